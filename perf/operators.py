@@ -208,7 +208,7 @@ def _prepare_sample(case, seed):
     # a bulk, and a few tokens well above it, as a trained head has them
     logits = 2.0 * _normal(gen, rows, vocab)
     few = min(vocab, 40)
-    places = torch.randint(0, vocab, (rows, few), generator=gen, device="cuda")
+    places = torch.rand((rows, vocab), generator=gen, device="cuda").topk(few, 1).indices  # no place twice
     logits.scatter_(1, places, 8 + 2.5 * _normal(gen, rows, few))
     logits[:, vocab - vocab // 16:] = -math.inf  # control tokens that a request may not draw
     u = torch.rand(rows, generator=gen, device="cuda")
