@@ -365,6 +365,129 @@ qtts_status qtts_generate_codes_batch(qtts_talker *t, qtts_predictor *p, int32_t
                                       const qtts_loop_params *params, const uint64_t *seeds, uint32_t *codes,
                                       int32_t *n_frames);
 
+/* ------------------------------------------------------------------------ */
+/* Serving many streams: a paged 8-bit cache, its attention, row sampling.    */
+/* No counterparts in the reference, whose cache is one f32 Vec per stream    */
+/* and whose sampler takes one row.                                           */
+/* ------------------------------------------------------------------------ */
+
+/* One layer's paged cache, in the caller's own device buffers (16-byte
+ * aligned).  A sequence's tokens fill pages of page_size; its page table says
+ * which page of the pool holds which tokens.  A full page is held as int8
+ * codes with one scale for each of its kv heads, K and V apart:
+ *   scale = max|x| / 127 over the block (f32),  code = 127 x / max|x| rounded
+ *   to the nearest, ties to even,  value = code * scale;
+ * a block of zeros has scale 0, a block with an Inf or NaN has scale NaN (its
+ * values read as NaN) and codes 0.  The page that a sequence is filling is
+ * held in f32 in the open rows of its slot, so that a block is rounded once
+ * and the cache does not depend on how its tokens were divided into calls. */
+typedef struct qtts_paged_kv {
+    int8_t *k_codes; /* [num_pages][kv_heads][page_size][head_dim] */
+    int8_t *v_codes; /* [num_pages][kv_heads][head_dim][page_size] */
+    float *k_scales; /* [num_pages][kv_heads] */
+    float *v_scales; /* [num_pages][kv_heads] */
+    float *k_open;   /* [num_slots][kv_heads][page_size][head_dim] */
+    float *v_open;   /* [num_slots][kv_heads][page_size][head_dim] */
+    int32_t num_pages;
+    int32_t kv_heads;
+    int32_t head_dim;  /* 64 or 128 */
+    int32_t page_size; /* 16, 32, 64 or 128 */
+    int32_t num_slots;
+} qtts_paged_kv;
+
+/* The sequences of one call.  The arrays are device memory and are read when
+ * the work runs, so a captured call follows what they hold at each replay.
+ * Sequence b has starts[b] tokens cached and takes rows row_offsets[b] up to
+ * row_offsets[b + 1] of the call's rows as its next tokens; rows past `rows`,
+ * and past max_rows of one sequence, are not looked at.  page_table row b
+ * holds its pages in order; an entry outside the pool is an absent page, whose
+ * tokens are neither written nor attended to (a window's dropped pages).  A
+ * sequence is left out as a whole, its cache untouched, where starts[b] is
+ * negative, its tokens pass max_pages * page_size (or the rotation's table) or
+ * slots[b] is outside the slots.  Pages may be shared for reading; the pages
+ * and slots that a call writes must be different ones. */
+typedef struct qtts_paged_seqs {
+    int32_t batch;
+    int32_t max_pages;          /* entries of a page_table row */
+    int32_t rows;               /* rows in the call's buffers */
+    int32_t max_rows;           /* most rows of one sequence */
+    const int32_t *page_table;  /* [batch][max_pages] */
+    const int32_t *slots;       /* [batch] */
+    const int32_t *starts;      /* [batch] */
+    const int32_t *row_offsets; /* [batch + 1] */
+} qtts_paged_seqs;
+
+/* New rows: per row, `heads` query heads (q may be NULL: none) and the cache's
+ * kv heads of head_dim floats, rows ld_* floats apart (a fused q|k|v product's
+ * parts).  Pointers are 16-byte aligned and strides multiples of 4. */
+typedef struct qtts_paged_rows {
+    const float *q, *k, *v;
+    float *q_out; /* [rows], ld_q_out apart; may be q itself with the same stride */
+    int32_t heads;
+    int32_t ld_q, ld_k, ld_v, ld_q_out;
+    const uint16_t *q_norm; /* [head_dim] binary16; NULL with k_norm: no norm */
+    const uint16_t *k_norm;
+    float eps;
+    int32_t rope_rows;     /* rows of the tables */
+    const float *rope_cos; /* [rope_rows][head_dim/2]; NULL with rope_sin: no rotation */
+    const float *rope_sin;
+} qtts_paged_rows;
+
+/* Appends each sequence's rows to its cache: per head RMSNorm (x * norm /
+ * sqrt(mean x^2 + eps)), the rotation of the halves at the token's position,
+ * in 64 bits and rounded to f32 once; v as it is.  Rotated queries go to q_out
+ * (rows of sequences left out and behind the last one stay as they were).
+ * Enqueued on the context stream, allocates nothing and can be captured. */
+qtts_status qtts_paged_append_device(qtts_ctx *ctx, const qtts_paged_kv *kv, const qtts_paged_seqs *seqs,
+                                     const qtts_paged_rows *rows);
+
+/* Attention of each sequence's rows over its cache after an append with the
+ * same qtts_paged_seqs: row i sees positions up to starts[b] + i, with
+ * window > 0 the last `window` of them, absent pages left out.  q and out hold
+ * heads * head_dim floats a row, ld_* apart (out may be q); head h reads kv head
+ * h / (heads / kv_heads).  scale multiplies the products (head_dim^-0.5).  A
+ * row that sees nothing, or of a sequence left out, is zeros; rows behind the
+ * last sequence stay as they were.  Enqueued on the context stream, allocates
+ * nothing and can be captured; its partial results lie in context scratch, so
+ * replay a graph in order with the context's calls. */
+qtts_status qtts_paged_attention_device(qtts_ctx *ctx, const qtts_paged_kv *kv, const qtts_paged_seqs *seqs,
+                                        int32_t heads, const float *d_q, int32_t ld_q, float scale, int32_t window,
+                                        float *d_out, int32_t ld_out);
+
+/* Cached tokens as f32 rows: sequence b, lens[b] tokens long (device, [batch];
+ * NULL: up to its last row asked for), gives positions starts[b] and on into
+ * rows row_offsets[b] up to row_offsets[b + 1] of k_out and v_out (kv_heads *
+ * head_dim floats a row, ld_* apart; either may be NULL).  Positions of
+ * absent pages read as zeros, as do those past lens[b]. */
+qtts_status qtts_paged_read_device(qtts_ctx *ctx, const qtts_paged_kv *kv, const qtts_paged_seqs *seqs,
+                                   const int32_t *d_lens, float *d_k_out, int32_t ld_k_out, float *d_v_out,
+                                   int32_t ld_v_out);
+
+/* Settings of each row's draw, device arrays of `rows` entries; NULL: 1, off,
+ * off, off. */
+typedef struct qtts_row_sampler {
+    const float *temperature; /* <= 0 or NaN: the largest logit, lowest index */
+    const int32_t *top_k;     /* the k largest; <= 0 or >= vocab: off */
+    const float *top_p;       /* the fewest largest with this share; >= 1 or NaN: off */
+    const float *min_p;       /* at least this share of the largest's; <= 0 or NaN: off */
+} qtts_row_sampler;
+
+/* Draws a token from each row of logits (rows of `vocab` floats, ld apart;
+ * 1 <= vocab <= 524288).  With w_i = exp((l_i - max) / temperature) and tokens
+ * ordered by logit, largest first, ties by index: top_k keeps the first k;
+ * top_p those of them whose predecessors' sum is below top_p times the sum;
+ * min_p those with w_i >= min_p; the first one stays always.  The token is the
+ * lowest index whose running sum over the kept ones, in index order, is above
+ * uniform[row] times their sum (uniform in [0, 1); NaN and below count as 0,
+ * 1 and above as the last).  Sums are exact to 2^-45 of the largest weight and
+ * do not depend on an order.  probs (or NULL) receives its share of the kept
+ * sum.  +Inf logits share the draw; a row of -Inf gives token -1 and share 0, a
+ * row with a NaN -1 and NaN.  Enqueued on the context stream, allocates
+ * nothing and can be captured (context scratch, as above). */
+qtts_status qtts_sample_rows_device(qtts_ctx *ctx, const float *d_logits, int64_t ld, int32_t rows, int32_t vocab,
+                                    const qtts_row_sampler *params, const float *d_uniform, int32_t *d_tokens,
+                                    float *d_probs);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,8 @@
 #include "../../include/qtts_synth.h"
 #include "engine.h"
 #include "internal.h"
+#include "paged_plan.h"
+#include "serve.h"
 
 using namespace qtts;
 
@@ -2894,9 +2896,121 @@ qtts_status qtts_sample_top_k(qtts_ctx *c, const float *logits, int32_t vocab, f
     return QTTS_OK;
 }
 
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Paged 8-bit cache and row sampling
+// ---------------------------------------------------------------------------
+namespace {
+
+// The context's device for a call, the caller's back afterwards.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(int device) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        if (before != device) (void)hipSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+qtts_status refuse(qtts_ctx *c, const Refusal &r) { return fail(c, r.status, r.why); }
+
+#define QTTS_CHECK(ctx, expr)                        \
+    do {                                             \
+        const Refusal r_ = (expr);                   \
+        if (r_.why) return refuse((ctx), r_);        \
+    } while (0)
+
+}  // namespace
+
+extern "C" {
+
+qtts_status qtts_paged_append_device(qtts_ctx *c, const qtts_paged_kv *kv, const qtts_paged_seqs *s,
+                                     const qtts_paged_rows *r) {
+    if (!c || !kv || !s || !r) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_append(*kv, *s, *r));
+    if (paged_empty(*s)) return QTTS_OK;
+    PagedAppendParams p{};
+    p.kv = *kv;
+    p.s = *s;
+    p.r = *r;
+    p.cap = (long long)s->max_pages * kv->page_size;
+    if (r->rope_cos) p.cap = std::min<long long>(p.cap, r->rope_rows);
+    DeviceGuard guard(c->device);
+    if (!launch_paged_append(c->stream, p)) return fail(c, QTTS_ERANGE, "paged append: more blocks than a launch holds");
+    return check_launch(c, "k_paged_append");
+}
+
+qtts_status qtts_paged_attention_device(qtts_ctx *c, const qtts_paged_kv *kv, const qtts_paged_seqs *s, int32_t heads,
+                                        const float *d_q, int32_t ld_q, float scale, int32_t window, float *d_out,
+                                        int32_t ld_out) {
+    if (!c || !kv || !s) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_attention(*kv, *s, heads, d_q, ld_q, scale, window, d_out, ld_out));
+    if (paged_empty(*s)) return QTTS_OK;
+    PagedAttnParams p{};
+    p.kv = *kv;
+    p.s = *s;
+    p.q = d_q;
+    p.out = d_out;
+    p.heads = heads;
+    p.ld_q = ld_q;
+    p.ld_out = ld_out;
+    p.scale = scale;
+    p.window = window;
+    DeviceGuard guard(c->device);
+    if (!launch_paged_attention(c->stream, p))
+        return fail(c, QTTS_ERANGE, "paged attention: more blocks than a launch holds");
+    return check_launch(c, "k_paged_attn");
+}
+
+qtts_status qtts_paged_read_device(qtts_ctx *c, const qtts_paged_kv *kv, const qtts_paged_seqs *s, const int32_t *d_lens,
+                                   float *d_k_out, int32_t ld_k_out, float *d_v_out, int32_t ld_v_out) {
+    if (!c || !kv || !s) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_read(*kv, *s, d_lens, d_k_out, ld_k_out, d_v_out, ld_v_out));
+    if (paged_empty(*s) || (!d_k_out && !d_v_out)) return QTTS_OK;
+    PagedReadParams p{};
+    p.kv = *kv;
+    p.s = *s;
+    p.lens = d_lens;
+    p.k_out = d_k_out;
+    p.v_out = d_v_out;
+    p.ld_k = ld_k_out;
+    p.ld_v = ld_v_out;
+    DeviceGuard guard(c->device);
+    if (!launch_paged_read(c->stream, p)) return fail(c, QTTS_ERANGE, "paged read: more blocks than a launch holds");
+    return check_launch(c, "k_paged_read");
+}
+
+qtts_status qtts_sample_rows_device(qtts_ctx *c, const float *d_logits, int64_t ld, int32_t rows, int32_t vocab,
+                                    const qtts_row_sampler *params, const float *d_uniform, int32_t *d_tokens,
+                                    float *d_probs) {
+    if (!c) return QTTS_EINVAL;
+    SampleRowsParams p{};
+    p.logits = d_logits;
+    p.ld = ld;
+    p.rows = rows;
+    p.vocab = vocab;
+    if (params) p.p = *params;
+    p.u = d_uniform;
+    p.tokens = d_tokens;
+    p.probs = d_probs;
+    QTTS_CHECK(c, check_sample_rows(d_logits, ld, rows, vocab, p.p, d_uniform, d_tokens, d_probs));
+    if (rows == 0) return QTTS_OK;
+    DeviceGuard guard(c->device);
+    launch_sample_rows(c->stream, p);
+    return check_launch(c, "k_sample_rows");
+}
+
+}  // extern "C"
+
 // ---------------------------------------------------------------------------
 // Frame loop
 // ---------------------------------------------------------------------------
+extern "C" {
+
 namespace {
 
 struct LoopCfg {

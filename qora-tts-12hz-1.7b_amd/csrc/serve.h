@@ -1,0 +1,56 @@
+// serve.h — kernel parameter blocks and launches of the serving operators: the
+// paged 8-bit cache (paged.hip) and row sampling (sample_rows.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/qtts.h"
+
+namespace qtts {
+
+struct PagedAppendParams {
+    qtts_paged_kv kv;
+    qtts_paged_seqs s;
+    qtts_paged_rows r;
+    int kv_items;   // pages one sequence's rows can touch
+    int q_items;    // blocks over one sequence's queries
+    long long cap;  // tokens a sequence may reach
+};
+
+struct PagedAttnParams {
+    qtts_paged_kv kv;
+    qtts_paged_seqs s;
+    const float *q;
+    float *out;
+    int heads, ld_q, ld_out;
+    float scale;
+    int window;
+};
+
+struct PagedReadParams {
+    qtts_paged_kv kv;
+    qtts_paged_seqs s;
+    const int32_t *lens;
+    float *k_out, *v_out;
+    int ld_k, ld_v;
+};
+
+struct SampleRowsParams {
+    const float *logits;
+    long long ld;
+    int rows, vocab;
+    qtts_row_sampler p;
+    const float *u;
+    int32_t *tokens;
+    float *probs;
+};
+
+// False: the call needs more blocks than one launch holds, nothing was launched.
+bool launch_paged_append(hipStream_t st, const PagedAppendParams &p);
+bool launch_paged_attention(hipStream_t st, const PagedAttnParams &p);
+bool launch_paged_read(hipStream_t st, const PagedReadParams &p);
+void launch_sample_rows(hipStream_t st, const SampleRowsParams &p);
+
+}  // namespace qtts

@@ -200,6 +200,31 @@ class LoopParams(C.Structure):
     ]
 
 
+class PagedKv(C.Structure):
+    """qtts_paged_kv: one layer's paged 8-bit cache, device pointers."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k_codes", "v_codes", "k_scales", "v_scales", "k_open", "v_open")] + [
+        (n, C.c_int32) for n in ("num_pages", "kv_heads", "head_dim", "page_size", "num_slots")]
+
+
+class PagedSeqs(C.Structure):
+    """qtts_paged_seqs: the sequences of one call, device pointers."""
+
+    _fields_ = [(n, C.c_int32) for n in ("batch", "max_pages", "rows", "max_rows")] + [
+        (n, C.c_void_p) for n in ("page_table", "slots", "starts", "row_offsets")]
+
+
+class PagedRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + [
+        (n, C.c_int32) for n in ("heads", "ld_q", "ld_k", "ld_v", "ld_q_out")] + [
+        ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float), ("rope_rows", C.c_int32),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p)]
+
+
+class RowSampler(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p")]
+
+
 _lib = None
 
 
@@ -292,6 +317,11 @@ def load_library(path: str = LIB_PATH):
         "qtts_prefill_talker": ([vp, vp, vp, i32, vp, f32p], i32),
         "qtts_generate_speech": ([vp, vp, vp, vp, i32, u32, u32, vp, vp, vp, C.POINTER(LoopParams), C.c_uint64, f32p,
                                   C.c_int64, C.POINTER(C.c_int64), C.POINTER(i32)], i32),
+        "qtts_paged_append_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), C.POINTER(PagedRows)], i32),
+        "qtts_paged_attention_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), i32, vp, i32, C.c_float, i32,
+                                         vp, i32], i32),
+        "qtts_paged_read_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), vp, vp, i32, vp, i32], i32),
+        "qtts_sample_rows_device": ([vp, vp, C.c_int64, i32, i32, C.POINTER(RowSampler), vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -320,6 +350,8 @@ def exported_symbols() -> List[str]:
         "qtts_model_file_talker", "qtts_model_file_predictor", "qtts_model_file_text", "qtts_model_file_info",
         "qtts_model_file_decoder", "qtts_decoder_upload", "qtts_decoder_free", "qtts_decoder_num_samples",
         "qtts_decode_to_audio", "qtts_decode_to_audio_device", "qtts_prefill_talker", "qtts_generate_speech",
+        "qtts_paged_append_device", "qtts_paged_attention_device", "qtts_paged_read_device",
+        "qtts_sample_rows_device",
     ]
 
 
@@ -870,6 +902,33 @@ class Context:
         self.check(self.lib.qtts_sample_top_k(self.h, _ptr(lg), lg.size, float(temperature), int(top_k),
                                               C.byref(state), C.byref(tok)))
         return int(tok.value), int(state.value)
+
+
+    # Paged 8-bit cache and row sampling (include/qtts.h).  Pointers are
+    # device addresses (0: none); the work goes on the context's stream.
+    def paged_append_device(self, kv: PagedKv, seqs: PagedSeqs, k: int, ld_k: int, v: int, ld_v: int, heads: int = 0,
+                            q: int = 0, ld_q: int = 0, q_out: int = 0, ld_q_out: int = 0, q_norm: int = 0,
+                            k_norm: int = 0, eps: float = 1e-6, rope_cos: int = 0, rope_sin: int = 0,
+                            rope_rows: int = 0):
+        rows = PagedRows(q, k, v, q_out, heads, ld_q, ld_k, ld_v, ld_q_out, q_norm, k_norm, eps, rope_rows, rope_cos,
+                         rope_sin)
+        self.check(self.lib.qtts_paged_append_device(self.h, C.byref(kv), C.byref(seqs), C.byref(rows)))
+
+    def paged_attention_device(self, kv: PagedKv, seqs: PagedSeqs, heads: int, q: int, ld_q: int, out: int,
+                               ld_out: int, scale: float, window: int = 0):
+        self.check(self.lib.qtts_paged_attention_device(self.h, C.byref(kv), C.byref(seqs), heads, q, ld_q, scale,
+                                                        window, out, ld_out))
+
+    def paged_read_device(self, kv: PagedKv, seqs: PagedSeqs, lens: int, k_out: int, ld_k_out: int, v_out: int,
+                          ld_v_out: int):
+        self.check(self.lib.qtts_paged_read_device(self.h, C.byref(kv), C.byref(seqs), lens, k_out, ld_k_out, v_out,
+                                                   ld_v_out))
+
+    def sample_rows_device(self, logits: int, ld: int, rows: int, vocab: int, uniform: int, tokens: int,
+                           probs: int = 0, temperature: int = 0, top_k: int = 0, top_p: int = 0, min_p: int = 0):
+        p = RowSampler(temperature, top_k, top_p, min_p)
+        self.check(self.lib.qtts_sample_rows_device(self.h, logits, ld, rows, vocab, C.byref(p), uniform, tokens,
+                                                    probs))
 
 
 class DeviceQ4(_DeviceObject):
