@@ -32,6 +32,7 @@ constexpr size_t kPartialFloats = (size_t)1 << 20;  // split-K partials
 constexpr int kCounters = 8192;
 constexpr size_t kAttnPartFloats = (size_t)4 << 20;
 constexpr int kAttnCounters = 1024;
+static_assert(kAttnPartFloats >= (size_t)kPagedPartFloats, "the paged attention's chunks fit");
 
 }  // namespace
 
@@ -43,6 +44,7 @@ struct qtts_ctx {
     unsigned *counters = nullptr;
     float *attn_part = nullptr;
     unsigned *attn_counters = nullptr;
+    unsigned *paged_counters = nullptr;
     // staging for the stand-alone operators
     float *d_in = nullptr;
     size_t d_in_cap = 0;
@@ -86,6 +88,7 @@ void ctx_release(qtts_ctx *c) {
     (void)hipFree(c->counters);
     (void)hipFree(c->attn_part);
     (void)hipFree(c->attn_counters);
+    (void)hipFree(c->paged_counters);
     (void)hipFree(c->d_in);
     (void)hipFree(c->d_out);
     (void)hipFree(c->d_small);
@@ -1588,9 +1591,11 @@ qtts_status qtts_ctx_create(int32_t device, qtts_ctx **out) {
     if (bad(hipMalloc(&c->counters, kCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->attn_part, kAttnPartFloats * sizeof(float)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->attn_counters, kAttnCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
+    if (bad(hipMalloc(&c->paged_counters, kPagedCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->d_small, 256))) return QTTS_ENOMEM;
     if (bad(hipMemset(c->counters, 0, kCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
     if (bad(hipMemset(c->attn_counters, 0, kAttnCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
+    if (bad(hipMemset(c->paged_counters, 0, kPagedCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
     if (bad(static_scratch_setup(device))) return QTTS_EDEVICE;
     if (bad(hipDeviceSynchronize())) return QTTS_EDEVICE;
     *out = c;
@@ -2960,6 +2965,8 @@ qtts_status qtts_paged_attention_device(qtts_ctx *c, const qtts_paged_kv *kv, co
     p.ld_out = ld_out;
     p.scale = scale;
     p.window = window;
+    p.part = c->attn_part;
+    p.counters = c->paged_counters;
     DeviceGuard guard(c->device);
     if (!launch_paged_attention(c->stream, p))
         return fail(c, QTTS_ERANGE, "paged attention: more blocks than a launch holds");

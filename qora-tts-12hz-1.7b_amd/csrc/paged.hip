@@ -178,63 +178,426 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
     if (j == 0 && begun && end % P != 0) open_rows(end / P * P, end);
 }
 
-// One block of four waves per (row, head): each wave takes every fourth token,
-// a lane HD / 64 of its dimensions.
-template <int HD>
-__global__ __launch_bounds__(256) void k_paged_attn_row(PagedAttnParams A) {
-    constexpr int E = HD / 64;
-    __shared__ float part[4][HD + 2];
-    const int P = A.kv.page_size, kvh = A.kv.kv_heads;
-    const int h = blockIdx.x % A.heads;
-    const int i = blockIdx.x / A.heads % A.s.max_rows, b = blockIdx.x / A.heads / A.s.max_rows;
+// ---------------------------------------------------------------------------
+// Attention.  Scores are computed transposed, S^T = K Q^T, and so is the
+// output, O^T = V^T P^T: the columns of every product are query rows (a row of
+// the call and one of the heads that share the kv head, "columns" below), and
+// the lane that holds a probability after the first product is the one that
+// feeds it to the second, with no exchange between lanes.  The order of tokens
+// in a contraction is free, so the pages are read 16 bytes a lane in an order
+// that makes it so.
+//
+// Codes are exact in binary16.  A query column is scaled by a power of two and
+// split into binary16 hi + lo (22 bits); a probability, with its page's scale of
+// V multiplied in, likewise; accumulation is in f32.  Both are scaled to below
+// 2^15, so that the least step of binary16 is 2^-39 of a column's largest.  The
+// exponent of a page's scale of V joins the score in the running maximum
+// (t = s + e), so that this holds of the weights whatever V's size is.
+// ---------------------------------------------------------------------------
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kRoom = 14;  // binary places that the split operands are raised by
+
+// Eight int8 codes as binary16: byte u = code + 128 becomes 1024 + u, whose
+// mantissa it is, minus 1152.
+__device__ __forceinline__ f16x8 codes_f16(unsigned w0, unsigned w1) {
+    const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    union {
+        f16x8 v;
+        f16x2 h[4];
+    } r;
+    w0 ^= 0x80808080u, w1 ^= 0x80808080u;
+    r.h[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u)) + off;
+    r.h[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u)) + off;
+    r.h[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u)) + off;
+    r.h[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)) + off;
+    return r.v;
+}
+
+// Maximum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float rows4_max(float v) {
+    v = halves_max(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float rows4_sum(float v) {
+    v = halves_sum(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// v[l] + v[l ^ 8] within rows of 16 lanes.
+__device__ __forceinline__ float sum_ror8(float v) { return v + dpp<0x128>(v); }
+
+// The exponent that joins a score: of V's scale there.  Its ends keep both the
+// split weights and the sum of probabilities (scaled back by it) in range; a
+// block of zeros weighs nothing, and takes a middle one that leaves the running
+// maximum to the others.
+__device__ __forceinline__ int fold_exponent(float x) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
+    return x == 0.0f ? -30 : e < -90 ? -90 : e > 121 ? 121 : e;
+}
+
+// Up to 16 columns of one kv head over one chunk of the tokens: a block of four
+// waves, each every fourth step of 64 tokens; chunks are joined by the block
+// that ends last.  Bound by reading the pages: 16 loads of 16 bytes a lane are
+// in flight per step, K's for the next step from when this step's scores are
+// done and V's from when its output is.
+//
+// Of a step's 64 tokens, lane (r = lane % 16, G = lane / 16) has scores of
+// tokens 16G + 4t + i in register i of tile t, for column r, and feeds them to
+// the output's contraction slots 8G + j of product s as tokens 16G + 8s + j:
+// its own.  K's tile t therefore holds token 16 (r / 4) + 4t + r % 4 in row r.
+//
+// WIDE = false: at most 8 columns, hi in operand columns 0-7 and lo in 8-15, one
+// product for both.  WIDE = true: 16 columns and two products.
+template <int HD, bool WIDE>
+__global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
+    constexpr int CT = WIDE ? 16 : 8;
+    constexpr int NK = HD / 64, ND = HD / 16;  // 16-byte pieces of a K row in a lane; dimension tiles
+    __shared__ float so[4][CT][HD + 4];
+    __shared__ float sm[4][CT], sl[4][CT];
+    __shared__ unsigned sarrived;
+    const int P = A.kv.page_size, kvh = A.kv.kv_heads, group = A.heads / kvh;
+    int id = blockIdx.x;
+    const int split = id % A.nsplit;
+    id /= A.nsplit;
+    const int pair = id;
+    const int tile = id % A.tiles;
+    id /= A.tiles;
+    const int head = id % kvh, b = id / kvh;
     const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, (long long)A.s.max_pages * P);
-    if (i >= q.rows) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int head = h / (A.heads / kvh);
-    const float *qr = A.q + (size_t)(q.row0 + i) * A.ld_q + (size_t)h * HD;
-    float m = -INFINITY, l = 0, o[E] = {}, x[E];
-    for (int e = 0; e < E; e++) x[e] = qr[lane + 64 * e];
-    if (q.ok) {
-        const int end = q.start + q.rows, full = end / P * P, pos = q.start + i;
-        const int low = A.window > 0 && pos - A.window >= 0 ? pos - A.window + 1 : 0;
-        for (int t = low + wave; t <= pos; t += 4) {
-            float s = 0, y[E];
-            if (t < full) {
-                const int id = q.pages[t / P];
-                if (id < 0 || id >= A.kv.num_pages) continue;
-                const size_t block = (size_t)id * kvh + head;
-                for (int e = 0; e < E; e++) {
-                    s += x[e] * (float)A.kv.k_codes[(block * P + t % P) * HD + lane + 64 * e];
-                    y[e] = (float)A.kv.v_codes[(block * HD + lane + 64 * e) * P + t % P] * A.kv.v_scales[block];
-                }
-                s *= A.kv.k_scales[block];
-            } else {
-                const size_t row = (((size_t)q.slot * kvh + head) * P + t % P) * HD;
-                for (int e = 0; e < E; e++) {
-                    s += x[e] * A.kv.k_open[row + lane + 64 * e];
-                    y[e] = A.kv.v_open[row + lane + 64 * e];
+    const int left = (int)min((long long)q.rows * group - (long long)tile * CT, (long long)CT);
+    if (left <= 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, G = lane >> 4;
+    auto out_of = [&](int n) {  // column n's place in the output
+        const int c = tile * CT + n;
+        return A.out + (size_t)(q.row0 + c / group) * A.ld_out + (size_t)(head * group + c % group) * HD;
+    };
+    if (!q.ok) {
+        if (split == 0)
+            for (int i = threadIdx.x; i < left * HD; i += 256) out_of(i / HD)[i % HD] = 0.0f;
+        return;
+    }
+    // what the columns see: tokens low .. high - 1
+    const int row_a = tile * CT / group, row_b = (tile * CT + left - 1) / group;
+    const int high = q.start + row_b + 1;
+    const int low = A.window > 0 ? max(0, q.start + row_a - A.window + 1) : 0;
+    const int first = low / A.chunk, last = (high - 1) / A.chunk;
+    if (split < first || split > last) return;
+    const int end = q.start + q.rows, full = end / P * P;
+
+    // this lane's column
+    const int n = WIDE ? r : r & 7;
+    const bool real = n < left;
+    const int col = tile * CT + (real ? n : 0);
+    const int pos = q.start + col / group;
+    const float *qr = A.q + (size_t)(q.row0 + col / group) * A.ld_q + (size_t)(head * group + col % group) * HD;
+    f16x8 qh[2 * NK], ql[2 * NK];
+    float qscale;
+    {
+        float x[2 * NK][8], top = 0;
+        unsigned bits = 0;
+#pragma unroll
+        for (int ks = 0; ks < 2 * NK; ks++) {
+            const float *p = qr + 64 * (ks / 2) + 16 * G + 8 * (ks % 2);
+            const float4 a = *reinterpret_cast<const float4 *>(p), c = *reinterpret_cast<const float4 *>(p + 4);
+            x[ks][0] = a.x, x[ks][1] = a.y, x[ks][2] = a.z, x[ks][3] = a.w;
+            x[ks][4] = c.x, x[ks][5] = c.y, x[ks][6] = c.z, x[ks][7] = c.w;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (!real) x[ks][j] = 0.0f;
+                bits = max(bits, __float_as_uint(x[ks][j]) & 0x7fffffffu);
+            }
+        }
+        top = rows4_max(__uint_as_float(min(bits, 0x7f7fffffu)));
+        const bool odd = bits >= 0x7f800000u;  // an Inf or NaN: the column is NaN
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        e = e < -126 ? -126 : e;
+#pragma unroll
+        for (int ks = 0; ks < 2 * NK; ks++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = odd ? __uint_as_float(0x7fc00000u) : ldexpf(x[ks][j], kRoom - e);
+                const _Float16 h = (_Float16)y;
+                const _Float16 l = (_Float16)(y - (float)h);
+                if (WIDE) {
+                    qh[ks][j] = h, ql[ks][j] = l;
+                } else {
+                    qh[ks][j] = r < 8 ? h : l;
                 }
             }
-            s = wave_sum(s) * A.scale;
-            const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
-            l = l * c + p;
-            for (int e = 0; e < E; e++) o[e] = o[e] * c + p * y[e];
+        }
+        qscale = ldexpf(A.scale * kLog2e, e - kRoom);
+    }
+
+    float m = -INFINITY, l = 0;
+    f32x4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = f32x4{0, 0, 0, 0};
+
+    auto raise = [&](float mx) {  // the running maximum, and what was summed under the last one
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= c;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= c;
             m = mn;
         }
+    };
+
+    // --- full pages ---
+    const int c0 = split * A.chunk;
+    const int stop = min(min(c0 + A.chunk, full), high);
+    int base = c0 + 64 * wave;
+    if (low > c0) base += (low - c0) / 256 * 256;
+    if (base + 64 <= low) base += 256;
+    u32x4 kr[4][NK], vr[ND];
+    float ks_, vs_;
+    bool there;
+    auto page_at = [&](int token) {  // an absent page reads as the pool's first, and is masked
+        return token < stop ? q.pages[token / P] : -1;
+    };
+    auto valid = [&](int pg) { return pg >= 0 && pg < A.kv.num_pages; };
+    auto load_k = [&](int at, int pg) {
+        const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
+        const int8_t *p = A.kv.k_codes + (block * P + (at + 16 * (r >> 2)) % P + (r & 3)) * HD + 16 * G;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int h = 0; h < NK; h++)
+                kr[t][h] = *glb(reinterpret_cast<const u32x4 *>(p + 4 * t * HD + 64 * h));
+    };
+    auto load_v = [&](int at, int pg) {
+        const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
+        const int8_t *p = A.kv.v_codes + (block * HD + r) * P + (at + 16 * G) % P;
+#pragma unroll
+        for (int d = 0; d < ND; d++) vr[d] = *glb(reinterpret_cast<const u32x4 *>(p + 16 * d * P));
+    };
+    auto load_scales = [&](int pg) {
+        const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
+        ks_ = A.kv.k_scales[block], vs_ = A.kv.v_scales[block];
+        there = valid(pg);
+    };
+    int pk = page_at(base + 16 * (r >> 2)), pv = page_at(base + 16 * G);
+    if (base < stop) {
+        load_k(base, pk);
+        load_v(base, pv);
+        load_scales(pv);
     }
-    for (int e = 0; e < E; e++) part[wave][lane + 64 * e] = o[e];
-    if (lane == 0) part[wave][HD] = m, part[wave][HD + 1] = l;
-    __syncthreads();
-    if (threadIdx.x < HD) {
-        float mx = -INFINITY, sum = 0, acc = 0;
-        for (int w = 0; w < 4; w++) mx = fmaxf(mx, part[w][HD]);
-        for (int w = 0; w < 4; w++) {
-            if (part[w][HD + 1] == 0.0f) continue;
-            const float c = expf(part[w][HD] - mx);
-            sum += c * part[w][HD + 1];
-            acc += c * part[w][threadIdx.x];
+    for (; base < stop; base += 256) {
+        const int next = base + 256;
+        const int pkn = page_at(next + 16 * (r >> 2)), pvn = page_at(next + 16 * G);
+        f32x4 s[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int h = 0; h < NK; h++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const f16x8 k = codes_f16(kr[t][h][2 * u], kr[t][h][2 * u + 1]);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[2 * h + u], acc, 0, 0, 0);
+                    if (WIDE) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[2 * h + u], acc, 0, 0, 0);
+                }
+            s[t] = acc;
         }
-        A.out[(size_t)(q.row0 + i) * A.ld_out + (size_t)h * HD + threadIdx.x] = sum == 0.0f ? 0.0f : acc / sum;
+        if (next < stop) load_k(next, pkn);
+        const float kq = qscale * ks_;
+        const int e = there ? fold_exponent(vs_) : 0;
+        const float f = there ? ldexpf(vs_, -e) : 1.0f, inv = ldexpf(1.0f, -e), ef = (float)e;
+        // every column sees all of the step's tokens unless the step passes
+        // the first column's position, the window's edge or an absent page
+        const bool plain = base + 63 <= q.start + row_a && base + 64 <= stop && base >= low &&
+                           (A.window == 0 || base > high - 1 - A.window) && __all(there);
+        float mx = -INFINITY, p[16];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x = WIDE ? s[t][i] : sum_ror8(s[t][i]);
+                x = fmaf(x, kq, ef);
+                if (!plain) {
+                    const int token = base + 16 * G + 4 * t + i;
+                    const bool seen = there && token <= pos && token < stop &&
+                                      (A.window == 0 || token > pos - A.window);
+                    x = seen ? x : -INFINITY;
+                }
+                p[4 * t + i] = x;
+                mx = fmaxf(mx, x);
+            }
+        raise(rows4_max(mx));
+        const float ms = m == -INFINITY ? 0.0f : m - kRoom;
+        float sum = 0;
+        f16x8 ph[2], pl[2];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float x = p[j];
+            const float y = __builtin_amdgcn_exp2f(x - ms);
+            sum += y;
+            float w = y * f;
+            if (!plain) w = x == -INFINITY ? 0.0f : w;
+            const _Float16 h = (_Float16)w;
+            const _Float16 lo = (_Float16)(w - (float)h);
+            if (WIDE) {
+                ph[j / 8][j % 8] = h, pl[j / 8][j % 8] = lo;
+            } else {
+                ph[j / 8][j % 8] = r < 8 ? h : lo;
+            }
+        }
+        l = fmaf(sum, inv, l);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const f16x8 v = codes_f16(vr[d][2 * u], vr[d][2 * u + 1]);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u], o[d], 0, 0, 0);
+                if (WIDE) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u], o[d], 0, 0, 0);
+            }
+        if (next < stop) {
+            load_v(next, pvn);
+            load_scales(pvn);
+        }
+    }
+
+    // --- the open page's rows, in f32 products, 16 tokens a step ---
+    const int open_hi = min(min(end, c0 + A.chunk), high);
+    for (int t0 = full + 16 * wave; t0 < open_hi; t0 += 64) {
+        if (t0 < c0 || t0 + 16 <= low) continue;
+        const size_t row = ((size_t)q.slot * kvh + head) * P;
+        const int kt = t0 + r;  // K: row r of the tile
+        const bool kin = kt < open_hi && kt >= low;
+        const float *kp = A.kv.k_open + (row + (kin ? kt % P : 0)) * HD + 4 * G;
+        f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < ND; c++) {
+            const float4 k = *reinterpret_cast<const float4 *>(kp + 16 * c);
+            float4 x = *reinterpret_cast<const float4 *>(qr + 16 * c + 4 * G);
+            if (!real || (!WIDE && r >= 8)) x = make_float4(0, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.x, x.x, s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.y, x.y, s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.z, x.z, s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.w, x.w, s, 0, 0, 0);
+        }
+        // V: token t0 + 4G + i, dimension 16 d + r.  What is not finite is left
+        // out of the products (0 * Inf would reach rows that do not see it) and
+        // added by itself below.
+        float v[4][ND], p[4], inv[4], mx = -INFINITY;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int token = t0 + 4 * G + i;
+            const bool in = token < open_hi && token >= low;
+            const float *vp = A.kv.v_open + (row + (in ? token % P : 0)) * HD + r;
+            float top = 0;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                float x = in ? vp[16 * d] : 0.0f;
+                if (!(fabsf(x) < INFINITY)) odd = true, x = 0.0f;
+                v[i][d] = x;
+                top = fmaxf(top, fabsf(x));
+            }
+            const int e = fold_exponent(row16_max(top) * (1.0f / 128.0f));
+            inv[i] = ldexpf(1.0f, -e);
+            const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
+            float x = fmaf(WIDE ? s[i] : sum_ror8(s[i]), A.scale * kLog2e, (float)e);
+            x = seen ? x : -INFINITY;
+            p[i] = x;
+            mx = fmaxf(mx, x);
+        }
+        raise(rows4_max(mx));
+        const float ms = m == -INFINITY ? 0.0f : m - kRoom;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float y = p[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms) * inv[i];
+            l += y;
+            p[i] = !WIDE && r >= 8 ? 0.0f : y;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d], p[i], o[d], 0, 0, 0);
+        if (__any(odd)) {
+            for (int g = 0; g < 4; g++) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int token = t0 + 4 * g + t;
+                    const float w = __shfl(p[t], r + 16 * g, 64);
+                    if (token >= open_hi || token < low) continue;
+                    const bool seen = token <= pos && (A.window == 0 || token > pos - A.window) && (WIDE || r < 8);
+                    const float *vp = A.kv.v_open + (row + token % P) * HD + 4 * G;
+#pragma unroll
+                    for (int d = 0; d < ND; d++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float x = vp[16 * d + i];
+                            if (seen && !(fabsf(x) < INFINITY)) o[d][i] += w * x;
+                        }
+                }
+            }
+        }
+    }
+
+    // --- the block's four waves ---
+    l = rows4_sum(l);
+    if (G == 0 && (WIDE || r < 8)) sm[wave][n] = m, sl[wave][n] = l;
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+        f32x4 x = o[d];
+        if (!WIDE)
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = sum_ror8(x[i]);
+        if (WIDE || r < 8) *reinterpret_cast<f32x4 *>(&so[wave][n][16 * d + 4 * G]) = x;
+    }
+    __syncthreads();
+    const int parts = last - first + 1;
+    float *part = A.part + ((size_t)pair * A.nsplit) * CT * (HD + 2);
+    for (int i = threadIdx.x; i < left * HD; i += 256) {
+        const int c = i / HD, d = i % HD;
+        float mx = -INFINITY, sum = 0, acc = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) mx = fmaxf(mx, sm[w][c]);
+        const float ms = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float x = __builtin_amdgcn_exp2f(sm[w][c] - ms);
+            sum = fmaf(x, sl[w][c], sum);
+            acc = fmaf(x, so[w][c][d], acc);
+        }
+        if (parts == 1) {
+            out_of(c)[d] = sum == 0.0f ? 0.0f : acc / sum;
+        } else {
+            float *to = part + ((size_t)(split - first) * CT + c) * (HD + 2);
+            st_dev(to + d, acc);
+            if (d == 0) st_dev(to + HD, mx), st_dev(to + HD + 1, sum);
+        }
+    }
+    if (parts == 1) return;
+    wait_stores();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sarrived = arrive_dev(A.counters + pair);
+        if (sarrived == (unsigned)parts - 1) reset_dev(A.counters + pair);
+    }
+    __syncthreads();
+    if (sarrived != (unsigned)parts - 1) return;
+    for (int i = threadIdx.x; i < left * HD; i += 256) {
+        const int c = i / HD, d = i % HD;
+        float mx = -INFINITY, sum = 0, acc = 0;
+        for (int k = 0; k < parts; k++) mx = fmaxf(mx, ld_dev(part + ((size_t)k * CT + c) * (HD + 2) + HD));
+        const float ms = mx == -INFINITY ? 0.0f : mx;
+        for (int k = 0; k < parts; k++) {
+            const float *from = part + ((size_t)k * CT + c) * (HD + 2);
+            const float x = __builtin_amdgcn_exp2f(ld_dev(from + HD) - ms);
+            sum = fmaf(x, ld_dev(from + HD + 1), sum);
+            acc = fmaf(x, ld_dev(from + d), acc);
+        }
+        out_of(c)[d] = sum == 0.0f ? 0.0f : acc / sum;
     }
 }
 
@@ -294,11 +657,27 @@ bool launch_paged_append(hipStream_t st, const PagedAppendParams &in) {
     return true;
 }
 
-bool launch_paged_attention(hipStream_t st, const PagedAttnParams &p) {
-    const long long blocks = (long long)p.s.batch * p.s.max_rows * p.heads;
+bool launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
+    PagedAttnParams p = in;
+    const int group = p.heads / p.kv.kv_heads, hd = p.kv.head_dim;
+    const long long cols = (long long)p.s.max_rows * group;
+    const bool wide = cols > 8;
+    const int ct = wide ? 16 : 8;
+    p.tiles = (int)((cols + ct - 1) / ct);
+    const long long pairs = (long long)p.s.batch * p.kv.kv_heads * p.tiles;
+    const AttnSplit plan = attn_split(pairs, (long long)p.s.max_pages * p.kv.page_size, (long long)ct * (hd + 2));
+    p.chunk = plan.chunk;
+    p.nsplit = plan.nsplit;
+    const long long blocks = pairs * p.nsplit;
     if (blocks > kPagedMaxBlocks) return false;
-    if (p.kv.head_dim == 64) hipLaunchKernelGGL(k_paged_attn_row<64>, dim3((unsigned)blocks), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(k_paged_attn_row<128>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    const dim3 grid((unsigned)blocks), block(256);
+    if (hd == 64) {
+        if (wide) hipLaunchKernelGGL((k_paged_attn_few<64, true>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((k_paged_attn_few<64, false>), grid, block, 0, st, p);
+    } else {
+        if (wide) hipLaunchKernelGGL((k_paged_attn_few<128, true>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((k_paged_attn_few<128, false>), grid, block, 0, st, p);
+    }
     return true;
 }
 

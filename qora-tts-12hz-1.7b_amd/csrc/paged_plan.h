@@ -25,6 +25,8 @@ struct Refusal {
 constexpr Refusal kAccepted{QTTS_OK, nullptr};
 constexpr long long kPagedMaxBlocks = (1LL << 31) - 1;  // of one launch
 constexpr int kSampleRowsMaxVocab = 1 << 19;
+constexpr long long kPagedBlocks = 1024;   // blocks that attention aims at
+constexpr long long kPagedMaxChunk = 2048;  // tokens a block takes at most where it can
 
 inline bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -140,6 +142,29 @@ inline Refusal check_sample_rows(const float *logits, int64_t ld, int32_t rows, 
         !aligned_to(p.temperature, 4) || !aligned_to(p.top_k, 4) || !aligned_to(p.top_p, 4) || !aligned_to(p.min_p, 4))
         return {QTTS_EINVAL, "sample_rows: misaligned argument"};
     return kAccepted;
+}
+
+// How attention divides a page table row's tokens over blocks.  A block takes
+// `chunk` tokens; results of several are joined through `part`, which holds
+// kPagedPartFloats, and a counter for each (sequence, kv head, column tile).
+constexpr long long kPagedPartFloats = 4LL << 20;
+constexpr long long kPagedCounters = 1 << 14;
+
+struct AttnSplit {
+    int chunk, nsplit;
+};
+
+inline AttnSplit attn_split(long long pairs, long long cap, long long floats) {
+    const long long steps = (cap + 255) / 256;  // of four waves
+    long long n = (kPagedBlocks + pairs - 1) / pairs;
+    n = n < (cap + kPagedMaxChunk - 1) / kPagedMaxChunk ? (cap + kPagedMaxChunk - 1) / kPagedMaxChunk : n;
+    const long long fits = pairs > kPagedCounters ? 1 : kPagedPartFloats / (pairs * floats);
+    n = n > fits ? fits : n;
+    n = n > steps ? steps : n;
+    n = n < 1 ? 1 : n;
+    const long long chunk = ((steps + n - 1) / n < 1 ? 1 : (steps + n - 1) / n) * 256;
+    const long long used = (cap + chunk - 1) / chunk;
+    return {(int)chunk, (int)(used < 1 ? 1 : used)};
 }
 
 // One sequence of a call as the kernels see it: whatever the device arrays

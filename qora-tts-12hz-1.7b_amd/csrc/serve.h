@@ -27,6 +27,11 @@ struct PagedAttnParams {
     int heads, ld_q, ld_out;
     float scale;
     int window;
+    // the launch's own
+    int tiles;           // column tiles of one sequence and kv head
+    int chunk, nsplit;   // tokens a block takes; blocks over a page table row
+    float *part;         // kPagedPartFloats: chunks' results
+    unsigned *counters;  // kPagedCounters, zero between launches
 };
 
 struct PagedReadParams {
