@@ -187,19 +187,16 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
 // in a contraction is free, so the pages are read 16 bytes a lane in an order
 // that makes it so.
 //
-// Codes are exact in binary16.  A query column is scaled by a power of two and
-// split into binary16 hi + lo (22 bits); a probability, with its page's scale of
-// V multiplied in, likewise; accumulation is in f32.  Both are scaled to below
-// 2^15, so that the least step of binary16 is 2^-39 of a column's largest.  The
-// exponent of a page's scale of V joins the score in the running maximum
-// (t = s + e), so that this holds of the weights whatever V's size is.
+// Weights of V's products are p times the page's scale of V.  The scale's
+// exponent joins the score in the running maximum (t = s + e), so that the
+// largest weight fills the operand's range whatever V's size is.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kRoom = 14;  // binary places that the split operands are raised by
 
 // Eight int8 codes as binary16: byte u = code + 128 becomes 1024 + u, whose
 // mantissa it is, minus 1152.
@@ -217,7 +214,16 @@ __device__ __forceinline__ f16x8 codes_f16(unsigned w0, unsigned w1) {
     return r.v;
 }
 
-// Maximum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+// Byte `digit` of four integers' balanced base-256 digits (-128 .. 127 but for
+// the highest): adding 128 to the lower digits carries, and taking it off each
+// is flipping its top bit.  `pick` selects the byte (digit | (digit + 4) << 8).
+__device__ __forceinline__ int digits4(int a, int b, int c, int d, unsigned pick, unsigned flip) {
+    const unsigned lo = __builtin_amdgcn_perm((unsigned)b + 0x808080u, (unsigned)a + 0x808080u, pick);
+    const unsigned hi = __builtin_amdgcn_perm((unsigned)d + 0x808080u, (unsigned)c + 0x808080u, pick);
+    return (int)((lo | hi << 16) ^ flip);
+}
+
+// Maximum and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float rows4_max(float v) {
     v = halves_max(v);
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -229,37 +235,51 @@ __device__ __forceinline__ float rows4_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// v[l] + v[l ^ 8] within rows of 16 lanes.
-__device__ __forceinline__ float sum_ror8(float v) { return v + dpp<0x128>(v); }
-
-// The exponent that joins a score: of V's scale there.  Its ends keep both the
-// split weights and the sum of probabilities (scaled back by it) in range; a
-// block of zeros weighs nothing, and takes a middle one that leaves the running
-// maximum to the others.
-__device__ __forceinline__ int fold_exponent(float x) {
-    const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
-    return x == 0.0f ? -30 : e < -90 ? -90 : e > 121 ? 121 : e;
+// Sum over the lanes l + 4 k of a row of 16, the same bits in each.
+__device__ __forceinline__ float digits_sum(float v) {
+    v += dpp<0x128>(v);  // row_ror:8
+    return v + dpp<0x124>(v);
 }
 
-// Up to 16 columns of one kv head over one chunk of the tokens: a block of four
+// The exponent that joins a score: of V's scale there.  Its ends keep both the
+// weights and the sum of probabilities (scaled back by it) in range; a block of
+// zeros weighs nothing, and takes a middle one that leaves the running maximum
+// to the others.
+__device__ __forceinline__ int fold_exponent(float x) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
+    return x == 0.0f ? -30 : e < -70 ? -70 : e > 121 ? 121 : e;
+}
+
+// Few columns of one kv head over one chunk of the tokens: a block of four
 // waves, each every fourth step of 64 tokens; chunks are joined by the block
 // that ends last.  Bound by reading the pages: 16 loads of 16 bytes a lane are
 // in flight per step, K's for the next step from when this step's scores are
 // done and V's from when its output is.
 //
 // Of a step's 64 tokens, lane (r = lane % 16, G = lane / 16) has scores of
-// tokens 16G + 4t + i in register i of tile t, for column r, and feeds them to
-// the output's contraction slots 8G + j of product s as tokens 16G + 8s + j:
-// its own.  K's tile t therefore holds token 16 (r / 4) + 4t + r % 4 in row r.
+// tokens 16G + 4t + i in register i of tile t, and feeds them to the output's
+// contraction as its slots of group G, which V's rows hold in that order.  K's
+// tile t therefore holds token 16 (r / 4) + 4t + r % 4 in row r.
 //
-// WIDE = false: at most 8 columns, hi in operand columns 0-7 and lo in 8-15, one
-// product for both.  WIDE = true: 16 columns and two products.
-template <int HD, bool WIDE>
+// I8: up to 4 columns, on int8 products: the codes go in as they are read.  A
+// query value (scaled to the column's largest) and a weight are 30-bit
+// integers, whose four base-256 digits take four operand columns: lane r holds
+// digit r / 4 of column r % 4.  Integer sums are exact; they join the f32 ones
+// when the running maximum rises.  Vector instructions a step: half of the f16
+// form's, which a chunk of one token's attention is bound by otherwise.
+//
+// Otherwise up to 16 columns on binary16 products: codes are exact in it, a
+// query value and a weight are split hi + lo (22 bits, scaled to below 2^15, so
+// that binary16's least step is 2^-39 of a column's largest).
+template <int HD, bool I8>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
-    constexpr int CT = WIDE ? 16 : 8;
+    constexpr int CT = I8 ? 4 : 16;
     constexpr int NK = HD / 64, ND = HD / 16;  // 16-byte pieces of a K row in a lane; dimension tiles
+    constexpr int kRoom = I8 ? 29 : 14;        // binary places of the largest weight
+    constexpr int kFlush = 1024;               // steps that int32 sums hold: 64 * 128 * 127 each
     __shared__ float so[4][CT][HD + 4];
     __shared__ float sm[4][CT], sl[4][CT];
+    __shared__ float fac[CT * kPagedMaxSplits];
     __shared__ unsigned sarrived;
     const int P = A.kv.page_size, kvh = A.kv.kv_heads, group = A.heads / kvh;
     int id = blockIdx.x;
@@ -269,10 +289,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
     const int tile = id % A.tiles;
     id /= A.tiles;
     const int head = id % kvh, b = id / kvh;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, G = lane >> 4;
     const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, (long long)A.s.max_pages * P);
     const int left = (int)min((long long)q.rows * group - (long long)tile * CT, (long long)CT);
     if (left <= 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, G = lane >> 4;
     auto out_of = [&](int n) {  // column n's place in the output
         const int c = tile * CT + n;
         return A.out + (size_t)(q.row0 + c / group) * A.ld_out + (size_t)(head * group + c % group) * HD;
@@ -282,83 +302,30 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
             for (int i = threadIdx.x; i < left * HD; i += 256) out_of(i / HD)[i % HD] = 0.0f;
         return;
     }
-    // what the columns see: tokens low .. high - 1
+    // What the columns see, tokens low .. high - 1, in equal chunks of whole
+    // steps: by this sequence's own length, not by its page table's.
     const int row_a = tile * CT / group, row_b = (tile * CT + left - 1) / group;
     const int high = q.start + row_b + 1;
     const int low = A.window > 0 ? max(0, q.start + row_a - A.window + 1) : 0;
-    const int first = low / A.chunk, last = (high - 1) / A.chunk;
-    if (split < first || split > last) return;
+    const int from = low & ~63, chunk = chunk_of(high - from, A.nsplit);
+    const int parts = (high - from + chunk - 1) / chunk;
+    if (split >= parts) return;
+    const int c0 = from + split * chunk;
     const int end = q.start + q.rows, full = end / P * P;
 
     // this lane's column
-    const int n = WIDE ? r : r & 7;
+    const int n = I8 ? r & 3 : r, digit = I8 ? r >> 2 : 0;
     const bool real = n < left;
     const int col = tile * CT + (real ? n : 0);
     const int pos = q.start + col / group;
     const float *qr = A.q + (size_t)(q.row0 + col / group) * A.ld_q + (size_t)(head * group + col % group) * HD;
-    f16x8 qh[2 * NK], ql[2 * NK];
-    float qscale;
-    {
-        float x[2 * NK][8], top = 0;
-        unsigned bits = 0;
-#pragma unroll
-        for (int ks = 0; ks < 2 * NK; ks++) {
-            const float *p = qr + 64 * (ks / 2) + 16 * G + 8 * (ks % 2);
-            const float4 a = *reinterpret_cast<const float4 *>(p), c = *reinterpret_cast<const float4 *>(p + 4);
-            x[ks][0] = a.x, x[ks][1] = a.y, x[ks][2] = a.z, x[ks][3] = a.w;
-            x[ks][4] = c.x, x[ks][5] = c.y, x[ks][6] = c.z, x[ks][7] = c.w;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (!real) x[ks][j] = 0.0f;
-                bits = max(bits, __float_as_uint(x[ks][j]) & 0x7fffffffu);
-            }
-        }
-        top = rows4_max(__uint_as_float(min(bits, 0x7f7fffffu)));
-        const bool odd = bits >= 0x7f800000u;  // an Inf or NaN: the column is NaN
-        int e = (int)(__float_as_uint(top) >> 23) - 127;
-        e = e < -126 ? -126 : e;
-#pragma unroll
-        for (int ks = 0; ks < 2 * NK; ks++) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = odd ? __uint_as_float(0x7fc00000u) : ldexpf(x[ks][j], kRoom - e);
-                const _Float16 h = (_Float16)y;
-                const _Float16 l = (_Float16)(y - (float)h);
-                if (WIDE) {
-                    qh[ks][j] = h, ql[ks][j] = l;
-                } else {
-                    qh[ks][j] = r < 8 ? h : l;
-                }
-            }
-        }
-        qscale = ldexpf(A.scale * kLog2e, e - kRoom);
-    }
 
-    float m = -INFINITY, l = 0;
-    f32x4 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f32x4{0, 0, 0, 0};
-
-    auto raise = [&](float mx) {  // the running maximum, and what was summed under the last one
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, mx);
-            const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            l *= c;
-#pragma unroll
-            for (int d = 0; d < ND; d++) o[d] *= c;
-            m = mn;
-        }
-    };
-
-    // --- full pages ---
-    const int c0 = split * A.chunk;
-    const int stop = min(min(c0 + A.chunk, full), high);
+    // --- full pages: the first step's loads ---
+    const int stop = min(min(c0 + chunk, full), high);
     int base = c0 + 64 * wave;
-    if (low > c0) base += (low - c0) / 256 * 256;
-    if (base + 64 <= low) base += 256;
     u32x4 kr[4][NK], vr[ND];
-    float ks_, vs_;
-    bool there;
+    float ks_ = 0, vs_ = 0;
+    bool there = false;
     auto page_at = [&](int token) {  // an absent page reads as the pool's first, and is masked
         return token < stop ? q.pages[token / P] : -1;
     };
@@ -383,128 +350,144 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
         ks_ = A.kv.k_scales[block], vs_ = A.kv.v_scales[block];
         there = valid(pg);
     };
-    int pk = page_at(base + 16 * (r >> 2)), pv = page_at(base + 16 * G);
+    // In this order, as loads come back in it: the pages' ids, the queries (made
+    // into operands meanwhile), the pages.
+    const int pk = page_at(base + 16 * (r >> 2)), pv = page_at(base + 16 * G);
+    float x[NK][16];
+#pragma unroll
+    for (int h = 0; h < NK; h++)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const float4 a = *reinterpret_cast<const float4 *>(qr + 64 * h + 16 * G + j);
+            x[h][j] = a.x, x[h][j + 1] = a.y, x[h][j + 2] = a.z, x[h][j + 3] = a.w;
+        }
     if (base < stop) {
         load_k(base, pk);
         load_v(base, pv);
         load_scales(pv);
     }
-    for (; base < stop; base += 256) {
-        const int next = base + 256;
-        const int pkn = page_at(next + 16 * (r >> 2)), pvn = page_at(next + 16 * G);
-        f32x4 s[4];
+
+    // --- the queries ---
+    i32x4 qi[NK];                // I8: digits of dimensions 64 h + 16 G + 0 .. 15
+    f16x8 qh[2 * NK], ql[2 * NK];  // else: hi and lo of 64 h + 16 G + 8 u + 0 .. 7 at 2 h + u
+    float qscale;
+    const unsigned pick = (unsigned)(digit | (digit + 4) << 8) | 0x0c0c0000u;
+    const unsigned flip = digit == 3 ? 0u : 0x80808080u;
+    {
+        unsigned bits = 0;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            f32x4 acc = {0, 0, 0, 0};
+        for (int h = 0; h < NK; h++)
 #pragma unroll
-            for (int h = 0; h < NK; h++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const f16x8 k = codes_f16(kr[t][h][2 * u], kr[t][h][2 * u + 1]);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[2 * h + u], acc, 0, 0, 0);
-                    if (WIDE) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[2 * h + u], acc, 0, 0, 0);
-                }
-            s[t] = acc;
-        }
-        if (next < stop) load_k(next, pkn);
-        const float kq = qscale * ks_;
-        const int e = there ? fold_exponent(vs_) : 0;
-        const float f = there ? ldexpf(vs_, -e) : 1.0f, inv = ldexpf(1.0f, -e), ef = (float)e;
-        // every column sees all of the step's tokens unless the step passes
-        // the first column's position, the window's edge or an absent page
-        const bool plain = base + 63 <= q.start + row_a && base + 64 <= stop && base >= low &&
-                           (A.window == 0 || base > high - 1 - A.window) && __all(there);
-        float mx = -INFINITY, p[16];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float x = WIDE ? s[t][i] : sum_ror8(s[t][i]);
-                x = fmaf(x, kq, ef);
-                if (!plain) {
-                    const int token = base + 16 * G + 4 * t + i;
-                    const bool seen = there && token <= pos && token < stop &&
-                                      (A.window == 0 || token > pos - A.window);
-                    x = seen ? x : -INFINITY;
-                }
-                p[4 * t + i] = x;
-                mx = fmaxf(mx, x);
+            for (int j = 0; j < 16; j++) {
+                if (!real) x[h][j] = 0.0f;
+                bits = max(bits, __float_as_uint(x[h][j]) & 0x7fffffffu);
             }
-        raise(rows4_max(mx));
-        const float ms = m == -INFINITY ? 0.0f : m - kRoom;
-        float sum = 0;
-        f16x8 ph[2], pl[2];
+        // an Inf or NaN anywhere makes the column NaN
+        const bool odd = rows4_max(bits >= 0x7f800000u ? 1.0f : 0.0f) > 0.0f;
+        const float top = rows4_max(__uint_as_float(min(bits, 0x7f7fffffu)));
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        e = e < -126 ? -126 : e;
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float x = p[j];
-            const float y = __builtin_amdgcn_exp2f(x - ms);
-            sum += y;
-            float w = y * f;
-            if (!plain) w = x == -INFINITY ? 0.0f : w;
-            const _Float16 h = (_Float16)w;
-            const _Float16 lo = (_Float16)(w - (float)h);
-            if (WIDE) {
-                ph[j / 8][j % 8] = h, pl[j / 8][j % 8] = lo;
+        for (int h = 0; h < NK; h++) {
+            if (I8) {
+                int v[16];
+#pragma unroll
+                for (int j = 0; j < 16; j++) v[j] = odd ? 0 : (int)rintf(ldexpf(x[h][j], 29 - e));
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    qi[h][j] = digits4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], pick, flip);
             } else {
-                ph[j / 8][j % 8] = r < 8 ? h : lo;
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const float y = odd ? 0.0f : ldexpf(x[h][j], 14 - e);
+                    const _Float16 a = (_Float16)y;
+                    qh[2 * h + j / 8][j % 8] = a;
+                    ql[2 * h + j / 8][j % 8] = (_Float16)(y - (float)a);
+                }
             }
         }
-        l = fmaf(sum, inv, l);
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const f16x8 v = codes_f16(vr[d][2 * u], vr[d][2 * u + 1]);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u], o[d], 0, 0, 0);
-                if (WIDE) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u], o[d], 0, 0, 0);
-            }
-        if (next < stop) {
-            load_v(next, pvn);
-            load_scales(pvn);
-        }
+        qscale = odd ? __uint_as_float(0x7fc00000u) : ldexpf(A.scale * kLog2e, I8 ? e - 29 + 8 * digit : e - 14);
     }
 
-    // --- the open page's rows, in f32 products, 16 tokens a step ---
-    const int open_hi = min(min(end, c0 + A.chunk), high);
+    float m = -INFINITY, l = 0;
+    f32x4 o[ND];
+    i32x4 oi[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = f32x4{0, 0, 0, 0}, oi[d] = i32x4{0, 0, 0, 0};
+    int held = 0;  // steps in oi
+
+    auto flush = [&]() {
+        if (I8 && held) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[d][i] += (float)oi[d][i];
+                oi[d] = i32x4{0, 0, 0, 0};
+            }
+            held = 0;
+        }
+    };
+    auto raise = [&](float mx) {  // the running maximum, and what was summed under the last one
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            flush();
+            l *= c;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= c;
+            m = mn;
+        }
+    };
+
+    // --- the open page's rows, in f32 products, 16 tokens a step (while the
+    // first step's pages are on their way) ---
+    const int open_hi = min(min(end, c0 + chunk), high);
     for (int t0 = full + 16 * wave; t0 < open_hi; t0 += 64) {
         if (t0 < c0 || t0 + 16 <= low) continue;
         const size_t row = ((size_t)q.slot * kvh + head) * P;
         const int kt = t0 + r;  // K: row r of the tile
         const bool kin = kt < open_hi && kt >= low;
         const float *kp = A.kv.k_open + (row + (kin ? kt % P : 0)) * HD + 4 * G;
-        f32x4 s = {0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < ND; c++) {
-            const float4 k = *reinterpret_cast<const float4 *>(kp + 16 * c);
-            float4 x = *reinterpret_cast<const float4 *>(qr + 16 * c + 4 * G);
-            if (!real || (!WIDE && r >= 8)) x = make_float4(0, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.x, x.x, s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.y, x.y, s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.z, x.z, s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.w, x.w, s, 0, 0, 0);
-        }
-        // V: token t0 + 4G + i, dimension 16 d + r.  What is not finite is left
-        // out of the products (0 * Inf would reach rows that do not see it) and
-        // added by itself below.
+        float4 kf[ND];
         float v[4][ND], p[4], inv[4], mx = -INFINITY;
-        bool odd = false;
+#pragma unroll
+        for (int c = 0; c < ND; c++) kf[c] = *reinterpret_cast<const float4 *>(kp + 16 * c);
+        // V: token t0 + 4G + i, dimension 16 d + r
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int token = t0 + 4 * G + i;
             const bool in = token < open_hi && token >= low;
             const float *vp = A.kv.v_open + (row + (in ? token % P : 0)) * HD + r;
+#pragma unroll
+            for (int d = 0; d < ND; d++) v[i][d] = in ? vp[16 * d] : 0.0f;
+        }
+        f32x4 s = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < ND; c++) {
+            float4 x = *reinterpret_cast<const float4 *>(qr + 16 * c + 4 * G);
+            if (!real || digit) x = make_float4(0, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].x, x.x, s, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].y, x.y, s1, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].z, x.z, s, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].w, x.w, s1, 0, 0, 0);
+        }
+        s += s1;
+        // What is not finite is left out of V's products (0 * Inf would reach
+        // rows that do not see it) and added by itself below.
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int token = t0 + 4 * G + i;
             float top = 0;
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                float x = in ? vp[16 * d] : 0.0f;
-                if (!(fabsf(x) < INFINITY)) odd = true, x = 0.0f;
-                v[i][d] = x;
-                top = fmaxf(top, fabsf(x));
+                if (!(fabsf(v[i][d]) < INFINITY)) odd = true, v[i][d] = 0.0f;
+                top = fmaxf(top, fabsf(v[i][d]));
             }
             const int e = fold_exponent(row16_max(top) * (1.0f / 128.0f));
             inv[i] = ldexpf(1.0f, -e);
             const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
-            float x = fmaf(WIDE ? s[i] : sum_ror8(s[i]), A.scale * kLog2e, (float)e);
+            float x = fmaf(I8 ? digits_sum(s[i]) : s[i], A.scale * kLog2e, (float)e);
             x = seen ? x : -INFINITY;
             p[i] = x;
             mx = fmaxf(mx, x);
@@ -515,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
         for (int i = 0; i < 4; i++) {
             const float y = p[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms) * inv[i];
             l += y;
-            p[i] = !WIDE && r >= 8 ? 0.0f : y;
+            p[i] = digit ? 0.0f : y;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -529,7 +512,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
                     const int token = t0 + 4 * g + t;
                     const float w = __shfl(p[t], r + 16 * g, 64);
                     if (token >= open_hi || token < low) continue;
-                    const bool seen = token <= pos && (A.window == 0 || token > pos - A.window) && (WIDE || r < 8);
+                    const bool seen = token <= pos && (A.window == 0 || token > pos - A.window) && !digit;
                     const float *vp = A.kv.v_open + (row + token % P) * HD + 4 * G;
 #pragma unroll
                     for (int d = 0; d < ND; d++)
@@ -543,20 +526,114 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
         }
     }
 
+    // --- full pages ---
+    for (; base < stop; base += 256) {
+        const int next = base + 256;
+        const int pkn = page_at(next + 16 * (r >> 2)), pvn = page_at(next + 16 * G);
+        float p[16];
+        const float kq = qscale * ks_;
+        const int e = there ? fold_exponent(vs_) : 0;
+        const float f = there ? ldexpf(vs_, -e) : 1.0f, inv = ldexpf(1.0f, -e);
+        if constexpr (I8) {
+            i32x4 s[4] = {};
+#pragma unroll
+            for (int h = 0; h < NK; h++)
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[t][h]), qi[h], s[t], 0, 0, 0);
+            const float ef = digit ? 0.0f : (float)e;
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[j] = digits_sum(fmaf((float)s[j / 4][j % 4], kq, ef));
+        } else {
+            f32x4 s[4] = {};
+#pragma unroll
+            for (int h = 0; h < NK; h++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        const f16x8 k = codes_f16(kr[t][h][2 * u], kr[t][h][2 * u + 1]);
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[2 * h + u], s[t], 0, 0, 0);
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[2 * h + u], s[t], 0, 0, 0);
+                    }
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[j] = fmaf(s[j / 4][j % 4], kq, (float)e);
+        }
+        if (next < stop) load_k(next, pkn);
+        // every column sees all of the step's tokens unless the step passes
+        // the first column's position, the window's edge or an absent page
+        const bool plain = base + 63 <= q.start + row_a && base + 64 <= stop && base >= low &&
+                           (A.window == 0 || base > high - 1 - A.window) && __all(there);
+        if (!plain) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int token = base + 16 * G + j;
+                const bool seen = there && token <= pos && token < stop && (A.window == 0 || token > pos - A.window);
+                p[j] = seen ? p[j] : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; j++) mx = fmaxf(mx, p[j]);
+        raise(rows4_max(mx));
+        const float ms = m == -INFINITY ? 0.0f : m - kRoom;
+        float sum = 0;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float y = __builtin_amdgcn_exp2f(p[j] - ms);
+            sum += y;
+            p[j] = p[j] == -INFINITY ? 0.0f : y * f;
+        }
+        l = fmaf(sum, inv, l);
+        if constexpr (I8) {
+            i32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                w[j] = digits4((int)(unsigned)p[4 * j], (int)(unsigned)p[4 * j + 1], (int)(unsigned)p[4 * j + 2],
+                               (int)(unsigned)p[4 * j + 3], pick, flip);
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                oi[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, vr[d]), w, oi[d], 0, 0, 0);
+            if (++held == kFlush) flush();
+        } else {
+            f16x8 ph[2], pl[2];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const _Float16 a = (_Float16)p[j];
+                ph[j / 8][j % 8] = a;
+                pl[j / 8][j % 8] = (_Float16)(p[j] - (float)a);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const f16x8 v = codes_f16(vr[d][2 * u], vr[d][2 * u + 1]);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u], o[d], 0, 0, 0);
+                }
+        }
+        if (next < stop) {
+            load_v(next, pvn);
+            load_scales(pvn);
+        }
+    }
+
     // --- the block's four waves ---
+    flush();
     l = rows4_sum(l);
-    if (G == 0 && (WIDE || r < 8)) sm[wave][n] = m, sl[wave][n] = l;
+    const bool writes = !I8 || digit == 0;
+    if (G == 0 && writes) sm[wave][n] = m, sl[wave][n] = l;
+    const float weight = ldexpf(1.0f, 8 * digit);
 #pragma unroll
     for (int d = 0; d < ND; d++) {
         f32x4 x = o[d];
-        if (!WIDE)
+        if (I8)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = sum_ror8(x[i]);
-        if (WIDE || r < 8) *reinterpret_cast<f32x4 *>(&so[wave][n][16 * d + 4 * G]) = x;
+            for (int i = 0; i < 4; i++) x[i] = digits_sum(x[i] * weight);
+        if (writes) *reinterpret_cast<f32x4 *>(&so[wave][n][16 * d + 4 * G]) = x;
     }
     __syncthreads();
-    const int parts = last - first + 1;
-    float *part = A.part + ((size_t)pair * A.nsplit) * CT * (HD + 2);
+    float *part = A.part + (size_t)pair * A.nsplit * CT * (HD + 2);
     for (int i = threadIdx.x; i < left * HD; i += 256) {
         const int c = i / HD, d = i % HD;
         float mx = -INFINITY, sum = 0, acc = 0;
@@ -572,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
         if (parts == 1) {
             out_of(c)[d] = sum == 0.0f ? 0.0f : acc / sum;
         } else {
-            float *to = part + ((size_t)(split - first) * CT + c) * (HD + 2);
+            float *to = part + ((size_t)split * CT + c) * (HD + 2);
             st_dev(to + d, acc);
             if (d == 0) st_dev(to + HD, mx), st_dev(to + HD + 1, sum);
         }
@@ -586,18 +663,51 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
     }
     __syncthreads();
     if (sarrived != (unsigned)parts - 1) return;
-    for (int i = threadIdx.x; i < left * HD; i += 256) {
-        const int c = i / HD, d = i % HD;
-        float mx = -INFINITY, sum = 0, acc = 0;
-        for (int k = 0; k < parts; k++) mx = fmaxf(mx, ld_dev(part + ((size_t)k * CT + c) * (HD + 2) + HD));
-        const float ms = mx == -INFINITY ? 0.0f : mx;
-        for (int k = 0; k < parts; k++) {
-            const float *from = part + ((size_t)k * CT + c) * (HD + 2);
-            const float x = __builtin_amdgcn_exp2f(ld_dev(from + HD) - ms);
-            sum = fmaf(x, ld_dev(from + HD + 1), sum);
-            acc = fmaf(x, ld_dev(from + d), acc);
+    // The parts' rows, eight loads in flight; the first eight of a thread's
+    // first value while the maxima and sums become every part's factor.
+    auto load8 = [&](float *x, int i, int k) {
+        const float *from = part + (size_t)(i / HD) * (HD + 2) + i % HD;
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = k + j < parts ? ld_dev(from + (size_t)(k + j) * CT * (HD + 2)) : 0.0f;
+    };
+    float y[8];
+    if ((int)threadIdx.x < left * HD) load8(y, threadIdx.x, 0);
+    for (int c = wave; c < left; c += 4) {
+        constexpr int N = kPagedMaxSplits / 64;
+        float pm[N], ps[N], mx = -INFINITY, sum = 0;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int k = lane + 64 * j;
+            const float *from = part + ((size_t)k * CT + c) * (HD + 2) + HD;
+            pm[j] = k < parts ? ld_dev(from) : -INFINITY;
+            ps[j] = k < parts ? ld_dev(from + 1) : 0.0f;
         }
-        out_of(c)[d] = sum == 0.0f ? 0.0f : acc / sum;
+#pragma unroll
+        for (int j = 0; j < N; j++) mx = fmaxf(mx, pm[j]);
+        mx = wave_max(mx);
+        const float ms = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const float f = __builtin_amdgcn_exp2f(pm[j] - ms);
+            if (lane + 64 * j < parts) fac[c * parts + lane + 64 * j] = f;
+            sum = fmaf(f, ps[j], sum);
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) sl[0][c] = sum;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < left * HD; i += 256) {
+        const float *fc = fac + i / HD * parts;
+        float acc = 0;
+        if (i != (int)threadIdx.x) load8(y, i, 0);
+        for (int k = 0; k < parts; k += 8) {
+            if (k) load8(y, i, k);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (k + j < parts) acc = fmaf(fc[k + j], y[j], acc);
+        }
+        const float sum = sl[0][i / HD];
+        out_of(i / HD)[i % HD] = sum == 0.0f ? 0.0f : acc / sum;
     }
 }
 
@@ -661,21 +771,19 @@ bool launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
     PagedAttnParams p = in;
     const int group = p.heads / p.kv.kv_heads, hd = p.kv.head_dim;
     const long long cols = (long long)p.s.max_rows * group;
-    const bool wide = cols > 8;
-    const int ct = wide ? 16 : 8;
+    const bool i8 = cols <= 4;
+    const int ct = i8 ? 4 : 16;
     p.tiles = (int)((cols + ct - 1) / ct);
     const long long pairs = (long long)p.s.batch * p.kv.kv_heads * p.tiles;
-    const AttnSplit plan = attn_split(pairs, (long long)p.s.max_pages * p.kv.page_size, (long long)ct * (hd + 2));
-    p.chunk = plan.chunk;
-    p.nsplit = plan.nsplit;
+    p.nsplit = attn_splits(pairs, (long long)p.s.max_pages * p.kv.page_size, (long long)ct * (hd + 2));
     const long long blocks = pairs * p.nsplit;
     if (blocks > kPagedMaxBlocks) return false;
     const dim3 grid((unsigned)blocks), block(256);
     if (hd == 64) {
-        if (wide) hipLaunchKernelGGL((k_paged_attn_few<64, true>), grid, block, 0, st, p);
+        if (i8) hipLaunchKernelGGL((k_paged_attn_few<64, true>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((k_paged_attn_few<64, false>), grid, block, 0, st, p);
     } else {
-        if (wide) hipLaunchKernelGGL((k_paged_attn_few<128, true>), grid, block, 0, st, p);
+        if (i8) hipLaunchKernelGGL((k_paged_attn_few<128, true>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((k_paged_attn_few<128, false>), grid, block, 0, st, p);
     }
     return true;

@@ -25,8 +25,6 @@ struct Refusal {
 constexpr Refusal kAccepted{QTTS_OK, nullptr};
 constexpr long long kPagedMaxBlocks = (1LL << 31) - 1;  // of one launch
 constexpr int kSampleRowsMaxVocab = 1 << 19;
-constexpr long long kPagedBlocks = 1024;   // blocks that attention aims at
-constexpr long long kPagedMaxChunk = 2048;  // tokens a block takes at most where it can
 
 inline bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -144,27 +142,35 @@ inline Refusal check_sample_rows(const float *logits, int64_t ld, int32_t rows, 
     return kAccepted;
 }
 
-// How attention divides a page table row's tokens over blocks.  A block takes
-// `chunk` tokens; results of several are joined through `part`, which holds
-// kPagedPartFloats, and a counter for each (sequence, kv head, column tile).
+// How attention divides a sequence's tokens over blocks.  Results of several are
+// joined through scratch of kPagedPartFloats, `floats` for each block, and a
+// counter for each pair (sequence and kv head, and column tile).
 constexpr long long kPagedPartFloats = 4LL << 20;
 constexpr long long kPagedCounters = 1 << 14;
+constexpr int kPagedMaxSplits = 256;
+// Two blocks a compute unit are one round of them.  Blocks of a second round
+// and smaller chunks cost more than they even out: 64 ragged sequences of up to
+// 8000 tokens (512 pairs) took 160 us with one block a pair, 180 us with four
+// and 204 us with eight; 4 of 32760 (32 pairs) 49 us with 16, 57 us with 32.
+constexpr long long kPagedBlocks = 512;
 
-struct AttnSplit {
-    int chunk, nsplit;
-};
-
-inline AttnSplit attn_split(long long pairs, long long cap, long long floats) {
-    const long long steps = (cap + 255) / 256;  // of four waves
-    long long n = (kPagedBlocks + pairs - 1) / pairs;
-    n = n < (cap + kPagedMaxChunk - 1) / kPagedMaxChunk ? (cap + kPagedMaxChunk - 1) / kPagedMaxChunk : n;
+// Blocks over one pair: the nearest to one round, at least 256 tokens each where
+// the page table row (`cap` tokens) is full.
+inline int attn_splits(long long pairs, long long cap, long long floats) {
+    const long long steps = (cap + 255) / 256;
     const long long fits = pairs > kPagedCounters ? 1 : kPagedPartFloats / (pairs * floats);
-    n = n > fits ? fits : n;
+    long long n = (kPagedBlocks + pairs / 2) / pairs;
     n = n > steps ? steps : n;
-    n = n < 1 ? 1 : n;
-    const long long chunk = ((steps + n - 1) / n < 1 ? 1 : (steps + n - 1) / n) * 256;
-    const long long used = (cap + chunk - 1) / chunk;
-    return {(int)chunk, (int)(used < 1 ? 1 : used)};
+    n = n > fits ? fits : n;
+    n = n > kPagedMaxSplits ? kPagedMaxSplits : n;
+    return (int)(n < 1 ? 1 : n);
+}
+
+// Tokens of one block where `nsplit` share `span` tokens: whole rounds of the
+// block's four waves, 64 tokens each.
+QTTS_HD int chunk_of(int span, int nsplit) {
+    const int each = span / nsplit + (span % nsplit != 0);
+    return (each + 255) / 256 * 256;
 }
 
 // One sequence of a call as the kernels see it: whatever the device arrays

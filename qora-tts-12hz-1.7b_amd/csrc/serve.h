@@ -29,7 +29,7 @@ struct PagedAttnParams {
     int window;
     // the launch's own
     int tiles;           // column tiles of one sequence and kv head
-    int chunk, nsplit;   // tokens a block takes; blocks over a page table row
+    int nsplit;          // blocks that share one tile's tokens
     float *part;         // kPagedPartFloats: chunks' results
     unsigned *counters;  // kPagedCounters, zero between launches
 };
