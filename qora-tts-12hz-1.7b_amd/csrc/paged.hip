@@ -187,9 +187,9 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
 // in a contraction is free, so the pages are read 16 bytes a lane in an order
 // that makes it so.
 //
-// Weights of V's products are p times the page's scale of V.  The scale's
-// exponent joins the score in the running maximum (t = s + e), so that the
-// largest weight fills the operand's range whatever V's size is.
+// Weights of V's products are p times the page's scale of V, whose logarithm
+// joins the score (t = s + log2 scale): the largest weight fills the operand's
+// range whatever V's size is.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -197,6 +197,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
+enum AttnMode { kAttnI8, kAttn16, kAttn32 };
 
 // Eight int8 codes as binary16: byte u = code + 128 becomes 1024 + u, whose
 // mantissa it is, minus 1152.
@@ -235,16 +236,22 @@ __device__ __forceinline__ float rows4_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The other row of 16 lanes in a half of the wave.
+__device__ __forceinline__ float dpp_row_pair(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return (threadIdx.x & 16) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
+}
+
 // Sum over the lanes l + 4 k of a row of 16, the same bits in each.
 __device__ __forceinline__ float digits_sum(float v) {
     v += dpp<0x128>(v);  // row_ror:8
     return v + dpp<0x124>(v);
 }
 
-// The exponent that joins a score: of V's scale there.  Its ends keep both the
-// weights and the sum of probabilities (scaled back by it) in range; a block of
-// zeros weighs nothing, and takes a middle one that leaves the running maximum
-// to the others.
+// The same of an open row, by its largest value's exponent.  Its ends keep both
+// the weights and the sum of probabilities (scaled back by it) in range; a row
+// of zeros weighs nothing, and takes a middle one that leaves the reference to
+// the others.
 __device__ __forceinline__ int fold_exponent(float x) {
     const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
     return x == 0.0f ? -30 : e < -70 ? -70 : e > 121 ? 121 : e;
@@ -271,25 +278,56 @@ __device__ __forceinline__ int fold_exponent(float x) {
 // Otherwise up to 16 columns on binary16 products: codes are exact in it, a
 // query value and a weight are split hi + lo (22 bits, scaled to below 2^15, so
 // that binary16's least step is 2^-39 of a column's largest).
-template <int HD, bool I8>
-__global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
-    constexpr int CT = I8 ? 4 : 16;
-    constexpr int NK = HD / 64, ND = HD / 16;  // 16-byte pieces of a K row in a lane; dimension tiles
-    constexpr int kRoom = I8 ? 29 : 14;        // binary places of the largest weight
-    constexpr int kFlush = 1024;               // steps that int32 sums hold: 64 * 128 * 127 each
+template <int HD, int MODE>
+__global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
+    constexpr bool I8 = MODE == kAttnI8;
+    constexpr int S = MODE == kAttn32 ? 32 : 16;  // side of a product's tile
+    constexpr int NG = 64 / S, NR = S * S / 64;   // lane groups, registers of a tile
+    constexpr int CT = I8 ? 4 : S;                // columns
+    constexpr int ST = 16 * NG, RT = 4 * ST;      // tokens of a wave's step, of the block's
+    constexpr int NT = ST / S;                    // token tiles of a step
+    constexpr int NK = HD / ST, ND = HD / S;      // 16-byte pieces of a K row in a lane; dimension tiles
+    // Weights are 2^(t - m); the reference m is set so that the largest is
+    // 2^kRoom, and again when one would pass 2^kLimit.
+    constexpr int kRoom = I8 ? 27 : 11, kLimit = I8 ? 30 : 15;
+    constexpr int kFlush = 1024;                  // steps that int32 sums hold: 64 * 128 * 127 each
+    typedef float Acc __attribute__((ext_vector_type(NR)));
     __shared__ float so[4][CT][HD + 4];
     __shared__ float sm[4][CT], sl[4][CT];
-    __shared__ float fac[CT * kPagedMaxSplits];
     __shared__ unsigned sarrived;
-    const int P = A.kv.page_size, kvh = A.kv.kv_heads, group = A.heads / kvh;
-    int id = blockIdx.x;
-    const int split = id % A.nsplit;
-    id /= A.nsplit;
-    const int pair = id;
-    const int tile = id % A.tiles;
-    id /= A.tiles;
-    const int head = id % kvh, b = id / kvh;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, G = lane >> 4;
+    static_assert(4 * (HD + 4) >= kPagedMaxSplits, "the parts' factors take so's place");
+    const int P = A.kv.page_size, sh = __builtin_ctz(P), kvh = A.kv.kv_heads, group = A.heads / kvh;
+    // Consecutive blocks lie on different XCDs.  Tiles of 32 share their pages:
+    // with kv heads innermost one head's are read through few caches, and the
+    // last rows, which see the most, go first.  Few columns read every page
+    // once, and faster with a pair's chunks spread (4 sequences of 32760: 48 us,
+    // 54 with heads innermost).
+    int id = blockIdx.x, head, b, split, tile;
+    if (S == 32) {
+        head = id % kvh, id /= kvh;
+        b = id % A.s.batch, id /= A.s.batch;
+        split = id % A.nsplit, tile = A.tiles - 1 - id / A.nsplit;
+    } else {
+        split = id % A.nsplit, id /= A.nsplit;
+        tile = id % A.tiles, id /= A.tiles;
+        head = id % kvh, b = id / kvh;
+    }
+    const size_t pair = ((size_t)b * kvh + head) * A.tiles + tile;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane % S, G = lane / S;
+    // the token (of a step's) in row r of K's tile 0: see above
+    const int krow = S == 16 ? 16 * (r >> 2) + (r & 3) : 16 * (r >> 2 & 1) + 8 * (r >> 4) + 4 * (r >> 3 & 1) + (r & 3);
+    auto group_max = [&](float v) { return NG == 4 ? rows4_max(v) : halves_max(v); };
+    auto group_add = [&](float v) { return NG == 4 ? rows4_sum(v) : halves_sum(v); };
+    // row of a product's tile that register i of this lane holds
+    auto row_of = [&](int i) { return S == 16 ? 4 * G + i : 8 * (i / 4) + 4 * G + i % 4; };
+    auto mma = [&](f16x8 x, f16x8 y, Acc c) {
+        if constexpr (S == 16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+    };
+    auto mma1 = [&](float x, float y, Acc c) {
+        if constexpr (S == 16) return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, c, 0, 0, 0);
+    };
     const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, (long long)A.s.max_pages * P);
     const int left = (int)min((long long)q.rows * group - (long long)tile * CT, (long long)CT);
     if (left <= 0) return;
@@ -311,7 +349,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
     const int parts = (high - from + chunk - 1) / chunk;
     if (split >= parts) return;
     const int c0 = from + split * chunk;
-    const int end = q.start + q.rows, full = end / P * P;
+    const int end = q.start + q.rows, full = end >> sh << sh;
 
     // this lane's column
     const int n = I8 ? r & 3 : r, digit = I8 ? r >> 2 : 0;
@@ -322,28 +360,28 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
 
     // --- full pages: the first step's loads ---
     const int stop = min(min(c0 + chunk, full), high);
-    int base = c0 + 64 * wave;
-    u32x4 kr[4][NK], vr[ND];
+    int base = c0 + ST * wave;
+    u32x4 kr[NT][NK], vr[ND];
     float ks_ = 0, vs_ = 0;
     bool there = false;
     auto page_at = [&](int token) {  // an absent page reads as the pool's first, and is masked
-        return token < stop ? q.pages[token / P] : -1;
+        return token < stop ? q.pages[token >> sh] : -1;
     };
     auto valid = [&](int pg) { return pg >= 0 && pg < A.kv.num_pages; };
     auto load_k = [&](int at, int pg) {
         const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
-        const int8_t *p = A.kv.k_codes + (block * P + (at + 16 * (r >> 2)) % P + (r & 3)) * HD + 16 * G;
+        const int8_t *p = A.kv.k_codes + (block * P + ((at + krow) & (P - 1))) * HD + 16 * G;
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int h = 0; h < NK; h++)
-                kr[t][h] = *glb(reinterpret_cast<const u32x4 *>(p + 4 * t * HD + 64 * h));
+                kr[t][h] = *glb(reinterpret_cast<const u32x4 *>(p + 4 * t * HD + ST * h));
     };
     auto load_v = [&](int at, int pg) {
         const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
-        const int8_t *p = A.kv.v_codes + (block * HD + r) * P + (at + 16 * G) % P;
+        const int8_t *p = A.kv.v_codes + (block * HD + r) * P + ((at + 16 * G) & (P - 1));
 #pragma unroll
-        for (int d = 0; d < ND; d++) vr[d] = *glb(reinterpret_cast<const u32x4 *>(p + 16 * d * P));
+        for (int d = 0; d < ND; d++) vr[d] = *glb(reinterpret_cast<const u32x4 *>(p + S * d * P));
     };
     auto load_scales = [&](int pg) {
         const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
@@ -352,24 +390,27 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
     };
     // In this order, as loads come back in it: the pages' ids, the queries (made
     // into operands meanwhile), the pages.
-    const int pk = page_at(base + 16 * (r >> 2)), pv = page_at(base + 16 * G);
+    const int pk = page_at(base + krow), pv = page_at(base + 16 * G);
     float x[NK][16];
 #pragma unroll
     for (int h = 0; h < NK; h++)
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
-            const float4 a = *reinterpret_cast<const float4 *>(qr + 64 * h + 16 * G + j);
+            const float4 a = *reinterpret_cast<const float4 *>(qr + ST * h + 16 * G + j);
             x[h][j] = a.x, x[h][j + 1] = a.y, x[h][j + 2] = a.z, x[h][j + 3] = a.w;
         }
-    if (base < stop) {
-        load_k(base, pk);
-        load_v(base, pv);
-        load_scales(pv);
-    }
+    auto load_first = [&]() {
+        if (base < stop) {
+            load_k(base, pk);
+            load_v(base, pv);
+            load_scales(pv);
+        }
+    };
+    if (S == 16) load_first();
 
     // --- the queries ---
-    i32x4 qi[NK];                // I8: digits of dimensions 64 h + 16 G + 0 .. 15
-    f16x8 qh[2 * NK], ql[2 * NK];  // else: hi and lo of 64 h + 16 G + 8 u + 0 .. 7 at 2 h + u
+    i32x4 qi[NK];                  // I8: digits of dimensions ST h + 16 G + 0 .. 15
+    f16x8 qh[2 * NK], ql[2 * NK];  // else: hi and lo of ST h + 16 G + 8 u + 0 .. 7 at 2 h + u
     float qscale;
     const unsigned pick = (unsigned)(digit | (digit + 4) << 8) | 0x0c0c0000u;
     const unsigned flip = digit == 3 ? 0u : 0x80808080u;
@@ -383,8 +424,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
                 bits = max(bits, __float_as_uint(x[h][j]) & 0x7fffffffu);
             }
         // an Inf or NaN anywhere makes the column NaN
-        const bool odd = rows4_max(bits >= 0x7f800000u ? 1.0f : 0.0f) > 0.0f;
-        const float top = rows4_max(__uint_as_float(min(bits, 0x7f7fffffu)));
+        const bool odd = group_max(bits >= 0x7f800000u ? 1.0f : 0.0f) > 0.0f;
+        const float top = group_max(__uint_as_float(min(bits, 0x7f7fffffu)));
         int e = (int)(__float_as_uint(top) >> 23) - 127;
         e = e < -126 ? -126 : e;
 #pragma unroll
@@ -410,26 +451,29 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
     }
 
     float m = -INFINITY, l = 0;
-    f32x4 o[ND];
-    i32x4 oi[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f32x4{0, 0, 0, 0}, oi[d] = i32x4{0, 0, 0, 0};
+    Acc o[ND] = {};
+    i32x4 oi[I8 ? ND : 1] = {};
     int held = 0;  // steps in oi
 
     auto flush = [&]() {
-        if (I8 && held) {
+        if constexpr (I8) {
+            if (held) {
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
+                for (int d = 0; d < ND; d++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[d][i] += (float)oi[d][i];
-                oi[d] = i32x4{0, 0, 0, 0};
+                    for (int i = 0; i < 4; i++) o[d][i] += (float)oi[d][i];
+                    oi[d] = i32x4{0, 0, 0, 0};
+                }
+                held = 0;
             }
-            held = 0;
         }
     };
-    auto raise = [&](float mx) {  // the running maximum, and what was summed under the last one
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, mx);
+    // A new reference where a column's largest t asks for it, and what was
+    // summed under the last one.
+    auto raise = [&](float top) {
+        const bool need = top > (m == -INFINITY ? -INFINITY : m + kLimit);
+        if (__any(need)) {
+            const float mn = need ? top - kRoom : m;
             const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
             flush();
             l *= c;
@@ -439,87 +483,100 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
         }
     };
 
-    // --- the open page's rows, in f32 products, 16 tokens a step (while the
+    // --- the open page's rows, in f32 products, S tokens a step (while the
     // first step's pages are on their way) ---
     const int open_hi = min(min(end, c0 + chunk), high);
-    for (int t0 = full + 16 * wave; t0 < open_hi; t0 += 64) {
-        if (t0 < c0 || t0 + 16 <= low) continue;
+    for (int t0 = full + S * wave; t0 < open_hi; t0 += 4 * S) {
+        if (t0 + S <= max(low, c0)) continue;
+        const int open_lo = max(low, c0);
         const size_t row = ((size_t)q.slot * kvh + head) * P;
         const int kt = t0 + r;  // K: row r of the tile
-        const bool kin = kt < open_hi && kt >= low;
-        const float *kp = A.kv.k_open + (row + (kin ? kt % P : 0)) * HD + 4 * G;
-        float4 kf[ND];
-        float v[4][ND], p[4], inv[4], mx = -INFINITY;
+        const bool kin = kt < open_hi && kt >= open_lo;
+        const float *kp = A.kv.k_open + (row + (kin ? (kt & (P - 1)) : 0)) * HD + 4 * G;
+        // V: dimension S d + r of the token of register i, BT registers at a
+        // time: all of them with tiles of 16, kept for the products; with tiles
+        // of 32 a half, read again for the products.
+        constexpr int BT = S == 16 ? NR : 8;
+        float v[BT][ND];
+        auto load_open = [&](int i0) {
 #pragma unroll
-        for (int c = 0; c < ND; c++) kf[c] = *reinterpret_cast<const float4 *>(kp + 16 * c);
-        // V: token t0 + 4G + i, dimension 16 d + r
+            for (int i = 0; i < BT; i++) {
+                const int token = t0 + row_of(i0 + i);
+                const bool in = token < open_hi && token >= open_lo;
+                const float *vp = A.kv.v_open + (row + (in ? (token & (P - 1)) : 0)) * HD + r;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int token = t0 + 4 * G + i;
-            const bool in = token < open_hi && token >= low;
-            const float *vp = A.kv.v_open + (row + (in ? token % P : 0)) * HD + r;
+                for (int d = 0; d < ND; d++) v[i][d] = vp[S * d];
 #pragma unroll
-            for (int d = 0; d < ND; d++) v[i][d] = in ? vp[16 * d] : 0.0f;
+                for (int d = 0; d < ND; d++) v[i][d] = in ? v[i][d] : 0.0f;
+            }
+        };
+        if (S == 16) load_open(0);
+        Acc s = {}, s1 = {};
+#pragma unroll
+        for (int c = 0; c < HD / (4 * NG); c++) {
+            const float4 y = *reinterpret_cast<const float4 *>(kp + 4 * NG * c);
+            float4 z = *reinterpret_cast<const float4 *>(qr + 4 * NG * c + 4 * G);
+            if (!real || digit) z = make_float4(0, 0, 0, 0);
+            s = mma1(y.x, z.x, s);
+            (S == 16 ? s1 : s) = mma1(y.y, z.y, S == 16 ? s1 : s);
+            s = mma1(y.z, z.z, s);
+            (S == 16 ? s1 : s) = mma1(y.w, z.w, S == 16 ? s1 : s);
         }
-        f32x4 s = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < ND; c++) {
-            float4 x = *reinterpret_cast<const float4 *>(qr + 16 * c + 4 * G);
-            if (!real || digit) x = make_float4(0, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].x, x.x, s, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].y, x.y, s1, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].z, x.z, s, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].w, x.w, s1, 0, 0, 0);
-        }
-        s += s1;
+        if (S == 16) s += s1;
         // What is not finite is left out of V's products (0 * Inf would reach
         // rows that do not see it) and added by itself below.
+        float p[NR], inv[NR], mx = -INFINITY;
         bool odd = false;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int token = t0 + 4 * G + i;
+        for (int i = 0; i < NR; i++) {
+            const int token = t0 + row_of(i);
+            if (S == 32 && i % BT == 0) load_open(i);
             float top = 0;
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                if (!(fabsf(v[i][d]) < INFINITY)) odd = true, v[i][d] = 0.0f;
-                top = fmaxf(top, fabsf(v[i][d]));
+                if (!(fabsf(v[i % BT][d]) < INFINITY)) odd = true, v[i % BT][d] = 0.0f;
+                top = fmaxf(top, fabsf(v[i % BT][d]));
             }
-            const int e = fold_exponent(row16_max(top) * (1.0f / 128.0f));
+            top = row16_max(top);
+            if (S == 32) top = fmaxf(top, dpp_row_pair(top));
+            const int e = fold_exponent(top * (1.0f / 128.0f));
             inv[i] = ldexpf(1.0f, -e);
-            const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
-            float x = fmaf(I8 ? digits_sum(s[i]) : s[i], A.scale * kLog2e, (float)e);
-            x = seen ? x : -INFINITY;
-            p[i] = x;
-            mx = fmaxf(mx, x);
+            const bool seen = token <= pos && token < open_hi && token >= open_lo &&
+                              (A.window == 0 || token > pos - A.window);
+            const float z = fmaf(I8 ? digits_sum(s[i]) : s[i], A.scale * kLog2e, (float)e);
+            p[i] = seen ? z : -INFINITY;
+            mx = fmaxf(mx, p[i]);
         }
-        raise(rows4_max(mx));
-        const float ms = m == -INFINITY ? 0.0f : m - kRoom;
+        raise(group_max(mx));
+        const float ms = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < NR; i++) {
             const float y = p[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms) * inv[i];
             l += y;
             p[i] = digit ? 0.0f : y;
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < NR; i++) {
+            if (S == 32 && i % BT == 0) load_open(i);
 #pragma unroll
             for (int d = 0; d < ND; d++)
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d], p[i], o[d], 0, 0, 0);
+                o[d] = mma1(S == 32 && !(fabsf(v[i % BT][d]) < INFINITY) ? 0.0f : v[i % BT][d], p[i], o[d]);
+        }
         if (__any(odd)) {
-            for (int g = 0; g < 4; g++) {
+            for (int g = 0; g < NG; g++) {
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int token = t0 + 4 * g + t;
-                    const float w = __shfl(p[t], r + 16 * g, 64);
-                    if (token >= open_hi || token < low) continue;
+                for (int t = 0; t < NR; t++) {
+                    const int token = t0 + row_of(t) + 4 * (g - G);  // of group g's register t
+                    const float w = __shfl(p[t], r + S * g, 64);
+                    if (token >= open_hi || token < open_lo) continue;
                     const bool seen = token <= pos && (A.window == 0 || token > pos - A.window) && !digit;
-                    const float *vp = A.kv.v_open + (row + token % P) * HD + 4 * G;
+                    const float *vp = A.kv.v_open + (row + (token & (P - 1))) * HD;
 #pragma unroll
                     for (int d = 0; d < ND; d++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float x = vp[16 * d + i];
-                            if (seen && !(fabsf(x) < INFINITY)) o[d][i] += w * x;
+                        for (int i = 0; i < NR; i++) {
+                            const float y = vp[S * d + row_of(i)];
+                            if (seen && !(fabsf(y) < INFINITY)) o[d][i] += w * y;
                         }
                 }
             }
@@ -527,13 +584,19 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
     }
 
     // --- full pages ---
-    for (; base < stop; base += 256) {
-        const int next = base + 256;
-        const int pkn = page_at(next + 16 * (r >> 2)), pvn = page_at(next + 16 * G);
+    if (S == 32) load_first();  // no registers to spare for them before
+    for (; base < stop; base += RT) {
+        const int next = base + RT;
+        const int pkn = page_at(next + krow), pvn = page_at(next + 16 * G);
         float p[16];
         const float kq = qscale * ks_;
-        const int e = there ? fold_exponent(vs_) : 0;
-        const float f = there ? ldexpf(vs_, -e) : 1.0f, inv = ldexpf(1.0f, -e);
+        // The page's scale of V joins the scores as its logarithm, and leaves
+        // the sum of probabilities as its inverse (blocks of zeros as a middle
+        // one; the least scales as 2^-70, and the rest as a factor).
+        const float least = 0x1p-70f;
+        const float vc = !there || vs_ == 0.0f ? 0x1p-30f : vs_ < least ? least : vs_;
+        const float lg = __builtin_amdgcn_logf(vc), inv = __builtin_amdgcn_rcpf(vc);
+        const float ms = m == -INFINITY ? 0.0f : m;
         if constexpr (I8) {
             i32x4 s[4] = {};
 #pragma unroll
@@ -541,28 +604,28 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
                     s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[t][h]), qi[h], s[t], 0, 0, 0);
-            const float ef = digit ? 0.0f : (float)e;
+            const float off = digit ? 0.0f : lg - ms;
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j] = digits_sum(fmaf((float)s[j / 4][j % 4], kq, ef));
+            for (int j = 0; j < 16; j++) p[j] = digits_sum(fmaf((float)s[j / 4][j % 4], kq, off));
         } else {
-            f32x4 s[4] = {};
+            Acc s[NT] = {};
 #pragma unroll
             for (int h = 0; h < NK; h++)
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int t = 0; t < 4; t++) {
-                        const f16x8 k = codes_f16(kr[t][h][2 * u], kr[t][h][2 * u + 1]);
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[2 * h + u], s[t], 0, 0, 0);
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[2 * h + u], s[t], 0, 0, 0);
+                    for (int t = 0; t < NT; t++) {
+                        const f16x8 c = codes_f16(kr[t][h][2 * u], kr[t][h][2 * u + 1]);
+                        s[t] = mma(c, qh[2 * h + u], s[t]);
+                        s[t] = mma(c, ql[2 * h + u], s[t]);
                     }
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j] = fmaf(s[j / 4][j % 4], kq, (float)e);
+            for (int j = 0; j < 16; j++) p[j] = fmaf(s[j / NR][j % NR], kq, lg - ms);
         }
         if (next < stop) load_k(next, pkn);
         // every column sees all of the step's tokens unless the step passes
         // the first column's position, the window's edge or an absent page
-        const bool plain = base + 63 <= q.start + row_a && base + 64 <= stop && base >= low &&
+        const bool plain = base + ST - 1 <= q.start + row_a && base + ST <= stop && base >= low &&
                            (A.window == 0 || base > high - 1 - A.window) && __all(there);
         if (!plain) {
 #pragma unroll
@@ -575,16 +638,22 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; j++) mx = fmaxf(mx, p[j]);
-        raise(rows4_max(mx));
-        const float ms = m == -INFINITY ? 0.0f : m - kRoom;
+        if (__any(mx > (m == -INFINITY ? -INFINITY : (float)kLimit))) {
+            raise(group_max(mx) + ms);
+            const float by = ms - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[j] += by;
+        }
         float sum = 0;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            const float y = __builtin_amdgcn_exp2f(p[j] - ms);
-            sum += y;
-            p[j] = p[j] == -INFINITY ? 0.0f : y * f;
+            p[j] = __builtin_amdgcn_exp2f(p[j]);
+            sum += p[j];
         }
         l = fmaf(sum, inv, l);
+        if (__any(there && vs_ < least && vs_ != 0.0f))
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[j] *= vs_ < least ? vs_ * 0x1p70f : 1.0f;
         if constexpr (I8) {
             i32x4 w;
 #pragma unroll
@@ -598,18 +667,20 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
         } else {
             f16x8 ph[2], pl[2];
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const _Float16 a = (_Float16)p[j];
-                ph[j / 8][j % 8] = a;
-                pl[j / 8][j % 8] = (_Float16)(p[j] - (float)a);
+            for (int j = 0; j < 16; j += 2) {  // hi rounded towards zero, lo holds the rest
+                const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]));
+                const f16x2 c = __builtin_bit_cast(
+                    f16x2, __builtin_amdgcn_cvt_pkrtz(p[j] - (float)a[0], p[j + 1] - (float)a[1]));
+                ph[j / 8][j % 8] = a[0], ph[j / 8][j % 8 + 1] = a[1];
+                pl[j / 8][j % 8] = c[0], pl[j / 8][j % 8 + 1] = c[1];
             }
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
                     const f16x8 v = codes_f16(vr[d][2 * u], vr[d][2 * u + 1]);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u], o[d], 0, 0, 0);
+                    o[d] = mma(v, ph[u], o[d]);
+                    o[d] = mma(v, pl[u], o[d]);
                 }
         }
         if (next < stop) {
@@ -620,38 +691,56 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
 
     // --- the block's four waves ---
     flush();
-    l = rows4_sum(l);
+    l = group_add(l);
     const bool writes = !I8 || digit == 0;
     if (G == 0 && writes) sm[wave][n] = m, sl[wave][n] = l;
     const float weight = ldexpf(1.0f, 8 * digit);
 #pragma unroll
     for (int d = 0; d < ND; d++) {
-        f32x4 x = o[d];
+        Acc z = o[d];
         if (I8)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = digits_sum(x[i] * weight);
-        if (writes) *reinterpret_cast<f32x4 *>(&so[wave][n][16 * d + 4 * G]) = x;
+            for (int i = 0; i < NR; i++) z[i] = digits_sum(z[i] * weight);
+        if (writes)
+#pragma unroll
+            for (int i = 0; i < NR; i += 4)
+                *reinterpret_cast<f32x4 *>(&so[wave][n][S * d + row_of(i)]) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
     }
     __syncthreads();
-    float *part = A.part + (size_t)pair * A.nsplit * CT * (HD + 2);
-    for (int i = threadIdx.x; i < left * HD; i += 256) {
-        const int c = i / HD, d = i % HD;
-        float mx = -INFINITY, sum = 0, acc = 0;
+    float *part = A.part + pair * A.nsplit * CT * (HD + 2);
+    if ((int)threadIdx.x < left) {  // the waves' factors, the column's sum
+        const int c = threadIdx.x;
+        float mx = -INFINITY, sum = 0;
 #pragma unroll
         for (int w = 0; w < 4; w++) mx = fmaxf(mx, sm[w][c]);
         const float ms = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const float x = __builtin_amdgcn_exp2f(sm[w][c] - ms);
-            sum = fmaf(x, sl[w][c], sum);
-            acc = fmaf(x, so[w][c][d], acc);
+            const float f = __builtin_amdgcn_exp2f(sm[w][c] - ms);
+            sum = fmaf(f, sl[w][c], sum);
+            sm[w][c] = f;
         }
         if (parts == 1) {
-            out_of(c)[d] = sum == 0.0f ? 0.0f : acc / sum;
+            sl[0][c] = sum;
         } else {
-            float *to = part + ((size_t)split * CT + c) * (HD + 2);
-            st_dev(to + d, acc);
-            if (d == 0) st_dev(to + HD, mx), st_dev(to + HD + 1, sum);
+            float *to = part + ((size_t)split * CT + c) * (HD + 2) + HD;
+            st_dev(to, mx), st_dev(to + 1, sum);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < left * (HD / 4); i += 256) {
+        const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) acc += sm[w][c] * *reinterpret_cast<const f32x4 *>(&so[w][c][d]);
+        if (parts == 1) {
+            const float sum = sl[0][c];
+            acc = sum == 0.0f ? f32x4{0, 0, 0, 0} : acc / sum;
+            *reinterpret_cast<f32x4 *>(out_of(c) + d) = acc;
+        } else {
+            float *to = part + ((size_t)split * CT + c) * (HD + 2) + d;
+#pragma unroll
+            for (int j = 0; j < 4; j++) st_dev(to + j, acc[j]);
         }
     }
     if (parts == 1) return;
@@ -670,6 +759,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_few(PagedAttnParams A) {
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = k + j < parts ? ld_dev(from + (size_t)(k + j) * CT * (HD + 2)) : 0.0f;
     };
+    float *fac = &so[0][0][0];
     float y[8];
     if ((int)threadIdx.x < left * HD) load8(y, threadIdx.x, 0);
     for (int c = wave; c < left; c += 4) {
@@ -753,6 +843,13 @@ void append_of(hipStream_t st, const PagedAppendParams &p, unsigned blocks) {
     }
 }
 
+template <int HD>
+void attn_of(hipStream_t st, const PagedAttnParams &p, AttnMode mode, unsigned blocks) {
+    if (mode == kAttnI8) hipLaunchKernelGGL((k_paged_attn<HD, kAttnI8>), dim3(blocks), dim3(256), 0, st, p);
+    else if (mode == kAttn16) hipLaunchKernelGGL((k_paged_attn<HD, kAttn16>), dim3(blocks), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_paged_attn<HD, kAttn32>), dim3(blocks), dim3(256), 0, st, p);
+}
+
 }  // namespace
 
 bool launch_paged_append(hipStream_t st, const PagedAppendParams &in) {
@@ -771,21 +868,15 @@ bool launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
     PagedAttnParams p = in;
     const int group = p.heads / p.kv.kv_heads, hd = p.kv.head_dim;
     const long long cols = (long long)p.s.max_rows * group;
-    const bool i8 = cols <= 4;
-    const int ct = i8 ? 4 : 16;
+    const AttnMode mode = cols <= 4 ? kAttnI8 : cols <= 16 ? kAttn16 : kAttn32;
+    const int ct = mode == kAttnI8 ? 4 : mode == kAttn16 ? 16 : 32;
     p.tiles = (int)((cols + ct - 1) / ct);
     const long long pairs = (long long)p.s.batch * p.kv.kv_heads * p.tiles;
     p.nsplit = attn_splits(pairs, (long long)p.s.max_pages * p.kv.page_size, (long long)ct * (hd + 2));
     const long long blocks = pairs * p.nsplit;
     if (blocks > kPagedMaxBlocks) return false;
-    const dim3 grid((unsigned)blocks), block(256);
-    if (hd == 64) {
-        if (i8) hipLaunchKernelGGL((k_paged_attn_few<64, true>), grid, block, 0, st, p);
-        else hipLaunchKernelGGL((k_paged_attn_few<64, false>), grid, block, 0, st, p);
-    } else {
-        if (i8) hipLaunchKernelGGL((k_paged_attn_few<128, true>), grid, block, 0, st, p);
-        else hipLaunchKernelGGL((k_paged_attn_few<128, false>), grid, block, 0, st, p);
-    }
+    if (hd == 64) attn_of<64>(st, p, mode, (unsigned)blocks);
+    else attn_of<128>(st, p, mode, (unsigned)blocks);
     return true;
 }
 
