@@ -388,7 +388,7 @@ typedef struct qtts_paged_kv {
     float *v_scales; /* [num_pages][kv_heads] */
     float *k_open;   /* [num_slots][kv_heads][page_size][head_dim] */
     float *v_open;   /* [num_slots][kv_heads][page_size][head_dim] */
-    int32_t num_pages;
+    int32_t num_pages; /* num_pages * kv_heads < 2^31 */
     int32_t kv_heads;
     int32_t head_dim;  /* 64 or 128 */
     int32_t page_size; /* 16, 32, 64 or 128 */

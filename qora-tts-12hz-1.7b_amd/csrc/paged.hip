@@ -4,6 +4,8 @@
 // f32 scale, K as [P][HD], V as [HD][P] (the product with the probabilities
 // contracts over tokens).  The page a sequence is filling lies in f32 in its
 // slot's open rows, so every block is rounded once, when it is full.
+#include <type_traits>
+
 #include "device_common.h"
 #include "paged_plan.h"
 #include "serve.h"
@@ -313,7 +315,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
         head = id % kvh, b = id / kvh;
     }
     const size_t pair = ((size_t)b * kvh + head) * A.tiles + tile;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane % S, G = lane / S;
+    const int lane = threadIdx.x & 63, r = lane % S, G = lane / S;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // the token (of a step's) in row r of K's tile 0: see above
     const int krow = S == 16 ? 16 * (r >> 2) + (r & 3) : 16 * (r >> 2 & 1) + 8 * (r >> 4) + 4 * (r >> 3 & 1) + (r & 3);
     auto group_max = [&](float v) { return NG == 4 ? rows4_max(v) : halves_max(v); };
@@ -362,15 +365,19 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
     const int stop = min(min(c0 + chunk, full), high);
     int base = c0 + ST * wave;
     u32x4 kr[NT][NK], vr[ND];
-    float ks_ = 0, vs_ = 0;
-    bool there = false;
-    auto page_at = [&](int token) {  // an absent page reads as the pool's first, and is masked
-        return token < stop ? q.pages[token >> sh] : -1;
+    // Loads come back in the order they are issued, so each is issued behind
+    // what is needed before it, and none hangs on a branch (which would make a
+    // wait for any of them a wait for all): past the last token, and for an
+    // absent page, they read the pool's first page, whose tokens are masked.
+    auto page_at = [&](int token) {
+        const int pg = q.pages[min(token, stop - 1) >> sh];
+        return token < stop && pg >= 0 && pg < A.kv.num_pages ? pg : -1;
     };
-    auto valid = [&](int pg) { return pg >= 0 && pg < A.kv.num_pages; };
+    auto block_of = [&](int pg) { return (unsigned)(max(pg, 0) * kvh + head); };
+    constexpr int kHdShift = HD == 64 ? 6 : 7;
     auto load_k = [&](int at, int pg) {
-        const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
-        const int8_t *p = A.kv.k_codes + (block * P + ((at + krow) & (P - 1))) * HD + 16 * G;
+        const int8_t *p = A.kv.k_codes + ((size_t)block_of(pg) << (sh + kHdShift)) +
+                          (((at + krow) & (P - 1)) << kHdShift) + 16 * G;
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -378,19 +385,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
                 kr[t][h] = *glb(reinterpret_cast<const u32x4 *>(p + 4 * t * HD + ST * h));
     };
     auto load_v = [&](int at, int pg) {
-        const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
-        const int8_t *p = A.kv.v_codes + (block * HD + r) * P + ((at + 16 * G) & (P - 1));
+        const int8_t *p = A.kv.v_codes + ((size_t)block_of(pg) << (sh + kHdShift)) + (r << sh) + ((at + 16 * G) & (P - 1));
 #pragma unroll
-        for (int d = 0; d < ND; d++) vr[d] = *glb(reinterpret_cast<const u32x4 *>(p + S * d * P));
+        for (int d = 0; d < ND; d++) vr[d] = *glb(reinterpret_cast<const u32x4 *>(p + ((S * d) << sh)));
     };
-    auto load_scales = [&](int pg) {
-        const size_t block = (size_t)(valid(pg) ? pg : 0) * kvh + head;
-        ks_ = A.kv.k_scales[block], vs_ = A.kv.v_scales[block];
-        there = valid(pg);
-    };
-    // In this order, as loads come back in it: the pages' ids, the queries (made
-    // into operands meanwhile), the pages.
-    const int pk = page_at(base + krow), pv = page_at(base + 16 * G);
+    const bool any = base < stop;
+    int pk = -1, pv = -1, pkn = -1, pvn = -1;  // this step's pages and the next one's
+    float ks_ = 0, vs_ = 0, ksn, vsn;
+    if (any) {
+        pk = page_at(base + krow), pv = page_at(base + 16 * G);
+        pkn = page_at(base + RT + krow), pvn = page_at(base + RT + 16 * G);
+    }
     float x[NK][16];
 #pragma unroll
     for (int h = 0; h < NK; h++)
@@ -400,10 +405,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
             x[h][j] = a.x, x[h][j + 1] = a.y, x[h][j + 2] = a.z, x[h][j + 3] = a.w;
         }
     auto load_first = [&]() {
-        if (base < stop) {
+        if (any) {
             load_k(base, pk);
+            ks_ = A.kv.k_scales[block_of(pv)], vs_ = A.kv.v_scales[block_of(pv)];
             load_v(base, pv);
-            load_scales(pv);
         }
     };
     if (S == 16) load_first();
@@ -585,18 +590,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
 
     // --- full pages ---
     if (S == 32) load_first();  // no registers to spare for them before
-    for (; base < stop; base += RT) {
+    auto step = [&](auto more) {  // more: another one follows, whose pages are asked for
         const int next = base + RT;
-        const int pkn = page_at(next + krow), pvn = page_at(next + 16 * G);
         float p[16];
-        const float kq = qscale * ks_;
-        // The page's scale of V joins the scores as its logarithm, and leaves
-        // the sum of probabilities as its inverse (blocks of zeros as a middle
-        // one; the least scales as 2^-70, and the rest as a factor).
-        const float least = 0x1p-70f;
-        const float vc = !there || vs_ == 0.0f ? 0x1p-30f : vs_ < least ? least : vs_;
-        const float lg = __builtin_amdgcn_logf(vc), inv = __builtin_amdgcn_rcpf(vc);
-        const float ms = m == -INFINITY ? 0.0f : m;
+        const bool there = pv >= 0;
         if constexpr (I8) {
             i32x4 s[4] = {};
 #pragma unroll
@@ -604,9 +601,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
                     s[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[t][h]), qi[h], s[t], 0, 0, 0);
-            const float off = digit ? 0.0f : lg - ms;
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j] = digits_sum(fmaf((float)s[j / 4][j % 4], kq, off));
+            for (int j = 0; j < 16; j++) p[j] = (float)s[j / 4][j % 4];
         } else {
             Acc s[NT] = {};
 #pragma unroll
@@ -620,9 +616,28 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
                         s[t] = mma(c, ql[2 * h + u], s[t]);
                     }
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j] = fmaf(s[j / NR][j % NR], kq, lg - ms);
+            for (int j = 0; j < 16; j++) p[j] = s[j / NR][j % NR];
         }
-        if (next < stop) load_k(next, pkn);
+        int pk2 = -1, pv2 = -1;
+        if constexpr (more) {
+            pk2 = page_at(next + RT + krow), pv2 = page_at(next + RT + 16 * G);
+            load_k(next, pkn);
+            ksn = A.kv.k_scales[block_of(pvn)], vsn = A.kv.v_scales[block_of(pvn)];
+        }
+        const float kq = qscale * ks_;
+        // The page's scale of V joins the scores as its logarithm, and leaves
+        // the sum of probabilities as its inverse (blocks of zeros as a middle
+        // one; the least scales as 2^-70, and the rest as a factor).
+        const float least = 0x1p-70f;
+        const float vc = !there || vs_ == 0.0f ? 0x1p-30f : vs_ < least ? least : vs_;
+        const float lg = __builtin_amdgcn_logf(vc), inv = __builtin_amdgcn_rcpf(vc);
+        const float ms = m == -INFINITY ? 0.0f : m;
+        const float off = digit ? 0.0f : lg - ms;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            p[j] = fmaf(p[j], kq, off);
+            if (I8) p[j] = digits_sum(p[j]);
+        }
         // every column sees all of the step's tokens unless the step passes
         // the first column's position, the window's edge or an absent page
         const bool plain = base + ST - 1 <= q.start + row_a && base + ST <= stop && base >= low &&
@@ -683,10 +698,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
                     o[d] = mma(v, pl[u], o[d]);
                 }
         }
-        if (next < stop) {
+        if constexpr (more) {
             load_v(next, pvn);
-            load_scales(pvn);
+            pv = pvn, pkn = pk2, pvn = pv2;
+            ks_ = ksn, vs_ = vsn;
         }
+    };
+    if (any) {
+        for (; base + RT < stop; base += RT) step(std::true_type{});
+        step(std::false_type{});
     }
 
     // --- the block's four waves ---

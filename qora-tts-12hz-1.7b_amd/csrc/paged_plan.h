@@ -36,6 +36,8 @@ inline Refusal check_paged(const qtts_paged_kv &kv, const qtts_paged_seqs &s) {
         return {QTTS_ESHAPE, "paged cache: page_size must be 16, 32, 64 or 128"};
     if (kv.num_pages < 1 || kv.kv_heads < 1 || kv.kv_heads > 1024 || kv.num_slots < 1)
         return {QTTS_ESHAPE, "paged cache: num_pages, kv_heads (to 1024) and num_slots must be positive"};
+    if ((long long)kv.num_pages * kv.kv_heads > kPagedMaxBlocks)
+        return {QTTS_ERANGE, "paged cache: more than 2^31 - 1 blocks (pages times kv heads)"};
     if (!kv.k_codes || !kv.v_codes || !kv.k_scales || !kv.v_scales || !kv.k_open || !kv.v_open)
         return {QTTS_EINVAL, "paged cache: null buffer"};
     if (!aligned_to(kv.k_codes, 16) || !aligned_to(kv.v_codes, 16) || !aligned_to(kv.k_open, 16) ||

@@ -91,6 +91,8 @@ CACHE_AND_SEQS = [
     (dict(page_size=48), dict(), ESHAPE),
     (dict(page_size=256), dict(), ESHAPE),
     (dict(num_pages=0), dict(), ESHAPE),
+    (dict(num_pages=1 << 30), dict(), ERANGE),
+    (dict(num_pages=(1 << 30) - 1), dict(), OK),
     (dict(num_pages=-1), dict(), ESHAPE),
     (dict(kv_heads=0), dict(), ESHAPE),
     (dict(num_slots=0), dict(), ESHAPE),
