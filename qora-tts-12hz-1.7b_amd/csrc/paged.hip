@@ -298,23 +298,26 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
     __shared__ float sm[4][CT], sl[4][CT];
     __shared__ unsigned sarrived;
     static_assert(4 * (HD + 4) >= kPagedMaxSplits, "the parts' factors take so's place");
+    static_assert(kPagedPartFloats >= 3LL * kPagedRound / 2 * CT * (HD + 2), "the parts fit");
     const int P = A.kv.page_size, sh = __builtin_ctz(P), kvh = A.kv.kv_heads, group = A.heads / kvh;
     // Consecutive blocks lie on different XCDs.  Tiles of 32 share their pages:
     // with kv heads innermost one head's are read through few caches, and the
     // last rows, which see the most, go first.  Few columns read every page
     // once, and faster with a pair's chunks spread (4 sequences of 32760: 48 us,
     // 54 with heads innermost).
-    int id = blockIdx.x, head, b, split, tile;
+    // Pairs past the plan's whole ones are divided over nsplit blocks.
+    int id = blockIdx.x, head, b, split = 0, tile, shared = 0, nsplit = 1;
+    if (id >= A.whole) {
+        shared = (id - A.whole) / A.nsplit, split = (id - A.whole) % A.nsplit;
+        id = A.whole + shared, nsplit = A.nsplit;
+    }
     if (S == 32) {
         head = id % kvh, id /= kvh;
-        b = id % A.s.batch, id /= A.s.batch;
-        split = id % A.nsplit, tile = A.tiles - 1 - id / A.nsplit;
+        b = id % A.s.batch, tile = A.tiles - 1 - id / A.s.batch;
     } else {
-        split = id % A.nsplit, id /= A.nsplit;
         tile = id % A.tiles, id /= A.tiles;
         head = id % kvh, b = id / kvh;
     }
-    const size_t pair = ((size_t)b * kvh + head) * A.tiles + tile;
     const int lane = threadIdx.x & 63, r = lane % S, G = lane / S;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // the token (of a step's) in row r of K's tile 0: see above
@@ -348,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
     const int row_a = tile * CT / group, row_b = (tile * CT + left - 1) / group;
     const int high = q.start + row_b + 1;
     const int low = A.window > 0 ? max(0, q.start + row_a - A.window + 1) : 0;
-    const int from = low & ~63, chunk = chunk_of(high - from, A.nsplit);
+    const int from = low & ~63, chunk = chunk_of(high - from, nsplit, attn_least(CT));
     const int parts = (high - from + chunk - 1) / chunk;
     if (split >= parts) return;
     const int c0 = from + split * chunk;
@@ -488,94 +491,136 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
         }
     };
 
-    // --- the open page's rows, in f32 products, S tokens a step (while the
-    // first step's pages are on their way) ---
-    const int open_hi = min(min(end, c0 + chunk), high);
-    for (int t0 = full + S * wave; t0 < open_hi; t0 += 4 * S) {
-        if (t0 + S <= max(low, c0)) continue;
-        const int open_lo = max(low, c0);
-        const size_t row = ((size_t)q.slot * kvh + head) * P;
-        const int kt = t0 + r;  // K: row r of the tile
-        const bool kin = kt < open_hi && kt >= open_lo;
-        const float *kp = A.kv.k_open + (row + (kin ? (kt & (P - 1)) : 0)) * HD + 4 * G;
-        // V: dimension S d + r of the token of register i, BT registers at a
-        // time: all of them with tiles of 16, kept for the products; with tiles
-        // of 32 a half, read again for the products.
-        constexpr int BT = S == 16 ? NR : 8;
-        float v[BT][ND];
-        auto load_open = [&](int i0) {
+    // --- the open page's rows, in f32 products, S tokens a step and a wave ---
+    // Tiles of 16 read them to registers (while the first step's pages are on
+    // their way); with tiles of 32, which have none to spare, the block brings
+    // K's and then V's to LDS, in the place of its result.
+    const int open_lo = max(max(full, low), c0), open_hi = min(min(end, c0 + chunk), high);
+    const float *k_open = A.kv.k_open + ((size_t)q.slot * kvh + head) * P * HD;
+    const float *v_open = A.kv.v_open + ((size_t)q.slot * kvh + head) * P * HD;
+    float(*rows)[HD + 4] = so[0];  // S == 32: row t - open_lo of the open page, 128 at most
+    auto stage = [&](const float *from) {
+        const int count = (open_hi - open_lo) * (HD / 4);
+        for (int i0 = threadIdx.x; i0 < count; i0 += 1024) {  // four loads in flight
+            f32x4 y[4];
 #pragma unroll
-            for (int i = 0; i < BT; i++) {
-                const int token = t0 + row_of(i0 + i);
-                const bool in = token < open_hi && token >= open_lo;
-                const float *vp = A.kv.v_open + (row + (in ? (token & (P - 1)) : 0)) * HD + r;
-#pragma unroll
-                for (int d = 0; d < ND; d++) v[i][d] = vp[S * d];
-#pragma unroll
-                for (int d = 0; d < ND; d++) v[i][d] = in ? v[i][d] : 0.0f;
+            for (int j = 0; j < 4; j++) {
+                const int i = min(i0 + 256 * j, count - 1), t = open_lo + i / (HD / 4);
+                y[j] = *glb(reinterpret_cast<const f32x4 *>(from + (t & (P - 1)) * HD + 4 * (i % (HD / 4))));
             }
-        };
-        if (S == 16) load_open(0);
-        Acc s = {}, s1 = {};
 #pragma unroll
-        for (int c = 0; c < HD / (4 * NG); c++) {
-            const float4 y = *reinterpret_cast<const float4 *>(kp + 4 * NG * c);
-            float4 z = *reinterpret_cast<const float4 *>(qr + 4 * NG * c + 4 * G);
-            if (!real || digit) z = make_float4(0, 0, 0, 0);
-            s = mma1(y.x, z.x, s);
-            (S == 16 ? s1 : s) = mma1(y.y, z.y, S == 16 ? s1 : s);
-            s = mma1(y.z, z.z, s);
-            (S == 16 ? s1 : s) = mma1(y.w, z.w, S == 16 ? s1 : s);
+            for (int j = 0; j < 4; j++) {
+                const int i = min(i0 + 256 * j, count - 1);
+                *reinterpret_cast<f32x4 *>(&rows[i / (HD / 4)][4 * (i % (HD / 4))]) = y[j];
+            }
         }
-        if (S == 16) s += s1;
+    };
+    auto open_tile = [&](int t0) {
+        const bool mine = t0 < open_hi;  // S == 32: others only take part in the staging
+        Acc s = {}, s1 = {};
+        float v[S == 16 ? NR : 1][ND];
+        if (S == 16) {
+            const int kt = t0 + r;  // K: row r of the tile
+            const float *kp = k_open + ((kt < open_hi ? kt : open_lo) & (P - 1)) * HD + 4 * G;
+            // V: dimension S d + r of the token of register i
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const int token = t0 + row_of(i);
+                const bool in = token < open_hi;
+                const float *vp = v_open + ((in ? token : open_lo) & (P - 1)) * HD + r;
+#pragma unroll
+                for (int d = 0; d < ND; d++) v[S == 16 ? i : 0][d] = vp[S * d];
+#pragma unroll
+                for (int d = 0; d < ND; d++) v[S == 16 ? i : 0][d] = in ? v[S == 16 ? i : 0][d] : 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < HD / (4 * NG); c++) {
+                const float4 y = *reinterpret_cast<const float4 *>(kp + 4 * NG * c);
+                float4 z = *reinterpret_cast<const float4 *>(qr + 4 * NG * c + 4 * G);
+                if (!real || digit) z = make_float4(0, 0, 0, 0);
+                s = mma1(y.x, z.x, s);
+                s1 = mma1(y.y, z.y, s1);
+                s = mma1(y.z, z.z, s);
+                s1 = mma1(y.w, z.w, s1);
+            }
+            s += s1;
+        } else {
+            stage(k_open);
+            __syncthreads();
+            if (mine) {
+                const float *kp = rows[min(t0 + r, open_hi - 1) - open_lo] + 16 * G;
+#pragma unroll
+                for (int h = 0; h < NK; h++)
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const f32x4 y = *reinterpret_cast<const f32x4 *>(kp + ST * h + j);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int at = 2 * h + (j + i) / 8;
+                            s = mma1(y[i], (float)qh[at][(j + i) % 8] + (float)ql[at][(j + i) % 8], s);
+                        }
+                    }
+            }
+            __syncthreads();
+            stage(v_open);
+            __syncthreads();
+        }
+        auto value = [&](int i, int d) {  // of V, 0 past the last token
+            if (S == 16) return v[S == 16 ? i : 0][d];
+            const int t = t0 + row_of(i);
+            const float y = rows[min(t, open_hi - 1) - open_lo][S * d + r];
+            return t < open_hi ? y : 0.0f;
+        };
         // What is not finite is left out of V's products (0 * Inf would reach
         // rows that do not see it) and added by itself below.
-        float p[NR], inv[NR], mx = -INFINITY;
+        float p[NR];
         bool odd = false;
+        if (mine) {
+            float mx = -INFINITY;
+            const float by = S == 16 ? A.scale * kLog2e : qscale;
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const int token = t0 + row_of(i);
-            if (S == 32 && i % BT == 0) load_open(i);
-            float top = 0;
+            for (int i = 0; i < NR; i++) {
+                const int token = t0 + row_of(i);
+                float top = 0;
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
-                if (!(fabsf(v[i % BT][d]) < INFINITY)) odd = true, v[i % BT][d] = 0.0f;
-                top = fmaxf(top, fabsf(v[i % BT][d]));
+                for (int d = 0; d < ND; d++) {
+                    const float y = fabsf(value(i, d));
+                    odd |= !(y < INFINITY);
+                    top = fmaxf(top, y < INFINITY ? y : 0.0f);
+                }
+                top = row16_max(top);
+                if (S == 32) top = fmaxf(top, dpp_row_pair(top));
+                const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
+                p[i] = seen ? (I8 ? digits_sum(s[i]) : s[i]) * by : -INFINITY;
+                mx = fmaxf(mx, p[i] + (float)fold_exponent(top * (1.0f / 128.0f)));
             }
-            top = row16_max(top);
-            if (S == 32) top = fmaxf(top, dpp_row_pair(top));
-            const int e = fold_exponent(top * (1.0f / 128.0f));
-            inv[i] = ldexpf(1.0f, -e);
-            const bool seen = token <= pos && token < open_hi && token >= open_lo &&
-                              (A.window == 0 || token > pos - A.window);
-            const float z = fmaf(I8 ? digits_sum(s[i]) : s[i], A.scale * kLog2e, (float)e);
-            p[i] = seen ? z : -INFINITY;
-            mx = fmaxf(mx, p[i]);
+            raise(group_max(mx));
+            const float ms = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const float y = __builtin_amdgcn_exp2f(p[i] - ms);
+                l += y;
+                p[i] = digit ? 0.0f : y;
+            }
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const float y = value(i, d);
+                    o[d] = mma1(fabsf(y) < INFINITY ? y : 0.0f, p[i], o[d]);
+                }
         }
-        raise(group_max(mx));
-        const float ms = m == -INFINITY ? 0.0f : m;
+        // (with tiles of 32 the block decides, as V's rows give way to the weights)
+        if (S == 32 ? __syncthreads_or(odd) : __any(odd)) {
+            if (mine) {
+                float *weight = &so[wave][0][0];  // [S tokens][S columns]
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const float y = p[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms) * inv[i];
-            l += y;
-            p[i] = digit ? 0.0f : y;
-        }
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            if (S == 32 && i % BT == 0) load_open(i);
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-                o[d] = mma1(S == 32 && !(fabsf(v[i % BT][d]) < INFINITY) ? 0.0f : v[i % BT][d], p[i], o[d]);
-        }
-        if (__any(odd)) {
-            for (int g = 0; g < NG; g++) {
-#pragma unroll
-                for (int t = 0; t < NR; t++) {
-                    const int token = t0 + row_of(t) + 4 * (g - G);  // of group g's register t
-                    const float w = __shfl(p[t], r + S * g, 64);
-                    if (token >= open_hi || token < open_lo) continue;
+                for (int i = 0; i < NR; i++) weight[row_of(i) * S + r] = p[i];
+#pragma unroll 1
+                for (int token = t0; token < min(t0 + S, open_hi); token++) {
+                    const float w = weight[(token - t0) * S + r];
                     const bool seen = token <= pos && (A.window == 0 || token > pos - A.window) && !digit;
-                    const float *vp = A.kv.v_open + (row + (token & (P - 1))) * HD;
+                    const float *vp = v_open + (token & (P - 1)) * HD;
 #pragma unroll
                     for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -586,6 +631,12 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
                 }
             }
         }
+        if (S == 32) __syncthreads();
+    };
+    if (S == 16) {
+        for (int t0 = open_lo + S * wave; t0 < open_hi; t0 += 4 * S) open_tile(t0);
+    } else if (open_lo < open_hi) {
+        open_tile(open_lo + S * wave);
     }
 
     // --- full pages ---
@@ -727,7 +778,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
                 *reinterpret_cast<f32x4 *>(&so[wave][n][S * d + row_of(i)]) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
     }
     __syncthreads();
-    float *part = A.part + pair * A.nsplit * CT * (HD + 2);
+    float *part = A.part + (size_t)shared * nsplit * CT * (HD + 2);
     if ((int)threadIdx.x < left) {  // the waves' factors, the column's sum
         const int c = threadIdx.x;
         float mx = -INFINITY, sum = 0;
@@ -760,37 +811,46 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
         } else {
             float *to = part + ((size_t)split * CT + c) * (HD + 2) + d;
 #pragma unroll
-            for (int j = 0; j < 4; j++) st_dev(to + j, acc[j]);
+            for (int j = 0; j < 4; j += 2)
+                st_dev_u64(reinterpret_cast<uint64_t *>(to + j),
+                           __float_as_uint(acc[j]) | (uint64_t)__float_as_uint(acc[j + 1]) << 32);
         }
     }
     if (parts == 1) return;
     wait_stores();
     __syncthreads();
     if (threadIdx.x == 0) {
-        sarrived = arrive_dev(A.counters + pair);
-        if (sarrived == (unsigned)parts - 1) reset_dev(A.counters + pair);
+        sarrived = arrive_dev(A.counters + shared);
+        if (sarrived == (unsigned)parts - 1) reset_dev(A.counters + shared);
     }
     __syncthreads();
     if (sarrived != (unsigned)parts - 1) return;
-    // The parts' rows, eight loads in flight; the first eight of a thread's
-    // first value while the maxima and sums become every part's factor.
-    auto load8 = [&](float *x, int i, int k) {
-        const float *from = part + (size_t)(i / HD) * (HD + 2) + i % HD;
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = k + j < parts ? ld_dev(from + (size_t)(k + j) * CT * (HD + 2)) : 0.0f;
-    };
+    // The parts' rows, two values a load and 16 loads in flight; the first ones
+    // while the maxima and sums become every part's factor.
+    constexpr int MI = CT * HD > 1024 ? CT * HD / 512 : 1, U = MI > 8 ? 1 : 16 / MI;
     float *fac = &so[0][0][0];
-    float y[8];
-    if ((int)threadIdx.x < left * HD) load8(y, threadIdx.x, 0);
+    uint64_t y[U][MI];
+    const int pairs = left * (HD / 2);  // of values
+    auto load_parts = [&](int k0) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                const int at = min((int)threadIdx.x + 256 * i, pairs - 1), k = min(k0 + u, parts - 1);
+                const float *from = part + ((size_t)k * CT + at / (HD / 2)) * (HD + 2) + 2 * (at % (HD / 2));
+                y[u][i] = ld_dev_u64(reinterpret_cast<const uint64_t *>(from));
+            }
+    };
+    load_parts(0);
     for (int c = wave; c < left; c += 4) {
         constexpr int N = kPagedMaxSplits / 64;
         float pm[N], ps[N], mx = -INFINITY, sum = 0;
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int k = lane + 64 * j;
-            const float *from = part + ((size_t)k * CT + c) * (HD + 2) + HD;
-            pm[j] = k < parts ? ld_dev(from) : -INFINITY;
-            ps[j] = k < parts ? ld_dev(from + 1) : 0.0f;
+            const float *from = part + ((size_t)min(lane + 64 * j, parts - 1) * CT + c) * (HD + 2) + HD;
+            const uint64_t z = ld_dev_u64(reinterpret_cast<const uint64_t *>(from));
+            pm[j] = lane + 64 * j < parts ? __uint_as_float((unsigned)z) : -INFINITY;
+            ps[j] = lane + 64 * j < parts ? __uint_as_float((unsigned)(z >> 32)) : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < N; j++) mx = fmaxf(mx, pm[j]);
@@ -806,18 +866,27 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
         if (lane == 0) sl[0][c] = sum;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < left * HD; i += 256) {
-        const float *fc = fac + i / HD * parts;
-        float acc = 0;
-        if (i != (int)threadIdx.x) load8(y, i, 0);
-        for (int k = 0; k < parts; k += 8) {
-            if (k) load8(y, i, k);
+    float acc[MI][2] = {};
+    for (int k0 = 0; k0 < parts; k0 += U) {
+        if (k0) load_parts(k0);
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (k + j < parts) acc = fmaf(fc[k + j], y[j], acc);
+        for (int i = 0; i < MI; i++) {
+            const int c = min((int)threadIdx.x + 256 * i, pairs - 1) / (HD / 2);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float f = k0 + u < parts ? fac[c * parts + k0 + u] : 0.0f;
+                acc[i][0] = fmaf(f, __uint_as_float((unsigned)y[u][i]), acc[i][0]);
+                acc[i][1] = fmaf(f, __uint_as_float((unsigned)(y[u][i] >> 32)), acc[i][1]);
+            }
         }
-        const float sum = sl[0][i / HD];
-        out_of(i / HD)[i % HD] = sum == 0.0f ? 0.0f : acc / sum;
+    }
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
+        const int at = threadIdx.x + 256 * i, c = at / (HD / 2);
+        if (at >= pairs) break;
+        const float sum = sl[0][c];
+        *reinterpret_cast<float2 *>(out_of(c) + 2 * (at % (HD / 2))) =
+            sum == 0.0f ? make_float2(0, 0) : make_float2(acc[i][0] / sum, acc[i][1] / sum);
     }
 }
 
@@ -892,8 +961,11 @@ bool launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
     const int ct = mode == kAttnI8 ? 4 : mode == kAttn16 ? 16 : 32;
     p.tiles = (int)((cols + ct - 1) / ct);
     const long long pairs = (long long)p.s.batch * p.kv.kv_heads * p.tiles;
-    p.nsplit = attn_splits(pairs, (long long)p.s.max_pages * p.kv.page_size, (long long)ct * (hd + 2));
-    const long long blocks = pairs * p.nsplit;
+    if (pairs > kPagedMaxBlocks) return false;
+    const AttnPlan plan = attn_plan(pairs, (long long)p.s.max_pages * p.kv.page_size, ct);
+    p.whole = plan.whole;
+    p.nsplit = plan.nsplit;
+    const long long blocks = plan.whole + (pairs - plan.whole) * plan.nsplit;
     if (blocks > kPagedMaxBlocks) return false;
     if (hd == 64) attn_of<64>(st, p, mode, (unsigned)blocks);
     else attn_of<128>(st, p, mode, (unsigned)blocks);

@@ -144,35 +144,42 @@ inline Refusal check_sample_rows(const float *logits, int64_t ld, int32_t rows, 
     return kAccepted;
 }
 
-// How attention divides a sequence's tokens over blocks.  Results of several are
-// joined through scratch of kPagedPartFloats, `floats` for each block, and a
-// counter for each pair (sequence and kv head, and column tile).
-constexpr long long kPagedPartFloats = 4LL << 20;
-constexpr long long kPagedCounters = 1 << 14;
+// How attention divides its pairs (a sequence and kv head, and column tile) over
+// blocks.  Two blocks a compute unit are one round of them.  A pair takes one
+// block in full rounds; the pairs of the last, incomplete round share it by
+// dividing their tokens, joined through scratch of kPagedPartFloats and a counter
+// each.  Smaller chunks everywhere cost more than they even out: 64 ragged
+// sequences of up to 8000 tokens (512 pairs) took 160 us with one block a pair,
+// 180 us with four and 204 us with eight; 4 of 32760 (32 pairs) 49 us with 16
+// blocks a pair, 57 us with 32.
+constexpr int kPagedRound = 512;
 constexpr int kPagedMaxSplits = 256;
-// Two blocks a compute unit are one round of them.  Blocks of a second round
-// and smaller chunks cost more than they even out: 64 ragged sequences of up to
-// 8000 tokens (512 pairs) took 160 us with one block a pair, 180 us with four
-// and 204 us with eight; 4 of 32760 (32 pairs) 49 us with 16, 57 us with 32.
-constexpr long long kPagedBlocks = 512;
+constexpr long long kPagedCounters = kPagedRound;
+constexpr long long kPagedPartFloats = 4LL << 20;  // 3/2 of a round's blocks of 32 columns, at least
 
-// Blocks over one pair: the nearest to one round, at least 256 tokens each where
-// the page table row (`cap` tokens) is full.
-inline int attn_splits(long long pairs, long long cap, long long floats) {
-    const long long steps = (cap + 255) / 256;
-    const long long fits = pairs > kPagedCounters ? 1 : kPagedPartFloats / (pairs * floats);
-    long long n = (kPagedBlocks + pairs / 2) / pairs;
+struct AttnPlan {
+    int whole;   // pairs of one block
+    int nsplit;  // blocks of each of the others
+};
+
+// Tokens that a block takes at least where it shares a pair: one step of its
+// waves, and with 32 columns four, as their joining costs more.
+QTTS_HD constexpr int attn_least(int columns) { return columns == 32 ? 512 : 256; }
+
+inline AttnPlan attn_plan(long long pairs, long long cap, int columns) {
+    const int least = attn_least(columns);
+    const long long steps = (cap + least - 1) / least, rest = pairs % kPagedRound;
+    long long n = rest ? (kPagedRound + rest / 2) / rest : 1;
     n = n > steps ? steps : n;
-    n = n > fits ? fits : n;
     n = n > kPagedMaxSplits ? kPagedMaxSplits : n;
-    return (int)(n < 1 ? 1 : n);
+    if (n <= 1) return {(int)pairs, 1};
+    return {(int)(pairs - rest), (int)n};
 }
 
-// Tokens of one block where `nsplit` share `span` tokens: whole rounds of the
-// block's four waves, 64 tokens each.
-QTTS_HD int chunk_of(int span, int nsplit) {
+// Tokens of one block where `nsplit` share `span` tokens.
+QTTS_HD int chunk_of(int span, int nsplit, int least) {
     const int each = span / nsplit + (span % nsplit != 0);
-    return (each + 255) / 256 * 256;
+    return (each + least - 1) / least * least;
 }
 
 // One sequence of a call as the kernels see it: whatever the device arrays

@@ -29,7 +29,7 @@ struct PagedAttnParams {
     int window;
     // the launch's own
     int tiles;           // column tiles of one sequence and kv head
-    int nsplit;          // blocks that share one tile's tokens
+    int whole, nsplit;   // AttnPlan
     float *part;         // kPagedPartFloats: chunks' results
     unsigned *counters;  // kPagedCounters, zero between launches
 };

@@ -33,6 +33,11 @@ extern "C" int sample(const float *l, int64_t ld, int rows, int vocab, const qtt
                       const int32_t *t, const float *pr) {
     return told(check_sample_rows(l, ld, rows, vocab, *p, u, t, pr));
 }
+extern "C" void plan(long long pairs, long long cap, int columns, long long *o) {
+    const AttnPlan p = attn_plan(pairs, cap, columns);
+    o[0] = p.whole; o[1] = p.nsplit; o[2] = kPagedMaxSplits; o[3] = kPagedPartFloats; o[4] = kPagedCounters;
+}
+extern "C" int chunk(int span, int nsplit, int round) { return chunk_of(span, nsplit, round); }
 extern "C" void seq(const qtts_paged_seqs *s, int b, int slots, long long cap, int *o) {
     const PagedSeq q = load_seq(*s, b, slots, cap);
     o[0] = q.start; o[1] = q.rows; o[2] = q.row0; o[3] = q.slot; o[4] = q.ok;
@@ -204,3 +209,25 @@ def test_any_device_arrays_stay_inside(lib):
                 assert 0 <= start and start + n <= cap and 0 <= slot < num_slots
                 served += n > 0
     assert served > 100
+
+
+def test_attention_plans(lib):
+    """Every pair gets its blocks, a round's scratch and counters hold the
+    shared ones, and the chunks of any span cover it."""
+    out = (C.c_longlong * 5)()
+    for pairs in list(range(1, 1600)) + [4096, 5000, 65536 * 3 + 7]:
+        for cap, columns in ((16, 4), (256, 32), (257, 4), (2048, 32), (32768, 16), (1 << 30, 32)):
+            lib.plan(C.c_longlong(pairs), C.c_longlong(cap), columns, out)
+            whole, nsplit, most, part, counters = list(out)
+            assert 0 <= whole <= pairs and nsplit >= 1
+            shared = pairs - whole
+            if shared == 0:
+                continue
+            assert nsplit > 1 and shared <= counters and nsplit <= most and nsplit <= -(-cap // 256)
+            assert shared * nsplit * 32 * 130 <= part
+            assert shared * nsplit <= 3 * 512 // 2 and whole % 512 == 0
+    for span in list(range(1, 700)) + [32761, 100000]:
+        for nsplit in (1, 2, 3, 16, 256):
+            for step in (256, 512):
+                chunk = lib.chunk(span, nsplit, step)
+                assert chunk % step == 0 and chunk * nsplit >= span and chunk < span / nsplit + step + 1
