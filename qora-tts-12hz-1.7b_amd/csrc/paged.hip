@@ -4,6 +4,7 @@
 // f32 scale, K as [P][HD], V as [HD][P] (the product with the probabilities
 // contracts over tokens).  The page a sequence is filling lies in f32 in its
 // slot's open rows, so every block is rounded once, when it is full.
+#include <algorithm>
 #include <type_traits>
 
 #include "device_common.h"
@@ -14,6 +15,7 @@ namespace qtts {
 
 namespace {
 
+// Sum over groups of `width` lanes.
 __device__ __forceinline__ double group_sum(double v, int width) {
     for (int off = width / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, width);
     return v;
@@ -21,107 +23,156 @@ __device__ __forceinline__ double group_sum(double v, int width) {
 
 // One head's vector spread over HD / 8 lanes: lane g of them holds elements
 // 4g..4g+3 of both halves, the pairs that the rotation mixes.
-template <int HD>
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4 load4(const float *p) { return *glb(reinterpret_cast<const f32x4 *>(p)); }
+__device__ __forceinline__ void store4(float *p, f32x4 v) { *glb(reinterpret_cast<f32x4 *>(p)) = v; }
+
 struct Pairs {
-    float lo[4], hi[4];
-    __device__ __forceinline__ void load(const float *p, int g) {
-        const float4 a = *reinterpret_cast<const float4 *>(p + 4 * g);
-        const float4 b = *reinterpret_cast<const float4 *>(p + HD / 2 + 4 * g);
-        lo[0] = a.x, lo[1] = a.y, lo[2] = a.z, lo[3] = a.w;
-        hi[0] = b.x, hi[1] = b.y, hi[2] = b.z, hi[3] = b.w;
+    f32x4 lo, hi;
+    __device__ __forceinline__ void load(const float *p, int g, int half) {
+        lo = load4(p + 4 * g);
+        hi = load4(p + half + 4 * g);
     }
-    __device__ __forceinline__ void store(float *p, int g) const {
-        *reinterpret_cast<float4 *>(p + 4 * g) = make_float4(lo[0], lo[1], lo[2], lo[3]);
-        *reinterpret_cast<float4 *>(p + HD / 2 + 4 * g) = make_float4(hi[0], hi[1], hi[2], hi[3]);
-    }
-    __device__ __forceinline__ void zero() {
-        for (int i = 0; i < 4; i++) lo[i] = hi[i] = 0.0f;
-    }
-    // Norm and rotation in 64 bits, rounded to f32 once: codes at the border
-    // between two steps then agree with the definition's.  The vector units
-    // run 64-bit products at the f32 rate, and the kernel waits for memory.
-    __device__ __forceinline__ void norm_rotate(const qtts_paged_rows &r, const uint16_t *norm, int pos, int g) {
-        double a[4], b[4];
-        for (int i = 0; i < 4; i++) a[i] = lo[i], b[i] = hi[i];
-        if (norm) {
-            double ss = 0;
-            for (int i = 0; i < 4; i++) ss += a[i] * a[i] + b[i] * b[i];
-            ss = group_sum(ss, HD / 8);
-            const double inv = 1.0 / sqrt(ss / HD + (double)r.eps);
-            for (int i = 0; i < 4; i++) {
-                a[i] *= (double)f16_to_f32(norm[4 * g + i]) * inv;
-                b[i] *= (double)f16_to_f32(norm[HD / 2 + 4 * g + i]) * inv;
-            }
-        }
-        if (r.rope_cos) {
-            const float *cs = r.rope_cos + (size_t)pos * (HD / 2) + 4 * g;
-            const float *sn = r.rope_sin + (size_t)pos * (HD / 2) + 4 * g;
-            for (int i = 0; i < 4; i++) {
-                const double c = cs[i], s = sn[i];
-                const double x = a[i] * c - b[i] * s, y = b[i] * c + a[i] * s;
-                a[i] = x, b[i] = y;
-            }
-        }
-        for (int i = 0; i < 4; i++) lo[i] = (float)a[i], hi[i] = (float)b[i];
-    }
-    // max |x|; an Inf or NaN gives NaN or Inf (the integer order of |x|).
-    __device__ __forceinline__ unsigned top_bits() const {
-        unsigned m = 0;
-        for (int i = 0; i < 4; i++) {
-            m = max(m, __float_as_uint(lo[i]) & 0x7fffffffu);
-            m = max(m, __float_as_uint(hi[i]) & 0x7fffffffu);
-        }
-        return m;
+    __device__ __forceinline__ void store(float *p, int g, int half) const {
+        store4(p + 4 * g, lo);
+        store4(p + half + 4 * g, hi);
     }
 };
 
-// rne(127 x / top), the quotient's border cases settled in 64 bits.
-__device__ __forceinline__ int quantize(float x, float top, float inv) {
-    const float t = x * inv;
-    const float r = rintf(t);
-    if (fabsf(t - r) < 0.4999f && top > 1e-30f) return (int)r;
-    return (int)rint((double)x * 127.0 / (double)top);
+// A position's cosines and sines, lane g's four.
+struct Turn {
+    f32x4 c, s;
+    __device__ __forceinline__ void load(const qtts_paged_rows &r, int pos, int g, int half) {
+        c = load4(r.rope_cos + (size_t)pos * half + 4 * g);
+        s = load4(r.rope_sin + (size_t)pos * half + 4 * g);
+    }
+};
+
+// Norm and rotation in 64 bits, rounded to f32 once: codes at the border
+// between two steps then agree with the definition's.  The vector units run
+// 64-bit products at the f32 rate, and the kernel waits for memory.
+template <int HD>
+__device__ __forceinline__ Pairs norm_rotate(const Pairs &x, const Turn &t, const uint16_t *norm, float eps, bool rope,
+                                             int g) {
+    double a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) a[i] = x.lo[i], b[i] = x.hi[i];
+    if (norm) {
+        double ss = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) ss += a[i] * a[i] + b[i] * b[i];
+        ss = group_sum(ss, HD / 8);
+        const double inv = 1.0 / sqrt(ss / HD + (double)eps);
+        const uint2 na = *reinterpret_cast<const uint2 *>(norm + 4 * g);
+        const uint2 nb = *reinterpret_cast<const uint2 *>(norm + HD / 2 + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            a[i] *= (double)f16_to_f32((uint16_t)((i < 2 ? na.x : na.y) >> 16 * (i & 1))) * inv;
+            b[i] *= (double)f16_to_f32((uint16_t)((i < 2 ? nb.x : nb.y) >> 16 * (i & 1))) * inv;
+        }
+    }
+    Pairs r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const double y = rope ? a[i] * (double)t.c[i] - b[i] * (double)t.s[i] : a[i];
+        const double z = rope ? b[i] * (double)t.c[i] + a[i] * (double)t.s[i] : b[i];
+        r.lo[i] = (float)y, r.hi[i] = (float)z;
+    }
+    return r;
 }
 
+// max |x| as bits; an Inf or NaN is the largest.
+__device__ __forceinline__ unsigned top_bits(f32x4 x, unsigned m) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
+}
+
+// A block's scale and what its codes are made with: rne(127 x / top).  The
+// f32 quotient is good to 2^-22 of its value; next to a border between two
+// codes, and where 127 / top leaves f32's range, the quotient is a 64-bit one.
+struct Quantizer {
+    float top, inv;
+    bool none;  // zeros, or not finite
+    __device__ __forceinline__ explicit Quantizer(unsigned bits) {
+        top = __uint_as_float(bits);
+        none = bits == 0 || bits >= 0x7f800000u;
+        inv = 127.0f / top;
+    }
+    __device__ __forceinline__ float scale() const {
+        return __float_as_uint(top) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : top / 127.0f;
+    }
+    __device__ __forceinline__ int code(float x) const {
+        if (none) return 0;
+        const float t = x * inv, r = rintf(t);
+        if (fabsf(t - r) < 0.4999f && top > 1e-30f) return (int)r;
+        return (int)rint((double)x * 127.0 / (double)top);
+    }
+    __device__ __forceinline__ unsigned code4(float a, float b, float c, float d) const {
+        return (unsigned)(code(a) & 255) | (unsigned)(code(b) & 255) << 8 | (unsigned)(code(c) & 255) << 16 |
+               (unsigned)code(d) << 24;
+    }
+};
+
+// A block for each (sequence, kv head, page that its rows touch, K or V), and for
+// NT / (HD / 8) groups of four query heads.  Bound by memory: rows are read once,
+// in 16-byte pieces all asked for before the first is used; a full page's codes
+// are written from registers, V's across (by way of LDS) in whole lines.
 template <int HD, int P>
 __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
-    constexpr int L = HD / 8;                                  // lanes of one head's vector
-    constexpr int NT = P * L < 256 ? P * L : 256;              // threads
-    constexpr int V = NT / L;                                  // vectors a pass
-    constexpr int PASS = P / V;
-    __shared__ unsigned tops[2][NT / 64];
-    const int per_seq = A.kv_items * A.kv.kv_heads + A.q_items;
+    constexpr int L = HD / 8, H = HD / 2;                 // lanes of one head's vector, its half
+    constexpr int NT = P * L < 256 ? P * L : 256;         // threads
+    constexpr int V = NT / L, PASS = P / V;               // K: vectors a pass
+    constexpr int D4 = HD / 4, TG = NT / D4;              // V: 4 dimensions of 4 tokens a thread
+    constexpr int VPASS = P / 4 > TG ? P / 4 / TG : 1;
+    constexpr int W = P / 4 + 1;                          // words of a dimension's row in LDS
+    __shared__ unsigned tops[NT / 64];
+    __shared__ unsigned vt[HD * W];
+    const qtts_paged_kv &kv = A.kv;
+    const int kv_blocks = 2 * A.kv_items * kv.kv_heads, per_seq = kv_blocks + A.q_items;
     const int b = blockIdx.x / per_seq, item = blockIdx.x % per_seq;
-    const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, A.cap);
+    const PagedSeq q = load_seq(A.s, b, kv.num_slots, A.cap);
     if (!q.ok || q.rows == 0) return;
-    const int g = threadIdx.x % L, v = threadIdx.x / L;
-    if (item >= A.kv_items * A.kv.kv_heads) {  // queries
-        const long long units = (long long)q.rows * A.r.heads;
-        const long long u0 = (long long)(item - A.kv_items * A.kv.kv_heads) * 64;
-        for (long long u = u0 + v; u < min(u0 + 64, units); u += V) {
-            const int row = (int)(u / A.r.heads), h = (int)(u % A.r.heads);
-            Pairs<HD> x;
-            x.load(A.r.q + (size_t)(q.row0 + row) * A.r.ld_q + (size_t)h * HD, g);
-            x.norm_rotate(A.r, A.r.q_norm, q.start + row, g);
-            x.store(A.r.q_out + (size_t)(q.row0 + row) * A.r.ld_q_out + (size_t)h * HD, g);
-        }
+    const int tid = threadIdx.x, g = tid % L, v = tid / L;
+    const bool rope = A.r.rope_cos != nullptr;
+    if (item >= kv_blocks) {  // queries: four heads of a row in each group of lanes
+        const int groups = (A.r.heads + 3) / 4;
+        const int at = (item - kv_blocks) * V + v;
+        if (at >= q.rows * groups) return;
+        const int row = at / groups, h0 = at % groups * 4, n = min(4, A.r.heads - h0);
+        const float *from = A.r.q + (size_t)(q.row0 + row) * A.r.ld_q + (size_t)h0 * HD;
+        float *to = A.r.q_out + (size_t)(q.row0 + row) * A.r.ld_q_out + (size_t)h0 * HD;
+        Pairs x[4];
+        Turn t;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i].load(from + min(i, n - 1) * HD, g, H);
+        if (rope) t.load(A.r, q.start + row, g, H);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < n) norm_rotate<HD>(x[i], t, A.r.q_norm, A.r.eps, rope, g).store(to + i * HD, g, H);
         return;
     }
-    const int head = item % A.kv.kv_heads, j = item / A.kv.kv_heads;
-    const int end = q.start + q.rows, first = q.start / P, page = first + j;
+    const bool is_v = item & 1;
+    const int head = item / 2 % kv.kv_heads, j = item / 2 / kv.kv_heads;
+    const int end = q.start + q.rows, page = q.start / P + j;
     if (page * P >= end) return;
-    const size_t open = ((size_t)q.slot * A.kv.kv_heads + head) * P * HD;
-    auto row_of = [&](const float *x, int ld, int pos) {
-        return x + (size_t)(q.row0 + pos - q.start) * ld + (size_t)head * HD;
+    float *open = (is_v ? kv.v_open : kv.k_open) + ((size_t)q.slot * kv.kv_heads + head) * P * HD;
+    const float *rows = (is_v ? A.r.v : A.r.k) + (size_t)head * HD;
+    const int ld = is_v ? A.r.ld_v : A.r.ld_k;
+    auto row_at = [&](int pos) {  // what the cache holds or takes at a position
+        return pos < q.start ? open + pos % P * HD : rows + (size_t)(q.row0 + pos - q.start) * ld;
     };
     auto open_rows = [&](int from, int to) {  // new rows of the page left open
         for (int pos = from + v; pos < to; pos += V) {
-            Pairs<HD> k, x;
-            k.load(row_of(A.r.k, A.r.ld_k, pos), g);
-            k.norm_rotate(A.r, A.r.k_norm, pos, g);
-            k.store(A.kv.k_open + open + (size_t)(pos % P) * HD, g);
-            x.load(row_of(A.r.v, A.r.ld_v, pos), g);
-            x.store(A.kv.v_open + open + (size_t)(pos % P) * HD, g);
+            Pairs x;
+            Turn t;
+            x.load(row_at(pos), g, H);
+            if (!is_v) {
+                if (rope) t.load(A.r, pos, g, H);
+                x = norm_rotate<HD>(x, t, A.r.k_norm, A.r.eps, rope, g);
+            }
+            x.store(open + pos % P * HD, g, H);
         }
     };
     // The rows left open go over the open rows of the page that was begun
@@ -131,49 +182,72 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
         if (j == 0 || !begun) open_rows(max(q.start, page * P), end);
         return;
     }
-    Pairs<HD> k[PASS], x[PASS];
-    unsigned top_k = 0, top_v = 0;
-#pragma unroll
-    for (int i = 0; i < PASS; i++) {
-        const int pos = page * P + i * V + v;
-        if (pos < q.start) {
-            k[i].load(A.kv.k_open + open + (size_t)(pos % P) * HD, g);
-            x[i].load(A.kv.v_open + open + (size_t)(pos % P) * HD, g);
-        } else {
-            k[i].load(row_of(A.r.k, A.r.ld_k, pos), g);
-            k[i].norm_rotate(A.r, A.r.k_norm, pos, g);
-            x[i].load(row_of(A.r.v, A.r.ld_v, pos), g);
-        }
-        top_k = max(top_k, k[i].top_bits());
-        top_v = max(top_v, x[i].top_bits());
-    }
-    for (int off = 32; off > 0; off >>= 1) {
-        top_k = max(top_k, (unsigned)__shfl_xor((int)top_k, off, 64));
-        top_v = max(top_v, (unsigned)__shfl_xor((int)top_v, off, 64));
-    }
-    if (threadIdx.x % 64 == 0) tops[0][threadIdx.x / 64] = top_k, tops[1][threadIdx.x / 64] = top_v;
-    __syncthreads();
-    for (int w = 0; w < NT / 64; w++) top_k = max(top_k, tops[0][w]), top_v = max(top_v, tops[1][w]);
     const int id = q.pages[page];
-    if (id >= 0 && id < A.kv.num_pages) {
-        const size_t block = (size_t)id * A.kv.kv_heads + head;
-        const bool fin_k = top_k < 0x7f800000u, fin_v = top_v < 0x7f800000u;
-        const float tk = __uint_as_float(top_k), tv = __uint_as_float(top_v);
-        const float ik = 127.0f / tk, iv = 127.0f / tv;
-        if (threadIdx.x == 0) {
-            A.kv.k_scales[block] = fin_k ? tk / 127.0f : __uint_as_float(0x7fc00000u);
-            A.kv.v_scales[block] = fin_v ? tv / 127.0f : __uint_as_float(0x7fc00000u);
-        }
-        int8_t *kc = A.kv.k_codes + block * P * HD, *vc = A.kv.v_codes + block * P * HD;
-        const bool zk = !fin_k || top_k == 0, zv = !fin_v || top_v == 0;
+    const bool in = id >= 0 && id < kv.num_pages;
+    const size_t block = (size_t)(in ? id : 0) * kv.kv_heads + head;
+    auto block_top = [&](unsigned top) {
+        for (int off = 32; off > 0; off >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, off, 64));
+        if (tid % 64 == 0) tops[tid / 64] = top;
+        __syncthreads();
+        for (int w = 0; w < NT / 64; w++) top = max(top, tops[w]);
+        return top;
+    };
+    unsigned top = 0;
+    if (!is_v) {
+        Pairs x[PASS];
+        Turn t[PASS];
 #pragma unroll
         for (int i = 0; i < PASS; i++) {
-            const int t = i * V + v;
-            for (int e = 0; e < 4; e++) {
-                kc[t * HD + 4 * g + e] = zk ? 0 : quantize(k[i].lo[e], tk, ik);
-                kc[t * HD + HD / 2 + 4 * g + e] = zk ? 0 : quantize(k[i].hi[e], tk, ik);
-                vc[(4 * g + e) * P + t] = zv ? 0 : quantize(x[i].lo[e], tv, iv);
-                vc[(HD / 2 + 4 * g + e) * P + t] = zv ? 0 : quantize(x[i].hi[e], tv, iv);
+            const int pos = page * P + i * V + v;
+            x[i].load(row_at(pos), g, H);
+            if (rope) t[i].load(A.r, pos, g, H);
+        }
+#pragma unroll
+        for (int i = 0; i < PASS; i++) {
+            if (page * P + i * V + v >= q.start) x[i] = norm_rotate<HD>(x[i], t[i], A.r.k_norm, A.r.eps, rope, g);
+            top = top_bits(x[i].hi, top_bits(x[i].lo, top));
+        }
+        const Quantizer z(block_top(top));
+        if (in) {
+            if (tid == 0) kv.k_scales[block] = z.scale();
+            unsigned *codes = reinterpret_cast<unsigned *>(kv.k_codes + block * P * HD);
+#pragma unroll
+            for (int i = 0; i < PASS; i++) {
+                unsigned *to = codes + (i * V + v) * (HD / 4) + g;
+                to[0] = z.code4(x[i].lo[0], x[i].lo[1], x[i].lo[2], x[i].lo[3]);
+                to[HD / 8] = z.code4(x[i].hi[0], x[i].hi[1], x[i].hi[2], x[i].hi[3]);
+            }
+        }
+    } else {
+        f32x4 x[VPASS][4];
+        const int d4 = tid % D4, tg = tid / D4;
+        const bool part = P / 4 >= TG || tg < P / 4;
+        if (part)
+#pragma unroll
+            for (int i = 0; i < VPASS; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[i][e] = load4(row_at(page * P + 4 * (i * TG + tg) + e) + 4 * d4);
+        if (part)
+#pragma unroll
+            for (int i = 0; i < VPASS; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = top_bits(x[i][e], top);
+        const Quantizer z(block_top(top));
+        if (in) {
+            if (tid == 0) kv.v_scales[block] = z.scale();
+            if (part)
+#pragma unroll
+                for (int i = 0; i < VPASS; i++) {
+                    unsigned *to = vt + 4 * d4 * W + i * TG + tg;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) to[e * W] = z.code4(x[i][0][e], x[i][1][e], x[i][2][e], x[i][3][e]);
+                }
+            __syncthreads();
+            uint4 *codes = reinterpret_cast<uint4 *>(kv.v_codes + block * P * HD);
+#pragma unroll
+            for (int i = tid; i < P * HD / 16; i += NT) {
+                const unsigned *from = vt + i / (P / 16) * W + i % (P / 16) * 4;
+                codes[i] = make_uint4(from[0], from[1], from[2], from[3]);
             }
         }
     }
@@ -195,7 +269,6 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -890,29 +963,56 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
     }
 }
 
-__global__ __launch_bounds__(256) void k_paged_read(PagedReadParams A, int tiles) {
-    const int P = A.kv.page_size, kvh = A.kv.kv_heads, hd = A.kv.head_dim, width = kvh * hd;
-    const int b = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+// A block of each (sequence, kv head, page that its positions touch): 4 tokens x
+// 4 dimensions a thread, so that V's codes, which lie across, are turned in
+// registers and every row is written 16 bytes a lane in a row.
+template <int HD>
+__global__ __launch_bounds__(256) void k_paged_read(PagedReadParams A, int items) {
+    constexpr int D4 = HD / 4;
+    const int P = A.kv.page_size, sh = __builtin_ctz(P), kvh = A.kv.kv_heads;
+    const int head = blockIdx.x % kvh, item = blockIdx.x / kvh % items, b = blockIdx.x / kvh / items;
     const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, (long long)A.s.max_pages * P);
     const int len = A.lens ? A.lens[b] : q.start + q.rows;
     const bool ok = q.ok && (long long)len <= (long long)A.s.max_pages * P;
-    for (int r = tile * 8; r < min(tile * 8 + 8, q.rows); r++) {
-        const int pos = q.start + r;
-        const bool have = ok && pos < len, open = have && pos >= len / P * P;
-        const int id = have && !open ? q.pages[pos / P] : -1;
-        for (int d = threadIdx.x; d < width; d += 256) {
-            const int head = d / hd, e = d % hd;
-            float k = 0, v = 0;
-            if (open) {
-                const size_t at = (((size_t)q.slot * kvh + head) * P + pos % P) * hd + e;
-                k = A.kv.k_open[at], v = A.kv.v_open[at];
-            } else if (id >= 0 && id < A.kv.num_pages) {
-                const size_t block = (size_t)id * kvh + head;
-                k = (float)A.kv.k_codes[(block * P + pos % P) * hd + e] * A.kv.k_scales[block];
-                v = (float)A.kv.v_codes[(block * hd + e) * P + pos % P] * A.kv.v_scales[block];
+    // positions of this block, by pages where they have any
+    const int first = ok ? q.start >> sh << sh : 0;
+    const int lo = max(first + item * P, ok ? q.start : 0);
+    const int hi = min(first + (item + 1) * P, ok ? q.start + q.rows : q.rows);
+    if (lo >= hi) return;
+    const int row0 = q.row0 - (ok ? q.start : 0);  // of position 0
+    const int full = ok ? len >> sh << sh : 0;
+    const int page = lo >> sh;
+    const int id = ok && lo < full ? q.pages[page] : -1;
+    const bool closed = id >= 0 && id < A.kv.num_pages;
+    const size_t block = (size_t)(closed ? id : 0) * kvh + head;
+    const float ks = closed ? A.kv.k_scales[block] : 0.0f, vs = closed ? A.kv.v_scales[block] : 0.0f;
+    const float *k_open = A.kv.k_open + ((size_t)(ok ? q.slot : 0) * kvh + head) * P * HD;
+    const float *v_open = A.kv.v_open + ((size_t)(ok ? q.slot : 0) * kvh + head) * P * HD;
+    const int8_t *kc = A.kv.k_codes + block * P * HD, *vc = A.kv.v_codes + block * P * HD;
+    const int t_lo = lo & ~3, parts = ((hi - t_lo + 3) >> 2) * D4;
+    auto byte = [](unsigned w, int i) { return (float)(int8_t)(w >> 8 * i); };
+    for (int i = threadIdx.x; i < parts; i += 256) {
+        const int d = 4 * (i % D4), t0 = t_lo + 4 * (i / D4);  // 4 tokens from t0, in one page
+        unsigned kw[4], vw[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            kw[e] = *reinterpret_cast<const unsigned *>(kc + (((t0 + e) & (P - 1)) * HD) + d);
+            vw[e] = *reinterpret_cast<const unsigned *>(vc + ((d + e) << sh) + (t0 & (P - 1)));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int t = t0 + e;
+            if (t < lo || t >= hi) continue;
+            f32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+            if (closed) {
+                k = f32x4{byte(kw[e], 0), byte(kw[e], 1), byte(kw[e], 2), byte(kw[e], 3)} * ks;
+                v = f32x4{byte(vw[0], e), byte(vw[1], e), byte(vw[2], e), byte(vw[3], e)} * vs;
+            } else if (ok && t >= full && t < len) {
+                k = load4(k_open + (t & (P - 1)) * HD + d);
+                v = load4(v_open + (t & (P - 1)) * HD + d);
             }
-            if (A.k_out) A.k_out[(size_t)(q.row0 + r) * A.ld_k + d] = k;
-            if (A.v_out) A.v_out[(size_t)(q.row0 + r) * A.ld_v + d] = v;
+            if (A.k_out) store4(A.k_out + (size_t)(row0 + t) * A.ld_k + head * HD + d, k);
+            if (A.v_out) store4(A.v_out + (size_t)(row0 + t) * A.ld_v + head * HD + d, v);
         }
     }
 }
@@ -945,9 +1045,12 @@ bool launch_paged_append(hipStream_t st, const PagedAppendParams &in) {
     PagedAppendParams p = in;
     const int P = p.kv.page_size;
     p.kv_items = (int)(((long long)p.s.max_rows + P - 2) / P + 1);
-    p.q_items = p.r.q ? (int)(((long long)p.s.max_rows * p.r.heads + 63) / 64) : 0;
-    const long long blocks = p.s.batch * ((long long)p.kv_items * p.kv.kv_heads + p.q_items);
-    if ((long long)p.s.max_rows * p.r.heads > kPagedMaxBlocks || blocks > kPagedMaxBlocks) return false;
+    const int NT = std::min(256, P * p.kv.head_dim / 8), groups = NT / (p.kv.head_dim / 8);
+    const long long parts = p.r.q ? (long long)p.s.max_rows * ((p.r.heads + 3) / 4) : 0;
+    if (parts > kPagedMaxBlocks) return false;
+    p.q_items = (int)((parts + groups - 1) / groups);
+    const long long blocks = p.s.batch * (2LL * p.kv_items * p.kv.kv_heads + p.q_items);
+    if (2LL * p.kv_items * p.kv.kv_heads > kPagedMaxBlocks || blocks > kPagedMaxBlocks) return false;
     if (p.kv.head_dim == 64) append_of<64>(st, p, (unsigned)blocks);
     else append_of<128>(st, p, (unsigned)blocks);
     return true;
@@ -973,10 +1076,11 @@ bool launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
 }
 
 bool launch_paged_read(hipStream_t st, const PagedReadParams &p) {
-    const int tiles = (p.s.max_rows + 7) / 8;
-    const long long blocks = (long long)p.s.batch * tiles;
+    const int P = p.kv.page_size, items = (int)(((long long)p.s.max_rows + P - 2) / P + 1);
+    const long long blocks = (long long)p.s.batch * items * p.kv.kv_heads;
     if (blocks > kPagedMaxBlocks) return false;
-    hipLaunchKernelGGL(k_paged_read, dim3((unsigned)blocks), dim3(256), 0, st, p, tiles);
+    if (p.kv.head_dim == 64) hipLaunchKernelGGL(k_paged_read<64>, dim3((unsigned)blocks), dim3(256), 0, st, p, items);
+    else hipLaunchKernelGGL(k_paged_read<128>, dim3((unsigned)blocks), dim3(256), 0, st, p, items);
     return true;
 }
 
