@@ -3004,6 +3004,8 @@ qtts_status qtts_sample_rows_device(qtts_ctx *c, const float *d_logits, int64_t 
     p.u = d_uniform;
     p.tokens = d_tokens;
     p.probs = d_probs;
+    p.scratch = c->attn_part;
+    p.scratch_bytes = kAttnPartFloats * sizeof(float);
     QTTS_CHECK(c, check_sample_rows(d_logits, ld, rows, vocab, p.p, d_uniform, d_tokens, d_probs));
     if (rows == 0) return QTTS_OK;
     DeviceGuard guard(c->device);

@@ -15,10 +15,31 @@ namespace qtts {
 
 namespace {
 
-// Sum over groups of `width` lanes.
-__device__ __forceinline__ double group_sum(double v, int width) {
-    for (int off = width / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, width);
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, 0xF, 0xF, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Sum over groups of 8 or 16 lanes, the same in each.
+template <int WIDTH>
+__device__ __forceinline__ double group_sum(double v) {
+    v += dpp64<kDppXor1>(v);
+    v += dpp64<kDppXor2>(v);
+    v += dpp64<kDppHalfMirror>(v);
+    if (WIDTH == 16) v += dpp64<kDppMirror>(v);
     return v;
+}
+
+// 1 / sqrt(x): the hardware's estimate and two steps of Newton's method.
+__device__ __forceinline__ double inv_sqrt(double x) {
+    if (!(x > 0.0 && x < (double)INFINITY)) return 1.0 / sqrt(x);
+    double y = __builtin_amdgcn_rsq(x);
+    y *= 1.5 - 0.5 * x * y * y;
+    y *= 1.5 - 0.5 * x * y * y;
+    return y;
 }
 
 // One head's vector spread over HD / 8 lanes: lane g of them holds elements
@@ -62,8 +83,7 @@ __device__ __forceinline__ Pairs norm_rotate(const Pairs &x, const Turn &t, cons
         double ss = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) ss += a[i] * a[i] + b[i] * b[i];
-        ss = group_sum(ss, HD / 8);
-        const double inv = 1.0 / sqrt(ss / HD + (double)eps);
+        const double inv = inv_sqrt(group_sum<HD / 8>(ss) * (1.0 / HD) + (double)eps);
         const uint2 na = *reinterpret_cast<const uint2 *>(norm + 4 * g);
         const uint2 nb = *reinterpret_cast<const uint2 *>(norm + HD / 2 + 4 * g);
 #pragma unroll

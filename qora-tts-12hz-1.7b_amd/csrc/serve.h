@@ -50,6 +50,8 @@ struct SampleRowsParams {
     const float *u;
     int32_t *tokens;
     float *probs;
+    void *scratch;         // for long rows: as many at once as it holds
+    size_t scratch_bytes;
 };
 
 // False: the call needs more blocks than one launch holds, nothing was launched.
