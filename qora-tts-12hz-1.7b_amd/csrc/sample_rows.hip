@@ -169,89 +169,171 @@ constexpr int kBrute = 256;  // a set this small is ranked by comparing all pair
 struct Space {
     double tab[64];
     u64 hist[256], wsum[16], base;
+    unsigned near[kBrute];
     unsigned digit, thr, ties, top, bad;
     int token;
 };
 
+// The prefix of n <= kBrute keys, near(i) in the order of their indices, of which
+// the first `count` stay (0: all) and then, where `by_sum`, those whose
+// predecessors' sum and `above` is below `need` (0: top-p's share of the sum).
+// NT / kBrute threads a key, or one, compare it with the others.
+template <int NT, class Key>
+__device__ Cut rank_all(const Key &near, int n, u64 count, bool by_sum, u64 above, u64 need, const RowSettings &S,
+                        const Weights &W, Space *sp) {
+    constexpr int PARTS = NT / kBrute;
+    static_assert(PARTS == 1 || PARTS == 4, "quads of lanes");
+    u64 *units = sp->hist;
+    const int i = threadIdx.x / PARTS, part = threadIdx.x % PARTS;
+    __syncthreads();
+    if (threadIdx.x == 0) sp->thr = 0xffffffffu, sp->ties = 0;
+    const bool in = i < n;
+    const unsigned k = in ? near(i) : 0;
+    const u64 mine = in && by_sum ? W.units(logit_of(k)) : 0;
+    if (in && part == 0) units[i] = mine;
+    __syncthreads();
+    unsigned rank = 0;
+    u64 ahead = 0;
+    if (in) {
+#pragma unroll 4
+        for (int j = part; j < n; j += PARTS) {
+            const unsigned o = near(j);
+            const bool before = o > k || (o == k && j < i);
+            rank += before;
+            ahead += before ? units[j] : 0;
+        }
+    }
+    for (int off = 1; off < PARTS; off <<= 1) {
+        rank += __shfl_xor((int)rank, off, 64);
+        ahead += (u64)__shfl_xor((long long)ahead, off, 64);
+    }
+    bool keep = in && (count == 0 || rank < count);
+    if (by_sum) {
+        if (need == 0) need = S.share_of(block_total<NT>(keep && part == 0 ? mine : 0, sp->wsum));
+        keep = keep && above + ahead < need;
+    }
+    if (keep) atomicMin(&sp->thr, k);
+    __syncthreads();
+    Cut c;
+    c.thr = sp->thr;
+    if (keep && part == 0 && k == c.thr) atomicAdd(&sp->ties, 1u);
+    __syncthreads();
+    c.ties = sp->ties;
+    return c;
+}
+
 // The prefix that top-k and top-p keep of n keys, key(i) in the order of their
 // indices; `need`: the sum that top-p's prefix reaches, 0: its share of the sum.
-// Small sets by comparing all pairs; others by 8 bits of the key at a time,
-// counts first and then sums.
+// Small sets at once.  Others by the logit's place on a line of 2^16 steps from
+// the largest down, 8 bits at a time, counts first and then sums, until what
+// shares the cut's step is a small set (many equal ones: by the key's digits).
 template <int NT, class Key>
 __device__ Cut cut_of(const Key &key, int n, const RowSettings &S, const Weights &W, u64 need, Space *sp) {
     const int tid = threadIdx.x;
     const bool sums = S.cuts_sum();
     Cut c;
     if (S.top_k == 0 && !sums) return c;
-    if (n <= kBrute) {
-        u64 *units = sp->hist;
-        __syncthreads();
-        if (tid == 0) sp->thr = 0xffffffffu, sp->ties = 0;
-        const bool in = tid < n;
-        const unsigned k = in ? key(tid) : 0;
-        const u64 mine = in ? W.units(logit_of(k)) : 0;
-        if (in) units[tid] = mine;
-        __syncthreads();
-        unsigned rank = 0;
-        u64 ahead = 0;
-        if (in)
-            for (int j = 0; j < n; j++) {
-                const unsigned o = key(j);
-                const bool before = o > k || (o == k && j < tid);
-                rank += before;
-                ahead += before ? units[j] : 0;
-            }
-        bool keep = in && (S.top_k == 0 || rank < (unsigned)S.top_k);
-        if (sums) {
-            if (need == 0) need = S.share_of(block_total<NT>(keep ? mine : 0, sp->wsum));
-            keep = keep && ahead < need;
-        }
-        if (keep) atomicMin(&sp->thr, k);
-        __syncthreads();
-        c.thr = sp->thr;
-        if (keep && k == c.thr) atomicAdd(&sp->ties, 1u);
-        __syncthreads();
-        c.ties = sp->ties;
-        return c;
+    if (n <= kBrute) return rank_all<NT>(key, n, S.top_k, sums, 0, need, S, W, sp);
+    // the least finite logit, and the line's scale
+    unsigned least = 0xffffffffu;
+    for (int i = tid; i < n; i += NT) {
+        const unsigned k = key(i);
+        least = min(least, k > key_of(-INFINITY) ? k : 0xffffffffu);
     }
-    auto select = [&](bool by_sum, u64 want, u64 *above) {
-        unsigned prefix = 0;
+    for (int off = 32; off > 0; off >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, off, 64));
+    __syncthreads();
+    if (tid == 0) sp->thr = 0xffffffffu;
+    __syncthreads();
+    if ((tid & 63) == 0) atomicMin(&sp->thr, least);
+    __syncthreads();
+    const float lo = logit_of(sp->thr);
+    __syncthreads();
+    float scale = 0;
+    auto line = [&](unsigned k) {  // halves, so that the difference stays in range
+        const float l = logit_of(k);
+        return l == W.mx ? 0 : (int)fminf((0.5f * W.mx - 0.5f * l) * scale, 65535.0f);
+    };
+    auto scan_digits = [&](bool down, u64 want, u64 base) {  // by the first wave: where the sum reaches `want`
+        if (tid < 64) {
+            u64 h[4], sum = 0;
+            for (int j = 0; j < 4; j++) sum += h[j] = sp->hist[down ? 255 - 4 * tid - j : 4 * tid + j];
+            u64 run = base + wave_scan(sum) - sum;
+            const bool mine = run < want && run + sum >= want, none = !__any(mine);
+            if (mine || (none && tid == 63)) {
+                int j = 0;
+                for (; j < 3 && run + h[j] < want; j++) run += h[j];
+                sp->digit = down ? 255 - 4 * tid - j : 4 * tid + j;
+                sp->base = run;
+            }
+        }
+        __syncthreads();
+    };
+    auto select = [&](bool by_sum, u64 want) {
+        const float range = 0.5f * W.mx - 0.5f * lo;
+        const float far = by_sum ? 16.0f * S.t : INFINITY;  // half of 46 octaves: no weights past them
+        const float span = range < far ? range : far;
+        scale = span > 0.0f ? 65535.0f / span : 0.0f;
+        if (!(scale < INFINITY)) scale = 3e38f;
         u64 base = 0;
+        int at = 0;  // the chosen steps' first digits
+        for (int round = 0; round < 2; round++) {
+            for (int i = tid; i < 256; i += NT) sp->hist[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += NT) {
+                const unsigned k = key(i);
+                if (k < c.thr) continue;
+                const int p = line(k);
+                if (round == 1 && p >> 8 != at) continue;
+                const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
+                if (w) atomicAdd(&sp->hist[round == 0 ? p >> 8 : p & 255], w);
+            }
+            __syncthreads();
+            scan_digits(false, want, base);
+            at = at << 8 | (int)sp->digit;
+            base = sp->base;
+            // what shares them, in order, if that is few
+            const int shift = round == 0 ? 8 : 0;
+            const int per = (n + NT - 1) / NT, lo_i = min(tid * per, n), hi_i = min(lo_i + per, n);
+            u64 have = 0, all;
+            for (int i = lo_i; i < hi_i; i++) {
+                const unsigned k = key(i);
+                have += k >= c.thr && line(k) >> shift == at;
+            }
+            int to = (int)(block_scan<NT>(have, sp->wsum, &all) - have);
+            if (all <= kBrute) {
+                for (int i = lo_i; i < hi_i; i++) {
+                    const unsigned k = key(i);
+                    if (k >= c.thr && line(k) >> shift == at) sp->near[to++] = k;
+                }
+                auto near = [&](int i) { return sp->near[i]; };
+                return by_sum ? rank_all<NT>(near, (int)all, 0, true, base, want, S, W, sp)
+                              : rank_all<NT>(near, (int)all, want - base, false, 0, 0, S, W, sp);
+            }
+        }
+        unsigned prefix = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
             __syncthreads();
             for (int i = tid; i < 256; i += NT) sp->hist[i] = 0;
             __syncthreads();
             for (int i = tid; i < n; i += NT) {
                 const unsigned k = key(i);
-                if (k < c.thr || (shift < 24 && k >> (shift + 8) != prefix)) continue;
+                if (k < c.thr || line(k) != at || (shift < 24 && k >> (shift + 8) != prefix)) continue;
                 const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
                 if (w) atomicAdd(&sp->hist[(k >> shift) & 255], w);
             }
             __syncthreads();
-            if (tid < 64) {  // from the top: a lane has digits 255 - 4 lane and the next three
-                u64 h[4], sum = 0;
-                for (int j = 0; j < 4; j++) sum += h[j] = sp->hist[255 - 4 * tid - j];
-                u64 run = base + wave_scan(sum) - sum;
-                const bool mine = run < want && run + sum >= want, none = !__any(mine);
-                if (mine || (none && tid == 63)) {
-                    int j = 0;
-                    for (; j < 3 && run + h[j] < want; j++) run += h[j];
-                    sp->digit = 255 - 4 * tid - j;
-                    sp->base = run;
-                }
-            }
-            __syncthreads();
+            scan_digits(true, want, base);
             prefix = prefix << 8 | sp->digit;
             base = sp->base;
         }
-        *above = base;
-        return prefix;
+        __syncthreads();
+        const u64 w = by_sum ? W.units(logit_of(prefix)) : (u64)1;
+        Cut d;
+        d.thr = prefix;
+        d.ties = w ? (want - base + w - 1) / w : ~0ull;
+        return d;
     };
-    if (S.top_k > 0) {
-        u64 above;
-        c.thr = select(false, (u64)S.top_k, &above);
-        c.ties = (u64)S.top_k - above;
-    }
+    if (S.top_k > 0) c = select(false, (u64)S.top_k);
     if (sums) {
         if (need == 0) {  // of those above thr, and `ties` at it
             u64 sum = 0;
@@ -262,11 +344,10 @@ __device__ Cut cut_of(const Key &key, int n, const RowSettings &S, const Weights
             sum = block_total<NT>(sum, sp->wsum);
             need = S.share_of(sum + (c.thr ? c.ties * W.units(logit_of(c.thr)) : 0));
         }
-        u64 above;
-        const unsigned t = select(true, need, &above);
-        const u64 w = W.units(logit_of(t)), m = w ? (need - above + w - 1) / w : ~0ull;
-        if (t > c.thr || c.thr == 0) c.thr = t, c.ties = m;
-        else c.ties = m < c.ties ? m : c.ties;
+        __syncthreads();
+        const Cut d = select(true, need);
+        if (d.thr > c.thr) c = d;
+        else c.ties = d.ties < c.ties ? d.ties : c.ties;
     }
     return c;
 }
@@ -314,52 +395,115 @@ __device__ __forceinline__ void drawn(const SampleRowsParams &P, int r, int toke
     if (P.probs) P.probs[r] = (float)(weight * kUnit / (double)total);
 }
 
-// The keys of `n` candidates among the row's, at least as large as the k-th
-// largest: at most top_k of the maxima of runs are above the k-th largest of
-// them, so that what is below it is not among the first k.  Ranked by comparing
-// all pairs; with top_k runs or fewer everything stays.
-template <int NT>
-__device__ unsigned least_of_runs(unsigned mine, int top_k, unsigned *tops, Space *sp) {
-    if (top_k >= NT) return 0;
-    tops[threadIdx.x] = mine;
-    __syncthreads();
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < NT; j++) {
-        const unsigned o = tops[j];
-        rank += o > mine || (o == mine && j < (int)threadIdx.x);
+// The whole end of a row whose candidates are at most a wave: n keys in the order
+// of their indices, cut and drawn from without a barrier.  place(i): the index.
+template <class Place>
+__device__ void finish_wave(const SampleRowsParams &P, int r, unsigned k, int n, const Place &place,
+                            const RowSettings &S, const Weights &W, u64 need) {
+    const int lane = threadIdx.x & 63;
+    const bool in = lane < n, sums = S.cuts_sum();
+    const float l = logit_of(k);
+    const u64 mine = in ? W.units(l) : 0;
+    unsigned rank = 0;
+    u64 ahead = 0;
+    for (int j = 0; j < n; j++) {
+        const unsigned o = (unsigned)__builtin_amdgcn_readlane((int)k, j);
+        const u64 w = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)mine, j) |
+                      (u64)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32;
+        const bool before = o > k || (o == k && j < lane);
+        rank += before;
+        ahead += before ? w : 0;
     }
-    if (rank == top_k - 1) sp->thr = mine;
+    bool keep = in && (S.top_k == 0 || rank < (unsigned)S.top_k);
+    if (sums) {
+        if (need == 0) need = S.share_of(wave_total(keep ? mine : 0));
+        keep = keep && ahead < need;
+    }
+    const u64 kept = keep && W.weight(l) >= S.least ? mine : 0;
+    const u64 upto = wave_scan(kept), total = (u64)__shfl((long long)upto, 63, 64);
+    const u64 target = S.target_of(P.u[r], total);
+    if (target >= upto - kept && target < upto) drawn(P, r, place(lane), W.weight(l), total);
+}
+
+// The first of 256 bins in `hist` (in LDS) where the sum from bin 0 reaches
+// `want`: by the first wave, for all after the barrier.
+__device__ __forceinline__ void first_bin(u64 want, Space *sp) {
+    if (threadIdx.x < 64) {
+        u64 h[4], sum = 0;
+        for (int j = 0; j < 4; j++) sum += h[j] = sp->hist[4 * threadIdx.x + j];
+        u64 run = wave_scan(sum) - sum;
+        const bool mine = run < want && run + sum >= want, none = !__any(mine);
+        if (mine || (none && threadIdx.x == 63)) {
+            int j = 0;
+            for (; j < 3 && run + h[j] < want; j++) run += h[j];
+            sp->digit = 4 * threadIdx.x + j;
+        }
+    }
     __syncthreads();
-    return sp->thr;
+}
+
+// A logit's place among 256 equal steps from the largest, down to `lo` (halves,
+// so that the difference stays in range).
+struct Line {
+    float mx, scale;
+    __device__ __forceinline__ Line(float top, float lo) : mx(top) {
+        const float range = 0.5f * top - 0.5f * lo;
+        scale = range > 0.0f ? 255.0f / range : 0.0f;
+        if (!(scale < INFINITY)) scale = 3e38f;
+    }
+    __device__ __forceinline__ int operator()(unsigned k) const {
+        const float l = logit_of(k);
+        return l == mx ? 0 : (int)fminf((0.5f * mx - 0.5f * l) * scale, 255.0f);
+    }
+};
+
+// Four logits of a row from the i-th, -Inf past the last: 16 bytes a lane where
+// the row's start allows it.
+__device__ __forceinline__ f32x4 load_logits(const float *x, int i, int V, bool aligned) {
+    if (aligned && i + 4 <= V) return *glb(reinterpret_cast<const f32x4 *>(x + i));
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = i + e < V ? x[min(i + e, V - 1)] : -INFINITY;
+    return v;
 }
 
 constexpr int kRowVocab = 8192;  // with the lists, a block's 64 KB of LDS
 
 template <int NT>
 __global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P) {
-    constexpr int kList = 4 * NT < 2048 ? 4 * NT : 2048;  // candidates
+    constexpr int kList = 2048;  // candidates
     extern __shared__ unsigned keys[];
     __shared__ Space sp;
-    __shared__ unsigned tops[NT], list[kList];
-    __shared__ int place[kList];
+    __shared__ unsigned list[kList], sleast;
+    __shared__ unsigned short place[kList];
     const int r = blockIdx.x, tid = threadIdx.x, V = P.vocab;
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
-    if (tid == 0) sp.top = 0, sp.bad = 0, sp.token = V;
+    const bool aligned = ((uintptr_t)x & 15) == 0;
+    if (tid == 0) sp.top = 0, sp.bad = 0, sp.token = V, sleast = 0xffffffffu;
     fill_table(sp.tab);
+    for (int i = tid; i < 256; i += NT) sp.hist[i] = 0;
     __syncthreads();
-    unsigned top = 0;
+    unsigned top = 0, least = 0xffffffffu;
     bool bad = false;
-    for (int i = tid; i < V; i += NT) {
-        const float l = x[i];
-        bad |= l != l;
-        const unsigned k = key_of(l);
-        keys[i] = k;
-        top = max(top, k);
+    for (int i0 = 4 * tid; i0 < V; i0 += 8 * NT) {  // two loads in flight
+        f32x4 v[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) v[j] = load_logits(x, i0 + 4 * NT * j, V, aligned);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = i0 + 4 * NT * j + e;
+                bad |= v[j][e] != v[j][e];
+                const unsigned k = key_of(v[j][e]);
+                if (i < V) keys[i] = k;
+                top = max(top, k);
+                least = min(least, v[j][e] > -INFINITY ? k : 0xffffffffu);
+            }
     }
-    top = wave_top(top);
-    if ((tid & 63) == 0) atomicMax(&sp.top, top);
+    top = wave_top(top), least = ~wave_top(~least);
+    if ((tid & 63) == 0) atomicMax(&sp.top, top), atomicMin(&sleast, least);
     if (bad) atomicOr(&sp.bad, 1u);
     __syncthreads();
     top = sp.top;
@@ -381,24 +525,43 @@ __global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P) {
     const Weights W = weights_of(S, mx, sp.tab);
     const unsigned *set = keys;
     int n = V;
+    u64 need = 0;
     bool listed = false;
-    if (S.top_k > 0 && V > kBrute) {  // candidates, in the order of their indices
-        const int per = (V + NT - 1) / NT, lo = min(tid * per, V), hi = min(lo + per, V);
-        unsigned run = 0;
-        for (int i = lo; i < hi; i++) run = max(run, keys[i]);
-        const unsigned least = least_of_runs<NT>(run, S.top_k, tops, &sp);
+    if (S.top_k > 0 || S.cuts_sum()) {
+        // Candidates, in the order of their indices: by steps down from the
+        // largest, up to the one where top-k's count or top-p's sum is reached.
+        const bool by_sum = S.top_k == 0;
+        const float lo = logit_of(sleast), far = mx - 32.0f * S.t;  // 46 octaves: no weights past them
+        const Line line(mx, by_sum && far > lo ? far : lo);
+        u64 sum = 0;
+        for (int i = tid; i < V; i += NT) {
+            const unsigned k = keys[i];
+            const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
+            if (w) atomicAdd(&sp.hist[line(k)], w);
+            sum += w;
+        }
+        if (by_sum) need = S.share_of(block_total<NT>(sum, sp.wsum));
+        __syncthreads();
+        first_bin(by_sum ? need : (u64)S.top_k, &sp);
+        const int bin = (int)sp.digit;
+        const int per = (V + NT - 1) / NT, lo_i = min(tid * per, V), hi_i = min(lo_i + per, V);
         u64 count = 0, total;
-        for (int i = lo; i < hi; i++) count += keys[i] >= least;
+        for (int i = lo_i; i < hi_i; i++) count += line(keys[i]) <= bin;
         int at = (int)(block_scan<NT>(count, sp.wsum, &total) - count);
         if (total <= kList) {
-            for (int i = lo; i < hi; i++)
-                if (keys[i] >= least) list[at] = keys[i], place[at++] = i;
+            for (int i = lo_i; i < hi_i; i++)
+                if (line(keys[i]) <= bin) list[at] = keys[i], place[at++] = (unsigned short)i;
             set = list, n = (int)total, listed = true;
             __syncthreads();
+            if (n <= 64) {
+                if (tid < 64)
+                    finish_wave(P, r, tid < n ? list[tid] : 0, n, [&](int i) { return (int)place[i]; }, S, W, need);
+                return;
+            }
         }
     }
     auto key = [&](int j) { return set[j]; };
-    const Cut c = cut_of<NT>(key, n, S, W, 0, &sp);
+    const Cut c = cut_of<NT>(key, n, S, W, need, &sp);
     u64 total;
     const int i = draw_of<NT>(key, n, c, S, W, P.u[r], 0, ~0ull, &total, &sp);
     if (i >= 0) drawn(P, r, listed ? place[i] : i, W.weight(logit_of(set[i])), total);
@@ -408,7 +571,7 @@ __global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P) {
 // Rows of more than kRowVocab logits
 // ---------------------------------------------------------------------------
 constexpr int kChunk = 4096, kGroup = 64;         // logits of a block, of a maximum
-constexpr int kNear = 2048;                       // tokens next to a cut that are held
+constexpr int kNear = 8192;                       // tokens next to a cut that are held
 constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk, kMaxGroups = kSampleRowsMaxVocab / kGroup;
 
 // A row's scratch.
@@ -418,11 +581,13 @@ struct RowScratch {
     unsigned top[kMaxChunks];         // its largest key
     int token[kMaxChunks];            // where that is first
     unsigned bad[kMaxChunks];         // a NaN
-    unsigned near_at[kMaxChunks];     // its tokens in the cut's bin, in `near`
+    unsigned low[kMaxChunks];         // the least of its groups' maxima above -Inf
+    unsigned near_at[kMaxChunks];     // its candidates (of top-p: in the cut's bin), in `near`
     unsigned near_n[kMaxChunks];
     unsigned near_all;
-    unsigned pad;
+    float least;                      // top-k's candidates are no smaller; +Inf: a NaN in the row
     unsigned near[kNear];             // keys
+    int near_i[kNear];                // and indices
     unsigned group[kMaxGroups];       // the largest key of each kGroup
 };
 
@@ -444,31 +609,21 @@ __device__ RowTop row_top(const RowScratch *R, int chunks, Space *sp) {
     return {sp->top, sp->bad != 0};
 }
 
-// Logits lo + 4 i .. of a row into registers, -Inf past the last: 16 bytes a lane
-// where the row's start allows it.
-__device__ __forceinline__ f32x4 load_logits(const float *x, int i, int V, bool aligned) {
-    if (aligned && i + 4 <= V) return *glb(reinterpret_cast<const f32x4 *>(x + i));
-    f32x4 v;
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = i + e < V ? x[min(i + e, V - 1)] : -INFINITY;
-    return v;
-}
-
 __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScratch *scratch, int row0) {
-    __shared__ unsigned stop, sbad;
+    __shared__ unsigned stop, sbad, slow;
     __shared__ int stoken;
     const int r = row0 + blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x, V = P.vocab;
     RowScratch *R = scratch + blockIdx.y;
     const float *x = P.logits + (size_t)r * P.ld;
     const bool aligned = ((uintptr_t)x & 15) == 0;
-    if (tid == 0) stop = 0, sbad = 0, stoken = V;
+    if (tid == 0) stop = 0, sbad = 0, slow = 0xffffffffu, stoken = V;
     for (int i = chunk * 256 + tid; i < kBins; i += gridDim.x * 256) R->hist[i] = 0;
     if (chunk == 0 && tid == 0) R->near_all = 0;
     __syncthreads();
     f32x4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = load_logits(x, chunk * kChunk + 1024 * j + 4 * tid, V, aligned);
-    unsigned top = 0;
+    unsigned top = 0, low = 0xffffffffu;
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -480,11 +635,12 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
         }
         for (int off = 1; off < 16; off <<= 1) g = max(g, (unsigned)__shfl_xor((int)g, off, 64));
         top = max(top, g);
+        low = min(low, g > key_of(-INFINITY) ? g : 0xffffffffu);
         const int at = chunk * kChunk + 1024 * j + 4 * tid;
         if ((tid & 15) == 0 && at < V) R->group[at / kGroup] = g;
     }
-    top = wave_top(top);
-    if ((tid & 63) == 0) atomicMax(&stop, top);
+    top = wave_top(top), low = ~wave_top(~low);
+    if ((tid & 63) == 0) atomicMax(&stop, top), atomicMin(&slow, low);
     if (bad) sbad = 1;
     __syncthreads();
     top = stop;
@@ -496,11 +652,48 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
             if (key_of(v[j][e]) == top) first = chunk * kChunk + 1024 * j + 4 * tid + e;
     if (first < V) atomicMin(&stoken, first);
     __syncthreads();
-    if (tid == 0) R->top[chunk] = top, R->bad[chunk] = sbad, R->token[chunk] = stoken;
+    if (tid == 0) R->top[chunk] = top, R->bad[chunk] = sbad, R->low[chunk] = slow, R->token[chunk] = stoken;
 }
 
-// Rows that top-k does not cut: units by bin where top-p does, else the chunk's
-// sum.
+// What top-k's candidates are no smaller than: a value that top_k of the groups'
+// maxima reach, by 256 steps down from the largest; every finite logit where
+// there are not that many groups.  (-Inf is never drawn, so it is no candidate.)
+__device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int groups, Space *sp) {
+    constexpr int N = 16;  // loads in flight: a row of 262144 in one step, kept for both passes
+    const int tid = threadIdx.x;
+    unsigned g[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) g[j] = R->group[min(tid + j * 256, groups - 1)];
+    if (tid == 0) sp->thr = 0xffffffffu, sp->ties = 0xffffffffu;
+    sp->hist[tid] = 0;
+    const RowTop t = row_top(R, chunks, sp);
+    float least = t.bad ? INFINITY : -3.402823466e38f;
+    if (S.top_k < groups && !t.bad) {
+        if (tid < chunks) atomicMin(&sp->thr, R->low[tid]);
+        __syncthreads();
+        const Line line(logit_of(t.top), logit_of(sp->thr));
+        auto each = [&](auto take) {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (tid + j * 256 < groups) take(g[j]);
+            for (int i = tid + N * 256; i < groups; i += 256) take(R->group[i]);
+        };
+        each([&](unsigned k) { atomicAdd(&sp->hist[line(k)], (u64)1); });
+        __syncthreads();
+        first_bin((u64)S.top_k, sp);
+        const int bin = (int)sp->digit;
+        unsigned low = 0xffffffffu;
+        each([&](unsigned k) { low = min(low, line(k) <= bin ? k : 0xffffffffu); });
+        low = ~wave_top(~low);
+        if ((tid & 63) == 0) atomicMin(&sp->ties, low);
+        __syncthreads();
+        least = fmaxf(least, logit_of(sp->ties));
+    }
+    if (tid == 0) R->least = least;
+}
+
+// Rows that top-k cuts: where its candidates end.  Others: units by bin where
+// top-p cuts them, else the chunk's sum.
 __global__ __launch_bounds__(256) void k_sample_sum(SampleRowsParams P, RowScratch *scratch, int row0) {
     __shared__ Space sp;
     __shared__ u64 hist[kBins];
@@ -508,7 +701,8 @@ __global__ __launch_bounds__(256) void k_sample_sum(SampleRowsParams P, RowScrat
     RowScratch *R = scratch + blockIdx.y;
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
-    if (S.greedy || S.top_k > 0) return;
+    if (S.greedy || (S.top_k > 0 && chunk > 0)) return;
+    if (S.top_k > 0) return find_least(R, S, gridDim.x, (V + kGroup - 1) / kGroup, &sp);
     const bool sums = S.cuts_sum(), aligned = ((uintptr_t)x & 15) == 0;
     f32x4 v[4];
 #pragma unroll
@@ -564,36 +758,54 @@ __device__ BinCut bin_cut(const RowScratch *R, const RowSettings &S, Space *sp) 
     return {sp->token, sp->base, need};
 }
 
-// Rows that top-p alone cuts: each chunk's kept sum before the cut's bin, and its
-// tokens in it, in the order of their indices.
+// A chunk's candidates, in the order of their indices.  For rows that top-k cuts:
+// what may be among the first top_k, from the groups whose maximum may.  (By the
+// one block that ends the row that took 36 us at 152000 logits and top_k = 2000,
+// bound by its instructions; here, beside other rows, 13.)  For rows that top-p
+// alone cuts: what shares the cut's bin, and the kept sum before that.
 __global__ __launch_bounds__(256) void k_sample_near(SampleRowsParams P, RowScratch *scratch, int row0) {
     __shared__ Space sp;
     const int r = row0 + blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x, V = P.vocab;
     RowScratch *R = scratch + blockIdx.y;
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
-    if (S.greedy || S.top_k > 0 || !S.cuts_sum()) return;
+    const bool first = S.top_k > 0;
+    if (S.greedy || !(first || S.cuts_sum())) return;
+    const int i0 = chunk * kChunk + 16 * tid;
     const bool aligned = ((uintptr_t)x & 15) == 0;
+    const float least = first ? R->least : 0.0f;
     f32x4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = load_logits(x, chunk * kChunk + 16 * tid + 4 * j, V, aligned);
-    fill_table(sp.tab);
-    const RowTop t = row_top(R, gridDim.x, &sp);
-    const float mx = logit_of(t.top);
-    if (t.bad || mx == -INFINITY) return;
-    const Weights W = weights_of(S, mx, sp.tab);
-    const BinCut b = bin_cut<256>(R, S, &sp);
-    u64 sum = 0, near = 0, all;
+    for (int j = 0; j < 4; j++) v[j] = -INFINITY;
+    if (i0 < V && (!first || R->group[i0 / kGroup] >= key_of(least))) {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+        for (int j = 0; j < 4; j++) v[j] = load_logits(x, i0 + 4 * j, V, aligned);
+    }
+    unsigned in = 0;  // which of the 16
+    u64 sum = 0, all;
+    if (first) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int bin = W.bin(v[j][e]);
-            if (bin < b.bin) sum += W.units(v[j][e], S.least);
-            near += bin == b.bin && chunk * kChunk + 16 * tid + 4 * j + e < V;
-        }
-    sum = block_total<256>(sum, sp.wsum);
-    unsigned at = (unsigned)(block_scan<256>(near, sp.wsum, &all) - near);
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) in |= (unsigned)(v[j][e] >= least) << (4 * j + e);
+    } else {
+        fill_table(sp.tab);
+        const RowTop t = row_top(R, gridDim.x, &sp);
+        const float mx = logit_of(t.top);
+        if (t.bad || mx == -INFINITY) return;
+        const Weights W = weights_of(S, mx, sp.tab);
+        const BinCut b = bin_cut<256>(R, S, &sp);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int bin = W.bin(v[j][e]);
+                if (bin < b.bin) sum += W.units(v[j][e], S.least);
+                in |= (unsigned)(bin == b.bin && i0 + 4 * j + e < V) << (4 * j + e);
+            }
+        sum = block_total<256>(sum, sp.wsum);
+    }
+    unsigned at = (unsigned)(block_scan<256>((u64)__popc(in), sp.wsum, &all) - __popc(in));
     if (tid == 0) {
         R->sum[chunk] = sum;
         R->near_n[chunk] = (unsigned)all;
@@ -606,25 +818,22 @@ __global__ __launch_bounds__(256) void k_sample_near(SampleRowsParams P, RowScra
     for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (W.bin(v[j][e]) == b.bin && chunk * kChunk + 16 * tid + 4 * j + e < V) {
-                if (at < kNear) R->near[at] = key_of(v[j][e]);
+            if (in >> (4 * j + e) & 1) {
+                if (at < kNear) R->near[at] = key_of(v[j][e]), R->near_i[at] = i0 + 4 * j + e;
                 at++;
             }
 }
 
 // The row's end: top-k's candidates, or where the chunks' sums say the draw falls.
-constexpr int kDrawThreads = 1024, kDrawList = 8192;
-static_assert(kDrawList >= kMaxGroups && kDrawList >= kNear, "either lies in LDS");
+constexpr int kDrawThreads = 1024;
 
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P, RowScratch *scratch, int row0) {
     constexpr int NT = kDrawThreads;
     __shared__ Space sp;
-    __shared__ unsigned keys[kDrawList];
-    __shared__ int place[kDrawList];
-    __shared__ unsigned short list[kMaxGroups];
+    __shared__ unsigned keys[kNear];
+    __shared__ int place[kNear];
     __shared__ int offset[kMaxChunks], ties[kMaxChunks];
-    const int r = row0 + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = P.vocab;
-    const int chunks = (V + kChunk - 1) / kChunk, groups = (V + kGroup - 1) / kGroup;
+    const int r = row0 + blockIdx.x, tid = threadIdx.x, V = P.vocab, chunks = (V + kChunk - 1) / kChunk;
     RowScratch *R = scratch + blockIdx.x;
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
@@ -654,63 +863,40 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
         if (i >= 0) drawn(P, r, i, W.weight(x[i]), total);
     };
     u64 total;
-    if (S.top_k > 0) {
-        // Candidates: as large as the top_k-th largest of the groups' maxima, from
-        // the groups that have such (to within a few times top_k tokens; many
-        // equal logits, or top_k past a few thousand, take the whole row).
-        for (int i = tid; i < groups; i += NT) keys[i] = R->group[i];
+    // Candidates into LDS, in the order of their indices.
+    const unsigned mine = tid < chunks ? R->near_n[tid] : 0;
+    unsigned first = 0;
+    u64 held = 0;
+    if (S.top_k > 0 || S.cuts_sum()) {
+        first = (unsigned)(block_scan<NT>(mine, sp.wsum, &held) - mine);
+        if (held > kNear) return whole();  // many equal logits, or top_k past a few thousand
+        if (tid < chunks) offset[tid] = (int)first - (int)R->near_at[tid];
         __syncthreads();
-        unsigned least = 0;
-        if (S.top_k < groups) {
-            RowSettings count = S;
-            count.top_p = 1.0f;
-            least = cut_of<NT>(near_key, groups, count, W, 0, &sp).thr;
-        }
-        const int per = (groups + NT - 1) / NT, lo = min(tid * per, groups), hi = min(lo + per, groups);
-        u64 n = 0, all;
-        for (int i = lo; i < hi; i++) n += keys[i] >= least;
-        int at = (int)(block_scan<NT>(n, sp.wsum, &all) - n);
-        for (int i = lo; i < hi; i++)
-            if (keys[i] >= least) list[at++] = (unsigned short)i;
-        __syncthreads();
-        // a wave's run of those groups, four at a time: counted, then written in
-        // the order of their indices
-        const int run = ((int)all + NT / 64 - 1) / (NT / 64);
-        const int g0 = min(wave * run, (int)all), g1 = min(g0 + run, (int)all);
-        auto each = [&](auto take) {
-            for (int g = g0; g < g1; g += 4) {
-                unsigned k[4];
-                int i[4];
+        for (int j0 = tid; j0 < (int)held; j0 += 4 * NT) {
+            unsigned k[4];
+            int i[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    i[j] = list[min(g + j, g1 - 1)] * kGroup + lane;
-                    k[j] = key_of(x[min(i[j], V - 1)]);
+            for (int j = 0; j < 4; j++) {
+                const int at = min(j0 + j * NT, (int)held - 1);
+                k[j] = R->near[at], i[j] = R->near_i[at];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j0 + j * NT < (int)held) {
+                    const int at = j0 + j * NT + offset[i[j] / kChunk];
+                    keys[at] = k[j], place[at] = i[j];
                 }
-#pragma unroll
-                for (int j = 0; j < 4; j++) take(i[j], k[j], g + j < g1 && i[j] < V && k[j] >= least);
-            }
-        };
-        u64 mine = 0;
-        each([&](int, unsigned, bool in) { mine += __popcll(__ballot(in)); });
-        if (lane == 0) sp.wsum[wave] = mine;
-        __syncthreads();
-        int to = 0, have = 0;
-        for (int w = 0; w < NT / 64; w++) {
-            if (w < wave) to += (int)sp.wsum[w];
-            have += (int)sp.wsum[w];
         }
-        if (have > kDrawList) return whole();
-        each([&](int i, unsigned k, bool in) {
-            const u64 who = __ballot(in);
-            if (in) {
-                const int p = to + __popcll(who & ((1ull << lane) - 1));
-                keys[p] = k, place[p] = i;
-            }
-            to += __popcll(who);
-        });
         __syncthreads();
-        const Cut c = cut_of<NT>(near_key, have, S, W, 0, &sp);
-        const int i = draw_of<NT>(near_key, have, c, S, W, u, 0, ~0ull, &total, &sp);
+    }
+    if (S.top_k > 0) {
+        const int n = (int)held;
+        if (n <= 64) {
+            if (tid < 64) finish_wave(P, r, tid < n ? keys[tid] : 0, n, [&](int i) { return place[i]; }, S, W, 0);
+            return;
+        }
+        const Cut c = cut_of<NT>(near_key, n, S, W, 0, &sp);
+        const int i = draw_of<NT>(near_key, n, c, S, W, u, 0, ~0ull, &total, &sp);
         if (i >= 0) drawn(P, r, place[i], W.weight(logit_of(keys[i])), total);
         return;
     }
@@ -718,27 +904,26 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
     u64 part = tid < chunks ? R->sum[tid] : 0;
     if (S.cuts_sum()) {
         const BinCut b = bin_cut<NT>(R, S, &sp);
-        const unsigned mine = tid < chunks ? R->near_n[tid] : 0;
-        u64 all;
-        const int first = (int)(block_scan<NT>(mine, sp.wsum, &all) - mine);
-        if (all > kNear) return whole();  // many equal or nearly equal logits
-        if (tid < chunks) offset[tid] = first;
-        __syncthreads();
-        for (int k = wave; k < chunks; k += NT / 64) {
-            const int n = (int)R->near_n[k], from = (int)R->near_at[k];
-            for (int j = lane; j < n; j += 64) keys[offset[k] + j] = R->near[from + j];
+        c = cut_of<NT>(near_key, (int)held, S, W, b.need - b.above, &sp);
+        // each chunk's ties before it and kept sum
+        static_assert(kMaxChunks <= 256, "sums in the histogram");
+        for (int i = tid; i < 256; i += NT) sp.hist[i] = 0;
+        if (tid < chunks) ties[tid] = 0;
+        const int per = ((int)held + NT - 1) / NT, lo = min(tid * per, (int)held), hi = min(lo + per, (int)held);
+        u64 count = 0, all;
+        for (int i = lo; i < hi; i++) count += keys[i] == c.thr;
+        u64 seen = block_scan<NT>(count, sp.wsum, &all) - count;  // with the barrier
+        for (int i = lo; i < hi; i++) {
+            const unsigned k = keys[i];
+            const int at = place[i] / kChunk;
+            if (k == c.thr) atomicAdd(&ties[at], 1);
+            if (k > c.thr || (k == c.thr && seen++ < c.ties)) atomicAdd(&sp.hist[at], W.units(logit_of(k), S.least));
         }
         __syncthreads();
-        c = cut_of<NT>(near_key, (int)all, S, W, b.need - b.above, &sp);
-        // each chunk's ties and kept sum
-        u64 count = 0, before;
-        for (unsigned j = 0; j < mine; j++) count += keys[first + j] == c.thr;
-        before = block_scan<NT>(count, sp.wsum, &all) - count;
-        if (tid < chunks) ties[tid] = (int)before;
-        for (unsigned j = 0; j < mine; j++) {
-            const unsigned k = keys[first + j];
-            if (k > c.thr || (k == c.thr && before++ < c.ties)) part += W.units(logit_of(k), S.least);
-        }
+        if (tid < chunks) part += sp.hist[tid], count = (u64)ties[tid];
+        else count = 0;
+        const u64 upto = block_scan<NT>(count, sp.wsum, &all);
+        if (tid < chunks) ties[tid] = (int)(upto - count);
     } else if (tid < chunks) {
         ties[tid] = 0;
     }
@@ -758,7 +943,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
 void launch_sample_rows(hipStream_t st, const SampleRowsParams &p) {
     if (p.vocab <= kRowVocab) {
         const unsigned lds = (unsigned)p.vocab * 4;
-        if (p.vocab <= 4096) hipLaunchKernelGGL(k_sample_row<256>, dim3((unsigned)p.rows), dim3(256), lds, st, p);
+        if (p.vocab <= 1024) hipLaunchKernelGGL(k_sample_row<256>, dim3((unsigned)p.rows), dim3(256), lds, st, p);
         else hipLaunchKernelGGL(k_sample_row<1024>, dim3((unsigned)p.rows), dim3(1024), lds, st, p);
         return;
     }
@@ -769,7 +954,7 @@ void launch_sample_rows(hipStream_t st, const SampleRowsParams &p) {
         const unsigned n = (unsigned)std::min(most, p.rows - row0);
         hipLaunchKernelGGL(k_sample_max, dim3(chunks, n), dim3(256), 0, st, p, scratch, row0);
         hipLaunchKernelGGL(k_sample_sum, dim3(chunks, n), dim3(256), 0, st, p, scratch, row0);
-        if (p.p.top_p) hipLaunchKernelGGL(k_sample_near, dim3(chunks, n), dim3(256), 0, st, p, scratch, row0);
+        if (p.p.top_p || p.p.top_k) hipLaunchKernelGGL(k_sample_near, dim3(chunks, n), dim3(256), 0, st, p, scratch, row0);
         hipLaunchKernelGGL(k_sample_draw, dim3(n), dim3(kDrawThreads), 0, st, p, scratch, row0);
     }
 }

@@ -212,3 +212,47 @@ def test_refusals(ctx):
         ctx.sample_rows_device(x.data_ptr(), 8, 2, 8, 0, x.data_ptr())
     assert e.value.status == qtts.QTTS_EINVAL
     ctx.sample_rows_device(0, 8, 0, 8, 0, 0)
+
+
+@pytest.mark.parametrize("vocab", [8193, 70003])
+def test_more_rows_than_the_scratch_holds(ctx, vocab):
+    """Long rows share the context's scratch in turns: in each the draws that the
+    same rows have among few."""
+    x = np.tile(rows_like_a_model(31, 20, vocab), (20, 1))
+    s, u = settings(32, 400), np.random.default_rng(33).random(400)
+    token, share = draw(ctx, x, u, **s)
+    for lo in range(0, 400, 50):
+        t, p = draw(ctx, x[lo:lo + 50], u[lo:lo + 50], **{n: a[lo:lo + 50] for n, a in s.items()})
+        assert np.array_equal(t, token[lo:lo + 50]) and np.array_equal(p, share[lo:lo + 50])
+    check(ctx, x[::23], u[::23], **{n: a[::23] for n, a in s.items()})
+
+
+@pytest.mark.parametrize("k", [64, 65, 257, 1999, 6000, 8300, 20000])
+@pytest.mark.parametrize("vocab", [8200, 33000, 151936])
+def test_many_candidates(ctx, k, vocab):
+    """Few to more than are held between the kernels; with and without top-p after
+    top-k, rows that do not begin on 16 bytes."""
+    rows = 6
+    r = np.random.default_rng(k)
+    x = r.standard_normal((rows, vocab)).astype(np.float32)
+    x[1] *= 6
+    x[2, :vocab // 2] = -np.inf
+    x[3, 100:4000] += 3  # most of them in one chunk
+    x[4] = np.round(x[4] * 64) / 64
+    p = [1.0, 0.9, 0.7, 0.95, 1.0, 0.3]
+    check(ctx, x, r.random(rows), [0.7, 1.0, 1.3, 0.9, 2.0, 1.0], [k] * rows, p, [0.0, 0.0, 1e-3, 0.0, 0.01, 0.0], ld=vocab + 3)
+
+
+@pytest.mark.parametrize("vocab", [8200, 33000, 151936])
+def test_many_tokens_at_the_cut(ctx, vocab):
+    """top-p alone, with from few to all of a row's tokens in one narrow step of
+    weight, in one chunk or in all of them."""
+    r = np.random.default_rng(vocab)
+    x = np.full((5, vocab), -20.0, np.float32)
+    for i, n in enumerate((300, 3000, 7000)):
+        at = r.choice(min(vocab, 9000 if i % 2 else vocab), n, replace=False)
+        x[i, at] = 1 + 1e-3 * r.standard_normal(n)
+    x[3] = 1e-4 * r.standard_normal(vocab)
+    x[4, 4096:8192] = 2 + 1e-4 * r.standard_normal(4096)
+    for p in (0.9, 0.31):
+        check(ctx, x, r.random(5), [1.0] * 5, None, [p] * 5, [0.0, 0.5, 0.0, 0.0, 0.9])
