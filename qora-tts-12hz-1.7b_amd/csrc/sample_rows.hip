@@ -158,227 +158,251 @@ __device__ __forceinline__ Weights weights_of(const RowSettings &S, float mx, co
     return {mx, 64 * 1.44269504088896340736 / (double)S.t, tab};
 }
 
-// What is kept of a set: keys above `thr`, and the first `ties` at it.
-struct Cut {
-    unsigned thr = 0;
-    u64 ties = ~0ull;
-};
+// The order of a row's tokens: larger logits first, equal ones by index.  What
+// top-k and top-p keep is all from some order on, the cut.
+__device__ __forceinline__ u64 order_of(unsigned key, int i) { return (u64)key << 32 | (unsigned)~i; }
+__device__ __forceinline__ unsigned key_in(u64 order) { return (unsigned)(order >> 32); }
+__device__ __forceinline__ int index_in(u64 order) { return (int)~(unsigned)order; }
 
 constexpr int kBrute = 256;  // a set this small is ranked by comparing all pairs
 
 struct Space {
     double tab[64];
-    u64 hist[256], wsum[16], base;
-    unsigned near[kBrute];
-    unsigned digit, thr, ties, top, bad;
+    u64 hist[256], wsum[16], near[kBrute], units[kBrute], base, cut;
+    unsigned rank[kBrute], digit, count, thr, top, bad;
     int token;
 };
 
-// The prefix of n <= kBrute keys, near(i) in the order of their indices, of which
-// the first `count` stay (0: all) and then, where `by_sum`, those whose
-// predecessors' sum and `above` is below `need` (0: top-p's share of the sum).
-// NT / kBrute threads a key, or one, compare it with the others.
-template <int NT, class Key>
-__device__ Cut rank_all(const Key &near, int n, u64 count, bool by_sum, u64 above, u64 need, const RowSettings &S,
-                        const Weights &W, Space *sp) {
-    constexpr int PARTS = NT / kBrute;
-    static_assert(PARTS == 1 || PARTS == 4, "quads of lanes");
-    u64 *units = sp->hist;
-    const int i = threadIdx.x / PARTS, part = threadIdx.x % PARTS;
+__device__ __forceinline__ u64 readlane64(u64 v, int j) {
+    return (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, j) |
+           (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), j) << 32;
+}
+
+// The cut of the n <= kBrute orders in sp->near (as they come), of which the first
+// `count` stay (0: all) and then, where `by_sum`, those whose predecessors' sum and
+// `above` is below `need` (0: top-p's share of the sum).  A lane holds every 64th
+// of them and a wave compares all with its share, which it has in scalar
+// registers: two instructions a pair, six with the sum (2.3 us for 206; with each
+// pair read from LDS by threads of their own it took 6.3).
+template <int NT>
+__device__ u64 rank_near(int n, u64 count, bool by_sum, u64 above, u64 need, const RowSettings &S, const Weights &W,
+                         Space *sp) {
+    constexpr int J = kBrute / (NT / 64), A = kBrute / 64;
+    const int tid = threadIdx.x, lane = tid & 63, j0 = __builtin_amdgcn_readfirstlane(tid >> 6) * J;
+    u64 *ahead = sp->hist;
     __syncthreads();
-    if (threadIdx.x == 0) sp->thr = 0xffffffffu, sp->ties = 0;
-    const bool in = i < n;
-    const unsigned k = in ? near(i) : 0;
-    const u64 mine = in && by_sum ? W.units(logit_of(k)) : 0;
-    if (in && part == 0) units[i] = mine;
+    u64 mine = 0;
+    if (tid < n) {
+        sp->rank[tid] = 0, ahead[tid] = 0;
+        if (by_sum) mine = W.units(logit_of(key_in(sp->near[tid])));
+        sp->units[tid] = mine;
+    }
+    if (tid == 0) sp->cut = ~0ull;
     __syncthreads();
-    unsigned rank = 0;
-    u64 ahead = 0;
-    if (in) {
-#pragma unroll 4
-        for (int j = part; j < n; j += PARTS) {
-            const unsigned o = near(j);
-            const bool before = o > k || (o == k && j < i);
-            rank += before;
-            ahead += before ? units[j] : 0;
-        }
+    u64 order[A], sum[A];
+    unsigned rank[A];
+#pragma unroll
+    for (int a = 0; a < A; a++) {
+        order[a] = 64 * a + lane < n ? sp->near[64 * a + lane] : ~0ull;
+        sum[a] = 0, rank[a] = 0;
     }
-    for (int off = 1; off < PARTS; off <<= 1) {
-        rank += __shfl_xor((int)rank, off, 64);
-        ahead += (u64)__shfl_xor((long long)ahead, off, 64);
-    }
-    bool keep = in && (count == 0 || rank < count);
+    const u64 share = sp->near[min(j0 + lane, kBrute - 1)], weigh = sp->units[min(j0 + lane, kBrute - 1)];
+    const int jn = min(J, n - j0);
     if (by_sum) {
-        if (need == 0) need = S.share_of(block_total<NT>(keep && part == 0 ? mine : 0, sp->wsum));
-        keep = keep && above + ahead < need;
-    }
-    if (keep) atomicMin(&sp->thr, k);
-    __syncthreads();
-    Cut c;
-    c.thr = sp->thr;
-    if (keep && part == 0 && k == c.thr) atomicAdd(&sp->ties, 1u);
-    __syncthreads();
-    c.ties = sp->ties;
-    return c;
-}
-
-// The prefix that top-k and top-p keep of n keys, key(i) in the order of their
-// indices; `need`: the sum that top-p's prefix reaches, 0: its share of the sum.
-// Small sets at once.  Others by the logit's place on a line of 2^16 steps from
-// the largest down, 8 bits at a time, counts first and then sums, until what
-// shares the cut's step is a small set (many equal ones: by the key's digits).
-template <int NT, class Key>
-__device__ Cut cut_of(const Key &key, int n, const RowSettings &S, const Weights &W, u64 need, Space *sp) {
-    const int tid = threadIdx.x;
-    const bool sums = S.cuts_sum();
-    Cut c;
-    if (S.top_k == 0 && !sums) return c;
-    if (n <= kBrute) return rank_all<NT>(key, n, S.top_k, sums, 0, need, S, W, sp);
-    // the least finite logit, and the line's scale
-    unsigned least = 0xffffffffu;
-    for (int i = tid; i < n; i += NT) {
-        const unsigned k = key(i);
-        least = min(least, k > key_of(-INFINITY) ? k : 0xffffffffu);
-    }
-    for (int off = 32; off > 0; off >>= 1) least = min(least, (unsigned)__shfl_xor((int)least, off, 64));
-    __syncthreads();
-    if (tid == 0) sp->thr = 0xffffffffu;
-    __syncthreads();
-    if ((tid & 63) == 0) atomicMin(&sp->thr, least);
-    __syncthreads();
-    const float lo = logit_of(sp->thr);
-    __syncthreads();
-    float scale = 0;
-    auto line = [&](unsigned k) {  // halves, so that the difference stays in range
-        const float l = logit_of(k);
-        return l == W.mx ? 0 : (int)fminf((0.5f * W.mx - 0.5f * l) * scale, 65535.0f);
-    };
-    auto scan_digits = [&](bool down, u64 want, u64 base) {  // by the first wave: where the sum reaches `want`
-        if (tid < 64) {
-            u64 h[4], sum = 0;
-            for (int j = 0; j < 4; j++) sum += h[j] = sp->hist[down ? 255 - 4 * tid - j : 4 * tid + j];
-            u64 run = base + wave_scan(sum) - sum;
-            const bool mine = run < want && run + sum >= want, none = !__any(mine);
-            if (mine || (none && tid == 63)) {
-                int j = 0;
-                for (; j < 3 && run + h[j] < want; j++) run += h[j];
-                sp->digit = down ? 255 - 4 * tid - j : 4 * tid + j;
-                sp->base = run;
+        for (int j = 0; j < jn; j++) {
+            const u64 o = readlane64(share, j), w = readlane64(weigh, j);
+#pragma unroll
+            for (int a = 0; a < A; a++) {
+                const bool before = o > order[a];
+                rank[a] += before;
+                sum[a] += before ? w : 0;
             }
         }
-        __syncthreads();
-    };
-    auto select = [&](bool by_sum, u64 want) {
-        const float range = 0.5f * W.mx - 0.5f * lo;
-        const float far = by_sum ? 16.0f * S.t : INFINITY;  // half of 46 octaves: no weights past them
-        const float span = range < far ? range : far;
-        scale = span > 0.0f ? 65535.0f / span : 0.0f;
+    } else {
+        for (int j = 0; j < jn; j++) {
+            const u64 o = readlane64(share, j);
+#pragma unroll
+            for (int a = 0; a < A; a++) rank[a] += o > order[a];
+        }
+    }
+    if (jn > 0) {
+#pragma unroll
+        for (int a = 0; a < A; a++)
+            if (64 * a + lane < n) {
+                atomicAdd(&sp->rank[64 * a + lane], rank[a]);
+                if (by_sum) atomicAdd(&ahead[64 * a + lane], sum[a]);
+            }
+    }
+    __syncthreads();
+    bool keep = tid < n && (count == 0 || sp->rank[tid] < count);
+    const u64 before = tid < n ? above + ahead[tid] : 0;
+    if (by_sum) {
+        if (need == 0) need = S.share_of(block_total<NT>(keep ? mine : 0, sp->wsum));
+        keep = keep && before < need;
+    }
+    if (keep) atomicMin(&sp->cut, sp->near[tid]);
+    __syncthreads();
+    return sp->cut;
+}
+
+// A logit's place among 2^16 equal steps from `hi` down to `lo` (halves, so that
+// the difference stays in range; what lies outside goes to the ends).
+struct Line {
+    float hi, scale;
+    __device__ __forceinline__ Line(float from, float to) : hi(from) {
+        const float range = 0.5f * from - 0.5f * to;
+        scale = range > 0.0f ? 65535.0f / range : 0.0f;
         if (!(scale < INFINITY)) scale = 3e38f;
-        u64 base = 0;
-        int at = 0;  // the chosen steps' first digits
-        for (int round = 0; round < 2; round++) {
-            for (int i = tid; i < 256; i += NT) sp->hist[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += NT) {
-                const unsigned k = key(i);
-                if (k < c.thr) continue;
-                const int p = line(k);
-                if (round == 1 && p >> 8 != at) continue;
-                const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
-                if (w) atomicAdd(&sp->hist[round == 0 ? p >> 8 : p & 255], w);
-            }
-            __syncthreads();
-            scan_digits(false, want, base);
-            at = at << 8 | (int)sp->digit;
-            base = sp->base;
-            // what shares them, in order, if that is few
-            const int shift = round == 0 ? 8 : 0;
-            const int per = (n + NT - 1) / NT, lo_i = min(tid * per, n), hi_i = min(lo_i + per, n);
-            u64 have = 0, all;
-            for (int i = lo_i; i < hi_i; i++) {
-                const unsigned k = key(i);
-                have += k >= c.thr && line(k) >> shift == at;
-            }
-            int to = (int)(block_scan<NT>(have, sp->wsum, &all) - have);
-            if (all <= kBrute) {
-                for (int i = lo_i; i < hi_i; i++) {
-                    const unsigned k = key(i);
-                    if (k >= c.thr && line(k) >> shift == at) sp->near[to++] = k;
-                }
-                auto near = [&](int i) { return sp->near[i]; };
-                return by_sum ? rank_all<NT>(near, (int)all, 0, true, base, want, S, W, sp)
-                              : rank_all<NT>(near, (int)all, want - base, false, 0, 0, S, W, sp);
-            }
-        }
-        unsigned prefix = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            for (int i = tid; i < 256; i += NT) sp->hist[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += NT) {
-                const unsigned k = key(i);
-                if (k < c.thr || line(k) != at || (shift < 24 && k >> (shift + 8) != prefix)) continue;
-                const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
-                if (w) atomicAdd(&sp->hist[(k >> shift) & 255], w);
-            }
-            __syncthreads();
-            scan_digits(true, want, base);
-            prefix = prefix << 8 | sp->digit;
-            base = sp->base;
-        }
-        __syncthreads();
-        const u64 w = by_sum ? W.units(logit_of(prefix)) : (u64)1;
-        Cut d;
-        d.thr = prefix;
-        d.ties = w ? (want - base + w - 1) / w : ~0ull;
-        return d;
-    };
-    if (S.top_k > 0) c = select(false, (u64)S.top_k);
-    if (sums) {
-        if (need == 0) {  // of those above thr, and `ties` at it
-            u64 sum = 0;
-            for (int i = tid; i < n; i += NT) {
-                const unsigned k = key(i);
-                if (k > c.thr) sum += W.units(logit_of(k));
-            }
-            sum = block_total<NT>(sum, sp->wsum);
-            need = S.share_of(sum + (c.thr ? c.ties * W.units(logit_of(c.thr)) : 0));
-        }
-        __syncthreads();
-        const Cut d = select(true, need);
-        if (d.thr > c.thr) c = d;
-        else c.ties = d.ties < c.ties ? d.ties : c.ties;
     }
-    return c;
+    __device__ __forceinline__ int operator()(unsigned k) const {
+        const float l = logit_of(k);
+        return l >= hi ? 0 : (int)fminf((0.5f * hi - 0.5f * l) * scale, 65535.0f);
+    }
+};
+
+// Where the sums of 256 bins, on top of `base`, reach `want` (the last where they
+// don't): sp->digit, and sp->base the sum before it.  By the first wave, for all
+// after the barrier.
+__device__ __forceinline__ void find_bin(bool down, u64 want, u64 base, Space *sp) {
+    const int tid = threadIdx.x;
+    if (tid < 64) {
+        u64 h[4], sum = 0;
+        for (int j = 0; j < 4; j++) sum += h[j] = sp->hist[down ? 255 - 4 * tid - j : 4 * tid + j];
+        u64 run = base + wave_scan(sum) - sum;
+        const bool mine = run < want && run + sum >= want, none = !__any(mine);
+        if (mine || (none && tid == 63)) {
+            int j = 0;
+            for (; j < 3 && run + h[j] < want; j++) run += h[j];
+            sp->digit = down ? 255 - 4 * tid - j : 4 * tid + j;
+            sp->base = run;
+        }
+    }
+    __syncthreads();
 }
 
-// The draw among n tokens in the order of their indices, keys through key(i):
-// which one it falls on and the sum it fell in, or -1 in the threads that do not
-// find it.  A thread takes a run of consecutive ones.  `tied`: ties before the
-// first; `target` ~0: uniform u's place in the sum, else this one.
+// The order, from `cut` on, at which the count or the sum of n keys reaches
+// `want`: by the keys' places on a line, 8 bits at a time, until what shares the
+// step is a small set (many equal ones: by the keys' digits, then by index).
+// `found`: the first 8 bits are in sp->digit, the sum before them in sp->base.
 template <int NT, class Key>
-__device__ int draw_of(const Key &key, int n, const Cut &c, const RowSettings &S, const Weights &W, float u, u64 tied,
+__device__ u64 select(const Key &key, int n, const Line &line, u64 cut, bool by_sum, u64 want, bool found,
+                      const RowSettings &S, const Weights &W, Space *sp) {
+    const int tid = threadIdx.x;
+    u64 base = 0;
+    int at = 0;  // the chosen step's first bits
+    for (int shift = 8; shift >= 0; shift -= 8) {
+        if (!found) {
+            __syncthreads();
+            for (int i = tid; i < 256; i += NT) sp->hist[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += NT) {
+                const unsigned k = key(i);
+                if (order_of(k, i) < cut) continue;
+                const int p = line(k);
+                if (shift == 0 && p >> 8 != at) continue;
+                const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
+                if (w) atomicAdd(&sp->hist[p >> shift & 255], w);
+            }
+            __syncthreads();
+            find_bin(false, want, base, sp);
+        }
+        found = false;
+        at = at << 8 | (int)sp->digit;
+        base = sp->base;
+        if (tid == 0) sp->count = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+            const unsigned k = key(i);
+            if (order_of(k, i) < cut || line(k) >> shift != at) continue;
+            const unsigned to = atomicAdd(&sp->count, 1u);
+            if (to < kBrute) sp->near[to] = order_of(k, i);
+        }
+        __syncthreads();
+        const int all = (int)sp->count;
+        if (all <= kBrute)
+            return by_sum ? rank_near<NT>(all, 0, true, base, want, S, W, sp)
+                          : rank_near<NT>(all, want - base, false, 0, 0, S, W, sp);
+    }
+    unsigned prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        for (int i = tid; i < 256; i += NT) sp->hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+            const unsigned k = key(i);
+            if (order_of(k, i) < cut || line(k) != at || (shift < 24 && k >> (shift + 8) != prefix)) continue;
+            const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
+            if (w) atomicAdd(&sp->hist[k >> shift & 255], w);
+        }
+        __syncthreads();
+        find_bin(true, want, base, sp);
+        prefix = prefix << 8 | sp->digit;
+        base = sp->base;
+    }
+    const u64 w = by_sum ? W.units(logit_of(prefix)) : (u64)1;
+    if (w == 0) return order_of(prefix, 0x7fffffff);
+    const u64 nth = (want - base + w - 1) / w;  // of those equal to it the last that stays
+    const int per = (n + NT - 1) / NT, lo = min(tid * per, n), hi = min(lo + per, n);
+    u64 count = 0, all;
+    for (int i = lo; i < hi; i++) count += key(i) == prefix;
+    u64 seen = block_scan<NT>(count, sp->wsum, &all) - count;
+    if (tid == 0) sp->token = 0x7fffffff;
+    __syncthreads();
+    if (seen < nth && seen + count >= nth)
+        for (int i = lo; i < hi; i++)
+            if (key(i) == prefix && ++seen == nth) sp->token = i;
+    __syncthreads();
+    return order_of(prefix, sp->token);
+}
+
+// The cut that top-k and top-p make in n keys, key(i) in the order of their
+// indices, which lie between lo and hi for the most part (0: none); `need`: the sum
+// that top-p's prefix reaches, 0: its share of the sum.  `found`: as for select,
+// by line's first 8 bits, for the first that cuts.
+template <int NT, class Key>
+__device__ u64 cut_of(const Key &key, int n, const Line &line, bool found, const RowSettings &S, const Weights &W,
+                      u64 need, Space *sp) {
+    const int tid = threadIdx.x;
+    const bool counts = S.top_k > 0 && S.top_k < n, sums = S.cuts_sum();
+    u64 cut = 0;
+    if (!counts && !sums) return cut;
+    if (n <= kBrute && !found) {
+        __syncthreads();
+        if (tid < n) sp->near[tid] = order_of(key(tid), tid);
+        return rank_near<NT>(n, counts ? S.top_k : 0, sums, 0, need, S, W, sp);
+    }
+    if (counts) cut = select<NT>(key, n, line, cut, false, (u64)S.top_k, found, S, W, sp);
+    if (!sums) return cut;
+    if (need == 0) {
+        u64 sum = 0;
+        for (int i = tid; i < n; i += NT) {
+            const unsigned k = key(i);
+            if (order_of(k, i) >= cut) sum += W.units(logit_of(k));
+        }
+        need = S.share_of(block_total<NT>(sum, sp->wsum));
+    }
+    const u64 least = select<NT>(key, n, line, cut, true, need, found && !counts, S, W, sp);
+    return least > cut ? least : cut;
+}
+
+// The draw among n tokens in the order of their indices, keys through key(i), the
+// first at `first` in the cut's terms: which one it falls on, or -1 in the threads
+// that do not find it.  A thread takes a run of consecutive ones.  `target` ~0:
+// uniform u's place in the sum, else this one.
+template <int NT, class Key>
+__device__ int draw_of(const Key &key, int first, int n, u64 cut, const RowSettings &S, const Weights &W, float u,
                        u64 target, u64 *total, Space *sp) {
     const int per = (n + NT - 1) / NT, lo = min((int)threadIdx.x * per, n), hi = min(lo + per, n);
-    u64 before = 0, all;
-    if (c.ties != ~0ull) {
-        u64 count = 0;
-        for (int i = lo; i < hi; i++) count += key(i) == c.thr;
-        before = tied + block_scan<NT>(count, sp->wsum, &all) - count;
-    }
-    u64 seen = before;
     auto kept = [&](int i) {
         const unsigned k = key(i);
-        if (k < c.thr || (k == c.thr && seen++ >= c.ties)) return (u64)0;
-        return W.units(logit_of(k), S.least);
+        return order_of(k, first + i) >= cut ? W.units(logit_of(k), S.least) : (u64)0;
     };
-    u64 sum = 0;
+    u64 sum = 0, all;
     for (int i = lo; i < hi; i++) sum += kept(i);
     const u64 upto = block_scan<NT>(sum, sp->wsum, &all);
     if (target == ~0ull) *total = all, target = S.target_of(u, all);
     if (target < upto - sum || target >= upto) return -1;
     u64 run = upto - sum;
-    seen = before;
     for (int i = lo; i < hi; i++) {
         run += kept(i);
         if (run > target) return i;
@@ -408,8 +432,7 @@ __device__ void finish_wave(const SampleRowsParams &P, int r, unsigned k, int n,
     u64 ahead = 0;
     for (int j = 0; j < n; j++) {
         const unsigned o = (unsigned)__builtin_amdgcn_readlane((int)k, j);
-        const u64 w = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)mine, j) |
-                      (u64)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32;
+        const u64 w = readlane64(mine, j);
         const bool before = o > k || (o == k && j < lane);
         rank += before;
         ahead += before ? w : 0;
@@ -425,38 +448,6 @@ __device__ void finish_wave(const SampleRowsParams &P, int r, unsigned k, int n,
     if (target >= upto - kept && target < upto) drawn(P, r, place(lane), W.weight(l), total);
 }
 
-// The first of 256 bins in `hist` (in LDS) where the sum from bin 0 reaches
-// `want`: by the first wave, for all after the barrier.
-__device__ __forceinline__ void first_bin(u64 want, Space *sp) {
-    if (threadIdx.x < 64) {
-        u64 h[4], sum = 0;
-        for (int j = 0; j < 4; j++) sum += h[j] = sp->hist[4 * threadIdx.x + j];
-        u64 run = wave_scan(sum) - sum;
-        const bool mine = run < want && run + sum >= want, none = !__any(mine);
-        if (mine || (none && threadIdx.x == 63)) {
-            int j = 0;
-            for (; j < 3 && run + h[j] < want; j++) run += h[j];
-            sp->digit = 4 * threadIdx.x + j;
-        }
-    }
-    __syncthreads();
-}
-
-// A logit's place among 256 equal steps from the largest, down to `lo` (halves,
-// so that the difference stays in range).
-struct Line {
-    float mx, scale;
-    __device__ __forceinline__ Line(float top, float lo) : mx(top) {
-        const float range = 0.5f * top - 0.5f * lo;
-        scale = range > 0.0f ? 255.0f / range : 0.0f;
-        if (!(scale < INFINITY)) scale = 3e38f;
-    }
-    __device__ __forceinline__ int operator()(unsigned k) const {
-        const float l = logit_of(k);
-        return l == mx ? 0 : (int)fminf((0.5f * mx - 0.5f * l) * scale, 255.0f);
-    }
-};
-
 // Four logits of a row from the i-th, -Inf past the last: 16 bytes a lane where
 // the row's start allows it.
 __device__ __forceinline__ f32x4 load_logits(const float *x, int i, int V, bool aligned) {
@@ -471,11 +462,10 @@ constexpr int kRowVocab = 8192;  // with the lists, a block's 64 KB of LDS
 
 template <int NT>
 __global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P) {
-    constexpr int kList = 2048;  // candidates
     extern __shared__ unsigned keys[];
     __shared__ Space sp;
-    __shared__ unsigned list[kList], sleast;
-    __shared__ unsigned short place[kList];
+    __shared__ unsigned sleast;
+    __shared__ int place[64];
     const int r = blockIdx.x, tid = threadIdx.x, V = P.vocab;
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
@@ -523,48 +513,41 @@ __global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P) {
         return;
     }
     const Weights W = weights_of(S, mx, sp.tab);
-    const unsigned *set = keys;
-    int n = V;
-    u64 need = 0;
-    bool listed = false;
+    auto key = [&](int j) { return keys[j]; };
+    const float lo = logit_of(sleast), far = mx - 32.0f * S.t;  // 46 octaves: no weights past them
+    const Line line(mx, S.top_k == 0 && far > lo ? far : lo);
+    u64 need = 0, total;
     if (S.top_k > 0 || S.cuts_sum()) {
-        // Candidates, in the order of their indices: by steps down from the
-        // largest, up to the one where top-k's count or top-p's sum is reached.
+        // Steps down from the largest to the one where top-k's count or top-p's
+        // sum is reached; a wave's worth of tokens ends here.
         const bool by_sum = S.top_k == 0;
-        const float lo = logit_of(sleast), far = mx - 32.0f * S.t;  // 46 octaves: no weights past them
-        const Line line(mx, by_sum && far > lo ? far : lo);
         u64 sum = 0;
         for (int i = tid; i < V; i += NT) {
             const unsigned k = keys[i];
             const u64 w = by_sum ? W.units(logit_of(k)) : (u64)1;
-            if (w) atomicAdd(&sp.hist[line(k)], w);
+            if (w) atomicAdd(&sp.hist[line(k) >> 8], w);
             sum += w;
         }
         if (by_sum) need = S.share_of(block_total<NT>(sum, sp.wsum));
         __syncthreads();
-        first_bin(by_sum ? need : (u64)S.top_k, &sp);
+        find_bin(false, by_sum ? need : (u64)S.top_k, 0, &sp);
         const int bin = (int)sp.digit;
         const int per = (V + NT - 1) / NT, lo_i = min(tid * per, V), hi_i = min(lo_i + per, V);
-        u64 count = 0, total;
-        for (int i = lo_i; i < hi_i; i++) count += line(keys[i]) <= bin;
-        int at = (int)(block_scan<NT>(count, sp.wsum, &total) - count);
-        if (total <= kList) {
+        u64 count = 0, n;
+        for (int i = lo_i; i < hi_i; i++) count += line(keys[i]) >> 8 <= bin;
+        int at = (int)(block_scan<NT>(count, sp.wsum, &n) - count);
+        if (n <= 64) {
             for (int i = lo_i; i < hi_i; i++)
-                if (line(keys[i]) <= bin) list[at] = keys[i], place[at++] = (unsigned short)i;
-            set = list, n = (int)total, listed = true;
+                if (line(keys[i]) >> 8 <= bin) place[at++] = i;
             __syncthreads();
-            if (n <= 64) {
-                if (tid < 64)
-                    finish_wave(P, r, tid < n ? list[tid] : 0, n, [&](int i) { return (int)place[i]; }, S, W, need);
-                return;
-            }
+            if (tid < 64)
+                finish_wave(P, r, tid < (int)n ? keys[place[tid]] : 0, (int)n, [&](int i) { return place[i]; }, S, W, need);
+            return;
         }
     }
-    auto key = [&](int j) { return set[j]; };
-    const Cut c = cut_of<NT>(key, n, S, W, need, &sp);
-    u64 total;
-    const int i = draw_of<NT>(key, n, c, S, W, P.u[r], 0, ~0ull, &total, &sp);
-    if (i >= 0) drawn(P, r, listed ? place[i] : i, W.weight(logit_of(set[i])), total);
+    const u64 cut = cut_of<NT>(key, V, line, true, S, W, need, &sp);
+    const int i = draw_of<NT>(key, 0, V, cut, S, W, P.u[r], ~0ull, &total, &sp);
+    if (i >= 0) drawn(P, r, i, W.weight(logit_of(keys[i])), total);
 }
 
 // ---------------------------------------------------------------------------
@@ -664,7 +647,7 @@ __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int 
     unsigned g[N];
 #pragma unroll
     for (int j = 0; j < N; j++) g[j] = R->group[min(tid + j * 256, groups - 1)];
-    if (tid == 0) sp->thr = 0xffffffffu, sp->ties = 0xffffffffu;
+    if (tid == 0) sp->thr = 0xffffffffu, sp->count = 0xffffffffu;
     sp->hist[tid] = 0;
     const RowTop t = row_top(R, chunks, sp);
     float least = t.bad ? INFINITY : -3.402823466e38f;
@@ -678,16 +661,16 @@ __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int 
                 if (tid + j * 256 < groups) take(g[j]);
             for (int i = tid + N * 256; i < groups; i += 256) take(R->group[i]);
         };
-        each([&](unsigned k) { atomicAdd(&sp->hist[line(k)], (u64)1); });
+        each([&](unsigned k) { atomicAdd(&sp->hist[line(k) >> 8], (u64)1); });
         __syncthreads();
-        first_bin((u64)S.top_k, sp);
+        find_bin(false, (u64)S.top_k, 0, sp);
         const int bin = (int)sp->digit;
         unsigned low = 0xffffffffu;
-        each([&](unsigned k) { low = min(low, line(k) <= bin ? k : 0xffffffffu); });
+        each([&](unsigned k) { low = min(low, line(k) >> 8 <= bin ? k : 0xffffffffu); });
         low = ~wave_top(~low);
-        if ((tid & 63) == 0) atomicMin(&sp->ties, low);
+        if ((tid & 63) == 0) atomicMin(&sp->count, low);
         __syncthreads();
-        least = fmaxf(least, logit_of(sp->ties));
+        least = fmaxf(least, logit_of(sp->count));
     }
     if (tid == 0) R->least = least;
 }
@@ -832,7 +815,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
     __shared__ Space sp;
     __shared__ unsigned keys[kNear];
     __shared__ int place[kNear];
-    __shared__ int offset[kMaxChunks], ties[kMaxChunks];
+    __shared__ int offset[kMaxChunks];
     const int r = row0 + blockIdx.x, tid = threadIdx.x, V = P.vocab, chunks = (V + kChunk - 1) / kChunk;
     RowScratch *R = scratch + blockIdx.x;
     const float *x = P.logits + (size_t)r * P.ld;
@@ -856,10 +839,10 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
     const float u = P.u[r];
     auto far_key = [&](int i) { return key_of(x[i]); };
     auto near_key = [&](int i) { return keys[i]; };
-    auto whole = [&]() {  // the row by its keys' digits, from memory: many passes
-        const Cut c = cut_of<NT>(far_key, V, S, W, 0, &sp);
+    auto whole = [&]() {  // the row from memory: many passes
+        const u64 cut = cut_of<NT>(far_key, V, Line(mx, mx - 32.0f * S.t), false, S, W, 0, &sp);
         u64 total;
-        const int i = draw_of<NT>(far_key, V, c, S, W, u, 0, ~0ull, &total, &sp);
+        const int i = draw_of<NT>(far_key, 0, V, cut, S, W, u, ~0ull, &total, &sp);
         if (i >= 0) drawn(P, r, i, W.weight(x[i]), total);
     };
     u64 total;
@@ -895,37 +878,24 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
             if (tid < 64) finish_wave(P, r, tid < n ? keys[tid] : 0, n, [&](int i) { return place[i]; }, S, W, 0);
             return;
         }
-        const Cut c = cut_of<NT>(near_key, n, S, W, 0, &sp);
-        const int i = draw_of<NT>(near_key, n, c, S, W, u, 0, ~0ull, &total, &sp);
+        const u64 cut = cut_of<NT>(near_key, n, Line(mx, R->least), false, S, W, 0, &sp);
+        const int i = draw_of<NT>(near_key, 0, n, cut, S, W, u, ~0ull, &total, &sp);
         if (i >= 0) drawn(P, r, place[i], W.weight(logit_of(keys[i])), total);
         return;
     }
-    Cut c;
-    u64 part = tid < chunks ? R->sum[tid] : 0;
+    u64 cut = 0, part = tid < chunks ? R->sum[tid] : 0;
     if (S.cuts_sum()) {
         const BinCut b = bin_cut<NT>(R, S, &sp);
-        c = cut_of<NT>(near_key, (int)held, S, W, b.need - b.above, &sp);
-        // each chunk's ties before it and kept sum
+        const Line line((float)((double)mx - 2 * b.bin / W.scale), (float)((double)mx - 2 * (b.bin + 1) / W.scale));
+        cut = cut_of<NT>(near_key, (int)held, line, false, S, W, b.need - b.above, &sp);
         static_assert(kMaxChunks <= 256, "sums in the histogram");
         for (int i = tid; i < 256; i += NT) sp.hist[i] = 0;
-        if (tid < chunks) ties[tid] = 0;
-        const int per = ((int)held + NT - 1) / NT, lo = min(tid * per, (int)held), hi = min(lo + per, (int)held);
-        u64 count = 0, all;
-        for (int i = lo; i < hi; i++) count += keys[i] == c.thr;
-        u64 seen = block_scan<NT>(count, sp.wsum, &all) - count;  // with the barrier
-        for (int i = lo; i < hi; i++) {
-            const unsigned k = keys[i];
-            const int at = place[i] / kChunk;
-            if (k == c.thr) atomicAdd(&ties[at], 1);
-            if (k > c.thr || (k == c.thr && seen++ < c.ties)) atomicAdd(&sp.hist[at], W.units(logit_of(k), S.least));
-        }
         __syncthreads();
-        if (tid < chunks) part += sp.hist[tid], count = (u64)ties[tid];
-        else count = 0;
-        const u64 upto = block_scan<NT>(count, sp.wsum, &all);
-        if (tid < chunks) ties[tid] = (int)(upto - count);
-    } else if (tid < chunks) {
-        ties[tid] = 0;
+        for (int i = tid; i < (int)held; i += NT)
+            if (order_of(keys[i], i) >= cut) atomicAdd(&sp.hist[place[i] / kChunk], W.units(logit_of(keys[i]), S.least));
+        __syncthreads();
+        if (tid < chunks) part += sp.hist[tid];
+        if (cut && index_in(cut) < (int)held) cut = order_of(key_in(cut), place[index_in(cut)]);  // in the row's terms
     }
     const u64 upto = block_scan<NT>(part, sp.wsum, &total);
     u64 target = S.target_of(u, total);
@@ -933,8 +903,8 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
     __syncthreads();
     const int chunk = sp.token, i0 = chunk * kChunk;
     target -= sp.base;
-    const int i = draw_of<NT>([&](int j) { return far_key(i0 + j); }, min(kChunk, V - i0), c, S, W, u,
-                              (u64)ties[chunk], target, &total, &sp);
+    const int i = draw_of<NT>([&](int j) { return far_key(i0 + j); }, i0, min(kChunk, V - i0), cut, S, W, u, target,
+                              &total, &sp);
     if (i >= 0) drawn(P, r, i0 + i, W.weight(x[i0 + i]), total);
 }
 
