@@ -182,8 +182,8 @@ __device__ __forceinline__ u64 readlane64(u64 v, int j) {
 // `count` stay (0: all) and then, where `by_sum`, those whose predecessors' sum and
 // `above` is below `need` (0: top-p's share of the sum).  A lane holds every 64th
 // of them and a wave compares all with its share, which it has in scalar
-// registers: two instructions a pair, six with the sum (2.3 us for 206; with each
-// pair read from LDS by threads of their own it took 6.3).
+// registers: two instructions a pair, six with the sum (226 by count 2.8 us, 215 by
+// sum 6.2; with each pair read from LDS and the cut by an atomic minimum 7.4 both).
 template <int NT>
 __device__ u64 rank_near(int n, u64 count, bool by_sum, u64 above, u64 need, const RowSettings &S, const Weights &W,
                          Space *sp) {
@@ -197,7 +197,7 @@ __device__ u64 rank_near(int n, u64 count, bool by_sum, u64 above, u64 need, con
         if (by_sum) mine = W.units(logit_of(key_in(sp->near[tid])));
         sp->units[tid] = mine;
     }
-    if (tid == 0) sp->cut = ~0ull;
+    if (tid == 0) sp->cut = 0;
     __syncthreads();
     u64 order[A], sum[A];
     unsigned rank[A];
@@ -234,13 +234,14 @@ __device__ u64 rank_near(int n, u64 count, bool by_sum, u64 above, u64 need, con
             }
     }
     __syncthreads();
-    bool keep = tid < n && (count == 0 || sp->rank[tid] < count);
-    const u64 before = tid < n ? above + ahead[tid] : 0;
-    if (by_sum) {
+    const bool keep = tid < n && (count == 0 || sp->rank[tid] < count);
+    if (by_sum) {  // the last that stays is where the sum arrives
+        const u64 before = tid < n ? above + ahead[tid] : 0;
         if (need == 0) need = S.share_of(block_total<NT>(keep ? mine : 0, sp->wsum));
-        keep = keep && before < need;
+        if (keep && before < need && before + mine >= need) sp->cut = sp->near[tid];
+    } else if (keep && sp->rank[tid] == count - 1) {
+        sp->cut = sp->near[tid];
     }
-    if (keep) atomicMin(&sp->cut, sp->near[tid]);
     __syncthreads();
     return sp->cut;
 }
