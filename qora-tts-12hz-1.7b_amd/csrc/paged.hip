@@ -920,7 +920,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnParams A) {
     if (sarrived != (unsigned)parts - 1) return;
     // The parts' rows, two values a load and 16 loads in flight; the first ones
     // while the maxima and sums become every part's factor.
-    constexpr int MI = CT * HD > 1024 ? CT * HD / 512 : 1, U = MI > 8 ? 1 : 16 / MI;
+    constexpr int MI = CT * HD > 512 ? CT * HD / 512 : 1, U = MI > 8 ? 1 : 16 / MI;
     float *fac = &so[0][0][0];
     uint64_t y[U][MI];
     const int pairs = left * (HD / 2);  // of values

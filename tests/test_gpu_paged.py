@@ -198,10 +198,11 @@ def test_blocks_of_odd_values(ctx):
     assert np.array_equal(k, held, equal_nan=True) and np.array_equal(v, held, equal_nan=True)
 
 
-def _check(got, q, k, v, start, scale, window, absent=()):
+def _check(got, q, k, v, start, scale, window, absent=(), step=0.0):
     ref, mass, slack = pm.attention(q, k, v, start, scale, window, absent)
     err = np.abs(got - ref)
     tol = mass * (2 * slack[..., None] + (k.shape[0] / 64 + 64) * 2.0 ** -24)
+    tol += step * np.abs(v).sum(0).repeat(q.shape[1] // v.shape[1], 0)
     assert np.all(np.isfinite(got))
     assert np.all(err <= tol), (float(err.max()), float((err / np.maximum(tol, 1e-30)).max()))
     # independent roundings add up as their squares do: far below the bound
@@ -257,6 +258,29 @@ def test_attention_many_rows(ctx, page, kvh, group, hd, window):
         _check(out[at:at + n].reshape(n, kvh * group, hd), q[at:at + n].reshape(n, kvh * group, hd), k, v, starts[b],
                hd ** -0.5, window)
         at += n
+
+
+@pytest.mark.parametrize("kvh,group,hd", [(1, 9, 64), (2, 16, 64), (1, 12, 128), (1, 3, 64), (3, 4, 128)])
+@pytest.mark.parametrize("rows", [1, 2, 3])
+def test_every_column_of_divided_tokens(ctx, kvh, group, hd, rows):
+    """Groups that fill a tile, or the next one partly, with each sequence's
+    tokens divided among blocks.
+
+    Some columns here have one token with nearly all the probability and a code
+    of 0 in a dimension, so that the output there is 1e-9 of V's size.  A weight
+    is held to a least step, not to a share of itself: as an integer of which the
+    column's largest is 2^27 or more (up to 4 columns), or as binary16 hi + lo,
+    steps of 2^-24, of which the largest is 2^11 or more.  Half a step is 2^-28 or
+    2^-36 of the largest weight, which is at most 1 of the sum, so an output is
+    off by at most that times sum |v| beside what the others may be."""
+    starts, counts = [2000, 700], [rows, rows]
+    c, held = _filled(ctx, kvh, hd, 32, starts, counts, seed=12)
+    q = _normal(13, 2 * rows, kvh * group * hd) * 2
+    got = c.attend(ctx, c.seqs(starts, counts), _up(q), kvh * group).cpu().numpy()
+    for b, (k, v) in enumerate(held):
+        at = slice(b * rows, b * rows + rows)
+        _check(got[at].reshape(rows, -1, hd), q[at].reshape(rows, -1, hd), k, v, starts[b], hd ** -0.5, 0,
+               step=2.0 ** (-28 if rows * group <= 4 else -36))
 
 
 @pytest.mark.parametrize("rows", [1, 5, 40])
