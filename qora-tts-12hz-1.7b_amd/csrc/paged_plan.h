@@ -162,6 +162,22 @@ struct AttnPlan {
     int nsplit;  // blocks of each of the others
 };
 
+// Columns (query rows of a kv head's group) that a block takes: 4 on int8
+// products, 16 or 32 on binary16 ones.  Where a page's bytes are the cost, few
+// columns cost as much as one: 16 sequences of 2064 tokens, 8 kv heads, took 20 us
+// at up to 4 columns on int8 products (21 on the others), at 8 columns 27 us on
+// int8 and 25 on binary16, at 16 columns 24 us (40 in tiles of 32).  Tiles of 32
+// halve the reading of pages and the products' operands, but leave half as many
+// blocks, which pays once those fill three quarters of a round: with 256 of them
+// (rows of 1024 columns behind 2000 tokens) 52 us against 45 in tiles of 16, with
+// 384 62 against 74, with 532 80 against 105.
+enum AttnMode { kAttnI8, kAttn16, kAttn32 };
+
+inline AttnMode attn_mode(long long columns, long long heads) {
+    if (columns <= 4) return kAttnI8;
+    return columns > 16 && (columns + 31) / 32 * heads >= kPagedRound * 3 / 4 ? kAttn32 : kAttn16;
+}
+
 // Tokens that a block takes at least where it shares a pair: one step of its
 // waves, and with 32 columns four, as their joining costs more.
 QTTS_HD constexpr int attn_least(int columns) { return columns == 32 ? 512 : 256; }
