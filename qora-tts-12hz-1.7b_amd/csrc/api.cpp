@@ -2945,7 +2945,7 @@ qtts_status qtts_paged_append_device(qtts_ctx *c, const qtts_paged_kv *kv, const
     p.cap = (long long)s->max_pages * kv->page_size;
     if (r->rope_cos) p.cap = std::min<long long>(p.cap, r->rope_rows);
     DeviceGuard guard(c->device);
-    if (!launch_paged_append(c->stream, p)) return fail(c, QTTS_ERANGE, "paged append: more blocks than a launch holds");
+    launch_paged_append(c->stream, p);
     return check_launch(c, "k_paged_append");
 }
 
@@ -2968,8 +2968,7 @@ qtts_status qtts_paged_attention_device(qtts_ctx *c, const qtts_paged_kv *kv, co
     p.part = c->attn_part;
     p.counters = c->paged_counters;
     DeviceGuard guard(c->device);
-    if (!launch_paged_attention(c->stream, p))
-        return fail(c, QTTS_ERANGE, "paged attention: more blocks than a launch holds");
+    launch_paged_attention(c->stream, p);
     return check_launch(c, "k_paged_attn");
 }
 
@@ -2987,7 +2986,7 @@ qtts_status qtts_paged_read_device(qtts_ctx *c, const qtts_paged_kv *kv, const q
     p.ld_k = ld_k_out;
     p.ld_v = ld_v_out;
     DeviceGuard guard(c->device);
-    if (!launch_paged_read(c->stream, p)) return fail(c, QTTS_ERANGE, "paged read: more blocks than a launch holds");
+    launch_paged_read(c->stream, p);
     return check_launch(c, "k_paged_read");
 }
 

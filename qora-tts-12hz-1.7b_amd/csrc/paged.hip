@@ -1063,47 +1063,30 @@ void attn_of(hipStream_t st, const PagedAttnParams &p, AttnMode mode, unsigned b
 
 }  // namespace
 
-bool launch_paged_append(hipStream_t st, const PagedAppendParams &in) {
+void launch_paged_append(hipStream_t st, const PagedAppendParams &in) {
     PagedAppendParams p = in;
-    const int P = p.kv.page_size;
-    p.kv_items = (int)(((long long)p.s.max_rows + P - 2) / P + 1);
-    const int NT = std::min(256, P * p.kv.head_dim / 8), groups = NT / (p.kv.head_dim / 8);
-    const long long parts = p.r.q ? (long long)p.s.max_rows * ((p.r.heads + 3) / 4) : 0;
-    if (parts > kPagedMaxBlocks) return false;
-    p.q_items = (int)((parts + groups - 1) / groups);
-    const long long blocks = p.s.batch * (2LL * p.kv_items * p.kv.kv_heads + p.q_items);
-    if (2LL * p.kv_items * p.kv.kv_heads > kPagedMaxBlocks || blocks > kPagedMaxBlocks) return false;
-    if (p.kv.head_dim == 64) append_of<64>(st, p, (unsigned)blocks);
-    else append_of<128>(st, p, (unsigned)blocks);
-    return true;
+    const AppendPlan plan = append_plan(p.kv, p.s, p.r);
+    p.kv_items = plan.kv_items;
+    p.q_items = (int)plan.q_items;
+    if (p.kv.head_dim == 64) append_of<64>(st, p, (unsigned)plan.blocks);
+    else append_of<128>(st, p, (unsigned)plan.blocks);
 }
 
-bool launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
+void launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
     PagedAttnParams p = in;
-    const int group = p.heads / p.kv.kv_heads, hd = p.kv.head_dim;
-    const long long cols = (long long)p.s.max_rows * group;
-    const AttnMode mode = attn_mode(cols, (long long)p.s.batch * p.kv.kv_heads);
-    const int ct = mode == kAttnI8 ? 4 : mode == kAttn16 ? 16 : 32;
-    p.tiles = (int)((cols + ct - 1) / ct);
-    const long long pairs = (long long)p.s.batch * p.kv.kv_heads * p.tiles;
-    if (pairs > kPagedMaxBlocks) return false;
-    const AttnPlan plan = attn_plan(pairs, (long long)p.s.max_pages * p.kv.page_size, ct);
-    p.whole = plan.whole;
-    p.nsplit = plan.nsplit;
-    const long long blocks = plan.whole + (pairs - plan.whole) * plan.nsplit;
-    if (blocks > kPagedMaxBlocks) return false;
-    if (hd == 64) attn_of<64>(st, p, mode, (unsigned)blocks);
-    else attn_of<128>(st, p, mode, (unsigned)blocks);
-    return true;
+    const AttnShape shape = attn_shape(p.kv, p.s, p.heads);
+    p.tiles = shape.tiles;
+    p.whole = shape.whole;
+    p.nsplit = shape.nsplit;
+    if (p.kv.head_dim == 64) attn_of<64>(st, p, shape.mode, (unsigned)shape.blocks);
+    else attn_of<128>(st, p, shape.mode, (unsigned)shape.blocks);
 }
 
-bool launch_paged_read(hipStream_t st, const PagedReadParams &p) {
-    const int P = p.kv.page_size, items = (int)(((long long)p.s.max_rows + P - 2) / P + 1);
-    const long long blocks = (long long)p.s.batch * items * p.kv.kv_heads;
-    if (blocks > kPagedMaxBlocks) return false;
-    if (p.kv.head_dim == 64) hipLaunchKernelGGL(k_paged_read<64>, dim3((unsigned)blocks), dim3(256), 0, st, p, items);
-    else hipLaunchKernelGGL(k_paged_read<128>, dim3((unsigned)blocks), dim3(256), 0, st, p, items);
-    return true;
+void launch_paged_read(hipStream_t st, const PagedReadParams &p) {
+    const int items = read_items(p.kv, p.s);
+    const unsigned blocks = (unsigned)read_blocks(p.kv, p.s);
+    if (p.kv.head_dim == 64) hipLaunchKernelGGL(k_paged_read<64>, dim3(blocks), dim3(256), 0, st, p, items);
+    else hipLaunchKernelGGL(k_paged_read<128>, dim3(blocks), dim3(256), 0, st, p, items);
 }
 
 }  // namespace qtts

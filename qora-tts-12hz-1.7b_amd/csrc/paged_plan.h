@@ -23,7 +23,7 @@ struct Refusal {
 };
 
 constexpr Refusal kAccepted{QTTS_OK, nullptr};
-constexpr long long kPagedMaxBlocks = (1LL << 31) - 1;  // of one launch
+constexpr long long kPagedMaxBlocks = (1LL << 24) - 1;  // of one launch: its threads are counted in 32 bits
 constexpr int kSampleRowsMaxVocab = 1 << 19;
 
 inline bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
@@ -36,7 +36,7 @@ inline Refusal check_paged(const qtts_paged_kv &kv, const qtts_paged_seqs &s) {
         return {QTTS_ESHAPE, "paged cache: page_size must be 16, 32, 64 or 128"};
     if (kv.num_pages < 1 || kv.kv_heads < 1 || kv.kv_heads > 1024 || kv.num_slots < 1)
         return {QTTS_ESHAPE, "paged cache: num_pages, kv_heads (to 1024) and num_slots must be positive"};
-    if ((long long)kv.num_pages * kv.kv_heads > kPagedMaxBlocks)
+    if ((long long)kv.num_pages * kv.kv_heads > (1LL << 31) - 1)
         return {QTTS_ERANGE, "paged cache: more than 2^31 - 1 blocks (pages times kv heads)"};
     if (!kv.k_codes || !kv.v_codes || !kv.k_scales || !kv.v_scales || !kv.k_open || !kv.v_open)
         return {QTTS_EINVAL, "paged cache: null buffer"};
@@ -78,6 +78,26 @@ inline Refusal check_heads(const qtts_paged_kv &kv, int32_t heads) {
         if (r_.why) return r_;         \
     } while (0)
 
+// Blocks of an append's sequence: K's and V's for every page that its rows touch
+// at most, and a share of the query heads each.
+struct AppendPlan {
+    int kv_items;       // pages
+    int threads;        // of a block
+    long long q_items;  // blocks of query heads
+    long long blocks;   // of the launch
+};
+
+inline AppendPlan append_plan(const qtts_paged_kv &kv, const qtts_paged_seqs &s, const qtts_paged_rows &r) {
+    const int P = kv.page_size, lanes = kv.head_dim / 8;
+    AppendPlan a;
+    a.kv_items = (int)(((long long)s.max_rows + P - 2) / P + 1);
+    a.threads = P * lanes < 256 ? P * lanes : 256;
+    const long long fours = r.q ? (long long)s.max_rows * ((r.heads + 3) / 4) : 0;
+    a.q_items = (fours + a.threads / lanes - 1) / (a.threads / lanes);
+    a.blocks = s.batch * (2LL * a.kv_items * kv.kv_heads + a.q_items);
+    return a;
+}
+
 inline Refusal check_append(const qtts_paged_kv &kv, const qtts_paged_seqs &s, const qtts_paged_rows &r) {
     QTTS_REFUSE(check_paged(kv, s));
     const long long hd = kv.head_dim, width = kv.kv_heads * hd;
@@ -103,44 +123,8 @@ inline Refusal check_append(const qtts_paged_kv &kv, const qtts_paged_seqs &s, c
         if (r.q == r.q_out && r.ld_q != r.ld_q_out)
             return {QTTS_EINVAL, "paged append: in place, q_out takes q's stride"};
     }
-    return kAccepted;
-}
-
-inline Refusal check_attention(const qtts_paged_kv &kv, const qtts_paged_seqs &s, int32_t heads, const float *q,
-                               int32_t ld_q, float scale, int32_t window, const float *out, int32_t ld_out) {
-    QTTS_REFUSE(check_paged(kv, s));
-    QTTS_REFUSE(check_heads(kv, heads));
-    if (window < 0) return {QTTS_EINVAL, "paged attention: window must not be negative"};
-    if (!std::isfinite(scale)) return {QTTS_EINVAL, "paged attention: scale must be finite"};
-    if (paged_empty(s)) return kAccepted;
-    QTTS_REFUSE(check_rows(q, ld_q, (long long)heads * kv.head_dim));
-    QTTS_REFUSE(check_rows(out, ld_out, (long long)heads * kv.head_dim));
-    if (q == out && ld_q != ld_out) return {QTTS_EINVAL, "paged attention: in place, out takes q's stride"};
-    return kAccepted;
-}
-
-inline Refusal check_read(const qtts_paged_kv &kv, const qtts_paged_seqs &s, const int32_t *lens, const float *k_out,
-                          int32_t ld_k, const float *v_out, int32_t ld_v) {
-    QTTS_REFUSE(check_paged(kv, s));
-    if (!aligned_to(lens, 4)) return {QTTS_EINVAL, "paged read: misaligned lens"};
-    if (paged_empty(s)) return kAccepted;
-    const long long width = (long long)kv.kv_heads * kv.head_dim;
-    if (k_out) QTTS_REFUSE(check_rows(k_out, ld_k, width));
-    if (v_out) QTTS_REFUSE(check_rows(v_out, ld_v, width));
-    return kAccepted;
-}
-
-inline Refusal check_sample_rows(const float *logits, int64_t ld, int32_t rows, int32_t vocab,
-                                 const qtts_row_sampler &p, const float *uniform, const int32_t *tokens,
-                                 const float *probs) {
-    if (vocab < 1 || vocab > kSampleRowsMaxVocab) return {QTTS_ESHAPE, "sample_rows: vocab must be 1..524288"};
-    if (rows < 0) return {QTTS_ESHAPE, "sample_rows: rows must not be negative"};
-    if (ld < vocab) return {QTTS_ESHAPE, "sample_rows: stride below the row"};
-    if (rows == 0) return kAccepted;
-    if (!logits || !uniform || !tokens) return {QTTS_EINVAL, "sample_rows: null argument"};
-    if (!aligned_to(logits, 4) || !aligned_to(uniform, 4) || !aligned_to(tokens, 4) || !aligned_to(probs, 4) ||
-        !aligned_to(p.temperature, 4) || !aligned_to(p.top_k, 4) || !aligned_to(p.top_p, 4) || !aligned_to(p.min_p, 4))
-        return {QTTS_EINVAL, "sample_rows: misaligned argument"};
+    if (append_plan(kv, s, r).blocks > kPagedMaxBlocks)
+        return {QTTS_ERANGE, "paged append: more blocks than a launch holds"};
     return kAccepted;
 }
 
@@ -190,6 +174,72 @@ inline AttnPlan attn_plan(long long pairs, long long cap, int columns) {
     n = n > kPagedMaxSplits ? kPagedMaxSplits : n;
     if (n <= 1) return {(int)pairs, 1};
     return {(int)(pairs - rest), (int)n};
+}
+
+struct AttnShape {
+    AttnMode mode;
+    int tiles;         // of columns, a sequence and kv head's
+    int whole, nsplit; // as in AttnPlan
+    long long blocks;  // of the launch
+};
+
+inline AttnShape attn_shape(const qtts_paged_kv &kv, const qtts_paged_seqs &s, int heads) {
+    const long long columns = (long long)s.max_rows * (heads / kv.kv_heads), kvs = (long long)s.batch * kv.kv_heads;
+    const AttnMode mode = attn_mode(columns, kvs);
+    const int each = mode == kAttnI8 ? 4 : mode == kAttn16 ? 16 : 32;
+    const long long tiles = (columns + each - 1) / each, pairs = kvs * tiles;
+    if (pairs > kPagedMaxBlocks) return {mode, 0, 0, 0, pairs};
+    const AttnPlan p = attn_plan(pairs, (long long)s.max_pages * kv.page_size, each);
+    return {mode, (int)tiles, p.whole, p.nsplit, p.whole + (pairs - p.whole) * p.nsplit};
+}
+
+// One for each page that a sequence's positions touch at most, and kv head.
+inline int read_items(const qtts_paged_kv &kv, const qtts_paged_seqs &s) {
+    return (int)(((long long)s.max_rows + kv.page_size - 2) / kv.page_size + 1);
+}
+inline long long read_blocks(const qtts_paged_kv &kv, const qtts_paged_seqs &s) {
+    return (long long)s.batch * read_items(kv, s) * kv.kv_heads;
+}
+
+inline Refusal check_attention(const qtts_paged_kv &kv, const qtts_paged_seqs &s, int32_t heads, const float *q,
+                               int32_t ld_q, float scale, int32_t window, const float *out, int32_t ld_out) {
+    QTTS_REFUSE(check_paged(kv, s));
+    QTTS_REFUSE(check_heads(kv, heads));
+    if (window < 0) return {QTTS_EINVAL, "paged attention: window must not be negative"};
+    if (!std::isfinite(scale)) return {QTTS_EINVAL, "paged attention: scale must be finite"};
+    if (paged_empty(s)) return kAccepted;
+    QTTS_REFUSE(check_rows(q, ld_q, (long long)heads * kv.head_dim));
+    QTTS_REFUSE(check_rows(out, ld_out, (long long)heads * kv.head_dim));
+    if (q == out && ld_q != ld_out) return {QTTS_EINVAL, "paged attention: in place, out takes q's stride"};
+    if (attn_shape(kv, s, heads).blocks > kPagedMaxBlocks)
+        return {QTTS_ERANGE, "paged attention: more blocks than a launch holds"};
+    return kAccepted;
+}
+
+inline Refusal check_read(const qtts_paged_kv &kv, const qtts_paged_seqs &s, const int32_t *lens, const float *k_out,
+                          int32_t ld_k, const float *v_out, int32_t ld_v) {
+    QTTS_REFUSE(check_paged(kv, s));
+    if (!aligned_to(lens, 4)) return {QTTS_EINVAL, "paged read: misaligned lens"};
+    if (paged_empty(s)) return kAccepted;
+    const long long width = (long long)kv.kv_heads * kv.head_dim;
+    if (k_out) QTTS_REFUSE(check_rows(k_out, ld_k, width));
+    if (v_out) QTTS_REFUSE(check_rows(v_out, ld_v, width));
+    if (read_blocks(kv, s) > kPagedMaxBlocks) return {QTTS_ERANGE, "paged read: more blocks than a launch holds"};
+    return kAccepted;
+}
+
+inline Refusal check_sample_rows(const float *logits, int64_t ld, int32_t rows, int32_t vocab,
+                                 const qtts_row_sampler &p, const float *uniform, const int32_t *tokens,
+                                 const float *probs) {
+    if (vocab < 1 || vocab > kSampleRowsMaxVocab) return {QTTS_ESHAPE, "sample_rows: vocab must be 1..524288"};
+    if (rows < 0) return {QTTS_ESHAPE, "sample_rows: rows must not be negative"};
+    if (ld < vocab) return {QTTS_ESHAPE, "sample_rows: stride below the row"};
+    if (rows == 0) return kAccepted;
+    if (!logits || !uniform || !tokens) return {QTTS_EINVAL, "sample_rows: null argument"};
+    if (!aligned_to(logits, 4) || !aligned_to(uniform, 4) || !aligned_to(tokens, 4) || !aligned_to(probs, 4) ||
+        !aligned_to(p.temperature, 4) || !aligned_to(p.top_k, 4) || !aligned_to(p.top_p, 4) || !aligned_to(p.min_p, 4))
+        return {QTTS_EINVAL, "sample_rows: misaligned argument"};
+    return kAccepted;
 }
 
 // Tokens of one block where `nsplit` share `span` tokens.

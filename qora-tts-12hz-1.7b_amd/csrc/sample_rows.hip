@@ -462,12 +462,12 @@ __device__ __forceinline__ f32x4 load_logits(const float *x, int i, int V, bool 
 constexpr int kRowVocab = 8192;  // with the lists, a block's 64 KB of LDS
 
 template <int NT>
-__global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P) {
+__global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P, int row0) {
     extern __shared__ unsigned keys[];
     __shared__ Space sp;
     __shared__ unsigned sleast;
     __shared__ int place[64];
-    const int r = blockIdx.x, tid = threadIdx.x, V = P.vocab;
+    const int r = row0 + blockIdx.x, tid = threadIdx.x, V = P.vocab;
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
     const bool aligned = ((uintptr_t)x & 15) == 0;
@@ -914,8 +914,13 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
 void launch_sample_rows(hipStream_t st, const SampleRowsParams &p) {
     if (p.vocab <= kRowVocab) {
         const unsigned lds = (unsigned)p.vocab * 4;
-        if (p.vocab <= 1024) hipLaunchKernelGGL(k_sample_row<256>, dim3((unsigned)p.rows), dim3(256), lds, st, p);
-        else hipLaunchKernelGGL(k_sample_row<1024>, dim3((unsigned)p.rows), dim3(1024), lds, st, p);
+        constexpr int most = (1 << 22) - 1;  // a launch's threads are counted in 32 bits
+        for (int row0 = 0; row0 < p.rows; row0 += most) {
+            const dim3 grid((unsigned)std::min(most, p.rows - row0));
+            if (p.vocab <= 1024) hipLaunchKernelGGL(k_sample_row<256>, grid, dim3(256), lds, st, p, row0);
+            else hipLaunchKernelGGL(k_sample_row<1024>, grid, dim3(1024), lds, st, p, row0);
+            if (p.rows - row0 <= most) break;
+        }
         return;
     }
     RowScratch *scratch = static_cast<RowScratch *>(p.scratch);

@@ -55,9 +55,9 @@ struct SampleRowsParams {
 };
 
 // False: the call needs more blocks than one launch holds, nothing was launched.
-bool launch_paged_append(hipStream_t st, const PagedAppendParams &p);
-bool launch_paged_attention(hipStream_t st, const PagedAttnParams &p);
-bool launch_paged_read(hipStream_t st, const PagedReadParams &p);
+void launch_paged_append(hipStream_t st, const PagedAppendParams &p);
+void launch_paged_attention(hipStream_t st, const PagedAttnParams &p);
+void launch_paged_read(hipStream_t st, const PagedReadParams &p);
 void launch_sample_rows(hipStream_t st, const SampleRowsParams &p);
 
 }  // namespace qtts

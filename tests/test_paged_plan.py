@@ -37,6 +37,10 @@ extern "C" void plan(long long pairs, long long cap, int columns, long long *o) 
     const AttnPlan p = attn_plan(pairs, cap, columns);
     o[0] = p.whole; o[1] = p.nsplit; o[2] = kPagedMaxSplits; o[3] = kPagedPartFloats; o[4] = kPagedCounters;
 }
+extern "C" void shape(const qtts_paged_kv *kv, const qtts_paged_seqs *s, int heads, long long *o) {
+    const AttnShape a = attn_shape(*kv, *s, heads);
+    o[0] = a.mode; o[1] = a.tiles; o[2] = a.whole; o[3] = a.blocks;
+}
 extern "C" int chunk(int span, int nsplit, int round) { return chunk_of(span, nsplit, round); }
 extern "C" void seq(const qtts_paged_seqs *s, int b, int slots, long long cap, int *o) {
     const PagedSeq q = load_seq(*s, b, slots, cap);
@@ -231,3 +235,36 @@ def test_attention_plans(lib):
             for step in (256, 512):
                 chunk = lib.chunk(span, nsplit, step)
                 assert chunk % step == 0 and chunk * nsplit >= span and chunk < span / nsplit + step + 1
+
+
+@pytest.mark.parametrize("append,attention,read,kv,seqs", [
+    (OK, OK, OK, dict(), dict(rows=1 << 20, max_rows=1 << 20)),
+    (OK, OK, OK, dict(kv_heads=4), dict(batch=65536, rows=65536, max_rows=1)),
+    (ERANGE, ERANGE, ERANGE, dict(kv_heads=256), dict(batch=65536, rows=65536, max_rows=1)),
+    (ERANGE, ERANGE, OK, dict(kv_heads=4), dict(batch=65536, rows=1 << 20, max_rows=1 << 10)),
+    (ERANGE, ERANGE, ERANGE, dict(), dict(batch=2, rows=1 << 30, max_rows=1 << 30)),
+])
+def test_more_blocks_than_a_launch_holds(lib, append, attention, read, kv, seqs):
+    """2^24 blocks of 256 threads: refused before anything is enqueued."""
+    k, s = _kv(**kv), _seqs(**seqs)
+    heads = 2 * k.kv_heads
+    wide = heads * k.head_dim
+    got = lib.append(C.byref(k), C.byref(s), C.byref(_rows(heads=heads, ld_q=wide, ld_q_out=wide, ld_k=wide, ld_v=wide)))
+    assert got == append, lib.reason()
+    assert lib.attention(C.byref(k), C.byref(s), heads, AT, wide, 0.1, 0, AT, wide) == attention, lib.reason()
+    assert lib.read_(C.byref(k), C.byref(s), None, AT, wide, AT, wide) == read, lib.reason()
+
+
+def test_columns_of_a_tile(lib):
+    """Few columns on int8 products, tiles of 32 only where they fill most of a
+    round; always enough tiles for all columns."""
+    out = (C.c_longlong * 4)()
+    for batch, kvh, group, rows, mode in ((1, 8, 2, 1, 0), (64, 8, 4, 1, 0), (64, 8, 5, 1, 1), (4, 8, 2, 8, 1),
+                                          (64, 8, 16, 1, 1), (64, 8, 17, 1, 2), (1, 8, 2, 512, 1), (1, 8, 2, 768, 2),
+                                          (16, 8, 2, 32, 1), (16, 8, 2, 33, 2)):
+        k, s = _kv(kv_heads=kvh), _seqs(batch=batch, rows=batch * rows, max_rows=rows)
+        lib.shape(C.byref(k), C.byref(s), kvh * group, out)
+        got, tiles, whole, blocks = list(out)
+        each = (4, 16, 32)[got]
+        assert got == mode and (tiles - 1) * each < group * rows <= tiles * each
+        assert batch * kvh * tiles <= blocks and whole <= batch * kvh * tiles
