@@ -5,14 +5,17 @@
 // integers of 2^-44 of the largest: sums do not depend on their order, and a
 // draw next to the border between two tokens falls as the 64-bit definition's
 // does.  What is kept is a prefix of the tokens in order (logit down, index up),
-// so that it is two numbers: a least key, and how many of those at it, the first
-// by index.
+// so that it is one number, the order of the last.
 //
 // Rows of up to kRowVocab logits take a block each, which holds the row's keys
 // in LDS (k_sample_row).  Longer rows are read in chunks by as many blocks as
-// they have: their maxima (k_sample_max), sums (k_sample_sum) and, where top-p
-// cuts without a top-k, the tokens next to the cut (k_sample_near); the row's
-// last block joins them and draws (k_sample_draw).
+// they have: their maxima (k_sample_max); where top-k's candidates end, or the
+// sums by weight (k_sample_sum); the candidates next to the cut
+// (k_sample_near).  One block a row joins them and draws (k_sample_draw).
+//
+// Measured: 64 rows of 151936, settings of every kind among them, 13 + 13 + 13
+// + 25 us (39 MB, which a copy reads in 8); all at top_k = 50, 14 + 9 + 7 + 10;
+// one row 6 + 7 + 4 + 9 us, all of it latency.
 #include <algorithm>
 
 #include "device_common.h"
@@ -459,8 +462,15 @@ __device__ __forceinline__ f32x4 load_logits(const float *x, int i, int V, bool 
     return v;
 }
 
-constexpr int kRowVocab = 8192;  // with the lists, a block's 64 KB of LDS
+// Rows that one block takes, in 48 KB of its LDS: 64 of 12000 logits in 35 us,
+// in chunks 61; one in 11 us, in chunks 16.
+constexpr int kRowVocab = 12288;
 
+// Bound by its steps' barriers and latencies, not by its bytes (64 rows of 2048:
+// 512 KB): 11 us where 50 tokens are kept and a wave finishes them, 16 us where
+// top-k and top-p both cut among many.  256 threads a row up to 1024 logits, which
+// have no more than four each (64 rows of 300: 11 us, with 1024 threads 12.5; of
+// 1500: 17 and 14).
 template <int NT>
 __global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P, int row0) {
     extern __shared__ unsigned keys[];
@@ -566,6 +576,7 @@ struct RowScratch {
     int token[kMaxChunks];            // where that is first
     unsigned bad[kMaxChunks];         // a NaN
     unsigned low[kMaxChunks];         // the least of its groups' maxima above -Inf
+    unsigned least_key[kMaxChunks];   // and of its logits
     unsigned near_at[kMaxChunks];     // its candidates (of top-p: in the cut's bin), in `near`
     unsigned near_n[kMaxChunks];
     unsigned near_all;
@@ -593,21 +604,24 @@ __device__ RowTop row_top(const RowScratch *R, int chunks, Space *sp) {
     return {sp->top, sp->bad != 0};
 }
 
+// The largest key of each group and chunk, and where the chunk's is first.  Bound
+// by memory: one load of the row, 16 bytes a lane and four in flight (64 rows of
+// 151936 in 13 us: 3 TB/s, from HBM).
 __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScratch *scratch, int row0) {
-    __shared__ unsigned stop, sbad, slow;
+    __shared__ unsigned stop, sbad, slow, sleast;
     __shared__ int stoken;
     const int r = row0 + blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x, V = P.vocab;
     RowScratch *R = scratch + blockIdx.y;
     const float *x = P.logits + (size_t)r * P.ld;
     const bool aligned = ((uintptr_t)x & 15) == 0;
-    if (tid == 0) stop = 0, sbad = 0, slow = 0xffffffffu, stoken = V;
+    if (tid == 0) stop = 0, sbad = 0, slow = sleast = 0xffffffffu, stoken = V;
     for (int i = chunk * 256 + tid; i < kBins; i += gridDim.x * 256) R->hist[i] = 0;
     if (chunk == 0 && tid == 0) R->near_all = 0;
     __syncthreads();
     f32x4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = load_logits(x, chunk * kChunk + 1024 * j + 4 * tid, V, aligned);
-    unsigned top = 0, low = 0xffffffffu;
+    unsigned top = 0, low = 0xffffffffu, least = 0xffffffffu;
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -616,6 +630,7 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
         for (int e = 0; e < 4; e++) {
             bad |= v[j][e] != v[j][e];
             g = max(g, key_of(v[j][e]));
+            least = min(least, v[j][e] > -INFINITY ? key_of(v[j][e]) : 0xffffffffu);
         }
         for (int off = 1; off < 16; off <<= 1) g = max(g, (unsigned)__shfl_xor((int)g, off, 64));
         top = max(top, g);
@@ -623,8 +638,8 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
         const int at = chunk * kChunk + 1024 * j + 4 * tid;
         if ((tid & 15) == 0 && at < V) R->group[at / kGroup] = g;
     }
-    top = wave_top(top), low = ~wave_top(~low);
-    if ((tid & 63) == 0) atomicMax(&stop, top), atomicMin(&slow, low);
+    top = wave_top(top), low = ~wave_top(~low), least = ~wave_top(~least);
+    if ((tid & 63) == 0) atomicMax(&stop, top), atomicMin(&slow, low), atomicMin(&sleast, least);
     if (bad) sbad = 1;
     __syncthreads();
     top = stop;
@@ -636,11 +651,11 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
             if (key_of(v[j][e]) == top) first = chunk * kChunk + 1024 * j + 4 * tid + e;
     if (first < V) atomicMin(&stoken, first);
     __syncthreads();
-    if (tid == 0) R->top[chunk] = top, R->bad[chunk] = sbad, R->low[chunk] = slow, R->token[chunk] = stoken;
+    if (tid == 0) R->top[chunk] = top, R->bad[chunk] = sbad, R->low[chunk] = slow, R->least_key[chunk] = sleast, R->token[chunk] = stoken;
 }
 
 // What top-k's candidates are no smaller than: a value that top_k of the groups'
-// maxima reach, by 256 steps down from the largest; every finite logit where
+// maxima reach, by 256 steps down from the largest; the least finite logit where
 // there are not that many groups.  (-Inf is never drawn, so it is no candidate.)
 __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int groups, Space *sp) {
     constexpr int N = 16;  // loads in flight: a row of 262144 in one step, kept for both passes
@@ -651,33 +666,38 @@ __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int 
     if (tid == 0) sp->thr = 0xffffffffu, sp->count = 0xffffffffu;
     sp->hist[tid] = 0;
     const RowTop t = row_top(R, chunks, sp);
-    float least = t.bad ? INFINITY : -3.402823466e38f;
-    if (S.top_k < groups && !t.bad) {
-        if (tid < chunks) atomicMin(&sp->thr, R->low[tid]);
+    float least = INFINITY;
+    if (!t.bad) {
+        const bool all = S.top_k >= groups;
+        if (tid < chunks) atomicMin(&sp->thr, all ? R->least_key[tid] : R->low[tid]);
         __syncthreads();
-        const Line line(logit_of(t.top), logit_of(sp->thr));
-        auto each = [&](auto take) {
+        least = logit_of(sp->thr);
+        if (!all) {
+            const Line line(logit_of(t.top), least);
+            auto each = [&](auto take) {
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if (tid + j * 256 < groups) take(g[j]);
-            for (int i = tid + N * 256; i < groups; i += 256) take(R->group[i]);
-        };
-        each([&](unsigned k) { atomicAdd(&sp->hist[line(k) >> 8], (u64)1); });
-        __syncthreads();
-        find_bin(false, (u64)S.top_k, 0, sp);
-        const int bin = (int)sp->digit;
-        unsigned low = 0xffffffffu;
-        each([&](unsigned k) { low = min(low, line(k) >> 8 <= bin ? k : 0xffffffffu); });
-        low = ~wave_top(~low);
-        if ((tid & 63) == 0) atomicMin(&sp->count, low);
-        __syncthreads();
-        least = fmaxf(least, logit_of(sp->count));
+                for (int j = 0; j < N; j++)
+                    if (tid + j * 256 < groups) take(g[j]);
+                for (int i = tid + N * 256; i < groups; i += 256) take(R->group[i]);
+            };
+            each([&](unsigned k) { atomicAdd(&sp->hist[line(k) >> 8], (u64)1); });
+            __syncthreads();
+            find_bin(false, (u64)S.top_k, 0, sp);
+            const int bin = (int)sp->digit;
+            unsigned low = 0xffffffffu;
+            each([&](unsigned k) { low = min(low, line(k) >> 8 <= bin && k > key_of(-INFINITY) ? k : 0xffffffffu); });
+            low = ~wave_top(~low);
+            if ((tid & 63) == 0) atomicMin(&sp->count, low);
+            __syncthreads();
+            least = logit_of(sp->count);
+        }
     }
     if (tid == 0) R->least = least;
 }
 
 // Rows that top-k cuts: where its candidates end.  Others: units by bin where
-// top-p cuts them, else the chunk's sum.
+// top-p cuts them, else the chunk's sum.  Bound by the 64-bit exponentials and,
+// by bin, the atomic sums in LDS (20 of 64 rows of 151936: 13 us).
 __global__ __launch_bounds__(256) void k_sample_sum(SampleRowsParams P, RowScratch *scratch, int row0) {
     __shared__ Space sp;
     __shared__ u64 hist[kBins];
@@ -809,6 +829,8 @@ __global__ __launch_bounds__(256) void k_sample_near(SampleRowsParams P, RowScra
 }
 
 // The row's end: top-k's candidates, or where the chunks' sums say the draw falls.
+// A row's few thousand candidates keep one block busy for up to 25 us (top_k =
+// 2000 and top-p after it: two cuts of 8 us), a few for 9.
 constexpr int kDrawThreads = 1024;
 
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P, RowScratch *scratch, int row0) {

@@ -13,7 +13,7 @@ import test_gpu_sample_rows as sampling
 
 pytestmark = pytest.mark.gpu
 
-HIDDEN, HEADS, KVH, HD, PAGE, VOCAB = 256, 8, 2, 64, 16, 9024  # a vocabulary of the sampler's long rows
+HIDDEN, HEADS, KVH, HD, PAGE, VOCAB = 256, 8, 2, 64, 16, 12320  # a vocabulary of the sampler's long rows
 QKV = (HEADS + 2 * KVH) * HD
 
 

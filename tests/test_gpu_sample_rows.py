@@ -214,7 +214,7 @@ def test_refusals(ctx):
     ctx.sample_rows_device(0, 8, 0, 8, 0, 0)
 
 
-@pytest.mark.parametrize("vocab", [8193, 70003])
+@pytest.mark.parametrize("vocab", [8193, 12289, 70003])
 def test_more_rows_than_the_scratch_holds(ctx, vocab):
     """Long rows share the context's scratch in turns: in each the draws that the
     same rows have among few."""
@@ -228,7 +228,7 @@ def test_more_rows_than_the_scratch_holds(ctx, vocab):
 
 
 @pytest.mark.parametrize("k", [64, 65, 257, 1999, 6000, 8300, 20000])
-@pytest.mark.parametrize("vocab", [8200, 33000, 151936])
+@pytest.mark.parametrize("vocab", [8200, 12288, 12289, 33000, 151936])
 def test_many_candidates(ctx, k, vocab):
     """Few to more than are held between the kernels; with and without top-p after
     top-k, rows that do not begin on 16 bytes."""
@@ -243,7 +243,7 @@ def test_many_candidates(ctx, k, vocab):
     check(ctx, x, r.random(rows), [0.7, 1.0, 1.3, 0.9, 2.0, 1.0], [k] * rows, p, [0.0, 0.0, 1e-3, 0.0, 0.01, 0.0], ld=vocab + 3)
 
 
-@pytest.mark.parametrize("vocab", [8200, 33000, 151936])
+@pytest.mark.parametrize("vocab", [8200, 12288, 12289, 33000, 151936])
 def test_many_tokens_at_the_cut(ctx, vocab):
     """top-p alone, with from few to all of a row's tokens in one narrow step of
     weight, in one chunk or in all of them."""
