@@ -13,9 +13,9 @@
 // sums by weight (k_sample_sum); the candidates next to the cut
 // (k_sample_near).  One block a row joins them and draws (k_sample_draw).
 //
-// Measured: 64 rows of 151936, settings of every kind among them, 13 + 13 + 13
+// Measured: 64 rows of 151936, settings of every kind among them, 14 + 12 + 13
 // + 25 us (39 MB, which a copy reads in 8); all at top_k = 50, 14 + 9 + 7 + 10;
-// one row 6 + 7 + 4 + 9 us, all of it latency.
+// one row 6 + 8 + 4 + 9 us, all of it latency.
 #include <algorithm>
 
 #include "device_common.h"
@@ -564,9 +564,19 @@ __global__ __launch_bounds__(NT) void k_sample_row(SampleRowsParams P, int row0)
 // ---------------------------------------------------------------------------
 // Rows of more than kRowVocab logits
 // ---------------------------------------------------------------------------
-constexpr int kChunk = 4096, kGroup = 64;         // logits of a block, of a maximum
+constexpr int kChunk = 4096;                      // logits of a block
 constexpr int kNear = 8192;                       // tokens next to a cut that are held
-constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk, kMaxGroups = kSampleRowsMaxVocab / kGroup;
+constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk;
+constexpr int kMaxGroups = 8192;
+
+// Logits of a maximum.  A top-k past the number of groups takes every finite logit
+// for a candidate, and the whole row from memory where those are more than are
+// held, so groups are as small as their places allow (64 rows of 32000, top_k =
+// 2000 and top-p among the settings: 121 us in groups of 16, 45 of 4).
+__host__ __device__ constexpr int group_of(int vocab) {
+    return vocab <= 4 * kMaxGroups ? 4 : vocab <= 16 * kMaxGroups ? 16 : 64;
+}
+static_assert(kSampleRowsMaxVocab <= 64 * kMaxGroups, "the groups fit");
 
 // A row's scratch.
 struct RowScratch {
@@ -583,7 +593,7 @@ struct RowScratch {
     float least;                      // top-k's candidates are no smaller; +Inf: a NaN in the row
     unsigned near[kNear];             // keys
     int near_i[kNear];                // and indices
-    unsigned group[kMaxGroups];       // the largest key of each kGroup
+    unsigned group[kMaxGroups];       // the largest key of each group
 };
 
 struct RowTop {
@@ -606,7 +616,8 @@ __device__ RowTop row_top(const RowScratch *R, int chunks, Space *sp) {
 
 // The largest key of each group and chunk, and where the chunk's is first.  Bound
 // by memory: one load of the row, 16 bytes a lane and four in flight (64 rows of
-// 151936 in 13 us: 3 TB/s, from HBM).
+// 151936 in 14 us: 2.8 TB/s, from HBM).
+template <int G>
 __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScratch *scratch, int row0) {
     __shared__ unsigned stop, sbad, slow, sleast;
     __shared__ int stoken;
@@ -621,6 +632,7 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
     f32x4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = load_logits(x, chunk * kChunk + 1024 * j + 4 * tid, V, aligned);
+    constexpr int lanes = G / 4;  // of a group
     unsigned top = 0, low = 0xffffffffu, least = 0xffffffffu;
     bool bad = false;
 #pragma unroll
@@ -632,11 +644,11 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
             g = max(g, key_of(v[j][e]));
             least = min(least, v[j][e] > -INFINITY ? key_of(v[j][e]) : 0xffffffffu);
         }
-        for (int off = 1; off < 16; off <<= 1) g = max(g, (unsigned)__shfl_xor((int)g, off, 64));
+        for (int off = 1; off < lanes; off <<= 1) g = max(g, (unsigned)__shfl_xor((int)g, off, 64));
         top = max(top, g);
         low = min(low, g > key_of(-INFINITY) ? g : 0xffffffffu);
         const int at = chunk * kChunk + 1024 * j + 4 * tid;
-        if ((tid & 15) == 0 && at < V) R->group[at / kGroup] = g;
+        if ((tid & (lanes - 1)) == 0 && at < V) R->group[at / (4 * lanes)] = g;
     }
     top = wave_top(top), low = ~wave_top(~low), least = ~wave_top(~least);
     if ((tid & 63) == 0) atomicMax(&stop, top), atomicMin(&slow, low), atomicMin(&sleast, least);
@@ -658,7 +670,7 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
 // maxima reach, by 256 steps down from the largest; the least finite logit where
 // there are not that many groups.  (-Inf is never drawn, so it is no candidate.)
 __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int groups, Space *sp) {
-    constexpr int N = 16;  // loads in flight: a row of 262144 in one step, kept for both passes
+    constexpr int N = kMaxGroups / 256;  // all in flight, and kept for both passes
     const int tid = threadIdx.x;
     unsigned g[N];
 #pragma unroll
@@ -678,7 +690,6 @@ __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int 
 #pragma unroll
                 for (int j = 0; j < N; j++)
                     if (tid + j * 256 < groups) take(g[j]);
-                for (int i = tid + N * 256; i < groups; i += 256) take(R->group[i]);
             };
             each([&](unsigned k) { atomicAdd(&sp->hist[line(k) >> 8], (u64)1); });
             __syncthreads();
@@ -697,7 +708,7 @@ __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int 
 
 // Rows that top-k cuts: where its candidates end.  Others: units by bin where
 // top-p cuts them, else the chunk's sum.  Bound by the 64-bit exponentials and,
-// by bin, the atomic sums in LDS (20 of 64 rows of 151936: 13 us).
+// by bin, the atomic sums in LDS (20 of 64 rows of 151936: 12 us).
 __global__ __launch_bounds__(256) void k_sample_sum(SampleRowsParams P, RowScratch *scratch, int row0) {
     __shared__ Space sp;
     __shared__ u64 hist[kBins];
@@ -706,7 +717,7 @@ __global__ __launch_bounds__(256) void k_sample_sum(SampleRowsParams P, RowScrat
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
     if (S.greedy || (S.top_k > 0 && chunk > 0)) return;
-    if (S.top_k > 0) return find_least(R, S, gridDim.x, (V + kGroup - 1) / kGroup, &sp);
+    if (S.top_k > 0) return find_least(R, S, gridDim.x, (V + group_of(V) - 1) / group_of(V), &sp);
     const bool sums = S.cuts_sum(), aligned = ((uintptr_t)x & 15) == 0;
     f32x4 v[4];
 #pragma unroll
@@ -781,7 +792,14 @@ __global__ __launch_bounds__(256) void k_sample_near(SampleRowsParams P, RowScra
     f32x4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = -INFINITY;
-    if (i0 < V && (!first || R->group[i0 / kGroup] >= key_of(least))) {
+    unsigned most = 0;  // of the groups that hold the 16
+    if (first && i0 < V) {
+        const unsigned *g = R->group + i0 / group_of(V);
+        if (group_of(V) == 4)
+            for (int e = 0; e < 4; e++) most = max(most, g[min(e, (V - i0 + 3) / 4 - 1)]);
+        else most = *g;
+    }
+    if (i0 < V && (!first || most >= key_of(least))) {
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = load_logits(x, i0 + 4 * j, V, aligned);
     }
@@ -950,9 +968,14 @@ void launch_sample_rows(hipStream_t st, const SampleRowsParams &p) {
     const unsigned chunks = (unsigned)((p.vocab + kChunk - 1) / kChunk);
     for (int row0 = 0; row0 < p.rows; row0 += most) {
         const unsigned n = (unsigned)std::min(most, p.rows - row0);
-        hipLaunchKernelGGL(k_sample_max, dim3(chunks, n), dim3(256), 0, st, p, scratch, row0);
-        hipLaunchKernelGGL(k_sample_sum, dim3(chunks, n), dim3(256), 0, st, p, scratch, row0);
-        if (p.p.top_p || p.p.top_k) hipLaunchKernelGGL(k_sample_near, dim3(chunks, n), dim3(256), 0, st, p, scratch, row0);
+        const dim3 grid(chunks, n);
+        switch (group_of(p.vocab)) {
+            case 4: hipLaunchKernelGGL(k_sample_max<4>, grid, dim3(256), 0, st, p, scratch, row0); break;
+            case 16: hipLaunchKernelGGL(k_sample_max<16>, grid, dim3(256), 0, st, p, scratch, row0); break;
+            default: hipLaunchKernelGGL(k_sample_max<64>, grid, dim3(256), 0, st, p, scratch, row0);
+        }
+        hipLaunchKernelGGL(k_sample_sum, grid, dim3(256), 0, st, p, scratch, row0);
+        if (p.p.top_p || p.p.top_k) hipLaunchKernelGGL(k_sample_near, grid, dim3(256), 0, st, p, scratch, row0);
         hipLaunchKernelGGL(k_sample_draw, dim3(n), dim3(kDrawThreads), 0, st, p, scratch, row0);
     }
 }
