@@ -404,8 +404,10 @@ typedef struct qtts_paged_kv {
  * tokens are neither written nor attended to (a window's dropped pages).  A
  * sequence is left out as a whole, its cache untouched, where starts[b] is
  * negative, its tokens pass max_pages * page_size (or the rotation's table) or
- * slots[b] is outside the slots.  Pages may be shared for reading; the pages
- * and slots that a call writes must be different ones. */
+ * slots[b] is outside the slots.  starts[b] may go back to a token of the page
+ * that is being filled or to a page's first; what was behind it is forgotten.
+ * Pages may be shared for reading; the pages and slots that a call writes must
+ * be different ones. */
 typedef struct qtts_paged_seqs {
     int32_t batch;
     int32_t max_pages;          /* entries of a page_table row */

@@ -161,6 +161,23 @@ def test_division_into_calls_does_not_matter(ctx):
             assert torch.equal(a, b)
 
 
+def test_going_back(ctx):
+    """To a token of the open page, to its first, to a full page's first: the
+    cache holds what was appended last, and attention sees no more."""
+    kvh, hd, page = 2, 64, 32
+    c = Cache(kvh, hd, page, 1, 5)
+    k, v = np.zeros((0, kvh, hd), np.float32), np.zeros((0, kvh, hd), np.float32)
+    for i, (start, rows) in enumerate([(0, 90), (70, 10), (64, 31), (32, 40), (72, 24), (96, 1), (96, 40), (0, 5)]):
+        nk, nv, q = (_normal(s + 3 * i, rows, kvh * hd) for s in (1, 2, 3))
+        c.append(ctx, c.seqs([start], [rows]), _up(nk), _up(nv))
+        k, v = (np.concatenate([a[:start], b.reshape(rows, kvh, hd)]) for a, b in ((k, nk), (v, nv)))
+        hk, hv = pm.held(k, page), pm.held(v, page)
+        gk, gv = c.read(ctx, c.seqs([0], [start + rows]))
+        assert np.array_equal(gk.reshape(hk.shape), hk) and np.array_equal(gv.reshape(hv.shape), hv)
+        got = c.attend(ctx, c.seqs([start], [rows]), _up(q), kvh).cpu().numpy()
+        _check(got.reshape(rows, kvh, hd), q.reshape(rows, kvh, hd), hk, hv, start, hd ** -0.5, 0)
+
+
 def test_blocks_of_odd_values(ctx):
     """Zeros, subnormals, the largest floats, Inf and NaN, exact ties."""
     page, hd = 16, 64
