@@ -287,7 +287,8 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
 //
 // Weights of V's products are p times the page's scale of V, whose logarithm
 // joins the score (t = s + log2 scale): the largest weight fills the operand's
-// range whatever V's size is.
+// range whatever V's size is.  The sum of probabilities has a reference of its own
+// and is taken from the weights (over the scale) where they hold it.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -344,13 +345,13 @@ __device__ __forceinline__ float digits_sum(float v) {
     return v + dpp<0x124>(v);
 }
 
-// The same of an open row, by its largest value's exponent.  Its ends keep both
-// the weights and the sum of probabilities (scaled back by it) in range; a row
-// of zeros weighs nothing, and takes a middle one that leaves the reference to
-// the others.
-__device__ __forceinline__ int fold_exponent(float x) {
-    const int e = (int)((__float_as_uint(x) >> 23) & 255) - 127;
-    return x == 0.0f ? -30 : e < -70 ? -70 : e > 121 ? 121 : e;
+// log2 of the scale that a row or block of zeros takes: below all others, so that
+// it leaves the reference to them.
+constexpr float kZeroScale = -200.0f;
+
+// The same of an open row, by its largest value's exponent.
+__device__ __forceinline__ float row_scale(float x) {
+    return x == 0.0f ? kZeroScale : (float)((int)((__float_as_uint(x) >> 23) & 255) - 127);
 }
 
 // Columns of one kv head over one chunk of the tokens: a block of four waves,
@@ -360,12 +361,12 @@ __device__ __forceinline__ int fold_exponent(float x) {
 // its output is.
 //
 // Few columns are bound by reading the pages: 64 sequences of up to 8000 tokens,
-// 8 kv heads of 128, 798 MB in 151 us (5.3 TB/s; a copy moves 5.1); 4 of 32760 in
+// 8 kv heads of 128, 798 MB in 153 us (5.2 TB/s; a copy moves 5.1); 4 of 32760 in
 // 46 us (4.8); 16 of 2064 in 20 us (2.7), of which 10 are a block's first loads
 // and the joining, as one sequence of 1064 tokens takes 11 us.  Many are bound by
 // vector instructions, codes to binary16 (160 of 440 a step) and the softmax, of
 // whose time the products cover half: 1064 rows of two heads behind 2000 tokens
-// 79 us, 0.28 PFLOP/s (0.56 as hi + lo).
+// 76 us, 0.29 PFLOP/s (0.58 as hi + lo).
 //
 // Of a step's 64 tokens, lane (r = lane % 16, G = lane / 16) has scores of
 // tokens 16G + 4t + i in register i of tile t, and feeds them to the output's
@@ -384,7 +385,7 @@ __device__ __forceinline__ int fold_exponent(float x) {
 // that binary16's least step is 2^-39 of a column's largest).
 //
 // Three blocks of 64 dimensions fit a CU's registers (tiles of 32 columns, 8
-// sequences of 500 rows, a window of 72: 31 us, 37 with two), two of 128.
+// sequences of 500 rows, a window of 72: 33 us, 38 with two), two of 128.
 template <int HD, int MODE>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnParams A) {
     constexpr bool I8 = MODE == kAttnI8;
@@ -401,9 +402,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     typedef float Acc __attribute__((ext_vector_type(NR)));
     __shared__ float so[4][CT][HD + 4];
     __shared__ float sm[4][CT], sl[4][CT];
+    __shared__ int sk[4][CT];
     __shared__ unsigned sarrived;
     static_assert(4 * (HD + 4) >= kPagedMaxSplits, "the parts' factors take so's place");
-    static_assert(kPagedPartFloats >= 3LL * kPagedRound / 2 * CT * (HD + 2), "the parts fit");
+    static_assert(kPagedPartFloats >= 3LL * kPagedRound / 2 * CT * (HD + 4), "the parts fit");
     const int P = A.kv.page_size, sh = __builtin_ctz(P), kvh = A.kv.kv_heads, group = A.heads / kvh;
     // Consecutive blocks lie on different XCDs.  Tiles of 32 share their pages:
     // with kv heads innermost one head's are read through few caches, and the
@@ -563,7 +565,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         qscale = odd ? __uint_as_float(0x7fc00000u) : ldexpf(A.scale * kLog2e, I8 ? e - 29 + 8 * digit : e - 14);
     }
 
+    // Weights of V are 2^(t - m); the sum of probabilities l is held relative to
+    // 2^(m - k), which stays within 2^60 of the largest: V's size, which is in t
+    // and m, takes nothing from it.
     float m = -INFINITY, l = 0;
+    int k = 0;
+    constexpr float kFar = 60.0f;
     Acc o[ND] = {};
     i32x4 oi[I8 ? ND : 1] = {};
     int held = 0;  // steps in oi
@@ -581,18 +588,27 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             }
         }
     };
+    // l's reference up to a probability of 2^rel of it, where that is far.
+    auto lift = [&](float rel) {
+        const int by = rel > kFar ? (int)rintf(rel) : 0;
+        k -= by;
+        l = ldexpf(l, -by);
+    };
     // A new reference where a column's largest t asks for it, and what was
-    // summed under the last one.
-    auto raise = [&](float top) {
-        const bool need = top > (m == -INFINITY ? -INFINITY : m + kLimit);
+    // summed under the last one; `prob`: the largest probability's logarithm.
+    auto raise = [&](float top, float prob) {
+        const bool first = m == -INFINITY, need = top > (first ? -INFINITY : m + kLimit);
         if (__any(need)) {
-            const float mn = need ? top - kRoom : m;
-            const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float mn = need ? top - kRoom : m, down = first ? 0.0f : m - mn;
+            const float c = first ? 0.0f : __builtin_amdgcn_exp2f(down);
             flush();
-            l *= c;
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= c;
+            const int by = (int)rintf(down);
+            l *= __builtin_amdgcn_exp2f(down - (float)by);
+            k = first && need ? (int)rintf(mn - prob) : k - by;
             m = mn;
+            if (need) lift(prob - m + (float)k);
         }
     };
 
@@ -681,7 +697,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         float p[NR];
         bool odd = false;
         if (mine) {
-            float mx = -INFINITY;
+            float mx = -INFINITY, prob = -INFINITY;
+            unsigned zeros = 0, smalls = 0;  // of the rows here
             const float by = S == 16 ? A.scale * kLog2e : qscale;
 #pragma unroll
             for (int i = 0; i < NR; i++) {
@@ -697,23 +714,32 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 if (S == 32) top = fmaxf(top, dpp_row_pair(top));
                 const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
                 p[i] = seen ? (I8 ? digits_sum(s[i]) : s[i]) * by : -INFINITY;
-                mx = fmaxf(mx, p[i] + (float)fold_exponent(top * (1.0f / 128.0f)));
+                const float big = row_scale(top);
+                zeros |= (unsigned)(big == kZeroScale) << i, smalls |= (unsigned)(big < -80.0f) << i;
+                mx = fmaxf(mx, p[i] + big - 7.0f);  // as a page's, whose codes go to 127
+                prob = fmaxf(prob, p[i]);
+                if (S == 32 && i % 4 == 3) asm volatile("" ::: "memory");  // a few rows of LDS at once
             }
-            raise(group_max(mx));
+            prob = group_max(prob);
+            raise(group_max(mx), prob);
             const float ms = m == -INFINITY ? 0.0f : m;
+            lift(prob - ms + (float)k);
 #pragma unroll
             for (int i = 0; i < NR; i++) {
-                const float y = __builtin_amdgcn_exp2f(p[i] - ms);
-                l += y;
-                p[i] = digit ? 0.0f : y;
+                l += __builtin_amdgcn_exp2f(p[i] - ms + (float)k);
+                // 2^60 of a small row's weight goes over to its values, and zeros have none
+                const float over = zeros >> i & 1 ? kZeroScale : smalls >> i & 1 ? -60.0f : 0.0f;
+                p[i] = digit ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms + over);
             }
 #pragma unroll
-            for (int i = 0; i < NR; i++)
+            for (int i = 0; i < NR; i++) {
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
                     const float y = value(i, d);
-                    o[d] = mma1(fabsf(y) < INFINITY ? y : 0.0f, p[i], o[d]);
+                    o[d] = mma1(fabsf(y) < INFINITY ? y * (smalls >> i & 1 ? 0x1p60f : 1.0f) : 0.0f, p[i], o[d]);
                 }
+                if (S == 32 && i % 4 == 3) asm volatile("" ::: "memory");  // as above
+            }
         }
         // (with tiles of 32 the block decides, as V's rows give way to the weights)
         if (S == 32 ? __syncthreads_or(odd) : __any(odd)) {
@@ -723,7 +749,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 for (int i = 0; i < NR; i++) weight[row_of(i) * S + r] = p[i];
 #pragma unroll 1
                 for (int token = t0; token < min(t0 + S, open_hi); token++) {
-                    const float w = weight[(token - t0) * S + r];
+                    const float w = fmaxf(weight[(token - t0) * S + r], 0x1p-126f);
                     const bool seen = token <= pos && (A.window == 0 || token > pos - A.window) && !digit;
                     const float *vp = v_open + (token & (P - 1)) * HD;
 #pragma unroll
@@ -732,6 +758,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                         for (int i = 0; i < NR; i++) {
                             const float y = vp[S * d + row_of(i)];
                             if (seen && !(fabsf(y) < INFINITY)) o[d][i] += w * y;
+                            if (i % 4 == 3) asm volatile("" ::: "memory");  // as above
                         }
                 }
             }
@@ -782,11 +809,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         }
         const float kq = qscale * ks_;
         // The page's scale of V joins the scores as its logarithm, and leaves
-        // the sum of probabilities as its inverse (blocks of zeros as a middle
-        // one; the least scales as 2^-70, and the rest as a factor).
-        const float least = 0x1p-70f;
-        const float vc = !there || vs_ == 0.0f ? 0x1p-30f : vs_ < least ? least : vs_;
-        const float lg = __builtin_amdgcn_logf(vc), inv = __builtin_amdgcn_rcpf(vc);
+        // the sum of probabilities as its inverse.
+        const bool small = vs_ < 0x1p-64f, zero = !there || vs_ == 0.0f;
+        const float vc = small ? vs_ * 0x1p64f : vs_;
+        const float lg = zero ? kZeroScale : __builtin_amdgcn_logf(vc) - (small ? 64.0f : 0.0f);
         const float ms = m == -INFINITY ? 0.0f : m;
         const float off = digit ? 0.0f : lg - ms;
 #pragma unroll
@@ -810,10 +836,21 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
         for (int j = 0; j < 16; j++) mx = fmaxf(mx, p[j]);
         if (__any(mx > (m == -INFINITY ? -INFINITY : (float)kLimit))) {
-            raise(group_max(mx) + ms);
+            raise(group_max(mx) + ms, group_max(mx - lg) + ms);
             const float by = ms - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
             for (int j = 0; j < 16; j++) p[j] += by;
+        }
+        // weights of a V that is so much smaller than the others' hold no
+        // probabilities: these are then taken by themselves
+        const bool apart = __any(there && (vs_ == 0.0f || (float)k - lg >= kFar));
+        if (apart) {
+            float prob = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; j++) prob = fmaxf(prob, p[j]);
+            lift(group_max(prob - lg) + (float)k);
+#pragma unroll
+            for (int j = 0; j < 16; j++) l += __builtin_amdgcn_exp2f(p[j] - lg + (float)k);
         }
         float sum = 0;
 #pragma unroll
@@ -821,10 +858,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             p[j] = __builtin_amdgcn_exp2f(p[j]);
             sum += p[j];
         }
-        l = fmaf(sum, inv, l);
-        if (__any(there && vs_ < least && vs_ != 0.0f))
-#pragma unroll
-            for (int j = 0; j < 16; j++) p[j] *= vs_ < least ? vs_ * 0x1p70f : 1.0f;
+        // (the sum is 0 where a lane's page is absent or all is masked, as a NaN scale)
+        if (!apart && sum != 0.0f) l = fmaf(sum, ldexpf(__builtin_amdgcn_rcpf(vc), small ? k + 64 : k), l);
         if constexpr (I8) {
             i32x4 w;
 #pragma unroll
@@ -869,7 +904,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     flush();
     l = group_add(l);
     const bool writes = !I8 || digit == 0;
-    if (G == 0 && writes) sm[wave][n] = m, sl[wave][n] = l;
+    if (G == 0 && writes) sm[wave][n] = m, sl[wave][n] = l, sk[wave][n] = k;
     const float weight = ldexpf(1.0f, 8 * digit);
 #pragma unroll
     for (int d = 0; d < ND; d++) {
@@ -883,24 +918,30 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 *reinterpret_cast<f32x4 *>(&so[wave][n][S * d + row_of(i)]) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
     }
     __syncthreads();
-    float *part = A.part + (size_t)shared * nsplit * CT * (HD + 2);
-    if ((int)threadIdx.x < left) {  // the waves' factors, the column's sum
+    // Joining, of waves and of parts: outputs relative to the largest reference,
+    // sums to the one whose power of two is nearest to the largest of theirs.
+    constexpr int PW = HD + 4;  // floats of a part's column: output, reference, sum, k
+    float *part = A.part + (size_t)shared * nsplit * CT * PW;
+    if ((int)threadIdx.x < left) {
         const int c = threadIdx.x;
-        float mx = -INFINITY, sum = 0;
+        float mx = -INFINITY, far = -INFINITY, sum = 0;
 #pragma unroll
         for (int w = 0; w < 4; w++) mx = fmaxf(mx, sm[w][c]);
         const float ms = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
+        for (int w = 0; w < 4; w++) far = fmaxf(far, sm[w][c] - ms - (float)sk[w][c]);
+        const int kj = far == -INFINITY ? 0 : -(int)rintf(far);
+#pragma unroll
         for (int w = 0; w < 4; w++) {
-            const float f = __builtin_amdgcn_exp2f(sm[w][c] - ms);
-            sum = fmaf(f, sl[w][c], sum);
-            sm[w][c] = f;
+            const float d = sm[w][c] - ms;
+            sum += sl[w][c] == 0.0f ? 0.0f : sl[w][c] * __builtin_amdgcn_exp2f(d == -INFINITY ? 0.0f : d + (float)(kj - sk[w][c]));
+            sm[w][c] = __builtin_amdgcn_exp2f(d);
         }
         if (parts == 1) {
-            sl[0][c] = sum;
+            sl[0][c] = sum, sk[0][c] = kj;
         } else {
-            float *to = part + ((size_t)split * CT + c) * (HD + 2) + HD;
-            st_dev(to, mx), st_dev(to + 1, sum);
+            float *to = part + ((size_t)split * CT + c) * PW + HD;
+            st_dev(to, mx), st_dev(to + 1, sum), st_dev(to + 2, (float)kj);
         }
     }
     __syncthreads();
@@ -912,9 +953,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         if (parts == 1) {
             const float sum = sl[0][c];
             acc = sum == 0.0f ? f32x4{0, 0, 0, 0} : acc / sum;
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[j] = ldexpf(acc[j], sk[0][c]);
             *reinterpret_cast<f32x4 *>(out_of(c) + d) = acc;
         } else {
-            float *to = part + ((size_t)split * CT + c) * (HD + 2) + d;
+            float *to = part + ((size_t)split * CT + c) * PW + d;
 #pragma unroll
             for (int j = 0; j < 4; j += 2)
                 st_dev_u64(reinterpret_cast<uint64_t *>(to + j),
@@ -942,18 +985,19 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
             for (int i = 0; i < MI; i++) {
                 const int at = min((int)threadIdx.x + 256 * i, pairs - 1), k = min(k0 + u, parts - 1);
-                const float *from = part + ((size_t)k * CT + at / (HD / 2)) * (HD + 2) + 2 * (at % (HD / 2));
+                const float *from = part + ((size_t)k * CT + at / (HD / 2)) * PW + 2 * (at % (HD / 2));
                 y[u][i] = ld_dev_u64(reinterpret_cast<const uint64_t *>(from));
             }
     };
     load_parts(0);
     for (int c = wave; c < left; c += 4) {
         constexpr int N = kPagedMaxSplits / 64;
-        float pm[N], ps[N], mx = -INFINITY, sum = 0;
+        float pm[N], ps[N], pk[N], mx = -INFINITY, far = -INFINITY, sum = 0;
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const float *from = part + ((size_t)min(lane + 64 * j, parts - 1) * CT + c) * (HD + 2) + HD;
+            const float *from = part + ((size_t)min(lane + 64 * j, parts - 1) * CT + c) * PW + HD;
             const uint64_t z = ld_dev_u64(reinterpret_cast<const uint64_t *>(from));
+            pk[j] = ld_dev(from + 2);
             pm[j] = lane + 64 * j < parts ? __uint_as_float((unsigned)z) : -INFINITY;
             ps[j] = lane + 64 * j < parts ? __uint_as_float((unsigned)(z >> 32)) : 0.0f;
         }
@@ -962,13 +1006,17 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         mx = wave_max(mx);
         const float ms = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
+        for (int j = 0; j < N; j++) far = fmaxf(far, pm[j] - ms - pk[j]);
+        far = wave_max(far);
+        const float kj = far == -INFINITY ? 0.0f : -rintf(far);
+#pragma unroll
         for (int j = 0; j < N; j++) {
-            const float f = __builtin_amdgcn_exp2f(pm[j] - ms);
-            if (lane + 64 * j < parts) fac[c * parts + lane + 64 * j] = f;
-            sum = fmaf(f, ps[j], sum);
+            const float d = pm[j] - ms;
+            if (lane + 64 * j < parts) fac[c * parts + lane + 64 * j] = __builtin_amdgcn_exp2f(d);
+            sum += ps[j] == 0.0f ? 0.0f : ps[j] * __builtin_amdgcn_exp2f(d == -INFINITY ? 0.0f : d + (kj - pk[j]));
         }
         sum = wave_sum(sum);
-        if (lane == 0) sl[0][c] = sum;
+        if (lane == 0) sl[0][c] = sum, sk[0][c] = (int)kj;
     }
     __syncthreads();
     float acc[MI][2] = {};
@@ -991,7 +1039,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         if (at >= pairs) break;
         const float sum = sl[0][c];
         *reinterpret_cast<float2 *>(out_of(c) + 2 * (at % (HD / 2))) =
-            sum == 0.0f ? make_float2(0, 0) : make_float2(acc[i][0] / sum, acc[i][1] / sum);
+            sum == 0.0f ? make_float2(0, 0)
+                        : make_float2(ldexpf(acc[i][0] / sum, sk[0][c]), ldexpf(acc[i][1] / sum, sk[0][c]));
     }
 }
 

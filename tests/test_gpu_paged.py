@@ -401,6 +401,56 @@ def test_values_that_a_mask_hides(ctx, rows):
         assert torch.isinf(two[-1, 2 * hd + 3]) and torch.isinf(two[-1, 3 * hd + 3])
 
 
+SIZES = [0, 1e-44, 1e-42, 1e-39, 1e-37, 1e-30, 1, 1e30, 1e37, 3e38]
+
+
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("group,rows", [(1, 1), (6, 1), (1, 5), (8, 12), (2, 40)])
+def test_values_of_every_size(ctx, group, rows, mixed):
+    """V from zeros and the least floats to the largest, one size to a sequence or
+    another in each page: pages whose values are nothing beside the others' keep
+    their probabilities.
+
+    Weights carry V's scale as its logarithm: it, its sum with a score and the
+    difference from a reference are each rounded below 512, by 2^-16, and so is the
+    reference: 4 ln 2 2^-16 < 2^-14 of a weight.  Then half a least step, 2^-28 of
+    the largest weight (see above) for each token, times its block's largest value,
+    and a step of the least floats."""
+    kvh, hd, page, n, each = 1, 64, 16, 100, len(SIZES)
+    k, q = _normal(1, each * n, kvh * hd), _normal(3, each * rows, kvh * group * hd)
+    v = np.clip(_normal(2, each * n, kvh * hd), -1, 1)
+    for b in range(each):
+        for at in range(0, n, page):
+            v[b * n + at:min(b * n + at + page, (b + 1) * n)] *= np.float32(SIZES[(b + mixed * at // page) % each])
+    c = Cache(kvh, hd, page, each, 7)
+    c.append(ctx, c.seqs([0] * each, [n] * each), _up(k), _up(v))
+    got = c.attend(ctx, c.seqs([n - rows] * each, [rows] * each), _up(q), kvh * group).cpu().numpy()
+    for b in range(each):
+        hk, hv = (pm.held(x[b * n:(b + 1) * n].reshape(n, kvh, hd), page) for x in (k, v))
+        mine = slice(b * rows, (b + 1) * rows)
+        ref, mass, slack = pm.attention(q[mine].reshape(rows, -1, hd), hk, hv, n - rows, hd ** -0.5, 0)
+        err = np.abs(got[mine].reshape(ref.shape) - ref)
+        tol = mass * (2 * slack[..., None] + 2.0 ** -14 + (n / 64 + 64) * 2.0 ** -24)
+        assert np.all(err <= tol + 2.0 ** -28 * n * np.abs(hv).max().astype(np.float64) + 2.0 ** -148), b
+
+
+@pytest.mark.parametrize("group,rows", [(1, 4), (1, 12), (4, 12), (2, 40)])
+def test_a_block_of_nan_in_the_middle_of_a_tile(ctx, group, rows):
+    """A page that reads as NaN begins between two rows of one tile: those before
+    it are as they were."""
+    kvh, hd, page = 2, 128, 16
+    start = 3 * page - rows // 2
+    c, _ = _filled(ctx, kvh, hd, page, [start], [rows + page], seed=4)
+    q, s = _up(_normal(5, rows + page, kvh * group * hd)), c.seqs([start], [rows + page])
+    ref = c.attend(ctx, s, q, kvh * group)
+    for scales in (c.v_scales, c.k_scales):
+        kept = scales.clone()
+        scales[int(c.table[0, 3])] = float("nan")
+        got = c.attend(ctx, s, q, kvh * group)
+        assert torch.equal(got[: rows // 2], ref[: rows // 2]) and torch.isnan(got[rows // 2:]).all()
+        scales.copy_(kept)
+
+
 def test_rows_of_nan_and_blocks_of_nan(ctx):
     """A NaN query gives its own row NaN; a block whose values read as NaN gives
     NaN to the rows that see it and to no others."""

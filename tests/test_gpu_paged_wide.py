@@ -61,6 +61,19 @@ def test_rows_of_nan_and_blocks_of_nan(ctx, padded):
     base.test_rows_of_nan_and_blocks_of_nan(ctx)
 
 
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("group,rows", [(1, 40), (8, 12)])
+def test_values_of_every_size(ctx, padded, group, rows, mixed):
+    padded(group)
+    base.test_values_of_every_size(ctx, group, rows, mixed)
+
+
+@pytest.mark.parametrize("group,rows", [(2, 40), (4, 12)])
+def test_a_block_of_nan_in_the_middle_of_a_tile(ctx, padded, group, rows):
+    padded(group)
+    base.test_a_block_of_nan_in_the_middle_of_a_tile(ctx, group, rows)
+
+
 @pytest.mark.parametrize("hd,page", [(64, 16), (128, 64)])
 def test_absent_pages(ctx, padded, hd, page):
     """Pages outside the pool, in tiles of 32 columns; a sequence without any."""
