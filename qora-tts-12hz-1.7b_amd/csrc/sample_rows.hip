@@ -675,13 +675,14 @@ __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int 
     unsigned g[N];
 #pragma unroll
     for (int j = 0; j < N; j++) g[j] = R->group[min(tid + j * 256, groups - 1)];
+    const bool all = S.top_k >= groups;
+    const unsigned lowest = (all ? R->least_key : R->low)[min(tid, chunks - 1)];
     if (tid == 0) sp->thr = 0xffffffffu, sp->count = 0xffffffffu;
     sp->hist[tid] = 0;
     const RowTop t = row_top(R, chunks, sp);
     float least = INFINITY;
     if (!t.bad) {
-        const bool all = S.top_k >= groups;
-        if (tid < chunks) atomicMin(&sp->thr, all ? R->least_key[tid] : R->low[tid]);
+        if (tid < chunks) atomicMin(&sp->thr, lowest);
         __syncthreads();
         least = logit_of(sp->thr);
         if (!all) {
@@ -861,6 +862,10 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
     RowScratch *R = scratch + blockIdx.x;
     const float *x = P.logits + (size_t)r * P.ld;
     const RowSettings S(P, r);
+    // asked for with the first loads, where they are needed or not
+    const int mine_at = min(tid, chunks - 1);
+    const unsigned near_n = R->near_n[mine_at], near_at = R->near_at[mine_at];
+    const float u = P.u[r], least = R->least;
     fill_table(sp.tab);
     const RowTop t = row_top(R, chunks, &sp);
     const float mx = logit_of(t.top);
@@ -877,7 +882,6 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
         return;
     }
     const Weights W = weights_of(S, mx, sp.tab);
-    const float u = P.u[r];
     auto far_key = [&](int i) { return key_of(x[i]); };
     auto near_key = [&](int i) { return keys[i]; };
     auto whole = [&]() {  // the row from memory: many passes
@@ -888,13 +892,13 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
     };
     u64 total;
     // Candidates into LDS, in the order of their indices.
-    const unsigned mine = tid < chunks ? R->near_n[tid] : 0;
+    const unsigned mine = tid < chunks ? near_n : 0;
     unsigned first = 0;
     u64 held = 0;
     if (S.top_k > 0 || S.cuts_sum()) {
         first = (unsigned)(block_scan<NT>(mine, sp.wsum, &held) - mine);
         if (held > kNear) return whole();  // many equal logits, or top_k past a few thousand
-        if (tid < chunks) offset[tid] = (int)first - (int)R->near_at[tid];
+        if (tid < chunks) offset[tid] = (int)first - (int)near_at;
         __syncthreads();
         for (int j0 = tid; j0 < (int)held; j0 += 4 * NT) {
             unsigned k[4];
@@ -919,7 +923,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleRowsParams P
             if (tid < 64) finish_wave(P, r, tid < n ? keys[tid] : 0, n, [&](int i) { return place[i]; }, S, W, 0);
             return;
         }
-        const u64 cut = cut_of<NT>(near_key, n, Line(mx, R->least), false, S, W, 0, &sp);
+        const u64 cut = cut_of<NT>(near_key, n, Line(mx, least), false, S, W, 0, &sp);
         const int i = draw_of<NT>(near_key, 0, n, cut, S, W, u, ~0ull, &total, &sp);
         if (i >= 0) drawn(P, r, place[i], W.weight(logit_of(keys[i])), total);
         return;
