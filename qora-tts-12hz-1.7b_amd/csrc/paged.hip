@@ -348,6 +348,7 @@ __device__ __forceinline__ float digits_sum(float v) {
 // log2 of the scale that a row or block of zeros takes: below all others, so that
 // it leaves the reference to them.
 constexpr float kZeroScale = -200.0f;
+constexpr float kSmallRow = -80.0f;  // below it a row's values are taken times 2^60
 
 // The same of an open row, by its largest value's exponent.
 __device__ __forceinline__ float row_scale(float x) {
@@ -366,7 +367,7 @@ __device__ __forceinline__ float row_scale(float x) {
 // and the joining, as one sequence of 1064 tokens takes 11 us.  Many are bound by
 // vector instructions, codes to binary16 (160 of 440 a step) and the softmax, of
 // whose time the products cover half: 1064 rows of two heads behind 2000 tokens
-// 76 us, 0.29 PFLOP/s (0.58 as hi + lo).
+// 75 us, 0.29 PFLOP/s (0.58 as hi + lo).
 //
 // Of a step's 64 tokens, lane (r = lane % 16, G = lane / 16) has scores of
 // tokens 16G + 4t + i in register i of tile t, and feeds them to the output's
@@ -385,7 +386,7 @@ __device__ __forceinline__ float row_scale(float x) {
 // that binary16's least step is 2^-39 of a column's largest).
 //
 // Three blocks of 64 dimensions fit a CU's registers (tiles of 32 columns, 8
-// sequences of 500 rows, a window of 72: 33 us, 38 with two), two of 128.
+// sequences of 500 rows, a window of 72: 32 us, 38 with two), two of 128.
 template <int HD, int MODE>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnParams A) {
     constexpr bool I8 = MODE == kAttnI8;
@@ -403,6 +404,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     __shared__ float so[4][CT][HD + 4];
     __shared__ float sm[4][CT], sl[4][CT];
     __shared__ int sk[4][CT];
+    __shared__ float srow[S == 32 ? 128 : 1];  // the open rows' largest |v|
     __shared__ unsigned sarrived;
     static_assert(4 * (HD + 4) >= kPagedMaxSplits, "the parts' factors take so's place");
     static_assert(kPagedPartFloats >= 3LL * kPagedRound / 2 * CT * (HD + 4), "the parts fit");
@@ -620,8 +622,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     const float *k_open = A.kv.k_open + ((size_t)q.slot * kvh + head) * P * HD;
     const float *v_open = A.kv.v_open + ((size_t)q.slot * kvh + head) * P * HD;
     float(*rows)[HD + 4] = so[0];  // S == 32: row t - open_lo of the open page, 128 at most
-    auto stage = [&](const float *from) {
+    // V's are staged as the products take them: what is not finite as 0, small
+    // rows times 2^60, their largest values in srow; returns whether something is
+    // not finite.
+    auto stage = [&](const float *from, bool values) {
         const int count = (open_hi - open_lo) * (HD / 4);
+        bool bad = false;
         for (int i0 = threadIdx.x; i0 < count; i0 += 1024) {  // four loads in flight
             f32x4 y[4];
 #pragma unroll
@@ -632,14 +638,30 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int i = min(i0 + 256 * j, count - 1);
-                *reinterpret_cast<f32x4 *>(&rows[i / (HD / 4)][4 * (i % (HD / 4))]) = y[j];
+                if (values) {
+                    float top = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool finite = fabsf(y[j][e]) < INFINITY;
+                        bad |= !finite;
+                        y[j][e] = finite ? y[j][e] : 0.0f;
+                        top = fmaxf(top, fabsf(y[j][e]));
+                    }
+                    top = row16_max(top);
+                    if (HD == 128) top = fmaxf(top, dpp_row_pair(top));
+                    if (row_scale(top) < kSmallRow) y[j] *= 0x1p60f;
+                    if (i0 + 256 * j < count) srow[i / (HD / 4)] = top;
+                }
+                if (i0 + 256 * j < count) *reinterpret_cast<f32x4 *>(&rows[i / (HD / 4)][4 * (i % (HD / 4))]) = y[j];
             }
         }
+        return bad;
     };
     auto open_tile = [&](int t0) {
         const bool mine = t0 < open_hi;  // S == 32: others only take part in the staging
         Acc s = {}, s1 = {};
         float v[S == 16 ? NR : 1][ND];
+        bool odd = false;
         if (S == 16) {
             const int kt = t0 + r;  // K: row r of the tile
             const float *kp = k_open + ((kt < open_hi ? kt : open_lo) & (P - 1)) * HD + 4 * G;
@@ -666,7 +688,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             }
             s += s1;
         } else {
-            stage(k_open);
+            stage(k_open, false);
             __syncthreads();
             if (mine) {
                 const float *kp = rows[min(t0 + r, open_hi - 1) - open_lo] + 16 * G;
@@ -683,19 +705,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                     }
             }
             __syncthreads();
-            stage(v_open);
+            odd = stage(v_open, true);
             __syncthreads();
         }
-        auto value = [&](int i, int d) {  // of V, 0 past the last token
-            if (S == 16) return v[S == 16 ? i : 0][d];
-            const int t = t0 + row_of(i);
-            const float y = rows[min(t, open_hi - 1) - open_lo][S * d + r];
-            return t < open_hi ? y : 0.0f;
-        };
         // What is not finite is left out of V's products (0 * Inf would reach
         // rows that do not see it) and added by itself below.
         float p[NR];
-        bool odd = false;
         if (mine) {
             float mx = -INFINITY, prob = -INFINITY;
             unsigned zeros = 0, smalls = 0;  // of the rows here
@@ -704,21 +719,23 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             for (int i = 0; i < NR; i++) {
                 const int token = t0 + row_of(i);
                 float top = 0;
+                if (S == 32) {
+                    top = srow[min(token, open_hi - 1) - open_lo];
+                } else {
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const float y = fabsf(value(i, d));
-                    odd |= !(y < INFINITY);
-                    top = fmaxf(top, y < INFINITY ? y : 0.0f);
+                    for (int d = 0; d < ND; d++) {
+                        const float y = fabsf(v[S == 16 ? i : 0][d]);
+                        odd |= !(y < INFINITY);
+                        top = fmaxf(top, y < INFINITY ? y : 0.0f);
+                    }
+                    top = row16_max(top);
                 }
-                top = row16_max(top);
-                if (S == 32) top = fmaxf(top, dpp_row_pair(top));
                 const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
                 p[i] = seen ? (I8 ? digits_sum(s[i]) : s[i]) * by : -INFINITY;
                 const float big = row_scale(top);
-                zeros |= (unsigned)(big == kZeroScale) << i, smalls |= (unsigned)(big < -80.0f) << i;
+                zeros |= (unsigned)(big == kZeroScale) << i, smalls |= (unsigned)(big < kSmallRow) << i;
                 mx = fmaxf(mx, p[i] + big - 7.0f);  // as a page's, whose codes go to 127
                 prob = fmaxf(prob, p[i]);
-                if (S == 32 && i % 4 == 3) asm volatile("" ::: "memory");  // a few rows of LDS at once
             }
             prob = group_max(prob);
             raise(group_max(mx), prob);
@@ -731,14 +748,29 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 const float over = zeros >> i & 1 ? kZeroScale : smalls >> i & 1 ? -60.0f : 0.0f;
                 p[i] = digit ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms + over);
             }
+            if (S == 32) {
 #pragma unroll
-            for (int i = 0; i < NR; i++) {
+                for (int i0 = 0; i0 < NR; i0 += 4) {  // four tokens' values ahead of their products
+                    float y[4][ND];
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const float y = value(i, d);
-                    o[d] = mma1(fabsf(y) < INFINITY ? y * (smalls >> i & 1 ? 0x1p60f : 1.0f) : 0.0f, p[i], o[d]);
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int d = 0; d < ND; d++)
+                            y[j][d] = rows[min(t0 + row_of(i0 + j), open_hi - 1) - open_lo][S * d + r];
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int d = 0; d < ND; d++) o[d] = mma1(y[j][d], p[i0 + j], o[d]);
                 }
-                if (S == 32 && i % 4 == 3) asm volatile("" ::: "memory");  // as above
+            } else {
+#pragma unroll
+                for (int i = 0; i < NR; i++)
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        const float y = v[S == 16 ? i : 0][d];
+                        o[d] = mma1(fabsf(y) < INFINITY ? y * (smalls >> i & 1 ? 0x1p60f : 1.0f) : 0.0f, p[i], o[d]);
+                    }
             }
         }
         // (with tiles of 32 the block decides, as V's rows give way to the weights)
