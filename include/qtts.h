@@ -460,7 +460,9 @@ qtts_status qtts_paged_attention_device(qtts_ctx *ctx, const qtts_paged_kv *kv, 
  * NULL: up to its last row asked for), gives positions starts[b] and on into
  * rows row_offsets[b] up to row_offsets[b + 1] of k_out and v_out (kv_heads *
  * head_dim floats a row, ld_* apart; either may be NULL).  Positions of
- * absent pages read as zeros, as do those past lens[b]. */
+ * absent pages read as zeros, as do those past lens[b] and the rows of a
+ * sequence left out; rows behind the last sequence stay as they were.  Enqueued
+ * on the context stream, allocates nothing and can be captured. */
 qtts_status qtts_paged_read_device(qtts_ctx *ctx, const qtts_paged_kv *kv, const qtts_paged_seqs *seqs,
                                    const int32_t *d_lens, float *d_k_out, int32_t ld_k_out, float *d_v_out,
                                    int32_t ld_v_out);
