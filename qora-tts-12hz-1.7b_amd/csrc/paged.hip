@@ -291,6 +291,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
 // and is taken from the weights (over the scale) where they hold it.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -344,6 +345,11 @@ __device__ __forceinline__ float digits_sum(float v) {
     v += dpp<0x128>(v);  // row_ror:8
     return v + dpp<0x124>(v);
 }
+
+// To the nearest integer: a weight's rounding has to favour no side, as thousands
+// of small ones add up beside a large one (truncated, 30000 tokens' share of 0.2
+// came out 1e-4 of it short).
+__device__ __forceinline__ int nearest(float x) { return (int)rintf(x); }
 
 // log2 of the scale that a row or block of zeros takes: below all others, so that
 // it leaves the reference to them.
@@ -896,8 +902,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             i32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                w[j] = digits4((int)(unsigned)p[4 * j], (int)(unsigned)p[4 * j + 1], (int)(unsigned)p[4 * j + 2],
-                               (int)(unsigned)p[4 * j + 3], pick, flip);
+                w[j] = digits4(nearest(p[4 * j]), nearest(p[4 * j + 1]), nearest(p[4 * j + 2]), nearest(p[4 * j + 3]),
+                               pick, flip);
 #pragma unroll
             for (int d = 0; d < ND; d++)
                 oi[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, vr[d]), w, oi[d], 0, 0, 0);
@@ -905,10 +911,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         } else {
             f16x8 ph[2], pl[2];
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {  // hi rounded towards zero, lo holds the rest
-                const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]));
-                const f16x2 c = __builtin_bit_cast(
-                    f16x2, __builtin_amdgcn_cvt_pkrtz(p[j] - (float)a[0], p[j + 1] - (float)a[1]));
+            for (int j = 0; j < 16; j += 2) {  // lo holds the rest; both to the nearest
+                const f16x2 a = __builtin_convertvector(f32x2{p[j], p[j + 1]}, f16x2);
+                const f16x2 c = __builtin_convertvector(f32x2{p[j] - (float)a[0], p[j + 1] - (float)a[1]}, f16x2);
                 ph[j / 8][j % 8] = a[0], ph[j / 8][j % 8 + 1] = a[1];
                 pl[j / 8][j % 8] = c[0], pl[j / 8][j % 8 + 1] = c[1];
             }

@@ -401,6 +401,24 @@ def test_values_that_a_mask_hides(ctx, rows):
         assert torch.isinf(two[-1, 2 * hd + 3]) and torch.isinf(two[-1, 3 * hd + 3])
 
 
+@pytest.mark.parametrize("group,rows", [(1, 1), (4, 1), (6, 1), (2, 20)])
+def test_many_small_weights_beside_a_large_one(ctx, group, rows):
+    """One token with most of the probability and thousands that share the rest, in
+    one block (of a batch that fills the card): roundings of small weights cancel,
+    none is towards one side, which would show as some 2e-5 of the output here."""
+    kvh, hd, page, n, pad = 1, 64, 64, 30000, 511
+    c = Cache(kvh, hd, page, 1, -(-(n + rows) // page))
+    q = np.tile(_normal(1, 1, hd), (rows, group)) + 0.01 * _normal(2, rows, group * hd)
+    k, v = 0.02 * _normal(3, n + rows, hd), 0.5 + 0.5 * np.abs(_normal(4, n + rows, hd))
+    k[1000] = q[0, :hd] * (np.log(4 * n) * hd ** 0.5 / (q[0, :hd] ** 2).sum())
+    c.append(ctx, c.seqs([0], [n + rows]), _up(k), _up(v))
+    s = c.seqs([0] * pad + [n], [0] * pad + [rows], table=c.table.expand(pad + 1, -1).contiguous(), slots=[0] * (pad + 1))
+    got = c.attend(ctx, s, _up(q), group).cpu().numpy().reshape(rows, group, hd)
+    hk, hv = (pm.held(x.reshape(n + rows, kvh, hd), page) for x in (k, v))
+    ref, _, _ = pm.attention(q.reshape(rows, group, hd), hk, hv, n, hd ** -0.5, 0)
+    assert np.abs(got / ref - 1).max() < 5e-6
+
+
 SIZES = [0, 1e-44, 1e-42, 1e-39, 1e-37, 1e-30, 1, 1e30, 1e37, 3e38]
 
 
