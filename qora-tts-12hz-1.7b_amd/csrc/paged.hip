@@ -346,10 +346,10 @@ __device__ __forceinline__ float digits_sum(float v) {
     return v + dpp<0x124>(v);
 }
 
-// To the nearest integer: a weight's rounding has to favour no side, as thousands
+// A weight's integer, the nearest: its rounding has to favour no side, as thousands
 // of small ones add up beside a large one (truncated, 30000 tokens' share of 0.2
 // came out 1e-4 of it short).
-__device__ __forceinline__ int nearest(float x) { return (int)rintf(x); }
+__device__ __forceinline__ int nearest(float x, float scale) { return (int)fmaf(x, scale, 0.5f); }
 
 // log2 of the scale that a row or block of zeros takes: below all others, so that
 // it leaves the reference to them.
@@ -403,8 +403,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     constexpr int NT = ST / S;                    // token tiles of a step
     constexpr int NK = HD / ST, ND = HD / S;      // 16-byte pieces of a K row in a lane; dimension tiles
     // Weights are 2^(t - m); the reference m is set so that the largest is
-    // 2^kRoom, and again when one would pass 2^kLimit.
-    constexpr int kRoom = I8 ? 27 : 11, kLimit = I8 ? 30 : 15;
+    // 2^kRoom, and again when one would pass 2^kLimit.  Integers take them times
+    // 2^27, so that t - m is small, and its rounding too, where the weight is large
+    // (binary16 would take a product each).
+    constexpr int kRoom = I8 ? 0 : 11, kLimit = I8 ? 3 : 15, kUnits = I8 ? 27 : 0;
     constexpr int kFlush = 1024;                  // steps that int32 sums hold: 64 * 128 * 127 each
     typedef float Acc __attribute__((ext_vector_type(NR)));
     __shared__ float so[4][CT][HD + 4];
@@ -752,7 +754,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 l += __builtin_amdgcn_exp2f(p[i] - ms + (float)k);
                 // 2^60 of a small row's weight goes over to its values, and zeros have none
                 const float over = zeros >> i & 1 ? kZeroScale : smalls >> i & 1 ? -60.0f : 0.0f;
-                p[i] = digit ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms + over);
+                p[i] = digit ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms + over) * (float)(1 << kUnits);
             }
             if (S == 32) {
 #pragma unroll
@@ -902,8 +904,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             i32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                w[j] = digits4(nearest(p[4 * j]), nearest(p[4 * j + 1]), nearest(p[4 * j + 2]), nearest(p[4 * j + 3]),
-                               pick, flip);
+                w[j] = digits4(nearest(p[4 * j], 0x1p27f), nearest(p[4 * j + 1], 0x1p27f),
+                               nearest(p[4 * j + 2], 0x1p27f), nearest(p[4 * j + 3], 0x1p27f), pick, flip);
 #pragma unroll
             for (int d = 0; d < ND; d++)
                 oi[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, vr[d]), w, oi[d], 0, 0, 0);
@@ -942,7 +944,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     l = group_add(l);
     const bool writes = !I8 || digit == 0;
     if (G == 0 && writes) sm[wave][n] = m, sl[wave][n] = l, sk[wave][n] = k;
-    const float weight = ldexpf(1.0f, 8 * digit);
+    const float weight = ldexpf(1.0f, 8 * digit - kUnits);
 #pragma unroll
     for (int d = 0; d < ND; d++) {
         Acc z = o[d];
