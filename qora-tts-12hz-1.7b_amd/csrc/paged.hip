@@ -387,9 +387,10 @@ __device__ __forceinline__ float row_scale(float x) {
 // when the running maximum rises.  Vector instructions a step: half of the f16
 // form's, which a chunk of one token's attention is bound by otherwise.
 //
-// Otherwise up to 16 columns on binary16 products: codes are exact in it, a
-// query value and a weight are split hi + lo (22 bits, scaled to below 2^15, so
-// that binary16's least step is 2^-39 of a column's largest).
+// Otherwise 16 or 32 columns on binary16 products: codes are exact in it, a query
+// value and a weight are split hi + lo: 22 bits, and no fewer than binary16's least
+// step leaves, 2^-38 of a column's largest query value and 2^-35 of its largest
+// weight.
 //
 // Three blocks of 64 dimensions fit a CU's registers (tiles of 32 columns, 8
 // sequences of 500 rows, a window of 72: 32 us, 38 with two), two of 128.
