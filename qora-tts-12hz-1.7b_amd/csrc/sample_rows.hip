@@ -569,9 +569,9 @@ constexpr int kNear = 8192;                       // tokens next to a cut that a
 constexpr int kMaxChunks = kSampleRowsMaxVocab / kChunk;
 constexpr int kMaxGroups = 8192;
 
-// Logits of a maximum.  A top-k past the number of groups takes every finite logit
-// for a candidate, and the whole row from memory where those are more than are
-// held, so groups are as small as their places allow (64 rows of 32000, top_k =
+// Logits of a maximum.  A top-k past the number of groups with a finite logit takes
+// every such logit for a candidate, and the whole row from memory where those are
+// more than are held, so groups are as small as their places allow (64 rows of 32000, top_k =
 // 2000 and top-p among the settings: 121 us in groups of 16, 45 of 4).
 __host__ __device__ constexpr int group_of(int vocab) {
     return vocab <= 4 * kMaxGroups ? 4 : vocab <= 16 * kMaxGroups ? 16 : 64;
@@ -667,37 +667,42 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleRowsParams P, RowScrat
 }
 
 // What top-k's candidates are no smaller than: a value that top_k of the groups'
-// maxima reach, by 256 steps down from the largest; the least finite logit where
-// there are not that many groups.  (-Inf is never drawn, so it is no candidate.)
+// maxima reach, by 256 steps down from the largest.  A group of -Inf alone holds no
+// candidate and is not counted (-Inf is never drawn); where fewer than top_k are
+// left, as in rows of which few tokens are allowed, the maxima say nothing of what
+// lies behind them in their groups, and it is the least finite logit.
 __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int groups, Space *sp) {
     constexpr int N = kMaxGroups / 256;  // all in flight, and kept for both passes
     const int tid = threadIdx.x;
     unsigned g[N];
 #pragma unroll
     for (int j = 0; j < N; j++) g[j] = R->group[min(tid + j * 256, groups - 1)];
-    const bool all = S.top_k >= groups;
-    const unsigned lowest = (all ? R->least_key : R->low)[min(tid, chunks - 1)];
-    if (tid == 0) sp->thr = 0xffffffffu, sp->count = 0xffffffffu;
+    const int mine = min(tid, chunks - 1);
+    const unsigned low_group = R->low[mine], low_logit = R->least_key[mine];
+    if (tid == 0) sp->thr = 0xffffffffu, sp->count = 0xffffffffu, sp->digit = 0xffffffffu;
     sp->hist[tid] = 0;
     const RowTop t = row_top(R, chunks, sp);
     float least = INFINITY;
     if (!t.bad) {
-        if (tid < chunks) atomicMin(&sp->thr, lowest);
-        __syncthreads();
-        least = logit_of(sp->thr);
-        if (!all) {
-            const Line line(logit_of(t.top), least);
-            auto each = [&](auto take) {
+        auto each = [&](auto take) {
 #pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (tid + j * 256 < groups) take(g[j]);
-            };
+            for (int j = 0; j < N; j++)
+                if (tid + j * 256 < groups && g[j] > key_of(-INFINITY)) take(g[j]);
+        };
+        u64 finite = 0;
+        each([&](unsigned) { finite++; });
+        if (tid < chunks) atomicMin(&sp->thr, low_group), atomicMin(&sp->digit, low_logit);
+        finite = block_total<256>(finite, sp->wsum);
+        if (finite < (u64)S.top_k) {
+            least = logit_of(sp->digit);
+        } else {
+            const Line line(logit_of(t.top), logit_of(sp->thr));
             each([&](unsigned k) { atomicAdd(&sp->hist[line(k) >> 8], (u64)1); });
             __syncthreads();
             find_bin(false, (u64)S.top_k, 0, sp);
             const int bin = (int)sp->digit;
             unsigned low = 0xffffffffu;
-            each([&](unsigned k) { low = min(low, line(k) >> 8 <= bin && k > key_of(-INFINITY) ? k : 0xffffffffu); });
+            each([&](unsigned k) { low = min(low, line(k) >> 8 <= bin ? k : 0xffffffffu); });
             low = ~wave_top(~low);
             if ((tid & 63) == 0) atomicMin(&sp->count, low);
             __syncthreads();
