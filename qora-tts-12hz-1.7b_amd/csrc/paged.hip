@@ -890,8 +890,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
             for (int j = 0; j < 16; j++) prob = fmaxf(prob, p[j]);
             lift(group_max(prob - lg) + (float)k);
+            // (a lane whose page is of scale NaN and masked has a NaN lg and no p)
 #pragma unroll
-            for (int j = 0; j < 16; j++) l += __builtin_amdgcn_exp2f(p[j] - lg + (float)k);
+            for (int j = 0; j < 16; j++) l += p[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[j] - lg + (float)k);
         }
         float sum = 0;
 #pragma unroll
