@@ -606,20 +606,25 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         l = ldexpf(l, -by);
     };
     // A new reference where a column's largest t asks for it, and what was
-    // summed under the last one; `prob`: the largest probability's logarithm.
+    // summed under the last one; `prob`: the largest probability's logarithm, of
+    // top's.  Scores may lie farther apart than an int holds, and top - kRoom is top
+    // where f32's steps are larger: what becomes a whole number is a difference.
     auto raise = [&](float top, float prob) {
         const bool first = m == -INFINITY, need = top > (first ? -INFINITY : m + kLimit);
         if (__any(need)) {
-            const float mn = need ? top - kRoom : m, down = first ? 0.0f : m - mn;
+            const float mn = need ? top - kRoom : m;
+            const float down = first ? 0.0f : fmaxf(m - mn, -4096.0f);  // 2^-4096 is nothing
             const float c = first ? 0.0f : __builtin_amdgcn_exp2f(down);
+            const float most = prob + (top - mn);  // of this reference
+            const float at = most == most ? fminf(fmaxf(most, -1024.0f), 1024.0f) : 0.0f;
             flush();
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= c;
             const int by = (int)rintf(down);
             l *= __builtin_amdgcn_exp2f(down - (float)by);
-            k = first && need ? (int)rintf(mn - prob) : k - by;
+            k = first && need ? -(int)rintf(at) : k - by;
             m = mn;
-            if (need) lift(prob - m + (float)k);
+            if (need) lift(at + (float)k);
         }
     };
 
@@ -723,32 +728,46 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         if (mine) {
             float mx = -INFINITY, prob = -INFINITY;
             unsigned zeros = 0, smalls = 0;  // of the rows here
+            float tops[S == 16 ? NR : 1];
             const float by = S == 16 ? A.scale * kLog2e : qscale;
+            auto size_of = [&](int i) {  // the logarithm of a row's V
+                return row_scale(S == 32 ? srow[min(t0 + row_of(i), open_hi - 1) - open_lo] : tops[S == 16 ? i : 0]);
+            };
 #pragma unroll
             for (int i = 0; i < NR; i++) {
                 const int token = t0 + row_of(i);
-                float top = 0;
-                if (S == 32) {
-                    top = srow[min(token, open_hi - 1) - open_lo];
-                } else {
+                if (S == 16) {
+                    float top = 0;
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         const float y = fabsf(v[S == 16 ? i : 0][d]);
                         odd |= !(y < INFINITY);
                         top = fmaxf(top, y < INFINITY ? y : 0.0f);
                     }
-                    top = row16_max(top);
+                    tops[S == 16 ? i : 0] = row16_max(top);
                 }
                 const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
                 p[i] = seen ? (I8 ? digits_sum(s[i]) : s[i]) * by : -INFINITY;
-                const float big = row_scale(top);
+                const float big = size_of(i);
                 zeros |= (unsigned)(big == kZeroScale) << i, smalls |= (unsigned)(big < kSmallRow) << i;
                 mx = fmaxf(mx, p[i] + big - 7.0f);  // as a page's, whose codes go to 127
-                prob = fmaxf(prob, p[i]);
             }
+            const float top = group_max(mx);
+            // Where f32's steps are whole units, a score is rounded as the reference
+            // is, with V's size, and p is taken from there on.
+            const bool coarse = fabsf(top) >= 0x1p24f && fabsf(top) < INFINITY;
+            if (__any(coarse)) {
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    const float big = size_of(i);
+                    p[i] = coarse ? (p[i] + big - 7.0f - top) + (7.0f - big) : p[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NR; i++) prob = fmaxf(prob, p[i]);
             prob = group_max(prob);
-            raise(group_max(mx), prob);
-            const float ms = m == -INFINITY ? 0.0f : m;
+            raise(top, coarse ? prob : prob - top);
+            const float ms = (m == -INFINITY ? 0.0f : m) - (coarse ? top : 0.0f);
             lift(prob - ms + (float)k);
 #pragma unroll
             for (int i = 0; i < NR; i++) {
@@ -877,10 +896,22 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
         for (int j = 0; j < 16; j++) mx = fmaxf(mx, p[j]);
         if (__any(mx > (m == -INFINITY ? -INFINITY : (float)kLimit))) {
-            raise(group_max(mx) + ms, group_max(mx - lg) + ms);
-            const float by = ms - (m == -INFINITY ? 0.0f : m);
+            const float top = group_max(mx);
+            raise(top + ms, group_max(mx - lg) - top);
+            const float mr = m == -INFINITY ? 0.0f : m, by = ms - mr;
+            const bool coarse = fmaxf(fabsf(ms), fabsf(mr)) >= 0x1p24f;
+            if (__any(coarse)) {
+                // Where f32's steps are whole units, p holds what a score's rounding
+                // leaves: the score is rounded as the reference is, and stays below it.
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j] += by;
+                for (int j = 0; j < 16; j++) {
+                    p[j] = coarse ? (p[j] + ms) - mr : p[j] + by;
+                    p[j] = p[j] > kLimit ? (float)kLimit : p[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) p[j] += by;
+            }
         }
         // weights of a V that is so much smaller than the others' hold no
         // probabilities: these are then taken by themselves
