@@ -729,7 +729,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             float mx = -INFINITY, prob = -INFINITY;
             unsigned zeros = 0, smalls = 0;  // of the rows here
             float tops[S == 16 ? NR : 1];
-            const float by = S == 16 ? A.scale * kLog2e : qscale;
+            // (qscale is NaN where the query is not finite: -Inf is no score)
+            const float by = S == 16 && qscale == qscale ? A.scale * kLog2e : qscale;
             auto size_of = [&](int i) {  // the logarithm of a row's V
                 return row_scale(S == 32 ? srow[min(t0 + row_of(i), open_hi - 1) - open_lo] : tops[S == 16 ? i : 0]);
             };
