@@ -748,7 +748,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                     tops[S == 16 ? i : 0] = row16_max(top);
                 }
                 const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
-                p[i] = seen ? (I8 ? digits_sum(s[i]) : s[i]) * by : -INFINITY;
+                // (the other digits' products are of zeros: none, or NaN with an Inf)
+                p[i] = seen ? (I8 ? digits_sum(digit ? 0.0f : s[i]) : s[i]) * by : -INFINITY;
                 const float big = size_of(i);
                 zeros |= (unsigned)(big == kZeroScale) << i, smalls |= (unsigned)(big < kSmallRow) << i;
                 mx = fmaxf(mx, p[i] + big - 7.0f);  // as a page's, whose codes go to 127

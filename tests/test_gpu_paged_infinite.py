@@ -1,5 +1,6 @@
-"""Paged attention: infinite queries.  A query with an Inf or NaN makes its row
-NaN, in the open page (which is held in float32) as in full ones."""
+"""Paged attention: infinite queries, and infinite keys in the open page (which
+is held in float32).  A query with an Inf or NaN makes its row NaN; a key whose
+score is -Inf has no weight."""
 import numpy as np
 import pytest
 import torch
@@ -33,7 +34,32 @@ def test_infinite_query(ctx, group, rows, n):
     _infinite_query(ctx, group, rows, n)
 
 
+def _infinite_key(ctx, group, rows, n):
+    """As if the token were not there: beside the same call with its score so low
+    that nothing is left of it."""
+    hd, page = 64, 64
+    k, v = base._normal(1, n, hd), base._normal(2, n, hd)
+    q = base._normal(3, rows, group * hd)
+    q[:, 5::hd] = 1 + np.abs(q[:, 5::hd])
+    gone = n - rows - 2  # seen by all rows
+    c = base.Cache(1, hd, page, 1, 4)
+    s = c.seqs([n - rows], [rows])
+    out = []
+    for low in (-1e30, -np.inf):
+        k[gone, 5] = low
+        c.append(ctx, c.seqs([0], [n]), base._up(k), base._up(v))
+        out.append(c.attend(ctx, s, base._up(q), group))
+    assert torch.isfinite(out[0]).all() and torch.equal(*out)
+
+
+@pytest.mark.parametrize("n", [30, 100])
+@pytest.mark.parametrize("group,rows", MODES)
+def test_infinite_key(ctx, group, rows, n):
+    _infinite_key(ctx, group, rows, n)
+
+
 @pytest.mark.parametrize("n", [30, 100])
 def test_tiles_of_32_columns(ctx, padded, n):
     padded(2)
     _infinite_query(ctx, 2, 20, n)
+    _infinite_key(ctx, 2, 20, n)
