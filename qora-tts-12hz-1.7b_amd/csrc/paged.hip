@@ -346,10 +346,15 @@ __device__ __forceinline__ float digits_sum(float v) {
     return v + dpp<0x124>(v);
 }
 
-// A weight's integer, the nearest: its rounding has to favour no side, as thousands
-// of small ones add up beside a large one (truncated, 30000 tokens' share of 0.2
-// came out 1e-4 of it short).
-__device__ __forceinline__ int nearest(float x, float scale) { return (int)fmaf(x, scale, 0.5f); }
+// A weight's integer, the nearest to it and to what the last one's rounding left,
+// which it hands on: thousands of weights about half a unit, or all alike, beside a
+// large one then sum up to what they are (30000 of 2^-28, 1e-4 of the sum: rounded
+// each for itself all of them were lost).  Not below 0, as a rest is -1/2 at least.
+__device__ __forceinline__ int nearest(float x, float scale, float &rest) {
+    const float y = fmaf(x, scale, rest), n = rintf(y);
+    rest = y - n;
+    return (int)n;
+}
 
 // log2 of the scale that a row or block of zeros takes: below all others, so that
 // it leaves the reference to them.
@@ -585,6 +590,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     Acc o[ND] = {};
     i32x4 oi[I8 ? ND : 1] = {};
     int held = 0;  // steps in oi
+    float rest[I8 ? 4 : 1] = {};  // of weights' integers, every fourth token's
 
     auto flush = [&]() {
         if constexpr (I8) {
@@ -622,6 +628,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             for (int d = 0; d < ND; d++) o[d] *= c;
             const int by = (int)rintf(down);
             l *= __builtin_amdgcn_exp2f(down - (float)by);
+#pragma unroll
+            for (int e = 0; e < (I8 ? 4 : 0); e++) rest[e] *= c;
             k = first && need ? -(int)rintf(at) : k - by;
             m = mn;
             if (need) lift(at + (float)k);
@@ -939,8 +947,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             i32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                w[j] = digits4(nearest(p[4 * j], 0x1p27f), nearest(p[4 * j + 1], 0x1p27f),
-                               nearest(p[4 * j + 2], 0x1p27f), nearest(p[4 * j + 3], 0x1p27f), pick, flip);
+                w[j] = digits4(nearest(p[4 * j], 0x1p27f, rest[0]), nearest(p[4 * j + 1], 0x1p27f, rest[1]),
+                               nearest(p[4 * j + 2], 0x1p27f, rest[2]), nearest(p[4 * j + 3], 0x1p27f, rest[3]), pick,
+                               flip);
 #pragma unroll
             for (int d = 0; d < ND; d++)
                 oi[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, vr[d]), w, oi[d], 0, 0, 0);
