@@ -403,8 +403,10 @@ typedef struct qtts_paged_kv {
  * holds its pages in order; an entry outside the pool is an absent page, whose
  * tokens are neither written nor attended to (a window's dropped pages).  A
  * sequence is left out as a whole, its cache untouched, where starts[b] is
- * negative, its tokens pass max_pages * page_size (or the rotation's table) or
- * slots[b] is outside the slots.  starts[b] may go back to a token of the page
+ * negative, its tokens pass max_pages * page_size or max_tokens or slots[b] is
+ * outside the slots.  (An append also leaves out what passes its rotation's
+ * table, which the other calls do not know: give them all the table's rows as
+ * max_tokens where max_pages * page_size is more.)  starts[b] may go back to a token of the page
  * that is being filled or to a page's first; what was behind it is forgotten.
  * Pages may be shared for reading; the pages and slots that a call writes must
  * be different ones. */
@@ -417,6 +419,7 @@ typedef struct qtts_paged_seqs {
     const int32_t *slots;       /* [batch] */
     const int32_t *starts;      /* [batch] */
     const int32_t *row_offsets; /* [batch + 1] */
+    int32_t max_tokens;         /* most tokens of a sequence; 0: max_pages * page_size */
 } qtts_paged_seqs;
 
 /* New rows: per row, `heads` query heads (q may be NULL: none) and the cache's

@@ -2942,7 +2942,7 @@ qtts_status qtts_paged_append_device(qtts_ctx *c, const qtts_paged_kv *kv, const
     p.kv = *kv;
     p.s = *s;
     p.r = *r;
-    p.cap = (long long)s->max_pages * kv->page_size;
+    p.cap = tokens_cap(*kv, *s);
     if (r->rope_cos) p.cap = std::min<long long>(p.cap, r->rope_rows);
     DeviceGuard guard(c->device);
     launch_paged_append(c->stream, p);

@@ -30,6 +30,12 @@ inline bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 
 
 inline bool paged_empty(const qtts_paged_seqs &s) { return s.batch == 0 || s.rows == 0 || s.max_rows == 0; }
 
+// Tokens that a sequence may reach.
+QTTS_HD long long tokens_cap(const qtts_paged_kv &kv, const qtts_paged_seqs &s) {
+    const long long held = (long long)s.max_pages * kv.page_size;
+    return s.max_tokens > 0 && s.max_tokens < held ? s.max_tokens : held;
+}
+
 inline Refusal check_paged(const qtts_paged_kv &kv, const qtts_paged_seqs &s) {
     if (kv.head_dim != 64 && kv.head_dim != 128) return {QTTS_ESHAPE, "paged cache: head_dim must be 64 or 128"};
     if (kv.page_size != 16 && kv.page_size != 32 && kv.page_size != 64 && kv.page_size != 128)
@@ -43,8 +49,9 @@ inline Refusal check_paged(const qtts_paged_kv &kv, const qtts_paged_seqs &s) {
     if (!aligned_to(kv.k_codes, 16) || !aligned_to(kv.v_codes, 16) || !aligned_to(kv.k_open, 16) ||
         !aligned_to(kv.v_open, 16) || !aligned_to(kv.k_scales, 4) || !aligned_to(kv.v_scales, 4))
         return {QTTS_EINVAL, "paged cache: buffers must be 16-byte aligned"};
-    if (s.batch < 0 || s.batch > 65536 || s.rows < 0 || s.max_rows < 0 || s.max_pages < 0)
-        return {QTTS_ESHAPE, "paged sequences: batch must be 0..65536, rows, max_rows and max_pages not negative"};
+    if (s.batch < 0 || s.batch > 65536 || s.rows < 0 || s.max_rows < 0 || s.max_pages < 0 || s.max_tokens < 0)
+        return {QTTS_ESHAPE,
+                "paged sequences: batch must be 0..65536, rows, max_rows, max_pages and max_tokens not negative"};
     if ((long long)s.max_pages * kv.page_size > (1LL << 30))
         return {QTTS_ERANGE, "paged sequences: more than 2^30 tokens in a page table row"};
     if (paged_empty(s)) return kAccepted;
@@ -189,7 +196,7 @@ inline AttnShape attn_shape(const qtts_paged_kv &kv, const qtts_paged_seqs &s, i
     const int each = mode == kAttnI8 ? 4 : mode == kAttn16 ? 16 : 32;
     const long long tiles = (columns + each - 1) / each, pairs = kvs * tiles;
     if (pairs > kPagedMaxBlocks) return {mode, 0, 0, 0, pairs};
-    const AttnPlan p = attn_plan(pairs, (long long)s.max_pages * kv.page_size, each);
+    const AttnPlan p = attn_plan(pairs, tokens_cap(kv, s), each);
     return {mode, (int)tiles, p.whole, p.nsplit, p.whole + (pairs - p.whole) * p.nsplit};
 }
 

@@ -208,10 +208,11 @@ class PagedKv(C.Structure):
 
 
 class PagedSeqs(C.Structure):
-    """qtts_paged_seqs: the sequences of one call, device pointers."""
+    """qtts_paged_seqs: the sequences of one call, device pointers; max_tokens
+    0 (or left out): what the page table holds."""
 
     _fields_ = [(n, C.c_int32) for n in ("batch", "max_pages", "rows", "max_rows")] + [
-        (n, C.c_void_p) for n in ("page_table", "slots", "starts", "row_offsets")]
+        (n, C.c_void_p) for n in ("page_table", "slots", "starts", "row_offsets")] + [("max_tokens", C.c_int32)]
 
 
 class PagedRows(C.Structure):
