@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     __shared__ float srow[S == 32 ? 128 : 1];  // the open rows' largest |v|
     __shared__ unsigned sarrived;
     static_assert(4 * (HD + 4) >= kPagedMaxSplits, "the parts' factors take so's place");
-    static_assert(kPagedPartFloats >= 3LL * kPagedRound / 2 * CT * (HD + 4), "the parts fit");
+    static_assert(kPagedPartFloats >= 3LL * kPagedRound / 2 * CT * part_floats(HD), "the parts fit");
     const int P = A.kv.page_size, sh = __builtin_ctz(P), kvh = A.kv.kv_heads, group = A.heads / kvh;
     // Consecutive blocks lie on different XCDs.  Tiles of 32 share their pages:
     // with kv heads innermost one head's are read through few caches, and the
@@ -1003,7 +1003,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     __syncthreads();
     // Joining, of waves and of parts: outputs relative to the largest reference,
     // sums to the one whose power of two is nearest to the largest of theirs.
-    constexpr int PW = HD + 4;  // floats of a part's column: output, reference, sum, k
+    constexpr int PW = part_floats(HD);
     float *part = A.part + (size_t)shared * nsplit * CT * PW;
     if ((int)threadIdx.x < left) {
         const int c = threadIdx.x;

@@ -148,6 +148,10 @@ constexpr int kPagedMaxSplits = 256;
 constexpr long long kPagedCounters = kPagedRound;
 constexpr long long kPagedPartFloats = 4LL << 20;  // 3/2 of a round's blocks of 32 columns, at least
 
+// Floats that a chunk's column takes there: its output, its reference, its sum and
+// the power of two that is the sum's (one more keeps the rows on 16 bytes).
+QTTS_HD constexpr int part_floats(int head_dim) { return head_dim + 4; }
+
 struct AttnPlan {
     int whole;   // pairs of one block
     int nsplit;  // blocks of each of the others
