@@ -679,34 +679,38 @@ __device__ void find_least(RowScratch *R, const RowSettings &S, int chunks, int 
     for (int j = 0; j < N; j++) g[j] = R->group[min(tid + j * 256, groups - 1)];
     const int mine = min(tid, chunks - 1);
     const unsigned low_group = R->low[mine], low_logit = R->least_key[mine];
-    if (tid == 0) sp->thr = 0xffffffffu, sp->count = 0xffffffffu, sp->digit = 0xffffffffu;
+    unsigned *lowest = sp->rank;  // of the logits
+    if (tid == 0) sp->thr = 0xffffffffu, sp->count = 0xffffffffu, *lowest = 0xffffffffu;
     sp->hist[tid] = 0;
     const RowTop t = row_top(R, chunks, sp);
     float least = INFINITY;
     if (!t.bad) {
+        // (a wave's own least first: an atomic minimum goes through its lanes one by one)
+        const unsigned wave_group = ~wave_top(tid < chunks ? ~low_group : 0);
+        const unsigned wave_logit = ~wave_top(tid < chunks ? ~low_logit : 0);
+        if ((tid & 63) == 0) atomicMin(&sp->thr, wave_group), atomicMin(lowest, wave_logit);
+        __syncthreads();
+        const Line line(logit_of(t.top), logit_of(sp->thr));
         auto each = [&](auto take) {
 #pragma unroll
             for (int j = 0; j < N; j++)
-                if (tid + j * 256 < groups && g[j] > key_of(-INFINITY)) take(g[j]);
+                if (tid + j * 256 < groups) take(g[j]);
         };
-        u64 finite = 0;
-        each([&](unsigned) { finite++; });
-        if (tid < chunks) atomicMin(&sp->thr, low_group), atomicMin(&sp->digit, low_logit);
-        finite = block_total<256>(finite, sp->wsum);
-        if (finite < (u64)S.top_k) {
-            least = logit_of(sp->digit);
-        } else {
-            const Line line(logit_of(t.top), logit_of(sp->thr));
-            each([&](unsigned k) { atomicAdd(&sp->hist[line(k) >> 8], (u64)1); });
-            __syncthreads();
-            find_bin(false, (u64)S.top_k, 0, sp);
-            const int bin = (int)sp->digit;
+        each([&](unsigned k) {
+            if (k > key_of(-INFINITY)) atomicAdd(&sp->hist[line(k) >> 8], (u64)1);
+        });
+        __syncthreads();
+        find_bin(false, (u64)S.top_k, 0, sp);
+        const int bin = (int)sp->digit;
+        if (sp->base + sp->hist[bin] >= (u64)S.top_k) {
             unsigned low = 0xffffffffu;
-            each([&](unsigned k) { low = min(low, line(k) >> 8 <= bin ? k : 0xffffffffu); });
+            each([&](unsigned k) { low = min(low, line(k) >> 8 <= bin && k > key_of(-INFINITY) ? k : 0xffffffffu); });
             low = ~wave_top(~low);
             if ((tid & 63) == 0) atomicMin(&sp->count, low);
             __syncthreads();
             least = logit_of(sp->count);
+        } else {
+            least = logit_of(*lowest);
         }
     }
     if (tid == 0) R->least = least;
