@@ -2942,8 +2942,8 @@ qtts_status qtts_paged_append_device(qtts_ctx *c, const qtts_paged_kv *kv, const
     p.kv = *kv;
     p.s = *s;
     p.r = *r;
-    p.cap = tokens_cap(*kv, *s);
-    if (r->rope_cos) p.cap = std::min<long long>(p.cap, r->rope_rows);
+    p.cap = (int)tokens_cap(*kv, *s);
+    if (r->rope_cos) p.cap = std::min(p.cap, r->rope_rows);
     DeviceGuard guard(c->device);
     launch_paged_append(c->stream, p);
     return check_launch(c, "k_paged_append");
@@ -2965,6 +2965,7 @@ qtts_status qtts_paged_attention_device(qtts_ctx *c, const qtts_paged_kv *kv, co
     p.ld_out = ld_out;
     p.scale = scale;
     p.window = window;
+    p.cap = (int)tokens_cap(*kv, *s);
     p.part = c->attn_part;
     p.counters = c->paged_counters;
     DeviceGuard guard(c->device);
@@ -2985,6 +2986,7 @@ qtts_status qtts_paged_read_device(qtts_ctx *c, const qtts_paged_kv *kv, const q
     p.v_out = d_v_out;
     p.ld_k = ld_k_out;
     p.ld_v = ld_v_out;
+    p.cap = (int)tokens_cap(*kv, *s);
     DeviceGuard guard(c->device);
     launch_paged_read(c->stream, p);
     return check_launch(c, "k_paged_read");

@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         if constexpr (S == 16) return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0);
         else return __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, c, 0, 0, 0);
     };
-    const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, tokens_cap(A.kv, A.s));
+    const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, A.cap);
     const int left = (int)min((long long)q.rows * group - (long long)tile * CT, (long long)CT);
     if (left <= 0) return;
     auto out_of = [&](int n) {  // column n's place in the output
@@ -1136,9 +1136,9 @@ __global__ __launch_bounds__(256) void k_paged_read(PagedReadParams A, int items
     constexpr int D4 = HD / 4;
     const int P = A.kv.page_size, sh = __builtin_ctz(P), kvh = A.kv.kv_heads;
     const int head = blockIdx.x % kvh, item = blockIdx.x / kvh % items, b = blockIdx.x / kvh / items;
-    const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, tokens_cap(A.kv, A.s));
+    const PagedSeq q = load_seq(A.s, b, A.kv.num_slots, A.cap);
     const int len = A.lens ? A.lens[b] : q.start + q.rows;
-    const bool ok = q.ok && (long long)len <= tokens_cap(A.kv, A.s);
+    const bool ok = q.ok && len <= A.cap;
     // positions of this block, by pages where they have any
     const int first = ok ? q.start >> sh << sh : 0;
     const int lo = max(first + item * P, ok ? q.start : 0);

@@ -16,7 +16,7 @@ struct PagedAppendParams {
     qtts_paged_rows r;
     int kv_items;   // pages one sequence's rows can touch
     int q_items;    // blocks over one sequence's queries
-    long long cap;  // tokens a sequence may reach
+    int cap;        // tokens a sequence may reach
 };
 
 struct PagedAttnParams {
@@ -27,6 +27,7 @@ struct PagedAttnParams {
     int heads, ld_q, ld_out;
     float scale;
     int window;
+    int cap;  // tokens a sequence may reach
     // the launch's own
     int tiles;           // column tiles of one sequence and kv head
     int whole, nsplit;   // AttnPlan
@@ -40,6 +41,7 @@ struct PagedReadParams {
     const int32_t *lens;
     float *k_out, *v_out;
     int ld_k, ld_v;
+    int cap;  // tokens a sequence may reach
 };
 
 struct SampleRowsParams {
@@ -54,7 +56,7 @@ struct SampleRowsParams {
     size_t scratch_bytes;
 };
 
-// False: the call needs more blocks than one launch holds, nothing was launched.
+// The host's checks (paged_plan.h) have refused what a launch cannot hold.
 void launch_paged_append(hipStream_t st, const PagedAppendParams &p);
 void launch_paged_attention(hipStream_t st, const PagedAttnParams &p);
 void launch_paged_read(hipStream_t st, const PagedReadParams &p);
