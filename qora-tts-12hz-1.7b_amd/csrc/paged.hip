@@ -542,7 +542,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     // --- the queries ---
     i32x4 qi[NK];                  // I8: digits of dimensions ST h + 16 G + 0 .. 15
     f16x8 qh[2 * NK], ql[2 * NK];  // else: hi and lo of ST h + 16 G + 8 u + 0 .. 7 at 2 h + u
-    float qscale;
+    float qscale, qsize, qrest;
     const unsigned pick = (unsigned)(digit | (digit + 4) << 8) | 0x0c0c0000u;
     const unsigned flip = digit == 3 ? 0u : 0x80808080u;
     {
@@ -578,7 +578,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 }
             }
         }
-        qscale = odd ? __uint_as_float(0x7fc00000u) : ldexpf(A.scale * kLog2e, I8 ? e - 29 + 8 * digit : e - 14);
+        // What an operand is to be multiplied by, in two factors: in one, a query of
+        // 2^-110 would leave it below f32's least normal value, and beside open keys of
+        // 2^113 an operand of 2^15 would leave f32 (tiles of 32 take it times qsize).
+        const int size = I8 ? e - 29 + 8 * digit : e - 14, h = max(size, -60);
+        qsize = ldexpf(1.0f, h), qrest = ldexpf(1.0f, size - h);
+        qscale = odd ? __uint_as_float(0x7fc00000u) : A.scale * kLog2e;
     }
 
     // Weights of V are 2^(t - m); the sum of probabilities l is held relative to
@@ -722,7 +727,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int at = 2 * h + (j + i) / 8;
-                            s = mma1(y[i], (float)qh[at][(j + i) % 8] + (float)ql[at][(j + i) % 8], s);
+                            s = mma1(y[i], ((float)qh[at][(j + i) % 8] + (float)ql[at][(j + i) % 8]) * qsize, s);
                         }
                     }
             }
@@ -738,7 +743,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             unsigned zeros = 0, smalls = 0;  // of the rows here
             float tops[S == 16 ? NR : 1];
             // (qscale is NaN where the query is not finite: -Inf is no score)
-            const float by = S == 16 && qscale == qscale ? A.scale * kLog2e : qscale;
+            const float by = S == 16 ? qscale : qscale * qrest;
             auto size_of = [&](int i) {  // the logarithm of a row's V
                 return row_scale(S == 32 ? srow[min(t0 + row_of(i), open_hi - 1) - open_lo] : tops[S == 16 ? i : 0]);
             };
@@ -877,7 +882,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             load_k(next, pkn);
             ksn = A.kv.k_scales[block_of(pvn)], vsn = A.kv.v_scales[block_of(pvn)];
         }
-        const float kq = qscale * ks_;
+        const float kq = qscale * qsize * ks_ * qrest;
         // The page's scale of V joins the scores as its logarithm, and leaves
         // the sum of probabilities as its inverse.
         const bool small = vs_ < 0x1p-64f, zero = !there || vs_ == 0.0f;
