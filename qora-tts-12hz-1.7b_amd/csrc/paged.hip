@@ -347,9 +347,10 @@ __device__ __forceinline__ float digits_sum(float v) {
 }
 
 // A weight's integer, the nearest to it and to what the last one's rounding left,
-// which it hands on: thousands of weights about half a unit, or all alike, beside a
+// which it hands on: thousands of weights below half a unit, or all alike, beside a
 // large one then sum up to what they are (30000 of 2^-28, 1e-4 of the sum: rounded
-// each for itself all of them were lost).  Not below 0, as a rest is -1/2 at least.
+// each for itself, to units of 2^-27, all of them were lost).  Each is off by a unit
+// at most, and not below 0, as a rest is -1/2 at least.
 __device__ __forceinline__ int nearest(float x, float scale, float &rest) {
     const float y = fmaf(x, scale, rest), n = rintf(y);
     rest = y - n;
@@ -410,9 +411,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     constexpr int NK = HD / ST, ND = HD / S;      // 16-byte pieces of a K row in a lane; dimension tiles
     // Weights are 2^(t - m); the reference m is set so that the largest is
     // 2^kRoom, and again when one would pass 2^kLimit.  Integers take them times
-    // 2^27, so that t - m is small, and its rounding too, where the weight is large
+    // 2^28, so that t - m is small, and its rounding too, where the weight is large
     // (binary16 would take a product each).
-    constexpr int kRoom = I8 ? 0 : 11, kLimit = I8 ? 3 : 15, kUnits = I8 ? 27 : 0;
+    constexpr int kRoom = I8 ? 0 : 11, kLimit = I8 ? 2 : 15, kUnits = I8 ? 28 : 0;
     constexpr int kFlush = 1024;                  // steps that int32 sums hold: 64 * 128 * 127 each
     typedef float Acc __attribute__((ext_vector_type(NR)));
     __shared__ float so[4][CT][HD + 4];
@@ -952,8 +953,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
             i32x4 w;
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                w[j] = digits4(nearest(p[4 * j], 0x1p27f, rest[0]), nearest(p[4 * j + 1], 0x1p27f, rest[1]),
-                               nearest(p[4 * j + 2], 0x1p27f, rest[2]), nearest(p[4 * j + 3], 0x1p27f, rest[3]), pick,
+                w[j] = digits4(nearest(p[4 * j], 0x1p28f, rest[0]), nearest(p[4 * j + 1], 0x1p28f, rest[1]),
+                               nearest(p[4 * j + 2], 0x1p28f, rest[2]), nearest(p[4 * j + 3], 0x1p28f, rest[3]), pick,
                                flip);
 #pragma unroll
             for (int d = 0; d < ND; d++)
