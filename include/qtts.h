@@ -406,10 +406,10 @@ typedef struct qtts_paged_kv {
  * negative, its tokens pass max_pages * page_size or max_tokens or slots[b] is
  * outside the slots.  (An append also leaves out what passes its rotation's
  * table, which the other calls do not know: give them all the table's rows as
- * max_tokens where max_pages * page_size is more.)  starts[b] may go back to a token of the page
- * that is being filled or to a page's first; what was behind it is forgotten.
- * Pages may be shared for reading; the pages and slots that a call writes must
- * be different ones. */
+ * max_tokens where max_pages * page_size is more.)  starts[b] may go back to a
+ * token of the page that is being filled or to a page's first; what was behind
+ * it is forgotten.  Pages may be shared for reading; the pages and slots that a
+ * call writes must be different ones. */
 typedef struct qtts_paged_seqs {
     int32_t batch;
     int32_t max_pages;          /* entries of a page_table row */
@@ -452,9 +452,13 @@ qtts_status qtts_paged_append_device(qtts_ctx *ctx, const qtts_paged_kv *kv, con
  * heads * head_dim floats a row, ld_* apart (out may be q); head h reads kv head
  * h / (heads / kv_heads).  scale multiplies the products (head_dim^-0.5).  A
  * row that sees nothing, or of a sequence left out, is zeros; rows behind the
- * last sequence stay as they were.  Enqueued on the context stream, allocates
- * nothing and can be captured; its partial results lie in context scratch, so
- * replay a graph in order with the context's calls. */
+ * last sequence stay as they were.  A query with an Inf or NaN makes its row
+ * NaN; a key whose score is -Inf has no weight.  Scores are float32 with its
+ * steps, which are whole units from 2^24 on, and its range.  Weights are held
+ * to 2^-28 of the row's largest or finer, and their sum closer than that.
+ * Enqueued on the context stream, allocates nothing and can be captured; its
+ * partial results lie in context scratch, so replay a graph in order with the
+ * context's calls. */
 qtts_status qtts_paged_attention_device(qtts_ctx *ctx, const qtts_paged_kv *kv, const qtts_paged_seqs *seqs,
                                         int32_t heads, const float *d_q, int32_t ld_q, float scale, int32_t window,
                                         float *d_out, int32_t ld_out);
@@ -486,10 +490,12 @@ typedef struct qtts_row_sampler {
  * min_p those with w_i >= min_p; the first one stays always.  The token is the
  * lowest index whose running sum over the kept ones, in index order, is above
  * uniform[row] times their sum (uniform in [0, 1); NaN and below count as 0,
- * 1 and above as the last).  Sums are exact to 2^-45 of the largest weight and
- * do not depend on an order.  probs (or NULL) receives its share of the kept
+ * 1 and above as the last).  A sum is exact to 2^-45 of the largest weight for
+ * each token of the row and does not depend on an order.  probs (or NULL) receives its share of the kept
  * sum.  +Inf logits share the draw; a row of -Inf gives token -1 and share 0, a
- * row with a NaN -1 and NaN.  Enqueued on the context stream, allocates
+ * row with a NaN -1 and NaN.  Tokens that are not allowed are best -Inf: low
+ * finite ones are candidates of top_k as others are, which in rows of more than
+ * 12288 logits takes many passes where thousands are alike.  Enqueued on the context stream, allocates
  * nothing and can be captured (context scratch, as above). */
 qtts_status qtts_sample_rows_device(qtts_ctx *ctx, const float *d_logits, int64_t ld, int32_t rows, int32_t vocab,
                                     const qtts_row_sampler *params, const float *d_uniform, int32_t *d_tokens,

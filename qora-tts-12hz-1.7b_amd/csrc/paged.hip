@@ -287,8 +287,10 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendParams A) {
 //
 // Weights of V's products are p times the page's scale of V, whose logarithm
 // joins the score (t = s + log2 scale): the largest weight fills the operand's
-// range whatever V's size is.  The sum of probabilities has a reference of its own
-// and is taken from the weights (over the scale) where they hold it.
+// range whatever V's size is, and t is rounded at its size (by some 2^-17 of a
+// weight where scales are 2^100 or 2^-100, 2^-21 where they are ordinary).  The
+// sum of probabilities has a reference of its own and is taken from the weights
+// (over the scale) where they hold it.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -375,11 +377,12 @@ __device__ __forceinline__ float row_scale(float x) {
 //
 // Few columns are bound by reading the pages: 64 sequences of up to 8000 tokens,
 // 8 kv heads of 128, 798 MB in 153 us (5.2 TB/s; a copy moves 5.1); 4 of 32760 in
-// 46 us (4.8); 16 of 2064 in 20 us (2.7), of which 10 are a block's first loads
-// and the joining, as one sequence of 1064 tokens takes 11 us.  Many are bound by
-// vector instructions, codes to binary16 (160 of 440 a step) and the softmax, of
-// whose time the products cover half: 1064 rows of two heads behind 2000 tokens
-// 75 us, 0.29 PFLOP/s (0.58 as hi + lo).
+// 47 us (4.7); 16 of 2064 in 21 us (2.6), of which 10 are a block's first loads
+// and the joining, as one sequence of 1064 tokens takes 12 us.  Many are bound by
+// vector instructions, codes to binary16 (160 of 440 a step) and the softmax: 1064
+// rows of two heads behind 2000 tokens 76 us, 0.29 PFLOP/s (0.58 as hi + lo), of
+// which vector instructions take 35 and products 18, with two waves a SIMD to
+// cover one by the other.
 //
 // Of a step's 64 tokens, lane (r = lane % 16, G = lane / 16) has scores of
 // tokens 16G + 4t + i in register i of tile t, and feeds them to the output's
@@ -390,8 +393,8 @@ __device__ __forceinline__ float row_scale(float x) {
 // query value (scaled to the column's largest) and a weight are 30-bit
 // integers, whose four base-256 digits take four operand columns: lane r holds
 // digit r / 4 of column r % 4.  Integer sums are exact; they join the f32 ones
-// when the running maximum rises.  Vector instructions a step: half of the f16
-// form's, which a chunk of one token's attention is bound by otherwise.
+// when the running maximum rises.  Vector instructions a step: about half of the
+// f16 form's, which a chunk of one token's attention is bound by otherwise.
 //
 // Otherwise 16 or 32 columns on binary16 products: codes are exact in it, a query
 // value and a weight are split hi + lo: 22 bits, and no fewer than binary16's least
@@ -399,7 +402,7 @@ __device__ __forceinline__ float row_scale(float x) {
 // weight.
 //
 // Three blocks of 64 dimensions fit a CU's registers (tiles of 32 columns, 8
-// sequences of 500 rows, a window of 72: 32 us, 38 with two), two of 128.
+// sequences of 500 rows, a window of 72: 33 us, 38 with two), two of 128.
 template <int HD, int MODE>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnParams A) {
     constexpr bool I8 = MODE == kAttnI8;

@@ -2,9 +2,9 @@
 // top-p, min-p, given uniform numbers.
 //
 // Weights w_i = exp((l_i - max) / T) are evaluated in 64 bits and summed as
-// integers of 2^-44 of the largest: sums do not depend on their order, and a
-// draw next to the border between two tokens falls as the 64-bit definition's
-// does.  What is kept is a prefix of the tokens in order (logit down, index up),
+// integers of 2^-44 of the largest, each to the nearest: sums do not depend on
+// their order, and a draw falls as the 64-bit definition's does but within 2^-45 a
+// token of the border between two.  What is kept is a prefix of the tokens in order (logit down, index up),
 // so that it is one number, the order of the last.
 //
 // Rows of up to kRowVocab logits take a block each, which holds the row's keys
@@ -15,7 +15,10 @@
 //
 // Measured: 64 rows of 151936, settings of every kind among them, 14 + 12 + 13
 // + 25 us (39 MB, which a copy reads in 8); all at top_k = 50, 14 + 9 + 7 + 10;
-// one row 6 + 8 + 4 + 9 us, all of it latency.
+// one row 6 + 7 + 4 + 9 us, all of it latency.  Rows of more than kNear candidates
+// (top_k past the groups that hold a finite logit, thousands of equal or masked
+// but finite ones) are cut from memory by one block: 0.2 to 1.1 ms a row of 151936,
+// 0.3 to 1.5 for 64.
 #include <algorithm>
 
 #include "device_common.h"

@@ -75,3 +75,15 @@ def test_every_allowed_token_is_drawn(ctx, vocab, n, k):
         u = (edges[:-1] + edges[1:]) / 2
         token, _ = base.draw(ctx, np.tile(row, (len(u), 1)), u, [0.9] * len(u), [k] * len(u))
         assert np.array_equal(token, kept)
+
+
+@pytest.mark.parametrize("low", [np.finfo(np.float32).min, -1e4])
+@pytest.mark.parametrize("vocab", [12288, 40000, 151936])
+def test_masked_by_a_low_value(ctx, vocab, low):
+    """A finite mask, which takes part in top-k and has no weight."""
+    x, u = masked(vocab, vocab, 10, 4)
+    y, v = masked(vocab + 1, vocab, vocab // 2, 4)
+    for a, b in ((x, u), (y, v)):
+        a = np.where(a == -np.inf, np.float32(low), a)
+        base.check(ctx, a, b, [0.8] * 4, [50] * 4)
+        base.check(ctx, a, b[::-1].copy(), [1.5] * 4, [0, 3, 2000, 0], [0.9, 1.0, 0.9, 1.0], [0.0, 0.0, 0.0, 0.05])
