@@ -362,7 +362,10 @@ __device__ __forceinline__ int nearest(float x, float scale, float &rest) {
 // log2 of the scale that a row or block of zeros takes: below all others, so that
 // it leaves the reference to them.
 constexpr float kZeroScale = -200.0f;
-constexpr float kSmallRow = -80.0f;  // below it a row's values are taken times 2^60
+// An open row's values are taken times 2^60 below this and 2^-60 above that: their
+// weights are 2^-120 of the probabilities beside values of 2^127, where the next
+// ones would fall below f32.
+constexpr float kSmallRow = -80.0f, kLargeRow = 80.0f;
 
 // The same of an open row, by its largest value's exponent.
 __device__ __forceinline__ float row_scale(float x) {
@@ -653,8 +656,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     const float *k_open = A.kv.k_open + ((size_t)q.slot * kvh + head) * P * HD;
     const float *v_open = A.kv.v_open + ((size_t)q.slot * kvh + head) * P * HD;
     float(*rows)[HD + 4] = so[0];  // S == 32: row t - open_lo of the open page, 128 at most
-    // V's are staged as the products take them: what is not finite as 0, small
-    // rows times 2^60, their largest values in srow; returns whether something is
+    // V's are staged as the products take them: what is not finite as 0, small rows
+    // times 2^60, large ones 2^-60, their largest values in srow; returns whether something is
     // not finite.
     auto stage = [&](const float *from, bool values) {
         const int count = (open_hi - open_lo) * (HD / 4);
@@ -680,7 +683,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                     }
                     top = row16_max(top);
                     if (HD == 128) top = fmaxf(top, dpp_row_pair(top));
-                    if (row_scale(top) < kSmallRow) y[j] *= 0x1p60f;
+                    y[j] *= row_scale(top) < kSmallRow ? 0x1p60f : row_scale(top) > kLargeRow ? 0x1p-60f : 1.0f;
                     if (i0 + 256 * j < count) srow[i / (HD / 4)] = top;
                 }
                 if (i0 + 256 * j < count) *reinterpret_cast<f32x4 *>(&rows[i / (HD / 4)][4 * (i % (HD / 4))]) = y[j];
@@ -744,7 +747,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         float p[NR];
         if (mine) {
             float mx = -INFINITY, prob = -INFINITY;
-            unsigned zeros = 0, smalls = 0;  // of the rows here
+            unsigned zeros = 0, smalls = 0, larges = 0;  // of the rows here
             float tops[S == 16 ? NR : 1];
             // (qscale is NaN where the query is not finite: -Inf is no score)
             const float by = S == 16 ? qscale : qscale * qrest;
@@ -768,7 +771,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 // (the other digits' products are of zeros: none, or NaN with an Inf)
                 p[i] = seen ? (I8 ? digits_sum(digit ? 0.0f : s[i]) : s[i]) * by : -INFINITY;
                 const float big = size_of(i);
-                zeros |= (unsigned)(big == kZeroScale) << i, smalls |= (unsigned)(big < kSmallRow) << i;
+                zeros |= (unsigned)(big == kZeroScale) << i;
+                smalls |= (unsigned)(big < kSmallRow) << i, larges |= (unsigned)(big > kLargeRow) << i;
                 mx = fmaxf(mx, p[i] + big - 7.0f);  // as a page's, whose codes go to 127
             }
             const float top = group_max(mx);
@@ -791,8 +795,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
             for (int i = 0; i < NR; i++) {
                 l += __builtin_amdgcn_exp2f(p[i] - ms + (float)k);
-                // 2^60 of a small row's weight goes over to its values, and zeros have none
-                const float over = zeros >> i & 1 ? kZeroScale : smalls >> i & 1 ? -60.0f : 0.0f;
+                // 2^60 of a small row's weight goes over to its values, of a large one's
+                // values to its weight, and zeros have none
+                const float over = zeros >> i & 1 ? kZeroScale : smalls >> i & 1 ? -60.0f : larges >> i & 1 ? 60.0f : 0.0f;
                 p[i] = digit ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms + over) * (float)(1 << kUnits);
             }
             if (S == 32) {
@@ -816,7 +821,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         const float y = v[S == 16 ? i : 0][d];
-                        o[d] = mma1(fabsf(y) < INFINITY ? y * (smalls >> i & 1 ? 0x1p60f : 1.0f) : 0.0f, p[i], o[d]);
+                        o[d] = mma1(fabsf(y) < INFINITY ? y * (smalls >> i & 1 ? 0x1p60f : larges >> i & 1 ? 0x1p-60f : 1.0f) : 0.0f,
+                                    p[i], o[d]);
                     }
             }
         }
