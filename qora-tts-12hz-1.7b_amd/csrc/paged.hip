@@ -797,7 +797,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 l += __builtin_amdgcn_exp2f(p[i] - ms + (float)k);
                 // 2^60 of a small row's weight goes over to its values, of a large one's
                 // values to its weight, and zeros have none
-                const float over = zeros >> i & 1 ? kZeroScale : smalls >> i & 1 ? -60.0f : larges >> i & 1 ? 60.0f : 0.0f;
+                const float over = zeros >> i & 1    ? kZeroScale
+                                   : smalls >> i & 1 ? -60.0f
+                                   : larges >> i & 1 ? 60.0f
+                                                     : 0.0f;
                 p[i] = digit ? 0.0f : __builtin_amdgcn_exp2f(p[i] - ms + over) * (float)(1 << kUnits);
             }
             if (S == 32) {
@@ -821,8 +824,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         const float y = v[S == 16 ? i : 0][d];
-                        o[d] = mma1(fabsf(y) < INFINITY ? y * (smalls >> i & 1 ? 0x1p60f : larges >> i & 1 ? 0x1p-60f : 1.0f) : 0.0f,
-                                    p[i], o[d]);
+                        const float by = smalls >> i & 1 ? 0x1p60f : larges >> i & 1 ? 0x1p-60f : 1.0f;
+                        o[d] = mma1(fabsf(y) < INFINITY ? y * by : 0.0f, p[i], o[d]);
                     }
             }
         }
