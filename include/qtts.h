@@ -501,6 +501,42 @@ qtts_status qtts_sample_rows_device(qtts_ctx *ctx, const float *d_logits, int64_
                                     const qtts_row_sampler *params, const float *d_uniform, int32_t *d_tokens,
                                     float *d_probs);
 
+/* ------------------------------------------------------------------------ */
+/* Products on weights in 8-bit floats.  No counterpart in the reference,     */
+/* whose weights are Q4.                                                      */
+/* ------------------------------------------------------------------------ */
+
+/* A weight of n outputs and k inputs in the caller's own device buffers: codes
+ * in e4m3 (sign, 4 bits of exponent, 3 of mantissa, largest 448, 0x7f and 0xff
+ * NaN), rows of k of them ld bytes apart (codes 16-byte aligned, ld a multiple of
+ * 16), and an f32 scale for each block of 128 x 128, the last ones of a side cut
+ * short: value = code * scale. */
+typedef struct qtts_fp8_weight {
+    const uint8_t *codes;  /* [n], ld apart */
+    const float *scales;   /* [(n + 127) / 128][(k + 127) / 128] */
+    int32_t n;             /* 1..131072 */
+    int32_t k;             /* 16..131072, a multiple of 16 */
+    int32_t ld;
+} qtts_fp8_weight;
+
+/* y = x W^T (+ add): x rows of k floats, y and add (NULL: none; may be y itself
+ * with the same stride) rows of n, ld_* floats apart; pointers 16-byte aligned,
+ * strides multiples of 4; y is neither x nor overlaps it.  Each 128 values of a
+ * row of x (the last ones fewer) go to e4m3 on the way, the nearest to x / s, ties
+ * to even, with s the least power of two with which they stay within 448 (2^-110
+ * at least).  Products of codes are exact, their sums f32.  A row with an Inf or
+ * NaN is NaN, as is a column whose weight or scale has one.  rows 0..2^24.
+ * Enqueued on the context stream, allocates nothing and can be captured (context
+ * scratch, as above).  How the sum over k is divided goes by the sizes of a call,
+ * so a row's last bits may depend on how many others there are. */
+qtts_status qtts_fp8_gemm_device(qtts_ctx *ctx, const qtts_fp8_weight *w, const float *d_x, int32_t ld_x, int32_t rows,
+                                 const float *d_add, int32_t ld_add, float *d_y, int32_t ld_y);
+
+/* Fills w's codes and scales from n rows of k floats, ld_src apart: the same
+ * powers of two for each block of 128 x 128; a block with an Inf or NaN has scale
+ * NaN and codes 0.  Enqueued on the context stream, can be captured. */
+qtts_status qtts_fp8_quantize_device(qtts_ctx *ctx, const float *d_src, int32_t ld_src, const qtts_fp8_weight *w);
+
 #ifdef __cplusplus
 }
 #endif

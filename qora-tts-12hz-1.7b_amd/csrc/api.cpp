@@ -20,6 +20,7 @@
 #include "../../include/qtts_decoder.h"
 #include "../../include/qtts_synth.h"
 #include "engine.h"
+#include "fp8_plan.h"
 #include "internal.h"
 #include "paged_plan.h"
 #include "serve.h"
@@ -33,6 +34,7 @@ constexpr int kCounters = 8192;
 constexpr size_t kAttnPartFloats = (size_t)4 << 20;
 constexpr int kAttnCounters = 1024;
 static_assert(kAttnPartFloats >= (size_t)kPagedPartFloats, "the paged attention's chunks fit");
+static_assert(kAttnPartFloats >= (size_t)kFp8PartFloats && kCounters >= kFp8Counters, "the split products' sums fit");
 
 }  // namespace
 
@@ -45,6 +47,7 @@ struct qtts_ctx {
     float *attn_part = nullptr;
     unsigned *attn_counters = nullptr;
     unsigned *paged_counters = nullptr;
+    uint8_t *fp8_x = nullptr;  // rows of the products on 8-bit floats
     // staging for the stand-alone operators
     float *d_in = nullptr;
     size_t d_in_cap = 0;
@@ -89,6 +92,7 @@ void ctx_release(qtts_ctx *c) {
     (void)hipFree(c->attn_part);
     (void)hipFree(c->attn_counters);
     (void)hipFree(c->paged_counters);
+    (void)hipFree(c->fp8_x);
     (void)hipFree(c->d_in);
     (void)hipFree(c->d_out);
     (void)hipFree(c->d_small);
@@ -1592,6 +1596,7 @@ qtts_status qtts_ctx_create(int32_t device, qtts_ctx **out) {
     if (bad(hipMalloc(&c->attn_part, kAttnPartFloats * sizeof(float)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->attn_counters, kAttnCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->paged_counters, kPagedCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
+    if (bad(hipMalloc(&c->fp8_x, kFp8ScratchBytes))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->d_small, 256))) return QTTS_ENOMEM;
     if (bad(hipMemset(c->counters, 0, kCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
     if (bad(hipMemset(c->attn_counters, 0, kAttnCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
@@ -3012,6 +3017,36 @@ qtts_status qtts_sample_rows_device(qtts_ctx *c, const float *d_logits, int64_t 
     DeviceGuard guard(c->device);
     launch_sample_rows(c->stream, p);
     return check_launch(c, "k_sample_rows");
+}
+
+qtts_status qtts_fp8_gemm_device(qtts_ctx *c, const qtts_fp8_weight *w, const float *d_x, int32_t ld_x, int32_t rows,
+                                 const float *d_add, int32_t ld_add, float *d_y, int32_t ld_y) {
+    if (!c || !w) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_fp8_gemm(*w, d_x, ld_x, rows, d_add, ld_add, d_y, ld_y));
+    if (rows == 0) return QTTS_OK;
+    Fp8Params p{};
+    p.w = *w;
+    p.x = d_x;
+    p.add = d_add;
+    p.y = d_y;
+    p.ld_x = ld_x;
+    p.ld_add = ld_add;
+    p.ld_y = ld_y;
+    p.rows = rows;
+    p.xc = c->fp8_x;
+    p.part = c->attn_part;
+    p.counters = c->counters;
+    DeviceGuard guard(c->device);
+    launch_fp8_gemm(c->stream, p);
+    return check_launch(c, "k_fp8_tile");
+}
+
+qtts_status qtts_fp8_quantize_device(qtts_ctx *c, const float *d_src, int32_t ld_src, const qtts_fp8_weight *w) {
+    if (!c || !w) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_fp8_quantize(d_src, ld_src, *w));
+    DeviceGuard guard(c->device);
+    launch_fp8_quantize(c->stream, d_src, ld_src, *w);
+    return check_launch(c, "k_fp8_weight");
 }
 
 }  // extern "C"

@@ -1,5 +1,6 @@
 // serve.h — kernel parameter blocks and launches of the serving operators: the
-// paged 8-bit cache (paged.hip) and row sampling (sample_rows.hip).
+// paged 8-bit cache (paged.hip), row sampling (sample_rows.hip) and products on
+// 8-bit floats (fp8.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -56,10 +57,25 @@ struct SampleRowsParams {
     size_t scratch_bytes;
 };
 
-// The host's checks (paged_plan.h) have refused what a launch cannot hold.
+struct Fp8Params {
+    qtts_fp8_weight w;
+    const float *x, *add;
+    float *y;
+    int ld_x, ld_add, ld_y, rows;
+    uint8_t *xc;          // kFp8ScratchBytes: rows as the products take them
+    float *part;          // kFp8PartFloats: split sums
+    unsigned *counters;   // kFp8Counters, zero between launches
+    // the launch's own
+    int kb;               // blocks of the contraction
+    int tiles_n, splits, each;  // Fp8Plan; blocks of a split
+};
+
+// The host's checks (paged_plan.h, fp8_plan.h) have refused what a launch cannot hold.
 void launch_paged_append(hipStream_t st, const PagedAppendParams &p);
 void launch_paged_attention(hipStream_t st, const PagedAttnParams &p);
 void launch_paged_read(hipStream_t st, const PagedReadParams &p);
 void launch_sample_rows(hipStream_t st, const SampleRowsParams &p);
+void launch_fp8_gemm(hipStream_t st, const Fp8Params &p);
+void launch_fp8_quantize(hipStream_t st, const float *src, int ld_src, const qtts_fp8_weight &w);
 
 }  // namespace qtts

@@ -226,6 +226,13 @@ class RowSampler(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p")]
 
 
+class Fp8Weight(C.Structure):
+    """qtts_fp8_weight: a weight in 8-bit floats, device pointers; ld: bytes
+    between rows."""
+
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p)] + [(n, C.c_int32) for n in ("n", "k", "ld")]
+
+
 _lib = None
 
 
@@ -323,6 +330,8 @@ def load_library(path: str = LIB_PATH):
                                          vp, i32], i32),
         "qtts_paged_read_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), vp, vp, i32, vp, i32], i32),
         "qtts_sample_rows_device": ([vp, vp, C.c_int64, i32, i32, C.POINTER(RowSampler), vp, vp, vp], i32),
+        "qtts_fp8_gemm_device": ([vp, C.POINTER(Fp8Weight), vp, i32, i32, vp, i32, vp, i32], i32),
+        "qtts_fp8_quantize_device": ([vp, vp, i32, C.POINTER(Fp8Weight)], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -352,7 +361,7 @@ def exported_symbols() -> List[str]:
         "qtts_model_file_decoder", "qtts_decoder_upload", "qtts_decoder_free", "qtts_decoder_num_samples",
         "qtts_decode_to_audio", "qtts_decode_to_audio_device", "qtts_prefill_talker", "qtts_generate_speech",
         "qtts_paged_append_device", "qtts_paged_attention_device", "qtts_paged_read_device",
-        "qtts_sample_rows_device",
+        "qtts_sample_rows_device", "qtts_fp8_gemm_device", "qtts_fp8_quantize_device",
     ]
 
 
@@ -930,6 +939,16 @@ class Context:
         p = RowSampler(temperature, top_k, top_p, min_p)
         self.check(self.lib.qtts_sample_rows_device(self.h, logits, ld, rows, vocab, C.byref(p), uniform, tokens,
                                                     probs))
+
+    # Products on weights in 8-bit floats (include/qtts.h), device addresses.
+    def fp8_gemm_device(self, w: Fp8Weight, x: int, ld_x: int, rows: int, y: int, ld_y: int, add: int = 0,
+                        ld_add: int = 0):
+        """y = x W^T (+ add)."""
+        self.check(self.lib.qtts_fp8_gemm_device(self.h, C.byref(w), x, ld_x, rows, add, ld_add, y, ld_y))
+
+    def fp8_quantize_device(self, src: int, ld_src: int, w: Fp8Weight):
+        """Fills w's codes and scales from f32 rows."""
+        self.check(self.lib.qtts_fp8_quantize_device(self.h, src, ld_src, C.byref(w)))
 
 
 class DeviceQ4(_DeviceObject):

@@ -1,0 +1,223 @@
+"""Products on weights in 8-bit floats (qtts_fp8_gemm_device) and the weights'
+quantizer, against their restatement in 64 bits (tests/fp8_model.py).
+
+Tolerances.  Codes and scales are equal.  A product of two codes is exact in
+f32 and so are the rows' powers of two; a weight's scale takes one rounding with
+its block's sum (a fused multiply-add).  A sum of 128 products, one of the
+blocks and joining at most 64 parts are f32 additions, each off by at most half
+a step of a partial sum, which is within the sum of magnitudes: (128 + blocks +
+64 + 2) * 2^-24 of that."""
+import numpy as np
+import pytest
+import torch
+
+import fp8_model as fm
+import qtts
+
+pytestmark = pytest.mark.gpu
+
+
+def _up(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def _padded(rows, width, ld, fill, dtype=torch.float32):
+    return torch.full((rows, ld), fill, dtype=dtype, device="cuda")
+
+
+class Weight:
+    def __init__(self, codes, scales, ld=None):
+        n, k = codes.shape
+        self.ld = k if ld is None else ld
+        # what lies behind a row's end is NaN
+        self.codes = torch.full((n, self.ld), 127, dtype=torch.uint8, device="cuda")
+        self.codes[:, :k] = _up(codes)
+        self.scales = _up(scales)
+        self.host = (codes, scales)
+        self.w = qtts.Fp8Weight(self.codes.data_ptr(), self.scales.data_ptr(), n, k, self.ld)
+
+
+def _weight(seed, n, k, ld=None):
+    r = np.random.default_rng(seed)
+    codes = r.integers(0, 256, (n, k)).astype(np.uint8)
+    codes[codes & 127 == 127] = 0x3a
+    scales = (np.exp(r.standard_normal((-(-n // 128), -(-k // 128)))) * 0.01).astype(np.float32)
+    return Weight(codes, scales, ld)
+
+
+def _rows(seed, rows, k):
+    r = np.random.default_rng(seed)
+    return (r.standard_normal((rows, k)) * np.exp(r.standard_normal(k))).astype(np.float32)
+
+
+def _gemm(ctx, w, x, add=None, ld_y=None, ld_x=None):
+    """y with what lies behind its rows and their ends checked to be as it was."""
+    rows, k = x.shape
+    n = w.w.n
+    ld_x, ld_y = ld_x or -(-k // 4) * 4, ld_y or -(-n // 4) * 4
+    dx = _padded(rows + 1, k, ld_x, float("nan"))
+    dx[:rows, :k] = _up(x)
+    y = _padded(rows + 2, n, ld_y, 7.0)
+    more = {}
+    if add is not None:
+        da = _padded(rows, n, ld_y + 8, float("nan"))
+        da[:, :n] = _up(add)
+        more = dict(add=da.data_ptr(), ld_add=ld_y + 8)
+    torch.cuda.synchronize()
+    ctx.fp8_gemm_device(w.w, dx.data_ptr(), ld_x, rows, y.data_ptr(), ld_y, **more)
+    ctx.synchronize()
+    y = y.cpu().numpy()
+    assert np.all(y[rows:] == 7.0) and np.all(y[:, n:] == 7.0)
+    return y[:rows, :n]
+
+
+def _check(got, x, w, add=None, tell=""):
+    ref, mass = fm.product(x, *w.host, add)
+    kb = -(-x.shape[1] // 128)
+    bound = (128 + kb + 66) * 2.0 ** -24 * mass + 2.0 ** -149
+    off = np.abs(got - ref)
+    assert np.all(off <= bound), (tell, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("k", [16, 48, 112, 128, 144, 256, 400, 1040])
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 33, 64, 129])
+def test_sizes(ctx, rows, k):
+    """Odd outputs, blocks cut short on either side."""
+    for n in (1, 31, 128, 197, 300):
+        w = _weight(n + k, n, k, ld=-(-k // 16) * 16 + 32)
+        x = _rows(rows + k, rows, k)
+        _check(_gemm(ctx, w, x, ld_x=k + 4, ld_y=-(-n // 4) * 4 + 4), x, w, tell=(rows, n, k))
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 4096, 2048), (3, 2048, 6144), (16, 2048, 6144), (40, 1000, 6144),
+                                      (200, 640, 2048), (515, 1100, 512), (700, 300, 8192)])
+def test_large(ctx, rows, n, k):
+    w, x, add = _weight(1, n, k), _rows(2, rows, k), _rows(3, rows, n)
+    _check(_gemm(ctx, w, x), x, w)
+    _check(_gemm(ctx, w, x, add=add), x, w, add)
+
+
+@pytest.mark.parametrize("rows", [5, 40])
+def test_residual_in_place(ctx, rows):
+    w, x, add = _weight(4, 260, 384), _rows(5, rows, 384), _rows(6, rows, 260)
+    dx, y = _up(x), _up(add)
+    torch.cuda.synchronize()
+    ctx.fp8_gemm_device(w.w, dx.data_ptr(), 384, rows, y.data_ptr(), 260, add=y.data_ptr(), ld_add=260)
+    ctx.synchronize()
+    _check(y.cpu().numpy(), x, w, add)
+
+
+def _edges():
+    """Rows of 128 values with every code's value, every border between two and
+    their neighbours, at several powers of two; zeros; the ends of f32."""
+    v = np.sort(fm.VALUES[~np.isnan(fm.VALUES)])
+    mid = (v[1:] + v[:-1]) / 2
+    near = [np.nextafter(mid.astype(np.float32), np.float32(s * np.inf)) for s in (1, -1)]
+    pool = np.concatenate([v, mid, *near]).astype(np.float32)
+    pool = np.concatenate([pool, np.zeros(-pool.size % 127, np.float32)]).reshape(-1, 127)
+    rows = [np.concatenate([p, [np.float32(448)]]) * np.float32(2.0 ** s)
+            for p in pool for s in (0, -3, 60, 118, -100, -117, -120, -126)]
+    for top in (448.0, np.nextafter(np.float32(448), np.float32(1e9)), 3.4028235e38, 1.1754944e-38, 1e-45, 0.0):
+        rows.append(np.linspace(-1, 1, 128).astype(np.float32) * np.float32(top))
+    return np.stack(rows).astype(np.float32)
+
+
+@pytest.mark.parametrize("each", [7, 64])
+def test_rows_are_rounded_exactly(ctx, each):
+    """Through a weight of ones on the diagonal a row comes back as its codes'
+    values."""
+    w = Weight(np.where(np.eye(128, dtype=bool), 0x38, 0).astype(np.uint8), np.ones((1, 1), np.float32))
+    x = _edges()
+    for at in range(0, x.shape[0], each):
+        part = x[at:at + each]
+        assert np.array_equal(_gemm(ctx, w, part), fm.blocks(part).astype(np.float32)), at
+
+
+@pytest.mark.parametrize("n,k", [(128, 128), (1, 16), (130, 272), (300, 1008)])
+def test_weights_are_rounded_exactly(ctx, n, k):
+    r = np.random.default_rng(n)
+    src = (r.standard_normal((n, k)) * np.exp(3 * r.standard_normal((n, 1)))).astype(np.float32)
+    edges = _edges().reshape(-1)
+    m = min(edges.size, src.size // 2)
+    src.reshape(-1)[:m] = edges[:m]
+    src[-1, -16:] = [0.0, -0.0] * 8
+    dsrc = _padded(n, k, k + 4, float("nan"))
+    dsrc[:, :k] = _up(src)
+    codes = torch.full((n + 1, k + 16), 99, dtype=torch.uint8, device="cuda")
+    scales = torch.full((-(-n // 128) * -(-k // 128) + 1,), 5.0, device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp8_quantize_device(dsrc.data_ptr(), k + 4, qtts.Fp8Weight(codes.data_ptr(), scales.data_ptr(), n, k, k + 16))
+    ctx.synchronize()
+    ref, s = fm.quantized(src)
+    codes, scales = codes.cpu().numpy(), scales.cpu().numpy()
+    assert np.array_equal(scales[:-1].reshape(s.shape), s) and scales[-1] == 5.0
+    assert np.array_equal(codes[:n, :k], ref)
+    assert np.all(codes[n:] == 99) and np.all(codes[:, k:] == 99)
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("rows", [3, 30])
+def test_not_finite(ctx, rows, bad):
+    """A row with an Inf or NaN is NaN, the others are not; a weight's code or
+    scale makes its outputs NaN; a block of a weight that is not finite has
+    scale NaN."""
+    n, k = 300, 272
+    w, x = _weight(8, n, k), _rows(9, rows, k)
+    x[1, 260] = bad
+    got = _gemm(ctx, w, x)
+    assert np.all(np.isnan(got[1]))
+    rest = [i for i in range(rows) if i != 1]
+    _check(got[rest], x[rest], w)
+    codes, scales = (a.copy() for a in w.host)
+    codes[17, 271], scales[1, 0] = 0xff, bad
+    x = np.abs(_rows(9, rows, k)) + 1
+    got = _gemm(ctx, Weight(codes, scales), x)
+    assert np.all(np.isnan(got[:, 17])) and not np.any(np.isfinite(got[:, 128:256]))
+    some = np.r_[0:17, 18:128, 256:300]
+    ref, mass = fm.product(x, w.host[0], w.host[1])
+    assert np.all(np.abs(got[:, some] - ref[:, some]) <= 200 * 2.0 ** -24 * mass[:, some])
+    src = _rows(10, n, k)
+    src[130, 200] = bad
+    dsrc, dc, ds = _up(src), torch.zeros((n, k), dtype=torch.uint8, device="cuda"), torch.zeros((3, 3), device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp8_quantize_device(dsrc.data_ptr(), k, qtts.Fp8Weight(dc.data_ptr(), ds.data_ptr(), n, k, k))
+    ctx.synchronize()
+    codes, scales = fm.quantized(src)
+    assert np.isnan(scales[1, 1]) and np.array_equal(ds.cpu().numpy(), scales, equal_nan=True)
+    assert np.array_equal(dc.cpu().numpy(), codes)
+
+
+def test_no_rows(ctx):
+    w = _weight(1, 32, 64)
+    ctx.fp8_gemm_device(w.w, 0, 64, 0, 0, 32)
+
+
+def test_graph_and_own_stream(ctx):
+    """Captured and replayed on other values, between plain calls that use the
+    scratch for other sizes."""
+    w, big = _weight(11, 640, 2048), _weight(12, 200, 1024)
+    xs = [_rows(20 + i, 40, 2048) for i in range(3)]
+    x, y = _up(xs[0]), torch.zeros((40, 640), device="cuda")
+    bx, by = _up(_rows(30, 300, 1024)), torch.zeros((300, 200), device="cuda")
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    call = lambda: ctx.fp8_gemm_device(w.w, x.data_ptr(), 2048, 40, y.data_ptr(), 640)
+    torch.cuda.synchronize()
+    alone = []
+    for a in xs:
+        x.copy_(_up(a))
+        torch.cuda.synchronize()
+        call()
+        ctx.synchronize()
+        alone.append(y.clone())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        call()
+    for i in (1, 2, 0, 2):
+        with torch.cuda.stream(stream):
+            x.copy_(_up(xs[i]))
+            ctx.fp8_gemm_device(big.w, bx.data_ptr(), 1024, 300, by.data_ptr(), 200)
+            g.replay()
+            ctx.fp8_gemm_device(big.w, bx.data_ptr(), 1024, 300, by.data_ptr(), 200)
+        torch.cuda.synchronize()
+        assert torch.equal(y, alone[i])
