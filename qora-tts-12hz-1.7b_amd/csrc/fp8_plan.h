@@ -16,6 +16,7 @@ constexpr long long kFp8MaxRows = 1LL << 24;
 constexpr size_t kFp8ScratchBytes = (size_t)64 << 20;  // a context's: rows, in bfloat16
 constexpr int kFp8RowStep = 256;                  // rows that a tile takes at most
 constexpr long long kFp8PartFloats = 4LL << 20;   // split sums
+constexpr int kFp8MaxSplits = 64;
 constexpr int kFp8Counters = 8192;                // a tile's, zero between launches
 
 inline int fp8_blocks(int k) { return (k + kFp8Block - 1) / kFp8Block; }
@@ -75,8 +76,9 @@ inline Fp8Plan fp8_plan(int rows, int n, int k) {
     p.splits = 1;
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     const int least = rows <= 16 ? 4 : 2;  // blocks of a split at least
-    long long want = rows <= 16 ? 512 / tiles : 512 / tiles;
+    long long want = 512 / tiles;
     if (want > kb / least) want = kb / least;
+    if (want > kFp8MaxSplits) want = kFp8MaxSplits;
     while (want > 1 && (tiles > kFp8Counters || tiles * want * p.bn * p.bm > kFp8PartFloats)) want--;
     if (want > 1) {
         const int each = (int)((kb + want - 1) / want);
