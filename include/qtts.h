@@ -474,6 +474,77 @@ qtts_status qtts_paged_read_device(qtts_ctx *ctx, const qtts_paged_kv *kv, const
                                    const int32_t *d_lens, float *d_k_out, int32_t ld_k_out, float *d_v_out,
                                    int32_t ld_v_out);
 
+/* The pages of a cache, whose owners are counted on the device, so that sequences
+ * can share beginnings, and the page table and slots of its sequences.  One pool
+ * serves every layer: layers hold a page under the same id and a slot's open rows
+ * under the same number.  refs[i] is how many table entries hold page i (and how
+ * many the caller keeps for himself); a page with 0 or below is free.  refs must be
+ * 16-byte aligned. */
+typedef struct qtts_paged_pool {
+    int32_t *refs;       /* [num_pages] */
+    int32_t *page_table; /* [batch][max_pages]; an entry outside the pool: no page */
+    int32_t *slots;      /* [batch], different ones */
+    int32_t num_pages;   /* 1..2^22 - 64 */
+    int32_t page_size;   /* 16, 32, 64 or 128 */
+    int32_t batch;       /* to 8192; batch * max_pages to 2^22 */
+    int32_t max_pages;
+} qtts_paged_pool;
+
+/* Sequences go on, fork, go back, drop what a window has passed, or end: row b of
+ * the table becomes row source[b] (device, [batch]; NULL: b) as it was before the
+ * call, up to tokens[b] tokens ([batch], 0..max_pages * page_size, clamped to it).
+ * A row that goes on from itself keeps its pages up to the last one begun; one that
+ * goes on from another shares that one's full pages.  A source outside the batch
+ * ends the row: it holds nothing.  With window > 0, pages whose tokens the next row
+ * of attention with this window and these sinks does not see are dropped.  What a
+ * row no longer holds is given back.  To go back into a full page, make tokens[b]
+ * its first token: a shared page is then not written again.
+ * Slots: a row that goes on from itself keeps its slot; the slot of one that only
+ * others go on from goes to the first of them; the other rows take those of the rows
+ * that ended, in order.  copied (NULL or [batch]) receives the slot whose open rows
+ * row b has to copy before its next append (qtts_paged_copy_open_device, every
+ * layer), or -1.
+ * Enqueued on the context stream, allocates nothing and can be captured; larger
+ * tables use context scratch, as attention does. */
+qtts_status qtts_paged_remap_device(qtts_ctx *ctx, const qtts_paged_pool *pool, const int32_t *d_source,
+                                    const int32_t *d_tokens, int32_t window, int32_t sinks, int32_t *d_copied);
+
+/* Gives row b pages for its tokens starts[b] .. ends[b] - 1 (device, [batch]) where
+ * the table has none: the lowest free ones, in order of rows and entries.  lacking
+ * (NULL or [batch]) receives 0 for a row that has them all now, -1 for one whose
+ * start is negative or whose end is below 0 or past the table, which is left out.
+ * From the first row that the free pages do not serve whole, rows receive none, and
+ * lacking says how many each wants.  Enqueued on the context stream, allocates
+ * nothing and can be captured (context scratch, as above). */
+qtts_status qtts_paged_reserve_device(qtts_ctx *ctx, const qtts_paged_pool *pool, const int32_t *d_starts,
+                                      const int32_t *d_ends, int32_t *d_lacking);
+
+/* Packs the pool: the pages in use become its first ones.  The i-th page in use
+ * behind that border takes the id of the i-th free one before it; refs and table
+ * follow.  from and to (device, [num_pages / 2]) receive the moves, -1 behind them,
+ * live (NULL or one int) how many pages are in use.  Then every layer copies its
+ * pages (qtts_paged_copy_pages_device with num_pages / 2) before they are read or
+ * written.  Enqueued on the context stream, allocates nothing and can be captured
+ * (context scratch, as above). */
+qtts_status qtts_paged_compact_device(qtts_ctx *ctx, const qtts_paged_pool *pool, int32_t *d_from, int32_t *d_to,
+                                      int32_t *d_live);
+
+/* Copies codes and scales of pages from[i] of one layer's cache to pages to[i] of
+ * another of the same page shape, or of the same one (device, [n]); a pair with a
+ * page outside its pool is left out.  A page that is written must not be in another
+ * pair.  The open rows may be NULL.  Enqueued on the context stream, allocates
+ * nothing and can be captured. */
+qtts_status qtts_paged_copy_pages_device(qtts_ctx *ctx, const qtts_paged_kv *from_kv, const qtts_paged_kv *to_kv,
+                                         int32_t n, const int32_t *d_from, const int32_t *d_to);
+
+/* Copies the open rows of slots from[i] to slots to[i] of one layer's cache, as
+ * many as tokens[i] tokens have behind their last full page (device, [n]); a pair
+ * with a slot outside the slots, or of one slot, is left out.  A slot that is
+ * written must not be in another pair.  The pages may be NULL.  Enqueued on the
+ * context stream, allocates nothing and can be captured. */
+qtts_status qtts_paged_copy_open_device(qtts_ctx *ctx, const qtts_paged_kv *kv, int32_t n, const int32_t *d_from,
+                                        const int32_t *d_to, const int32_t *d_tokens);
+
 /* Settings of each row's draw, device arrays of `rows` entries; NULL: 1, off,
  * off, off. */
 typedef struct qtts_row_sampler {

@@ -23,6 +23,7 @@
 #include "fp8_plan.h"
 #include "internal.h"
 #include "paged_plan.h"
+#include "pages_plan.h"
 #include "serve.h"
 
 using namespace qtts;
@@ -35,6 +36,7 @@ constexpr size_t kAttnPartFloats = (size_t)4 << 20;
 constexpr int kAttnCounters = 1024;
 static_assert(kAttnPartFloats >= (size_t)kPagedPartFloats, "the paged attention's chunks fit");
 static_assert(kAttnPartFloats >= (size_t)kFp8PartFloats && kCounters >= kFp8Counters, "the split products' sums fit");
+static_assert(kAttnPartFloats >= (size_t)kPoolEntries && kAttnPartFloats > (size_t)kPoolPages, "a page table's copy fits");
 
 }  // namespace
 
@@ -2995,6 +2997,55 @@ qtts_status qtts_paged_read_device(qtts_ctx *c, const qtts_paged_kv *kv, const q
     DeviceGuard guard(c->device);
     launch_paged_read(c->stream, p);
     return check_launch(c, "k_paged_read");
+}
+
+qtts_status qtts_paged_remap_device(qtts_ctx *c, const qtts_paged_pool *pool, const int32_t *d_source,
+                                    const int32_t *d_tokens, int32_t window, int32_t sinks, int32_t *d_copied) {
+    if (!c || !pool) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_remap(*pool, d_source, d_tokens, window, sinks, d_copied));
+    if (pool->batch == 0) return QTTS_OK;
+    DeviceGuard guard(c->device);
+    launch_paged_remap(c->stream, {*pool, d_source, d_tokens, window, sinks, d_copied, (int32_t *)c->attn_part});
+    return check_launch(c, "k_paged_remap");
+}
+
+qtts_status qtts_paged_reserve_device(qtts_ctx *c, const qtts_paged_pool *pool, const int32_t *d_starts,
+                                      const int32_t *d_ends, int32_t *d_lacking) {
+    if (!c || !pool) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_reserve(*pool, d_starts, d_ends, d_lacking));
+    if (pool->batch == 0) return QTTS_OK;
+    DeviceGuard guard(c->device);
+    launch_paged_reserve(c->stream, {*pool, d_starts, d_ends, d_lacking, (int32_t *)c->attn_part});
+    return check_launch(c, "k_paged_reserve");
+}
+
+qtts_status qtts_paged_compact_device(qtts_ctx *c, const qtts_paged_pool *pool, int32_t *d_from, int32_t *d_to,
+                                      int32_t *d_live) {
+    if (!c || !pool) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_compact(*pool, d_from, d_to, d_live));
+    DeviceGuard guard(c->device);
+    launch_paged_compact(c->stream, {*pool, d_from, d_to, d_live, (int32_t *)c->attn_part});
+    return check_launch(c, "k_paged_compact");
+}
+
+qtts_status qtts_paged_copy_pages_device(qtts_ctx *c, const qtts_paged_kv *from_kv, const qtts_paged_kv *to_kv,
+                                         int32_t n, const int32_t *d_from, const int32_t *d_to) {
+    if (!c || !from_kv || !to_kv) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_copy_pages(*from_kv, *to_kv, n, d_from, d_to));
+    if (n == 0) return QTTS_OK;
+    DeviceGuard guard(c->device);
+    launch_paged_copy_pages(c->stream, {*from_kv, *to_kv, d_from, d_to}, n);
+    return check_launch(c, "k_paged_copy_pages");
+}
+
+qtts_status qtts_paged_copy_open_device(qtts_ctx *c, const qtts_paged_kv *kv, int32_t n, const int32_t *d_from,
+                                        const int32_t *d_to, const int32_t *d_tokens) {
+    if (!c || !kv) return QTTS_EINVAL;
+    QTTS_CHECK(c, check_copy_open(*kv, n, d_from, d_to, d_tokens));
+    if (n == 0) return QTTS_OK;
+    DeviceGuard guard(c->device);
+    launch_paged_copy_open(c->stream, {*kv, d_from, d_to, d_tokens}, n);
+    return check_launch(c, "k_paged_copy_open");
 }
 
 qtts_status qtts_sample_rows_device(qtts_ctx *c, const float *d_logits, int64_t ld, int32_t rows, int32_t vocab,

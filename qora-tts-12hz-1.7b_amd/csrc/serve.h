@@ -1,5 +1,5 @@
 // serve.h — kernel parameter blocks and launches of the serving operators: the
-// paged 8-bit cache (paged.hip), row sampling (sample_rows.hip) and products on
+// paged 8-bit cache (paged.hip) and its pages (pages.hip), row sampling (sample_rows.hip) and products on
 // 8-bit floats (fp8.hip).
 #pragma once
 
@@ -45,6 +45,37 @@ struct PagedReadParams {
     int cap;  // tokens a sequence may reach
 };
 
+struct RemapParams {
+    qtts_paged_pool pool;
+    const int32_t *source, *tokens;
+    int window, sinks;
+    int32_t *copied;
+    int32_t *scratch;  // kPoolEntries
+};
+
+struct ReserveParams {
+    qtts_paged_pool pool;
+    const int32_t *starts, *ends;
+    int32_t *lacking;
+    int32_t *scratch;  // num_pages
+};
+
+struct CompactParams {
+    qtts_paged_pool pool;
+    int32_t *from, *to, *live;
+    int32_t *scratch;  // num_pages + 1
+};
+
+struct CopyPagesParams {
+    qtts_paged_kv a, b;
+    const int32_t *from, *to;
+};
+
+struct CopyOpenParams {
+    qtts_paged_kv kv;
+    const int32_t *from, *to, *tokens;
+};
+
 struct SampleRowsParams {
     const float *logits;
     long long ld;
@@ -70,10 +101,15 @@ struct Fp8Params {
     int tiles_n, splits, each;  // Fp8Plan; blocks of a split
 };
 
-// The host's checks (paged_plan.h, fp8_plan.h) have refused what a launch cannot hold.
+// The host's checks (paged_plan.h, pages_plan.h, fp8_plan.h) have refused what a launch cannot hold.
 void launch_paged_append(hipStream_t st, const PagedAppendParams &p);
 void launch_paged_attention(hipStream_t st, const PagedAttnParams &p);
 void launch_paged_read(hipStream_t st, const PagedReadParams &p);
+void launch_paged_remap(hipStream_t st, const RemapParams &p);
+void launch_paged_reserve(hipStream_t st, const ReserveParams &p);
+void launch_paged_compact(hipStream_t st, const CompactParams &p);
+void launch_paged_copy_pages(hipStream_t st, const CopyPagesParams &p, int n);
+void launch_paged_copy_open(hipStream_t st, const CopyOpenParams &p, int n);
 void launch_sample_rows(hipStream_t st, const SampleRowsParams &p);
 void launch_fp8_gemm(hipStream_t st, const Fp8Params &p);
 void launch_fp8_quantize(hipStream_t st, const float *src, int ld_src, const qtts_fp8_weight &w);

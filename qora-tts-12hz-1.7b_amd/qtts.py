@@ -222,6 +222,14 @@ class PagedRows(C.Structure):
         ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p)]
 
 
+class PagedPool(C.Structure):
+    """qtts_paged_pool: a cache's pages with their owners counted, its page
+    table and slots, device pointers."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("refs", "page_table", "slots")] + [
+        (n, C.c_int32) for n in ("num_pages", "page_size", "batch", "max_pages")]
+
+
 class RowSampler(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p")]
 
@@ -329,6 +337,11 @@ def load_library(path: str = LIB_PATH):
         "qtts_paged_attention_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), i32, vp, i32, C.c_float, i32,
                                          vp, i32], i32),
         "qtts_paged_read_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), vp, vp, i32, vp, i32], i32),
+        "qtts_paged_remap_device": ([vp, C.POINTER(PagedPool), vp, vp, i32, i32, vp], i32),
+        "qtts_paged_reserve_device": ([vp, C.POINTER(PagedPool), vp, vp, vp], i32),
+        "qtts_paged_compact_device": ([vp, C.POINTER(PagedPool), vp, vp, vp], i32),
+        "qtts_paged_copy_pages_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedKv), i32, vp, vp], i32),
+        "qtts_paged_copy_open_device": ([vp, C.POINTER(PagedKv), i32, vp, vp, vp], i32),
         "qtts_sample_rows_device": ([vp, vp, C.c_int64, i32, i32, C.POINTER(RowSampler), vp, vp, vp], i32),
         "qtts_fp8_gemm_device": ([vp, C.POINTER(Fp8Weight), vp, i32, i32, vp, i32, vp, i32], i32),
         "qtts_fp8_quantize_device": ([vp, vp, i32, C.POINTER(Fp8Weight)], i32),
@@ -361,7 +374,8 @@ def exported_symbols() -> List[str]:
         "qtts_model_file_decoder", "qtts_decoder_upload", "qtts_decoder_free", "qtts_decoder_num_samples",
         "qtts_decode_to_audio", "qtts_decode_to_audio_device", "qtts_prefill_talker", "qtts_generate_speech",
         "qtts_paged_append_device", "qtts_paged_attention_device", "qtts_paged_read_device",
-        "qtts_sample_rows_device", "qtts_fp8_gemm_device", "qtts_fp8_quantize_device",
+        "qtts_paged_remap_device", "qtts_paged_reserve_device", "qtts_paged_compact_device",
+        "qtts_paged_copy_pages_device", "qtts_paged_copy_open_device", "qtts_sample_rows_device", "qtts_fp8_gemm_device", "qtts_fp8_quantize_device",
     ]
 
 
@@ -933,6 +947,26 @@ class Context:
                           ld_v_out: int):
         self.check(self.lib.qtts_paged_read_device(self.h, C.byref(kv), C.byref(seqs), lens, k_out, ld_k_out, v_out,
                                                    ld_v_out))
+
+    def paged_remap_device(self, pool: PagedPool, source: int, tokens: int, window: int = 0, sinks: int = 0,
+                           copied: int = 0):
+        """Rows go on, fork, go back, drop pages behind a window, or end."""
+        self.check(self.lib.qtts_paged_remap_device(self.h, C.byref(pool), source, tokens, window, sinks, copied))
+
+    def paged_reserve_device(self, pool: PagedPool, starts: int, ends: int, lacking: int = 0):
+        """Pages for each row's next tokens."""
+        self.check(self.lib.qtts_paged_reserve_device(self.h, C.byref(pool), starts, ends, lacking))
+
+    def paged_compact_device(self, pool: PagedPool, moved_from: int, moved_to: int, live: int = 0):
+        """The pages in use become the pool's first; the moves are every layer's to copy."""
+        self.check(self.lib.qtts_paged_compact_device(self.h, C.byref(pool), moved_from, moved_to, live))
+
+    def paged_copy_pages_device(self, from_kv: PagedKv, to_kv: PagedKv, n: int, pages_from: int, pages_to: int):
+        self.check(self.lib.qtts_paged_copy_pages_device(self.h, C.byref(from_kv), C.byref(to_kv), n, pages_from,
+                                                         pages_to))
+
+    def paged_copy_open_device(self, kv: PagedKv, n: int, slots_from: int, slots_to: int, tokens: int):
+        self.check(self.lib.qtts_paged_copy_open_device(self.h, C.byref(kv), n, slots_from, slots_to, tokens))
 
     def sample_rows_device(self, logits: int, ld: int, rows: int, vocab: int, uniform: int, tokens: int,
                            probs: int = 0, temperature: int = 0, top_k: int = 0, top_p: int = 0, min_p: int = 0):
