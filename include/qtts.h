@@ -463,6 +463,13 @@ qtts_status qtts_paged_attention_device(qtts_ctx *ctx, const qtts_paged_kv *kv, 
                                         int32_t heads, const float *d_q, int32_t ld_q, float scale, int32_t window,
                                         float *d_out, int32_t ld_out);
 
+/* The same with sinks: under a window (window > 0) every row sees the first `sinks`
+ * tokens of its sequence too, as far as they are before it.  What a row does not see
+ * is not read, so a stream of any length costs its sinks and its window. */
+qtts_status qtts_paged_attention_sinks_device(qtts_ctx *ctx, const qtts_paged_kv *kv, const qtts_paged_seqs *seqs,
+                                              int32_t heads, const float *d_q, int32_t ld_q, float scale,
+                                              int32_t window, int32_t sinks, float *d_out, int32_t ld_out);
+
 /* Cached tokens as f32 rows: sequence b, lens[b] tokens long (device, [batch];
  * NULL: up to its last row asked for), gives positions starts[b] and on into
  * rows row_offsets[b] up to row_offsets[b + 1] of k_out and v_out (kv_heads *

@@ -2959,8 +2959,14 @@ qtts_status qtts_paged_append_device(qtts_ctx *c, const qtts_paged_kv *kv, const
 qtts_status qtts_paged_attention_device(qtts_ctx *c, const qtts_paged_kv *kv, const qtts_paged_seqs *s, int32_t heads,
                                         const float *d_q, int32_t ld_q, float scale, int32_t window, float *d_out,
                                         int32_t ld_out) {
+    return qtts_paged_attention_sinks_device(c, kv, s, heads, d_q, ld_q, scale, window, 0, d_out, ld_out);
+}
+
+qtts_status qtts_paged_attention_sinks_device(qtts_ctx *c, const qtts_paged_kv *kv, const qtts_paged_seqs *s,
+                                              int32_t heads, const float *d_q, int32_t ld_q, float scale,
+                                              int32_t window, int32_t sinks, float *d_out, int32_t ld_out) {
     if (!c || !kv || !s) return QTTS_EINVAL;
-    QTTS_CHECK(c, check_attention(*kv, *s, heads, d_q, ld_q, scale, window, d_out, ld_out));
+    QTTS_CHECK(c, check_attention_sinks(*kv, *s, heads, d_q, ld_q, scale, window, sinks, d_out, ld_out));
     if (paged_empty(*s)) return QTTS_OK;
     PagedAttnParams p{};
     p.kv = *kv;
@@ -2972,6 +2978,7 @@ qtts_status qtts_paged_attention_device(qtts_ctx *c, const qtts_paged_kv *kv, co
     p.ld_out = ld_out;
     p.scale = scale;
     p.window = window;
+    p.sinks = sinks;
     p.cap = (int)tokens_cap(*kv, *s);
     p.part = c->attn_part;
     p.counters = c->paged_counters;

@@ -406,7 +406,12 @@ __device__ __forceinline__ float row_scale(float x) {
 //
 // Three blocks of 64 dimensions fit a CU's registers (tiles of 32 columns, 8
 // sequences of 500 rows, a window of 72: 33 us, 38 with two), two of 128.
-template <int HD, int MODE>
+//
+// SINKS: with a window, the first tokens stay visible.  The tokens that a tile sees
+// are then two stretches, the sinks' and the window's, each begun at a multiple of
+// 64: they are numbered through, chunks and steps divide that numbering, and a
+// step, which never lies in both, adds the hole between them to its tokens.
+template <int HD, int MODE, bool SINKS>
 __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnParams A) {
     constexpr bool I8 = MODE == kAttnI8;
     constexpr int S = MODE == kAttn32 ? 32 : 16;  // side of a product's tile
@@ -480,12 +485,21 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     // steps: by this sequence's own length, not by its page table's.
     const int row_a = tile * CT / group, row_b = (tile * CT + left - 1) / group;
     const int high = q.start + row_b + 1;
-    const int low = A.window > 0 ? max(0, q.start + row_a - A.window + 1) : 0;
-    const int from = low & ~63, chunk = chunk_of(high - from, nsplit, attn_least(CT));
-    const int parts = (high - from + chunk - 1) / chunk;
+    int low = A.window > 0 ? max(0, q.start + row_a - A.window + 1) : 0, from = low & ~63;
+    // Numbers from `edge` on are `hole` below their tokens.  (Where there is a hole
+    // the sinks lie in full pages: they end 64 tokens before the window begins.)
+    const SeenHole gap = SINKS ? seen_hole(low, high, A.sinks) : SeenHole{0, 0};
+    const int hole = gap.hole, edge = gap.edge;
+    if (SINKS) from = 0, low = hole ? low : 0;
+    const int chunk = chunk_of(high - hole - from, nsplit, attn_least(CT));
+    const int parts = (high - hole - from + chunk - 1) / chunk;
     if (split >= parts) return;
     const int c0 = from + split * chunk;
     const int end = q.start + q.rows, full = end >> sh << sh;
+    auto token_of = [&](int number) { return SINKS ? number + (number >= edge ? hole : 0) : number; };
+    auto in_window = [&](int token, int pos) {
+        return A.window == 0 || token > pos - A.window || (SINKS && token < A.sinks);
+    };
 
     // this lane's column
     const int n = I8 ? r & 3 : r, digit = I8 ? r >> 2 : 0;
@@ -495,7 +509,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     const float *qr = A.q + (size_t)(q.row0 + col / group) * A.ld_q + (size_t)(head * group + col % group) * HD;
 
     // --- full pages: the first step's loads ---
-    const int stop = min(min(c0 + chunk, full), high);
+    const int stop = SINKS && hole ? min(c0 + chunk, max(edge, min(full, high) - hole)) : min(min(c0 + chunk, full), high);
     int base = c0 + ST * wave;
     u32x4 kr[NT][NK], vr[ND];
     // Loads come back in the order they are issued, so each is issued behind
@@ -503,7 +517,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     // wait for any of them a wait for all): past the last token, and for an
     // absent page, they read the pool's first page, whose tokens are masked.
     auto page_at = [&](int token) {
-        const int pg = q.pages[min(token, stop - 1) >> sh];
+        const int pg = q.pages[token_of(min(token, stop - 1)) >> sh];
         return token < stop && pg >= 0 && pg < A.kv.num_pages ? pg : -1;
     };
     auto block_of = [&](int pg) { return (unsigned)(max(pg, 0) * kvh + head); };
@@ -539,9 +553,9 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         }
     auto load_first = [&]() {
         if (any) {
-            load_k(base, pk);
+            load_k(token_of(base), pk);
             ks_ = A.kv.k_scales[block_of(pv)], vs_ = A.kv.v_scales[block_of(pv)];
-            load_v(base, pv);
+            load_v(token_of(base), pv);
         }
     };
     if (S == 16) load_first();
@@ -652,7 +666,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
     // Tiles of 16 read them to registers (while the first step's pages are on
     // their way); with tiles of 32, which have none to spare, the block brings
     // K's and then V's to LDS, in the place of its result.
-    const int open_lo = max(max(full, low), c0), open_hi = min(min(end, c0 + chunk), high);
+    const int open_lo = max(max(full, low), c0 + hole), open_hi = min(min(end, c0 + chunk + hole), high);
     const float *k_open = A.kv.k_open + ((size_t)q.slot * kvh + head) * P * HD;
     const float *v_open = A.kv.v_open + ((size_t)q.slot * kvh + head) * P * HD;
     float(*rows)[HD + 4] = so[0];  // S == 32: row t - open_lo of the open page, 128 at most
@@ -767,7 +781,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                     }
                     tops[S == 16 ? i : 0] = row16_max(top);
                 }
-                const bool seen = token <= pos && token < open_hi && (A.window == 0 || token > pos - A.window);
+                const bool seen = token <= pos && token < open_hi && in_window(token, pos);
                 // (the other digits' products are of zeros: none, or NaN with an Inf)
                 p[i] = seen ? (I8 ? digits_sum(digit ? 0.0f : s[i]) : s[i]) * by : -INFINITY;
                 const float big = size_of(i);
@@ -838,7 +852,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
 #pragma unroll 1
                 for (int token = t0; token < min(t0 + S, open_hi); token++) {
                     const float w = fmaxf(weight[(token - t0) * S + r], 0x1p-126f);
-                    const bool seen = token <= pos && (A.window == 0 || token > pos - A.window) && !digit;
+                    const bool seen = token <= pos && in_window(token, pos) && !digit;
                     const float *vp = v_open + (token & (P - 1)) * HD;
 #pragma unroll
                     for (int d = 0; d < ND; d++)
@@ -892,7 +906,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         int pk2 = -1, pv2 = -1;
         if constexpr (more) {
             pk2 = page_at(next + RT + krow), pv2 = page_at(next + RT + 16 * G);
-            load_k(next, pkn);
+            load_k(token_of(next), pkn);
             ksn = A.kv.k_scales[block_of(pvn)], vsn = A.kv.v_scales[block_of(pvn)];
         }
         const float kq = qscale * qsize * ks_ * qrest;
@@ -910,13 +924,14 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
         }
         // every column sees all of the step's tokens unless the step passes
         // the first column's position, the window's edge or an absent page
-        const bool plain = base + ST - 1 <= q.start + row_a && base + ST <= stop && base >= low &&
-                           (A.window == 0 || base > high - 1 - A.window) && __all(there);
+        const int at = token_of(base);
+        const bool plain = at + ST - 1 <= q.start + row_a && base + ST <= stop && (SINKS || base >= low) &&
+                           (A.window == 0 || at > high - 1 - A.window || (SINKS && at + ST <= A.sinks)) && __all(there);
         if (!plain) {
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                const int token = base + 16 * G + j;
-                const bool seen = there && token <= pos && token < stop && (A.window == 0 || token > pos - A.window);
+                const int token = at + 16 * G + j;
+                const bool seen = there && token <= pos && base + 16 * G + j < stop && in_window(token, pos);
                 p[j] = seen ? p[j] : -INFINITY;
             }
         }
@@ -991,7 +1006,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 3 : 2) void k_paged_attn(PagedAttnP
                 }
         }
         if constexpr (more) {
-            load_v(next, pvn);
+            load_v(token_of(next), pvn);
             pv = pvn, pkn = pk2, pvn = pv2;
             ks_ = ksn, vs_ = vsn;
         }
@@ -1215,11 +1230,17 @@ void append_of(hipStream_t st, const PagedAppendParams &p, unsigned blocks) {
     }
 }
 
-template <int HD>
+template <int HD, bool SINKS>
 void attn_of(hipStream_t st, const PagedAttnParams &p, AttnMode mode, unsigned blocks) {
-    if (mode == kAttnI8) hipLaunchKernelGGL((k_paged_attn<HD, kAttnI8>), dim3(blocks), dim3(256), 0, st, p);
-    else if (mode == kAttn16) hipLaunchKernelGGL((k_paged_attn<HD, kAttn16>), dim3(blocks), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_paged_attn<HD, kAttn32>), dim3(blocks), dim3(256), 0, st, p);
+    if (mode == kAttnI8) hipLaunchKernelGGL((k_paged_attn<HD, kAttnI8, SINKS>), dim3(blocks), dim3(256), 0, st, p);
+    else if (mode == kAttn16) hipLaunchKernelGGL((k_paged_attn<HD, kAttn16, SINKS>), dim3(blocks), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_paged_attn<HD, kAttn32, SINKS>), dim3(blocks), dim3(256), 0, st, p);
+}
+
+template <bool SINKS>
+void attn_dims(hipStream_t st, const PagedAttnParams &p, AttnMode mode, unsigned blocks) {
+    if (p.kv.head_dim == 64) attn_of<64, SINKS>(st, p, mode, blocks);
+    else attn_of<128, SINKS>(st, p, mode, blocks);
 }
 
 }  // namespace
@@ -1235,12 +1256,13 @@ void launch_paged_append(hipStream_t st, const PagedAppendParams &in) {
 
 void launch_paged_attention(hipStream_t st, const PagedAttnParams &in) {
     PagedAttnParams p = in;
-    const AttnShape shape = attn_shape(p.kv, p.s, p.heads);
+    const bool sinks = p.sinks > 0 && p.window > 0;
+    const AttnShape shape = attn_shape(p.kv, p.s, p.heads, sinks ? seen_span(p.window, p.sinks) : 0);
     p.tiles = shape.tiles;
     p.whole = shape.whole;
     p.nsplit = shape.nsplit;
-    if (p.kv.head_dim == 64) attn_of<64>(st, p, shape.mode, (unsigned)shape.blocks);
-    else attn_of<128>(st, p, shape.mode, (unsigned)shape.blocks);
+    if (sinks) attn_dims<true>(st, p, shape.mode, (unsigned)shape.blocks);
+    else attn_dims<false>(st, p, shape.mode, (unsigned)shape.blocks);
 }
 
 void launch_paged_read(hipStream_t st, const PagedReadParams &p) {

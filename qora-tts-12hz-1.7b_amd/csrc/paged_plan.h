@@ -194,13 +194,20 @@ struct AttnShape {
     long long blocks;  // of the launch
 };
 
-inline AttnShape attn_shape(const qtts_paged_kv &kv, const qtts_paged_seqs &s, int heads) {
+// Tokens that a tile of 32 rows sees at most under a window and with sinks, whose
+// stretches begin at multiples of 64.
+inline long long seen_span(int window, int sinks) { return (long long)window + sinks + 64 + 64 + 32; }
+
+// `span`: tokens that a tile sees at most, where the plan is to go by it (0: by what
+// a sequence may reach).
+inline AttnShape attn_shape(const qtts_paged_kv &kv, const qtts_paged_seqs &s, int heads, long long span = 0) {
     const long long columns = (long long)s.max_rows * (heads / kv.kv_heads), kvs = (long long)s.batch * kv.kv_heads;
     const AttnMode mode = attn_mode(columns, kvs);
     const int each = mode == kAttnI8 ? 4 : mode == kAttn16 ? 16 : 32;
     const long long tiles = (columns + each - 1) / each, pairs = kvs * tiles;
     if (pairs > kPagedMaxBlocks) return {mode, 0, 0, 0, pairs};
-    const AttnPlan p = attn_plan(pairs, tokens_cap(kv, s), each);
+    const long long cap = tokens_cap(kv, s);
+    const AttnPlan p = attn_plan(pairs, span > 0 && span < cap ? span : cap, each);
     return {mode, (int)tiles, p.whole, p.nsplit, p.whole + (pairs - p.whole) * p.nsplit};
 }
 
@@ -223,6 +230,17 @@ inline Refusal check_attention(const qtts_paged_kv &kv, const qtts_paged_seqs &s
     QTTS_REFUSE(check_rows(out, ld_out, (long long)heads * kv.head_dim));
     if (q == out && ld_q != ld_out) return {QTTS_EINVAL, "paged attention: in place, out takes q's stride"};
     if (attn_shape(kv, s, heads).blocks > kPagedMaxBlocks)
+        return {QTTS_ERANGE, "paged attention: more blocks than a launch holds"};
+    return kAccepted;
+}
+
+inline Refusal check_attention_sinks(const qtts_paged_kv &kv, const qtts_paged_seqs &s, int32_t heads, const float *q,
+                                     int32_t ld_q, float scale, int32_t window, int32_t sinks, const float *out,
+                                     int32_t ld_out) {
+    if (sinks < 0) return {QTTS_EINVAL, "paged attention: sinks must not be negative"};
+    QTTS_REFUSE(check_attention(kv, s, heads, q, ld_q, scale, window, out, ld_out));
+    if (paged_empty(s) || sinks == 0 || window == 0) return kAccepted;
+    if (attn_shape(kv, s, heads, seen_span(window, sinks)).blocks > kPagedMaxBlocks)
         return {QTTS_ERANGE, "paged attention: more blocks than a launch holds"};
     return kAccepted;
 }
@@ -251,6 +269,17 @@ inline Refusal check_sample_rows(const float *logits, int64_t ld, int32_t rows, 
         !aligned_to(p.temperature, 4) || !aligned_to(p.top_k, 4) || !aligned_to(p.top_p, 4) || !aligned_to(p.min_p, 4))
         return {QTTS_EINVAL, "sample_rows: misaligned argument"};
     return kAccepted;
+}
+
+// The tokens between the first `sinks` and a window that begins at `low`, in whole
+// 64s: numbers from `edge` on are `hole` below their tokens.  No hole where the two
+// meet.
+struct SeenHole {
+    int hole, edge;
+};
+QTTS_HD SeenHole seen_hole(int low, int high, int sinks) {
+    const int edge = ((sinks < high ? sinks : high) + 63) & ~63, from = low & ~63;
+    return {from > edge ? from - edge : 0, edge};
 }
 
 // Tokens of one block where `nsplit` share `span` tokens.

@@ -27,7 +27,7 @@ struct PagedAttnParams {
     float *out;
     int heads, ld_q, ld_out;
     float scale;
-    int window;
+    int window, sinks;
     int cap;  // tokens a sequence may reach
     // the launch's own
     int tiles;           // column tiles of one sequence and kv head

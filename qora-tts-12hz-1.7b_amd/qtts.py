@@ -336,6 +336,8 @@ def load_library(path: str = LIB_PATH):
         "qtts_paged_append_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), C.POINTER(PagedRows)], i32),
         "qtts_paged_attention_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), i32, vp, i32, C.c_float, i32,
                                          vp, i32], i32),
+        "qtts_paged_attention_sinks_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), i32, vp, i32, C.c_float,
+                                               i32, i32, vp, i32], i32),
         "qtts_paged_read_device": ([vp, C.POINTER(PagedKv), C.POINTER(PagedSeqs), vp, vp, i32, vp, i32], i32),
         "qtts_paged_remap_device": ([vp, C.POINTER(PagedPool), vp, vp, i32, i32, vp], i32),
         "qtts_paged_reserve_device": ([vp, C.POINTER(PagedPool), vp, vp, vp], i32),
@@ -373,7 +375,8 @@ def exported_symbols() -> List[str]:
         "qtts_model_file_talker", "qtts_model_file_predictor", "qtts_model_file_text", "qtts_model_file_info",
         "qtts_model_file_decoder", "qtts_decoder_upload", "qtts_decoder_free", "qtts_decoder_num_samples",
         "qtts_decode_to_audio", "qtts_decode_to_audio_device", "qtts_prefill_talker", "qtts_generate_speech",
-        "qtts_paged_append_device", "qtts_paged_attention_device", "qtts_paged_read_device",
+        "qtts_paged_append_device", "qtts_paged_attention_device", "qtts_paged_attention_sinks_device",
+        "qtts_paged_read_device",
         "qtts_paged_remap_device", "qtts_paged_reserve_device", "qtts_paged_compact_device",
         "qtts_paged_copy_pages_device", "qtts_paged_copy_open_device", "qtts_sample_rows_device", "qtts_fp8_gemm_device", "qtts_fp8_quantize_device",
     ]
@@ -939,9 +942,9 @@ class Context:
         self.check(self.lib.qtts_paged_append_device(self.h, C.byref(kv), C.byref(seqs), C.byref(rows)))
 
     def paged_attention_device(self, kv: PagedKv, seqs: PagedSeqs, heads: int, q: int, ld_q: int, out: int,
-                               ld_out: int, scale: float, window: int = 0):
-        self.check(self.lib.qtts_paged_attention_device(self.h, C.byref(kv), C.byref(seqs), heads, q, ld_q, scale,
-                                                        window, out, ld_out))
+                               ld_out: int, scale: float, window: int = 0, sinks: int = 0):
+        self.check(self.lib.qtts_paged_attention_sinks_device(self.h, C.byref(kv), C.byref(seqs), heads, q, ld_q,
+                                                              scale, window, sinks, out, ld_out))
 
     def paged_read_device(self, kv: PagedKv, seqs: PagedSeqs, lens: int, k_out: int, ld_k_out: int, v_out: int,
                           ld_v_out: int):
