@@ -603,7 +603,8 @@ typedef struct qtts_fp8_weight {
  * row of x (the last ones fewer) go to e4m3 on the way, the nearest to x / s, ties
  * to even, with s the least power of two with which they stay within 448 (2^-110
  * at least).  Products of codes are exact, their sums f32.  A row with an Inf or
- * NaN is NaN, as is a column whose weight or scale has one.  rows 0..2^24.
+ * NaN is NaN, as is a column whose weight or scale has one (codes under a scale of 0
+ * count as 0).  rows 0..2^24.
  * Enqueued on the context stream, allocates nothing and can be captured (context
  * scratch, as above).  How the sum over k is divided goes by the sizes of a call,
  * so a row's last bits may depend on how many others there are. */

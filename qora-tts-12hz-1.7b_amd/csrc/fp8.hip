@@ -11,6 +11,7 @@
 // (measured term by term, with and without their scaling): 2.3e-5 of a result on
 // ordinary values, where f32 sums are at 1e-7.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.h"
 #include "fp8_plan.h"
@@ -76,22 +77,47 @@ __device__ __forceinline__ unsigned half_max(unsigned v) {
     return v;
 }
 
-// Rows of x as the products take them, [rows][kb * 128] with zeros behind k.  32
-// lanes a block of 128.
-__global__ __launch_bounds__(256) void k_fp8_rows(Fp8Params A) {
-    const int lane = threadIdx.x & 31;
-    const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), blocks = (long long)A.rows * A.kb;
-    if (at >= blocks) return;
-    const int row = (int)(at / A.kb), b = (int)(at % A.kb), col = b * kFp8Block + 4 * lane;
-    f32x4 x = {0, 0, 0, 0};
-    if (col < A.w.k) x = load4(A.x + (size_t)row * A.ld_x + col);
+// Where a row's 16-byte pieces lie in LDS, of four: at place_of(piece) exclusive-or a
+// quarter of the row's number.  A read of 16 bytes a lane takes lanes 0-3, 12-15 and
+// 20-27 together, then 4-11, 16-19 and 28-31: their pieces, of two kinds, are then in
+// different banks (with the piece's own number they meet in pairs, and a read takes
+// twice as long).
+__device__ __forceinline__ int place_of(int piece) { return (piece & 1 ? 3 : 0) ^ (piece >> 1); }
+
+// 128 values of a row as the products take them, in 8 bits and back: four a lane of 32.
+__device__ __forceinline__ u32x2 block_values(f32x4 x) {
     const int e = scale_exponent(half_max(top4(x, 0)));
     const int c = codes4(x, e);
     const float s = e == 255 ? 1.0f : power_of(e);
-    int lo = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, false));
-    int hi = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, true));
-    if (e == 255) lo = hi = 0x7fc07fc0;
-    reinterpret_cast<int2 *>(A.xc)[(size_t)at * 32 + lane] = make_int2(lo, hi);
+    const unsigned lo = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, false));
+    const unsigned hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, true));
+    return e == 255 ? u32x2{0x7fc07fc0u, 0x7fc07fc0u} : u32x2{lo, hi};
+}
+
+// Rows lie in pieces of 1 KB, 16 of them and half of 64 of the contraction (of every 16
+// the first 8, or the others), as they are to lie in LDS.
+// All rows to scratch, [row / 16][k / 64][half], zeros behind k.  32 lanes a block of 128,
+// kRowsAhead blocks one after another whose loads are in flight together.
+constexpr int kRowsAhead = 4;
+__global__ __launch_bounds__(256) void k_fp8_rows(Fp8Params A) {
+    const int lane = threadIdx.x & 31;
+    const long long at = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kRowsAhead, blocks = (long long)A.rows * A.kb;
+    f32x4 x[kRowsAhead];
+#pragma unroll
+    for (int i = 0; i < kRowsAhead; i++) {
+        const long long b = min(at + i, blocks - 1);
+        const int col = (int)(b % A.kb) * kFp8Block + 4 * lane;
+        x[i] = load4(A.x + (size_t)(b / A.kb) * A.ld_x + (col < A.w.k ? col : 0));
+        if (col >= A.w.k) x[i] = f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsAhead; i++) {
+        if (at + i >= blocks) return;
+        const int row = (int)((at + i) / A.kb), b = (int)((at + i) % A.kb);
+        uint8_t *to = A.xc + ((size_t)(row >> 4) * A.kb + b) * 4096 + (lane >> 4) * 2048 + (lane & 2) * 512;
+        const int place = place_of(lane >> 2 & 3) ^ (row >> 2 & 3);
+        *glb(reinterpret_cast<u32x2 *>(to + (row & 15) * 64 + place * 16 + (lane & 1) * 8)) = block_values(x[i]);
+    }
 }
 
 // A weight in 8 bits, a block of 128 x 128 each: the same scales.
@@ -121,28 +147,39 @@ __global__ __launch_bounds__(256) void k_fp8_weight(const float *src, int ld_src
 }
 
 // A weight's scale in two factors: a power of two that its codes take as they
-// become bfloat16, within 2^-110 and 2^110, and the rest, for the block's sum.  A
-// sum then is of the result's size: a large x beside a small scale does not leave f32.
+// become bfloat16, within 2^-117 and 2^117, and the rest (1 to 2, but at the ends of
+// f32).  A sum then is of the result's size: a large x beside a small scale does not
+// leave f32.
 struct Scale {
     float power, rest;
+    bool none, bad;  // 0; Inf or NaN
     __device__ __forceinline__ explicit Scale(float s) {
-        const int e = (int)(__float_as_uint(s) >> 23 & 255), c = e == 255 ? 127 : min(max(e, 17), 237);
-        power = power_of(c);
-        rest = s * power_of(254 - c);
+        const int e = (int)(__float_as_uint(s) >> 23 & 255), c = min(max(e, 10), 244);
+        none = s == 0.0f, bad = e == 255;
+        power = none || bad ? 1.0f : power_of(c);
+        rest = none || bad ? 1.0f : s * power_of(254 - c);
     }
 };
 
 // 16 weight rows by 16 rows of x, 32 of the contraction.  Lane (r = lane % 16, G =
 // lane / 16) holds 8 values of row r of either operand and the result's rows 4 G..
-// of column r.  Which 8 of a block's 128 is free; step q = 2 h + u takes 64 h + 16 G
-// + 8 u and on, so that a lane reads codes 16 bytes at a time.
+// of column r.  Which 8 is free: of 64, half u takes 16 G + 8 u and on, so that a lane
+// reads codes 16 bytes at a time.
 __device__ __forceinline__ f32x4 mma(bf16x8 w, bf16x8 x, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ void fma4(f32x4 &acc, float s, f32x4 p) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = fmaf(s, p[i], acc[i]);
+template <int N, class F>
+__device__ __forceinline__ void each(F &&f) {
+    if constexpr (N > 0) {
+        each<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+
+// Four columns of a row of a split's sums.
+__device__ __forceinline__ float *part_of(const Fp8Params &A, int split, int row, int n) {
+    return A.part + ((size_t)split * A.rows + row) * ((A.w.n + 3) & ~3) + n;
 }
 
 // Four columns of a row of y.
@@ -157,215 +194,296 @@ __device__ __forceinline__ void put(const Fp8Params &A, int row, int n, f32x4 v)
     }
 }
 
-// BN weight rows by BM rows of x a block, WN by WM waves; both operands' blocks
-// of 128 come to LDS directly, the next ones while these are used.
+// 16 bytes a lane from memory to LDS, 1 KB in a row from `to` on.  Written out, as the
+// compiler has every read of LDS wait for all such loads before it; whoever uses
+// what they bring waits for them himself.
+__device__ __forceinline__ void to_lds(const uint8_t *base, unsigned offset, unsigned to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to));
+}
+__device__ __forceinline__ unsigned lds_address(void *p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)p;
+}
+
+// BN weight rows by BM rows of x a block, WN by WM waves.  A step is 64 of the
+// contraction in two halves of x; both operands come to LDS directly, two steps
+// ahead: x by halves in rings of three, codes by blocks of 128 in a ring of two, in
+// whole lines of 128 bytes (16 rows of 64 bytes a load reach half the rate from L2: 71
+// GB/s a CU with all of them loading, 132).  The one barrier of a step lies between
+// its halves: behind it the second half, the next step's codes and its first half are
+// read and multiplied in one stretch, so that neither the reads nor the codes'
+// conversion wait for a barrier of their own.
+//
+// Sums are held in units of the current block's `rest`, one multiplication for each
+// 128: a second set of sums for the block would take the registers of the tile.
+//
+// 256 x 256, 8192 rows, 2048 to 12288: 350 us, 1.18 PFLOP/s, where 8192 cubed in
+// bfloat16 is 1.24 in the library.  Of a step's 2950 cycles the products take 2048 (two
+// waves a SIMD); the multiplications, the conversions and the loads' addresses, some
+// 300 each, overlap with them in part, and at 1.9 to 2.1 GHz the card's power bounds
+// both.  Measured on the way: all loads right behind the barrier 3400 cycles, two
+// barriers' worth of reads in one place 4000; a pattern of products and other
+// instructions imposed on the compiler's order 3150 to 4200.
 template <int BN, int BM, int WN, int WM>
 __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
     constexpr int W = WN * WM, NF = BN / WN / 16, MF = BM / WM / 16;
     static_assert(BN / WN <= kFp8Block && kFp8Block % (BN / WN) == 0, "one scale a wave");
-    constexpr int LA = BN / 8 / W, LB = BM / 4 / W;  // loads of 1 KB a wave
-    __shared__ __align__(16) uint8_t sa[2][BN * 128], sb[2][BM * 256];
+    constexpr int LA = BN / 8 / W, LB = BM / 16 / W;  // loads of 1 KB a wave, of codes and of half of x
+    constexpr int kCodes = BN * 128, kHalf = BM * 64;
+    __shared__ __align__(16) uint8_t ring[2 * kCodes + 6 * kHalf];  // codes [2], x [3][2]
+    const unsigned ring_at = lds_address(ring);
     const int lane = threadIdx.x & 63, r = lane & 15, G = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
     int id = blockIdx.x;
     const int split = id % A.splits;
     id /= A.splits;
     const int n0 = id % A.tiles_n * BN, m0 = id / A.tiles_n * BM;
-    const int first = split * A.each, last = min(first + A.each, A.kb);
-    // A load brings 8 rows of codes or 4 of x.  A row's 16-byte pieces lie in LDS at
-    // their number exclusive-or the row's (half of it for codes, whose rows are half
-    // as long), so that 16 rows' same piece is in different banks.
-    const uint8_t *wa[LA], *xb[LB];
-    int pa[LA];
+    const int first = 2 * split * A.each, last = min(first + 2 * A.each, (A.w.k + 63) / 64);
+    // A load of codes brings 8 rows of 128 bytes; their eight pieces lie in LDS at
+    // their number exclusive-or half of the row's.
+    const uint8_t *codes = A.w.codes + (size_t)n0 * A.w.ld, *xs = A.xc + (size_t)(m0 / 16 + wave * LB) * A.kb * 4096;
+    unsigned row_at[LA];
+    int piece[LA];
 #pragma unroll
     for (int i = 0; i < LA; i++) {
         const int row = (wave * LA + i) * 8 + (lane >> 3);
-        wa[i] = A.w.codes + (size_t)min(n0 + row, A.w.n - 1) * A.w.ld;
-        pa[i] = 16 * ((lane & 7) ^ (row >> 1 & 7));
+        row_at[i] = (unsigned)min(row, A.w.n - 1 - n0) * (unsigned)A.w.ld;
+        piece[i] = 16 * ((lane & 7) ^ (row >> 1 & 7));
     }
-#pragma unroll
-    for (int i = 0; i < LB; i++) {
-        const int row = (wave * LB + i) * 4 + (lane >> 4);
-        xb[i] = A.xc + (size_t)(m0 + row) * A.kb * 256 + 16 * ((lane & 15) ^ (row & 15));
-    }
-    typedef __attribute__((address_space(1))) void gvoid;
-    typedef __attribute__((address_space(3))) void lvoid;
-    auto load = [&](int to, int b) {
-#pragma unroll
-        for (int i = 0; i < LA; i++) {
-            // behind k a row's first piece: x has zeros there
-            const int at = b * 128 + pa[i];
-            __builtin_amdgcn_global_load_lds((gvoid *)(wa[i] + (at < A.w.k ? at : b * 128)),
-                                             (lvoid *)(sa[to] + (wave * LA + i) * 1024), 16, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < LB; i++)
-            __builtin_amdgcn_global_load_lds((gvoid *)(xb[i] + (size_t)b * 256),
-                                             (lvoid *)(sb[to] + (wave * LB + i) * 1024), 16, 0, 0);
+    auto load_half = [&](int slot, int s, int u, int i) {
+        to_lds(xs + ((size_t)i * A.kb * 4096 + (size_t)s * 2048 + u * 1024), lane * 16,
+               ring_at + 2 * kCodes + (2 * slot + u) * kHalf + (wave * LB + i) * 1024);
     };
-    const float *ws = A.w.scales + (size_t)(min(n0 + wn * NF * 16, A.w.n - 1) / kFp8Block) * A.kb;
+    auto load_codes = [&](int s, int i) {  // of the block that begins with step s
+        // behind k a row's first codes: x has zeros there
+        const unsigned at = piece[i] < A.w.k - s * 64 ? piece[i] : 0;
+        to_lds(codes + (size_t)s * 64, row_at[i] + at, ring_at + (s >> 1 & 1) * kCodes + (wave * LA + i) * 1024);
+    };
+    // where this lane reads: its row of a fragment, its piece
+    const int my_code = r * 128 + 16 * (G ^ (r >> 1)), my_x = r * 64 + 16 * (place_of(G) ^ (r >> 2));
+    auto codes_at = [&](int s, int i) {
+        return *reinterpret_cast<const i32x4 *>(ring + (s >> 1 & 1) * kCodes + (wn * NF + i) * 2048 +
+                                                (my_code ^ (s & 1) * 64));
+    };
+    auto half_at = [&](int slot, int u, int j) {
+        return *reinterpret_cast<const bf16x8 *>(ring + 2 * kCodes + (2 * slot + u) * kHalf + (wm * MF + j) * 1024 + my_x);
+    };
+    // (scalar loads: they do not wait behind the others)
+    const KCONST float *ws =
+        (const KCONST float *)(A.w.scales + (size_t)(min(n0 + wn * NF * 16, A.w.n - 1) / kFp8Block) * A.kb);
     f32x4 acc[NF][MF] = {};
-    load(first & 1, first);
-    __syncthreads();
-    for (int b = first; b < last; b++) {
-        const Scale s(ws[b]);
-        if (b + 1 < last) load((b + 1) & 1, b + 1);
-        bf16x8 w[NF][4];
+    float next = ws[first >> 1], power = 1.0f, rest = 1.0f;
+    bool none = false, bad = false;
+    i32x4 c[NF];    // this step's codes
+    bf16x8 w[NF];   // the half at hand
+    auto half = [&](int slot, int u, float by, bool scaled, auto &&between) {
+        each<MF>([&](auto j) {
+            const bf16x8 x = half_at(slot, u, j);
 #pragma unroll
-        for (int i = 0; i < NF; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int row = (wn * NF + i) * 16 + r;
-                const i32x4 c = *reinterpret_cast<const i32x4 *>(sa[b & 1] + row * 128 + 16 * ((4 * h + G) ^ (row >> 1 & 7)));
-                w[i][2 * h] = values8(c[0], c[1], s.power);
-                w[i][2 * h + 1] = values8(c[2], c[3], s.power);
+            for (int i = 0; i < NF; i++) {
+                if (scaled) acc[i][j] *= by;  // just before its products, behind others'
+                acc[i][j] = mma(w[i], x, acc[i][j]);
             }
-#pragma unroll
-        for (int j = 0; j < MF; j++) {
-            const uint8_t *row = sb[b & 1] + ((wm * MF + j) * 16 + r) * 256;
-            f32x4 p[NF] = {};
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const bf16x8 x = *reinterpret_cast<const bf16x8 *>(row + 16 * ((8 * (q >> 1) + 2 * G + (q & 1)) ^ r));
-#pragma unroll
-                for (int i = 0; i < NF; i++) p[i] = mma(w[i][q], x, p[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < NF; i++) fma4(acc[i][j], s.rest, p[i]);
-        }
-        __syncthreads();
-    }
-    if (A.splits > 1) {
-        // parts: [tile][split][fragment][lane], joined in order by the last
-        float *part = A.part + (size_t)id * A.splits * BN * BM;
-        float *mine = part + (size_t)split * BN * BM + wave * NF * MF * 256 + lane * 4;
-#pragma unroll
+            between(j);
+        });
+    };
+    auto nothing = [](int) {};
+    float by = 1.0f;
+    auto new_block = [&](int s) {  // its scale
+        const Scale z(next);
+        next = ws[min((s >> 1) + 1, A.kb - 1)];
+        power = z.power, none = z.none, bad |= z.bad;
+        by = rest * __builtin_amdgcn_rcpf(z.rest), rest = z.rest;
+    };
+    // codes under a scale of 0 are zeros; every wave that reads these writes them
+    auto clear_codes = [&](int s) {
         for (int i = 0; i < NF; i++)
+            *reinterpret_cast<i32x4 *>(ring + (s >> 1 & 1) * kCodes + (wn * NF + i) * 2048 + (my_code ^ (s & 1) * 64)) =
+                i32x4{0, 0, 0, 0};
+    };
+    // a step's codes, its first half and the conversion for the second
+    auto begin = [&](int slot, int s, auto block) {
 #pragma unroll
-            for (int j = 0; j < MF; j++)
-#pragma unroll
-                for (int h = 0; h < 4; h += 2)
-                    st_dev_u64(reinterpret_cast<uint64_t *>(mine + (i * MF + j) * 256 + h),
-                               __float_as_uint(acc[i][j][h]) | (uint64_t)__float_as_uint(acc[i][j][h + 1]) << 32);
-        __shared__ unsigned arrived;
-        wait_stores();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            arrived = arrive_dev(A.counters + id);
-            if (arrived == (unsigned)A.splits - 1) reset_dev(A.counters + id);
+        for (int i = 0; i < NF; i++) {
+            c[i] = codes_at(s, i);
+            w[i] = values8(c[i][0], c[i][1], power);
         }
-        __syncthreads();
-        if (arrived != (unsigned)A.splits - 1) return;
+        half(slot, 0, by, block, nothing);
 #pragma unroll
-        for (int i = 0; i < NF; i++)
-#pragma unroll
-            for (int j = 0; j < MF; j++) acc[i][j] = f32x4{0, 0, 0, 0};
-        for (int k = 0; k < A.splits; k++) {
-            const float *from = part + (size_t)k * BN * BM + wave * NF * MF * 256 + lane * 4;
-#pragma unroll
-            for (int i = 0; i < NF; i++)
-#pragma unroll
-                for (int j = 0; j < MF; j++)
-#pragma unroll
-                    for (int h = 0; h < 4; h += 2) {
-                        const uint64_t v = ld_dev_u64(reinterpret_cast<const uint64_t *>(from + (i * MF + j) * 256 + h));
-                        acc[i][j][h] += __uint_as_float((unsigned)v);
-                        acc[i][j][h + 1] += __uint_as_float((unsigned)(v >> 32));
-                    }
+        for (int i = 0; i < NF; i++) w[i] = values8(c[i][2], c[i][3], power);
+    };
+    // From the middle of step s to that of the next one.  At the barrier what is read
+    // behind it is here (what the last step asked for may be on its way), and what the
+    // loads behind it go over has been read.  They are spread among the products, as
+    // both waves of a SIMD come from the barrier together.  far: there are three more
+    // steps, and the loads are on no branch.
+    auto through = [&](int slot, int s, auto odd, auto far) {
+        constexpr int kAway = 2 * LB + (odd ? 0 : LA), kNew = 2 * LB + (odd ? LA : 0), kEach = (kNew + MF - 1) / MF;
+        const int next_slot = slot == 2 ? 0 : slot + 1;
+        if (odd) new_block(s + 1);
+        if (far || s + 2 < last) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kAway) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        auto load = [&](auto l) {  // the new loads in their order
+            if constexpr (l < LB) load_half(slot == 0 ? 2 : slot - 1, s + 2, 1, l);
+            else if constexpr (odd && l < LB + LA) load_codes(s + 3, l - LB);
+            else if constexpr (l < kNew) load_half(slot, s + 3, 0, l - (kNew - LB));
+        };
+        if (!far) {
+            if (s + 2 < last) each<LB>(load);
+            if (s + 3 < last)
+                each<kNew>([&](auto l) {
+                    if constexpr (l >= LB) load(l);
+                });
         }
+        if (none) clear_codes(s + 1);
+        half(slot, 1, 1.0f, false, [&](auto j) {
+            if constexpr (far)
+                each<kEach>([&](auto e) { load(std::integral_constant<int, j * kEach + e>{}); });
+        });
+        begin(next_slot, s + 1, odd);
+        return next_slot;
+    };
+    const auto yes = std::true_type{};
+    const auto no = std::false_type{};
+    each<LA>([&](auto i) { load_codes(first, i); });
+    each<LB>([&](auto i) { load_half(0, first, 0, i), load_half(0, first, 1, i); });
+    if (first + 1 < last) each<LB>([&](auto i) { load_half(1, first + 1, 0, i), load_half(1, first + 1, 1, i); });
+    if (first + 2 < last) {
+        each<LA>([&](auto i) { load_codes(first + 2, i); });
+        each<LB>([&](auto i) { load_half(2, first + 2, 0, i); });
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    new_block(first);
+    if (none) clear_codes(first);
+    int slot = 0, s = first;
+    begin(slot, first, yes);
+    for (; s + 4 < last; s += 2) {
+        slot = through(slot, s, no, yes);
+        slot = through(slot, s + 1, yes, yes);
+    }
+    for (; s + 2 < last; s += 2) {
+        slot = through(slot, s, no, no);
+        slot = through(slot, s + 1, yes, no);
+    }
+    if (s + 1 < last) slot = through(slot, s, no, no);
+    half(slot, 1, 1.0f, false, nothing);
+    if (bad) rest = __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) acc[i][j] *= rest;
 #pragma unroll
     for (int j = 0; j < MF; j++) {
         const int row = m0 + (wm * MF + j) * 16 + r;
 #pragma unroll
         for (int i = 0; i < NF; i++) {
             const int n = n0 + (wn * NF + i) * 16 + 4 * G;
-            if (row < A.rows && n < A.w.n) put(A, row, n, acc[i][j]);
+            if (row >= A.rows || n >= A.w.n) continue;
+            if (A.splits > 1) *glb(reinterpret_cast<f32x4 *>(part_of(A, split, row, n))) = acc[i][j];
+            else put(A, row, n, acc[i][j]);
         }
     }
 }
 
-// Up to 16 rows: 32 weight rows a block, whose blocks of 128 its four waves take
-// in turn, straight from memory to registers.  The lane that feeds x to the matrix
-// instruction brings it to 8 bits itself.
-__global__ __launch_bounds__(256, 2) void k_fp8_few(Fp8Params A) {
-    constexpr int NF = 2;
-    __shared__ f32x4 so[4][NF][64];
+// The splits' sums, in their order.  Four columns a thread.
+__global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
+    const int fours = (A.w.n + 3) / 4;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (long long)A.rows * fours) return;
+    const int row = (int)(at / fours), n = (int)(at % fours) * 4;
+    f32x4 v = {0, 0, 0, 0};
+    for (int k0 = 0; k0 < A.splits; k0 += 8) {
+        f32x4 p[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) p[k] = load4(part_of(A, min(k0 + k, A.splits - 1), row, n));
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k0 + k < A.splits) v += p[k];
+    }
+    put(A, row, n, v);
+}
+
+// A few rows (kFewRows): 16 weight rows a block, whose blocks of 128 its W waves take in
+// turn, straight from memory to registers, four asked for at once; meanwhile the block
+// brings x to 8 bits, into LDS.  Bound by reading the weight and by one chain of
+// latencies: one row, 2048 to 12288, 25 MB in 7.7 us (3.3 TB/s); 6144 to 2048 8.5 us.
+// (With the contraction divided over blocks and joined through memory 12 us, most of it
+// the joining.)
+template <int W>
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A) {
+    extern __shared__ __align__(16) uint8_t lds[];  // sums of the waves, then x, [row][128s][half of 64][piece]
+    f32x4 *so = reinterpret_cast<f32x4 *>(lds);
+    uint8_t *xs = lds + W * 1024;
     const int lane = threadIdx.x & 63, r = lane & 15, G = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int split = blockIdx.x % A.splits, id = blockIdx.x / A.splits, n0 = id * 16 * NF;
-    const int first = split * A.each, last = min(first + A.each, A.kb);
-    const uint8_t *wr[NF];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
+    const uint8_t *wr = A.w.codes + (size_t)min(n0 + r, A.w.n - 1) * A.w.ld;
+    const KCONST float *ws = (const KCONST float *)(A.w.scales + (size_t)(n0 / kFp8Block) * A.kb);
+    i32x4 w[4][2];
+    float scale[4];
+    auto ask = [&](int b0) {
 #pragma unroll
-    for (int i = 0; i < NF; i++) wr[i] = A.w.codes + (size_t)min(n0 + 16 * i + r, A.w.n - 1) * A.w.ld;
-    const float *xr = A.x + (size_t)min(r, A.rows - 1) * A.ld_x;
-    const float *ws = A.w.scales + (size_t)(n0 / kFp8Block) * A.kb;
-    f32x4 acc[NF] = {};
-    for (int b = first + wave; b < last; b += 4) {
-        i32x4 w[NF][2];
-        f32x4 x[8];
+        for (int a = 0; a < 4; a++) {
+            const int b = min(b0 + W * a, A.kb - 1);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int at = b * 128 + 64 * h + 16 * G, to = at < A.w.k ? at : b * 128;
-#pragma unroll
-            for (int i = 0; i < NF; i++) w[i][h] = *glb(reinterpret_cast<const i32x4 *>(wr[i] + to));
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[4 * h + j] = load4(xr + to + 4 * j);
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[4 * h + j] = at < A.w.k ? x[4 * h + j] : f32x4{0, 0, 0, 0};
-        }
-        unsigned top = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) top = top4(x[j], top);
-        for (int off = 16; off < 64; off <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, off, 64));
-        const int e = scale_exponent(top);
-        const float sx = e == 255 ? __uint_as_float(0x7fc00000u) : 1.0f;  // a row that is not finite
-        const Scale s(ws[b]);
-        f32x4 p[NF] = {};
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const bf16x8 v = values8(codes4(x[2 * q], e), codes4(x[2 * q + 1], e), e == 255 ? 1.0f : power_of(e));
-#pragma unroll
-            for (int i = 0; i < NF; i++)
-                p[i] = mma(values8(w[i][q >> 1][2 * (q & 1)], w[i][q >> 1][2 * (q & 1) + 1], s.power), v, p[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NF; i++) fma4(acc[i], s.rest * sx, p[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NF; i++) so[wave][i][lane] = acc[i];
-    __syncthreads();
-    if (wave >= NF) return;
-    f32x4 v = so[0][wave][lane];
-#pragma unroll
-    for (int k = 1; k < 4; k++) v += so[k][wave][lane];
-    const int n = n0 + 16 * wave + 4 * G;
-    if (A.splits > 1) {
-        // each wave joins its own 16 columns
-        float *part = A.part + ((size_t)id * NF + wave) * A.splits * 256;
-        float *mine = part + split * 256 + lane * 4;
-        for (int h = 0; h < 4; h += 2)
-            st_dev_u64(reinterpret_cast<uint64_t *>(mine + h),
-                       __float_as_uint(v[h]) | (uint64_t)__float_as_uint(v[h + 1]) << 32);
-        wait_stores();
-        unsigned arrived = 0;
-        unsigned *counter = A.counters + id * NF + wave;
-        if (lane == 0) {
-            arrived = arrive_dev(counter);
-            if (arrived == (unsigned)A.splits - 1) reset_dev(counter);
-        }
-        arrived = __builtin_amdgcn_readfirstlane(arrived);
-        if (arrived != (unsigned)A.splits - 1) return;
-        v = f32x4{0, 0, 0, 0};
-        for (int k = 0; k < A.splits; k++)
-#pragma unroll
-            for (int h = 0; h < 4; h += 2) {
-                const uint64_t z = ld_dev_u64(reinterpret_cast<const uint64_t *>(part + k * 256 + lane * 4 + h));
-                v[h] += __uint_as_float((unsigned)z);
-                v[h + 1] += __uint_as_float((unsigned)(z >> 32));
+            for (int h = 0; h < 2; h++) {
+                const int at = b * 128 + 64 * h + 16 * G;  // behind k any codes: x has zeros there
+                w[a][h] = __builtin_nontemporal_load(glb(reinterpret_cast<const i32x4 *>(wr + (at < A.w.k ? at : 0))));
             }
+            scale[a] = ws[b];
+        }
+    };
+    ask(wave);
+    const int items = A.rows * A.kb;  // 32 lanes a row's block of 128
+    for (int i0 = threadIdx.x >> 5; i0 < items; i0 += 8 * W) {
+        f32x4 x[4];
+        const int l = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int it = min(i0 + 2 * W * i, items - 1), col = it % A.kb * kFp8Block + 4 * l;
+            x[i] = load4(A.x + (size_t)(it / A.kb) * A.ld_x + (col < A.w.k ? col : 0));
+            if (col >= A.w.k) x[i] = f32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int it = i0 + 2 * W * i;
+            const u32x2 v = block_values(x[i]);
+            if (it < items)
+                *reinterpret_cast<u32x2 *>(xs + it * 256 + (l >> 4) * 128 + (l & 2) * 32 + (l >> 2 & 3) * 16 + (l & 1) * 8) = v;
+        }
     }
-    if (r < A.rows && n < A.w.n) put(A, r, n, v);
+    __syncthreads();
+    const uint8_t *xr = xs + min(r, A.rows - 1) * A.kb * 256 + 16 * G;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int b0 = wave; b0 < A.kb; b0 += 4 * W) {
+        if (b0 != wave) ask(b0);
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            const int b = b0 + W * a;
+            if (b >= A.kb) break;
+            const Scale s(scale[a]);
+            const int mask = s.none ? 0 : -1;  // codes under a scale of 0 are zeros
+            f32x4 p = {0, 0, 0, 0};
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const i32x4 c = w[a][q >> 1];
+                p = mma(values8(c[2 * (q & 1)] & mask, c[2 * (q & 1) + 1] & mask, s.power),
+                        *reinterpret_cast<const bf16x8 *>(xr + b * 256 + q * 64), p);
+            }
+            const float by = s.bad ? __uint_as_float(0x7fc00000u) : s.rest;
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(by, p[i], acc[i]);
+        }
+    }
+    so[threadIdx.x] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int k = 1; k < W; k++) acc += so[k * 64 + lane];
+    const int n = n0 + 4 * G;
+    if (r < A.rows && n < A.w.n) put(A, r, n, acc);
 }
 
 }  // namespace
@@ -382,15 +500,25 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
         const Fp8Plan plan = fp8_plan(p.rows, p.w.n, p.w.k);
         p.tiles_n = plan.tiles_n;
         p.splits = plan.splits;
-        p.each = (p.kb + plan.splits - 1) / plan.splits;
+        p.each = plan.each;
         const unsigned blocks = (unsigned)plan.tiles_n * plan.tiles_m * plan.splits;
         if (plan.bm <= 16) {
-            hipLaunchKernelGGL(k_fp8_few, dim3(blocks), dim3(256), 0, st, p);
+            const size_t lds = (size_t)plan.waves * 1024 + (size_t)p.rows * p.kb * 256;
+            if (plan.waves == 4) hipLaunchKernelGGL(k_fp8_few<4>, dim3(blocks), dim3(256), lds, st, p);
+            else if (plan.waves == 8) hipLaunchKernelGGL(k_fp8_few<8>, dim3(blocks), dim3(512), lds, st, p);
+            else hipLaunchKernelGGL(k_fp8_few<16>, dim3(blocks), dim3(1024), lds, st, p);
             continue;
         }
-        const long long rows_blocks = ((long long)p.rows * p.kb + 7) / 8;
+        const long long each = 8 * kRowsAhead, rows_blocks = ((long long)p.rows * p.kb + each - 1) / each;
         hipLaunchKernelGGL(k_fp8_rows, dim3((unsigned)rows_blocks), dim3(256), 0, st, p);
-        hipLaunchKernelGGL((k_fp8_tile<256, 128, 4, 2>), dim3(blocks), dim3(512), 0, st, p);
+        if (plan.bm == 256) hipLaunchKernelGGL((k_fp8_tile<256, 256, 4, 2>), dim3(blocks), dim3(512), 0, st, p);
+        else if (plan.bn == 256) hipLaunchKernelGGL((k_fp8_tile<256, 128, 4, 2>), dim3(blocks), dim3(512), 0, st, p);
+        else if (plan.bm == 128) hipLaunchKernelGGL((k_fp8_tile<128, 128, 2, 2>), dim3(blocks), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((k_fp8_tile<64, 64, 2, 2>), dim3(blocks), dim3(256), 0, st, p);
+        if (plan.splits > 1) {
+            const long long fours = (long long)p.rows * ((p.w.n + 3) / 4);
+            hipLaunchKernelGGL(k_fp8_join, dim3((unsigned)((fours + 255) / 256)), dim3(256), 0, st, p);
+        }
     }
 }
 

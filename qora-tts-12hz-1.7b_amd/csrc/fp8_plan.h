@@ -13,11 +13,12 @@ namespace qtts {
 constexpr int kFp8Block = 128;                    // side of a weight's block, length of a row's
 constexpr int kFp8MaxSide = 1 << 17;              // of n and k
 constexpr long long kFp8MaxRows = 1LL << 24;
-constexpr size_t kFp8ScratchBytes = (size_t)64 << 20;  // a context's: rows, in bfloat16
+constexpr size_t kFp8ScratchBytes = (size_t)128 << 20;  // a context's: rows, in bfloat16
 constexpr int kFp8RowStep = 256;                  // rows that a tile takes at most
-constexpr long long kFp8PartFloats = 4LL << 20;   // split sums
-constexpr int kFp8MaxSplits = 64;
-constexpr int kFp8Counters = 8192;                // a tile's, zero between launches
+constexpr int kFp8MaxSplits = 16;                 // parts of a sum
+constexpr long long kFp8PartFloats = 4LL << 20;   // all parts' sums
+constexpr int kFewRows = 4;                       // that a kernel of their own takes,
+constexpr int kFewItems = 256;                    // with so many blocks of 128: 64 KB of LDS
 
 inline int fp8_blocks(int k) { return (k + kFp8Block - 1) / kFp8Block; }
 
@@ -59,32 +60,60 @@ inline Refusal check_fp8_quantize(const float *src, int32_t ld_src, const qtts_f
     return check_rows(src, ld_src, w.k);
 }
 
-// A product's tiles: BN columns of the output (rows of the weight) by BM rows,
-// blocks of 128 of the contraction divided over `splits` blocks of a tile.
+// A product's tiles: bn columns of the output (rows of the weight) by bm rows; the
+// blocks of 128 of the contraction are divided over `splits` blocks of a tile, `each`
+// of them each.
 struct Fp8Plan {
-    int bn, bm;     // bm <= 16: the kernel for few rows
-    int tiles_n, tiles_m, splits;
+    int bn, bm;  // bm == 16: the kernel for a few rows
+    int tiles_n, tiles_m, splits, each;
+    long long ns;  // what it is taken to cost
+    int waves;     // of a block, for a few rows
 };
 
+// A tile's step of 64, in ns: with a CU to itself and where blocks fill it, as measured
+// (4096 deep, 64 to 4096 blocks).
+struct Fp8Tile {
+    int bn, bm, alone, full;
+};
+constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1620, 1900}, {256, 128, 1000, 1080}, {128, 128, 600, 540}, {64, 64, 330, 200}};
+
+inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
+    const int kb = fp8_blocks(k);
+    Fp8Plan p{bn, bm, (n + bn - 1) / bn, (rows + bm - 1) / bm, 1, 0, 0, 0};
+    p.each = (kb + splits - 1) / splits;
+    p.splits = (kb + p.each - 1) / p.each;
+    p.each = (kb + p.splits - 1) / p.splits;
+    return p;
+}
+
+// The tile and number of splits that are taken to cost least.  A block's start costs
+// some 2 us, a CU works off ceil(blocks / CUs) of them, and joining costs a launch and
+// the parts' way to memory and back.  What it chooses is within 10 % of the best of
+// all of them but for a few sizes: 1064 x 2048 -> 4096, 64 x 64 30 us (chosen), 128 x
+// 128 31, 256 x 256 52; 8192 rows of it 90 (4096 rows), 134 and 124 (chosen); 128 x 6144
+// -> 2048 in 64 x 64, 14 us in four parts, 37 in one; 512 x 1552 -> 1001 10 us in one,
+// 12 in four.
 inline Fp8Plan fp8_plan(int rows, int n, int k) {
     const int kb = fp8_blocks(k);
-    Fp8Plan p;
-    p.bn = rows <= 16 ? 32 : 256;
-    p.bm = rows <= 16 ? 16 : 128;
-    p.tiles_n = (n + p.bn - 1) / p.bn;
-    p.tiles_m = (rows + p.bm - 1) / p.bm;
-    p.splits = 1;
-    const long long tiles = (long long)p.tiles_n * p.tiles_m;
-    const int least = rows <= 16 ? 4 : 2;  // blocks of a split at least
-    long long want = 512 / tiles;
-    if (want > kb / least) want = kb / least;
-    if (want > kFp8MaxSplits) want = kFp8MaxSplits;
-    while (want > 1 && (tiles > kFp8Counters || tiles * want * p.bn * p.bm > kFp8PartFloats)) want--;
-    if (want > 1) {
-        const int each = (int)((kb + want - 1) / want);
-        p.splits = (kb + each - 1) / each;
+    if (rows <= kFewRows && rows * kb <= kFewItems) {
+        // waves enough to fill the card with a few tiles, but a block of 128 for each
+        Fp8Plan p = fp8_divided(rows, n, k, 16, 16, 1);
+        p.waves = p.tiles_n >= 512 || kb <= 4 ? 4 : p.tiles_n >= 256 || kb <= 8 ? 8 : 16;
+        return p;
     }
-    return p;
+    Fp8Plan best{};
+    for (const Fp8Tile &t : kFp8Tiles)
+        for (int splits = 1; splits <= kFp8MaxSplits && splits <= kb; splits++) {
+            Fp8Plan p = fp8_divided(rows, n, k, t.bn, t.bm, splits);
+            if (p.splits != splits) continue;
+            const long long out = (long long)rows * ((n + 3) & ~3);
+            if (splits > 1 && splits * out > kFp8PartFloats) break;
+            const long long blocks = (long long)p.tiles_n * p.tiles_m * splits, full = (blocks + 255) / 256 * t.full;
+            p.ns = 2000 + 2LL * p.each * (full > t.alone ? full : t.alone);
+            if (splits > 1) p.ns += 2500 + splits * out * 8 / 4000;
+            if (best.bn == 0 || p.ns < best.ns) best = p;
+        }
+    return best;
 }
 
 }  // namespace qtts

@@ -95,7 +95,6 @@ struct Fp8Params {
     int ld_x, ld_add, ld_y, rows;
     uint8_t *xc;          // kFp8ScratchBytes: rows as the products take them
     float *part;          // kFp8PartFloats: split sums
-    unsigned *counters;   // kFp8Counters, zero between launches
     // the launch's own
     int kb;               // blocks of the contraction
     int tiles_n, splits, each;  // Fp8Plan; blocks of a split

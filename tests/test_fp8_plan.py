@@ -25,8 +25,8 @@ extern "C" int quantize(const float *src, int ld, const qtts_fp8_weight *w) { re
 extern "C" void plan(int rows, int n, int k, long long *o) {
     const Fp8Plan p = fp8_plan(rows, n, k);
     o[0] = p.bn; o[1] = p.bm; o[2] = p.tiles_n; o[3] = p.tiles_m; o[4] = p.splits;
-    o[5] = fp8_rows_at_once(k); o[6] = kFp8PartFloats; o[7] = kFp8Counters; o[8] = kFp8RowStep;
-    o[9] = (long long)kFp8ScratchBytes; o[10] = fp8_blocks(k);
+    o[5] = fp8_rows_at_once(k); o[6] = kFp8PartFloats; o[7] = kFp8MaxSplits; o[8] = kFp8RowStep;
+    o[9] = (long long)kFp8ScratchBytes; o[10] = fp8_blocks(k); o[11] = p.waves; o[12] = p.each;
 }
 """
 
@@ -90,22 +90,24 @@ def test_sources(lib):
 
 
 def test_plans(lib):
-    """Tiles cover the output, splits the contraction, none of them empty; parts,
-    counters and the rows' scratch hold what a launch uses."""
-    o = (C.c_longlong * 11)()
+    """Tiles cover the output, splits the contraction, none of them empty; parts
+    and the rows' scratch hold what a launch uses."""
+    o = (C.c_longlong * 13)()
     for rows in [*range(1, 300, 7), 512, 1064, 4096, 8192, 100000]:
         for n in (1, 31, 128, 1000, 2048, 12288, 131072):
             for k in (16, 128, 144, 2048, 6144, 131072):
                 lib.plan(rows, n, k, o)
-                bn, bm, tn, tm, splits, at_once, part, counters, step, scratch, kb = list(o)
+                bn, bm, tn, tm, splits, at_once, part, most, step, scratch, kb, waves, per = list(o)
                 assert (tn - 1) * bn < n <= tn * bn and (tm - 1) * bm < rows <= tm * bm
                 assert step % bm == 0 and at_once % step == 0 and at_once >= step
                 assert at_once * kb * 256 <= scratch
-                assert 1 <= splits <= min(kb, 64)
-                each = -(-kb // splits)
-                assert (splits - 1) * each < kb <= splits * each
+                assert 1 <= splits <= min(kb, most) and most <= 64
+                assert (splits - 1) * per < kb <= splits * per
                 if splits > 1:
-                    assert tn * tm * splits * bn * bm <= part and tn * tm * (2 if bm == 16 else 1) <= counters
+                    assert min(rows, at_once) * -(-n // 4) * 4 * splits <= part
+                if bm == 16:  # the kernel for a few rows: its LDS
+                    assert splits == 1 and rows <= 16 and waves in (4, 8, 16)
+                    assert waves * 1024 + rows * kb * 256 <= 160 * 1024
 
 
 def test_oracle_rounds_to_the_nearest():
