@@ -71,10 +71,19 @@ __device__ __forceinline__ unsigned top4(f32x4 x, unsigned m) {
     return m;
 }
 
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_bits(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+
 // Largest over 32 lanes, of magnitudes as bits (as integers: a NaN is the largest).
 __device__ __forceinline__ unsigned half_max(unsigned v) {
-    for (int off = 16; off > 0; off >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, off, 32));
-    return v;
+    v = max(v, dpp_bits<kDppXor1>(v));
+    v = max(v, dpp_bits<kDppXor2>(v));
+    v = max(v, dpp_bits<kDppHalfMirror>(v));
+    v = max(v, dpp_bits<kDppMirror>(v));
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max((unsigned)r[0], (unsigned)r[1]);
 }
 
 // Where a row's 16-byte pieces lie in LDS, of four: at place_of(piece) exclusive-or a

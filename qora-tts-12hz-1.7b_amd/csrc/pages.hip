@@ -17,15 +17,21 @@ namespace {
 
 constexpr int kThreads = kRemapThreads, kWaves = kThreads / 64;
 
+// Sum over the lanes up to this one: rows of 16 by shifts, then their last lanes' sums.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+
 // Exclusive sum over the block's threads, and the total; `sums`: kWaves ints.
 __device__ __forceinline__ int block_rank(int v, int *sums, int &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int y = __shfl_up(x, off, 64);
-        if (lane >= off) x += y;
-    }
+    const int x = wave_scan(v);
     __syncthreads();  // the last call's sums have been read
     if (lane == 63) sums[wave] = x;
     __syncthreads();
@@ -88,33 +94,48 @@ __device__ void hand_on_slots(const RemapParams &A, Slots &S) {
     }
 }
 
-// What entry i becomes; references change where it does.
-__device__ __forceinline__ int remapped(const RemapParams &A, int i) {
-    const int b = i / A.pool.max_pages, j = i % A.pool.max_pages;
-    const Heir h = heir_of(A.pool, A.source, A.tokens, b);
-    const int old = A.pool.page_table[i];
-    int now = -1;
-    if (h.source >= 0 && page_kept(j, h.tokens, h.source == b, A.pool.page_size, A.window, A.sinks))
-        now = h.source == b ? old : A.pool.page_table[(size_t)h.source * A.pool.max_pages + j];
-    if (!in_pool(A.pool, now)) now = -1;
-    if (old != now) {
-        if (in_pool(A.pool, old)) atomicSub(A.pool.refs + old, 1);
-        if (now >= 0) atomicAdd(A.pool.refs + now, 1);
+// What N entries from `first` on, kThreads apart, become; references change where they
+// do; the table has entries.  Loads of one kind are asked for together, one kind after another: what an entry
+// was, its row's heir, the heir's entry.
+template <int N>
+__device__ __forceinline__ void remapped(const RemapParams &A, int first, int (&now)[N]) {
+    const int n = A.pool.batch * A.pool.max_pages, wide = A.pool.max_pages;
+    int old[N], from[N];
+    Heir h[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int i = min(first + k * kThreads, n - 1);
+        old[k] = A.pool.page_table[i];
+        h[k] = heir_of(A.pool, A.source, A.tokens, i / wide);
     }
-    return now;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int i = min(first + k * kThreads, n - 1), b = i / wide, j = i % wide;
+        const bool kept = h[k].source >= 0 &&
+                          page_kept(j, h[k].tokens, h[k].source == b, A.pool.page_size, A.window, A.sinks);
+        from[k] = kept ? h[k].source * wide + j : -1;
+        now[k] = A.pool.page_table[max(from[k], 0)];
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        if (from[k] < 0 || !in_pool(A.pool, now[k])) now[k] = -1;
+        if (first + k * kThreads < n && old[k] != now[k]) {
+            if (in_pool(A.pool, old[k])) atomicSub(A.pool.refs + old[k], 1);
+            if (now[k] >= 0) atomicAdd(A.pool.refs + now[k], 1);
+        }
+    }
 }
 
-// Tables of up to kRemapThreads * kRemapEach entries: all read, then written.
+// Tables of up to kRemapThreads * kRemapEach entries: block 0 reads them all, then
+// writes; block 1 hands on the slots.  8 rows of 18: 4 us.  64 of 127 13 us, most of it
+// one CU's atomics: 4.1 + 2.3 us in many blocks and two launches.
 __global__ __launch_bounds__(kThreads) void k_paged_remap_one(RemapParams A) {
     __shared__ Slots S;
+    if (blockIdx.x == 1) return hand_on_slots(A, S);
     const int n = A.pool.batch * A.pool.max_pages;
+    if (n == 0) return;
     int now[kRemapEach];
-#pragma unroll
-    for (int k = 0; k < kRemapEach; k++) {
-        const int i = k * kThreads + threadIdx.x;
-        now[k] = i < n ? remapped(A, i) : -1;
-    }
-    hand_on_slots(A, S);
+    remapped(A, threadIdx.x, now);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kRemapEach; k++) {
@@ -128,7 +149,9 @@ __global__ __launch_bounds__(kThreads) void k_paged_remap(RemapParams A) {
     __shared__ Slots S;
     if (blockIdx.x == 0) return hand_on_slots(A, S);
     const int i = (blockIdx.x - 1) * kThreads + threadIdx.x;
-    if (i < A.pool.batch * A.pool.max_pages) A.scratch[i] = remapped(A, i);
+    int now[1];
+    remapped(A, i, now);
+    if (i < A.pool.batch * A.pool.max_pages) A.scratch[i] = now[0];
 }
 
 __global__ __launch_bounds__(256) void k_paged_remap_store(RemapParams A) {
@@ -153,19 +176,34 @@ __device__ __forceinline__ void load_refs(const qtts_paged_pool &p, int at, int 
 }
 
 // Pages for each row's span, in order of rows and entries, the lowest free ones
-// first; from the first row that cannot be served whole on, none.
+// first; from the first row that cannot be served whole on, none.  16 lanes a row, as
+// most rows want a page or two; the pages found lie in LDS as far as they fit.  64
+// rows, some of them new with up to 31 pages, of 14046: 8 us, a chain of latencies
+// (spans, references, ranks, entries).
+constexpr int kFoundLds = 8192;
 __global__ __launch_bounds__(kThreads) void k_paged_reserve(ReserveParams A) {
     __shared__ int need[kPoolBatch];
+    __shared__ int found_ids[kFoundLds];
     __shared__ int sums[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, batch = A.pool.batch;
+    constexpr int kRows = kThreads / 16;
+    const int tid = threadIdx.x, lane = tid & 15, at64 = tid & 48, batch = A.pool.batch;
     int refs[16];
     load_refs(A.pool, 0, refs);
-    for (int b = wave; b < batch; b += kWaves) {
+    // whether this lane's entry, j0 + lane of a span, wants a page, and the row's lanes' answers
+    auto wants = [&](const int32_t *row, const Span &s, int j0, unsigned &all) {
+        const bool want = j0 + lane < s.last && !in_pool(A.pool, row[min(j0 + lane, s.last - 1)]);
+        all = (unsigned)(__ballot(want) >> at64) & 0xffffu;
+        return want;
+    };
+    for (int b = tid >> 4; b < batch; b += kRows) {
         const Span s = reserve_span(A.pool, A.starts[b], A.ends[b]);
         const int32_t *row = A.pool.page_table + (size_t)b * A.pool.max_pages;
         int n = 0;
-        for (int j0 = s.first; j0 < s.last; j0 += 64)
-            n += __popcll(__ballot(j0 + lane < s.last && !in_pool(A.pool, row[min(j0 + lane, s.last - 1)])));
+        for (int j0 = s.first; j0 < s.last; j0 += 16) {
+            unsigned all;
+            wants(row, s, j0, all);
+            n += __popc(all);
+        }
         if (lane == 0) need[b] = n;
     }
     __syncthreads();
@@ -187,14 +225,16 @@ __global__ __launch_bounds__(kThreads) void k_paged_reserve(ReserveParams A) {
 #pragma unroll
         for (int k = 0; k < 16; k++)
             if (refs[k] <= 0) {
-                if (rank < total) A.scratch[rank] = at + 16 * tid + k;
+                const int id = at + 16 * tid + k;
+                if (rank < kFoundLds) found_ids[rank] = id;
+                else if (rank < total) A.scratch[rank] = id;
                 rank++;
             }
         found += n;
     }
     found = min(found, total);
     __syncthreads();
-    for (int b = wave; b < batch; b += kWaves) {
+    for (int b = tid >> 4; b < batch; b += kRows) {
         const Span s = reserve_span(A.pool, A.starts[b], A.ends[b]);
         const int base = need[b], end = b + 1 < batch ? need[b + 1] : total;
         const bool served = end <= found;
@@ -202,24 +242,28 @@ __global__ __launch_bounds__(kThreads) void k_paged_reserve(ReserveParams A) {
         if (!served || base == end) continue;
         int32_t *row = A.pool.page_table + (size_t)b * A.pool.max_pages;
         int rank = base;
-        for (int j0 = s.first; j0 < s.last; j0 += 64) {
-            const bool want = j0 + lane < s.last && !in_pool(A.pool, row[min(j0 + lane, s.last - 1)]);
-            const uint64_t all = __ballot(want);
-            if (want) {
-                const int id = A.scratch[rank + __popcll(all & ((1ull << lane) - 1))];
+        for (int j0 = s.first; j0 < s.last; j0 += 16) {
+            unsigned all;
+            if (wants(row, s, j0, all)) {
+                const int r = rank + __popc(all & ((1u << lane) - 1));
+                const int id = r < kFoundLds ? found_ids[r] : A.scratch[r];
                 row[j0 + lane] = id;
                 A.pool.refs[id] = 1;
             }
-            rank += __popcll(all);
+            rank += __popc(all);
         }
     }
 }
 
 // Which pages move where so that those in use are the pool's first: the i-th in use
 // behind that border to the i-th free one before it.  Their new names go to scratch,
-// the border to its end.  One block.
+// the border to its end.  One block; the moves of a pool of one chunk stay in LDS (12532
+// pages, 2300 moves: 10.5 us, 12.5 by way of the lists).
+template <bool ONE>
 __global__ __launch_bounds__(kThreads) void k_paged_compact(CompactParams A) {
     __shared__ int sums[kWaves];
+    constexpr int kMoves = ONE ? kPoolChunk / 2 : 1;
+    __shared__ int from[kMoves], held[kMoves], to[kMoves];  // held: the page's references
     const int tid = threadIdx.x, n = A.pool.num_pages;
     int refs[16], live = 0;
     for (int at = 0; at < n; at += kPoolChunk) {
@@ -232,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void k_paged_compact(CompactParams A) {
     }
     int moves = 0, holes = 0;
     for (int at = 0; at < n; at += kPoolChunk) {
-        if (n > kPoolChunk) load_refs(A.pool, at, refs);
+        if (!ONE) load_refs(A.pool, at, refs);
         const int first = at + 16 * tid;
         int movers = 0, free = 0, m, h;
 #pragma unroll
@@ -241,29 +285,34 @@ __global__ __launch_bounds__(kThreads) void k_paged_compact(CompactParams A) {
             movers += id < n && id >= live && refs[k] > 0;
             free += id < live && refs[k] <= 0;
         }
-        int rank_m = moves + block_rank(movers, sums, m), rank_h = holes + block_rank(free, sums, h);
+        // (a chunk's counts of both in one scan)
+        const int both = block_rank(movers << 16 | free, sums, m);
+        int rank_m = moves + (both >> 16), rank_h = holes + (both & 0xffff);
+        h = m & 0xffff, m >>= 16;
 #pragma unroll
         for (int k = 0; k < 16; k++) {
             const int id = first + k;
             if (id < n && id >= live) {
-                if (refs[k] > 0) A.from[rank_m++] = id;
-                else A.scratch[id] = id;
+                if (refs[k] <= 0) A.scratch[id] = id;
+                else if (ONE) from[rank_m] = id, held[rank_m++] = refs[k];
+                else A.from[rank_m++] = id;
             } else if (id < live && refs[k] <= 0) {
-                A.to[rank_h++] = id;
+                if (ONE) to[rank_h++] = id;
+                else A.to[rank_h++] = id;
             }
         }
         moves += m, holes += h;
     }
     __syncthreads();
     for (int i = tid; i < n / 2; i += kThreads) {
+        int a = -1, b = -1;
         if (i < moves) {
-            const int a = A.from[i], b = A.to[i];
+            a = ONE ? from[i] : A.from[i], b = ONE ? to[i] : A.to[i];
             A.scratch[a] = b;
-            A.pool.refs[b] = A.pool.refs[a];
+            A.pool.refs[b] = ONE ? held[i] : A.pool.refs[a];
             A.pool.refs[a] = 0;
-        } else {
-            A.from[i] = A.to[i] = -1;
         }
+        if (ONE || i >= moves) A.from[i] = a, A.to[i] = b;
     }
     if (tid == 0) {
         A.scratch[n] = live;
@@ -294,7 +343,8 @@ __device__ __forceinline__ void copy_bytes(void *to, const void *from, int bytes
     }
 }
 
-// A block for K or V of each pair of pages.
+// A block for K or V of each pair of pages.  Bound by memory: 2270 of 131 KB each way,
+// 0.6 GB in 100 us (5.9 TB/s), blocks of pairs that are not there among them.
 __global__ __launch_bounds__(256) void k_paged_copy_pages(CopyPagesParams A) {
     const int pair = blockIdx.x >> 1, from = A.from[pair], to = A.to[pair], heads = A.a.kv_heads;
     if (from < 0 || from >= A.a.num_pages || to < 0 || to >= A.b.num_pages) return;
@@ -325,7 +375,7 @@ __global__ __launch_bounds__(256) void k_paged_copy_open(CopyOpenParams A) {
 void launch_paged_remap(hipStream_t st, const RemapParams &p) {
     const long long n = (long long)p.pool.batch * p.pool.max_pages;
     if (n <= kRemapThreads * kRemapEach) {
-        hipLaunchKernelGGL(k_paged_remap_one, dim3(1), dim3(kThreads), 0, st, p);
+        hipLaunchKernelGGL(k_paged_remap_one, dim3(2), dim3(kThreads), 0, st, p);
         return;
     }
     hipLaunchKernelGGL(k_paged_remap, dim3(1 + (unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, p);
@@ -337,7 +387,8 @@ void launch_paged_reserve(hipStream_t st, const ReserveParams &p) {
 }
 
 void launch_paged_compact(hipStream_t st, const CompactParams &p) {
-    hipLaunchKernelGGL(k_paged_compact, dim3(1), dim3(kThreads), 0, st, p);
+    if (p.pool.num_pages <= kPoolChunk) hipLaunchKernelGGL(k_paged_compact<true>, dim3(1), dim3(kThreads), 0, st, p);
+    else hipLaunchKernelGGL(k_paged_compact<false>, dim3(1), dim3(kThreads), 0, st, p);
     const long long n = (long long)p.pool.batch * p.pool.max_pages;
     if (n) hipLaunchKernelGGL(k_paged_rename, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);
 }

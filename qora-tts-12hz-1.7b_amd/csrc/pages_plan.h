@@ -14,10 +14,10 @@ namespace qtts {
 constexpr int kPoolBatch = 8192;                    // rows whose slots one block hands on through LDS
 constexpr long long kPoolEntries = 4LL << 20;       // of a page table: its copy lies in scratch
 constexpr int kPoolPages = (4 << 20) - 64;          // names of pages, and their number, in scratch
-// Entries that one block remaps in its registers; more go through scratch, in two
-// launches.
-constexpr int kRemapThreads = 1024, kRemapEach = 8;
-constexpr int kPoolChunk = 16384;                   // pages that a block looks at in one go
+// Entries that one block remaps in its registers, in 3.5 us; more go through scratch in
+// two launches, which take 6.5 (one block 9 to 13 for 8128).
+constexpr int kRemapThreads = 1024, kRemapEach = 2;
+constexpr int kPoolChunk = 16384;                   // pages that a block looks at in one go (counted in 16 bits)
 
 inline Refusal check_pool(const qtts_paged_pool &p) {
     if (p.page_size != 16 && p.page_size != 32 && p.page_size != 64 && p.page_size != 128)
