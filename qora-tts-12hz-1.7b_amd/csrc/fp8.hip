@@ -415,13 +415,14 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
     put(A, row, n, v);
 }
 
-// A few rows (kFewRows): 16 weight rows a block, whose blocks of 128 its W waves take in
-// turn, straight from memory to registers, four asked for at once; meanwhile the block
-// brings x to 8 bits, into LDS.  Bound by reading the weight and by one chain of
+// Up to 16 rows: 16 weight rows a block, whose blocks of 128 its W waves take in turn,
+// straight from memory to registers, four asked for at once.  OWN: of up to kFewRows
+// rows the block meanwhile brings x to 8 bits itself, into LDS; more come from scratch,
+// which k_fp8_rows has filled.  Bound by reading the weight and by one chain of
 // latencies: one row, 2048 to 12288, 25 MB in 7.7 us (3.3 TB/s); 6144 to 2048 8.5 us.
 // (With the contraction divided over blocks and joined through memory 12 us, most of it
 // the joining.)
-template <int W>
+template <int W, bool OWN>
 __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A) {
     extern __shared__ __align__(16) uint8_t lds[];  // sums of the waves, then x, [row][128s][half of 64][piece]
     f32x4 *so = reinterpret_cast<f32x4 *>(lds);
@@ -431,11 +432,17 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A)
     const uint8_t *wr = A.w.codes + (size_t)min(n0 + r, A.w.n - 1) * A.w.ld;
     const KCONST float *ws = (const KCONST float *)(A.w.scales + (size_t)(n0 / kFp8Block) * A.kb);
     i32x4 w[4][2];
+    bf16x8 xv[OWN ? 1 : 4][4];
     float scale[4];
+    const uint8_t *xr = OWN ? xs + min(r, A.rows - 1) * A.kb * 256 + 16 * G : A.xc + r * 64 + 16 * (place_of(G) ^ (r >> 2));
     auto ask = [&](int b0) {
 #pragma unroll
         for (int a = 0; a < 4; a++) {
             const int b = min(b0 + W * a, A.kb - 1);
+            if (!OWN)
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    xv[OWN ? 0 : a][q] = *glb(reinterpret_cast<const bf16x8 *>(xr + (size_t)b * 4096 + q * 1024));
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int at = b * 128 + 64 * h + 16 * G;  // behind k any codes: x has zeros there
@@ -445,7 +452,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A)
         }
     };
     ask(wave);
-    const int items = A.rows * A.kb;  // 32 lanes a row's block of 128
+    const int items = OWN ? A.rows * A.kb : 0;  // 32 lanes a row's block of 128
     for (int i0 = threadIdx.x >> 5; i0 < items; i0 += 8 * W) {
         f32x4 x[4];
         const int l = threadIdx.x & 31;
@@ -463,8 +470,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A)
                 *reinterpret_cast<u32x2 *>(xs + it * 256 + (l >> 4) * 128 + (l & 2) * 32 + (l >> 2 & 3) * 16 + (l & 1) * 8) = v;
         }
     }
-    __syncthreads();
-    const uint8_t *xr = xs + min(r, A.rows - 1) * A.kb * 256 + 16 * G;
+    if (OWN) __syncthreads();
     f32x4 acc = {0, 0, 0, 0};
     for (int b0 = wave; b0 < A.kb; b0 += 4 * W) {
         if (b0 != wave) ask(b0);
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A)
             for (int q = 0; q < 4; q++) {
                 const i32x4 c = w[a][q >> 1];
                 p = mma(values8(c[2 * (q & 1)] & mask, c[2 * (q & 1) + 1] & mask, s.power),
-                        *reinterpret_cast<const bf16x8 *>(xr + b * 256 + q * 64), p);
+                        OWN ? *reinterpret_cast<const bf16x8 *>(xr + b * 256 + q * 64) : xv[OWN ? 0 : a][q], p);
             }
             const float by = s.bad ? __uint_as_float(0x7fc00000u) : s.rest;
 #pragma unroll
@@ -493,6 +499,14 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A)
     for (int k = 1; k < W; k++) acc += so[k * 64 + lane];
     const int n = n0 + 4 * G;
     if (r < A.rows && n < A.w.n) put(A, r, n, acc);
+}
+
+template <bool OWN>
+void few_of(hipStream_t st, const Fp8Params &p, int waves, unsigned blocks, size_t x_bytes) {
+    const size_t lds = (size_t)waves * 1024 + x_bytes;
+    if (waves == 4) hipLaunchKernelGGL((k_fp8_few<4, OWN>), dim3(blocks), dim3(256), lds, st, p);
+    else if (waves == 8) hipLaunchKernelGGL((k_fp8_few<8, OWN>), dim3(blocks), dim3(512), lds, st, p);
+    else hipLaunchKernelGGL((k_fp8_few<16, OWN>), dim3(blocks), dim3(1024), lds, st, p);
 }
 
 }  // namespace
@@ -511,15 +525,16 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
         p.splits = plan.splits;
         p.each = plan.each;
         const unsigned blocks = (unsigned)plan.tiles_n * plan.tiles_m * plan.splits;
-        if (plan.bm <= 16) {
-            const size_t lds = (size_t)plan.waves * 1024 + (size_t)p.rows * p.kb * 256;
-            if (plan.waves == 4) hipLaunchKernelGGL(k_fp8_few<4>, dim3(blocks), dim3(256), lds, st, p);
-            else if (plan.waves == 8) hipLaunchKernelGGL(k_fp8_few<8>, dim3(blocks), dim3(512), lds, st, p);
-            else hipLaunchKernelGGL(k_fp8_few<16>, dim3(blocks), dim3(1024), lds, st, p);
+        const bool own = plan.bm == 16 && fp8_own_rows(p.rows, p.kb);
+        if (!own) {
+            const long long each = 8 * kRowsAhead, rows_blocks = ((long long)p.rows * p.kb + each - 1) / each;
+            hipLaunchKernelGGL(k_fp8_rows, dim3((unsigned)rows_blocks), dim3(256), 0, st, p);
+        }
+        if (plan.bm == 16) {
+            if (own) few_of<true>(st, p, plan.waves, blocks, (size_t)p.rows * p.kb * 256);
+            else few_of<false>(st, p, plan.waves, blocks, 0);
             continue;
         }
-        const long long each = 8 * kRowsAhead, rows_blocks = ((long long)p.rows * p.kb + each - 1) / each;
-        hipLaunchKernelGGL(k_fp8_rows, dim3((unsigned)rows_blocks), dim3(256), 0, st, p);
         if (plan.bm == 256) hipLaunchKernelGGL((k_fp8_tile<256, 256, 4, 2>), dim3(blocks), dim3(512), 0, st, p);
         else if (plan.bn == 256) hipLaunchKernelGGL((k_fp8_tile<256, 128, 4, 2>), dim3(blocks), dim3(512), 0, st, p);
         else if (plan.bm == 128) hipLaunchKernelGGL((k_fp8_tile<128, 128, 2, 2>), dim3(blocks), dim3(256), 0, st, p);

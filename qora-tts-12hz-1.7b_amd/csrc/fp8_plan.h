@@ -17,7 +17,7 @@ constexpr size_t kFp8ScratchBytes = (size_t)128 << 20;  // a context's: rows, in
 constexpr int kFp8RowStep = 256;                  // rows that a tile takes at most
 constexpr int kFp8MaxSplits = 16;                 // parts of a sum
 constexpr long long kFp8PartFloats = 4LL << 20;   // all parts' sums
-constexpr int kFewRows = 4;                       // that a kernel of their own takes,
+constexpr int kFewRows = 4;                       // that each block brings to 8 bits itself,
 constexpr int kFewItems = 256;                    // with so many blocks of 128: 64 KB of LDS
 
 inline int fp8_blocks(int k) { return (k + kFp8Block - 1) / kFp8Block; }
@@ -64,7 +64,7 @@ inline Refusal check_fp8_quantize(const float *src, int32_t ld_src, const qtts_f
 // blocks of 128 of the contraction are divided over `splits` blocks of a tile, `each`
 // of them each.
 struct Fp8Plan {
-    int bn, bm;  // bm == 16: the kernel for a few rows
+    int bn, bm;  // bm == 16: the kernel for up to 16 rows
     int tiles_n, tiles_m, splits, each;
     long long ns;  // what it is taken to cost
     int waves;     // of a block, for a few rows
@@ -77,6 +77,9 @@ struct Fp8Tile {
 };
 constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1620, 1900}, {256, 128, 1000, 1080}, {128, 128, 600, 540}, {64, 64, 330, 200}};
 
+// Whether the kernel for up to 16 rows brings them to 8 bits itself, in each block anew.
+inline bool fp8_own_rows(int rows, int kb) { return rows <= kFewRows && rows * kb <= kFewItems; }
+
 inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
     const int kb = fp8_blocks(k);
     Fp8Plan p{bn, bm, (n + bn - 1) / bn, (rows + bm - 1) / bm, 1, 0, 0, 0};
@@ -87,15 +90,15 @@ inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
 }
 
 // The tile and number of splits that are taken to cost least.  A block's start costs
-// some 2 us, a CU works off ceil(blocks / CUs) of them, and joining costs a launch and
-// the parts' way to memory and back.  What it chooses is within 10 % of the best of
+// some 2 us, a CU works off ceil(blocks / CUs) of them, and joining costs a launch, the
+// host's share of it too, and the parts' way to memory and back.  What it chooses is within 10 % of the best of
 // all of them but for a few sizes: 1064 x 2048 -> 4096, 64 x 64 30 us (chosen), 128 x
 // 128 31, 256 x 256 52; 8192 rows of it 90 (4096 rows), 134 and 124 (chosen); 128 x 6144
 // -> 2048 in 64 x 64, 14 us in four parts, 37 in one; 512 x 1552 -> 1001 10 us in one,
 // 12 in four.
 inline Fp8Plan fp8_plan(int rows, int n, int k) {
     const int kb = fp8_blocks(k);
-    if (rows <= kFewRows && rows * kb <= kFewItems) {
+    if (rows <= 16) {
         // waves enough to fill the card with a few tiles, but a block of 128 for each
         Fp8Plan p = fp8_divided(rows, n, k, 16, 16, 1);
         p.waves = p.tiles_n >= 512 || kb <= 4 ? 4 : p.tiles_n >= 256 || kb <= 8 ? 8 : 16;
@@ -110,7 +113,7 @@ inline Fp8Plan fp8_plan(int rows, int n, int k) {
             if (splits > 1 && splits * out > kFp8PartFloats) break;
             const long long blocks = (long long)p.tiles_n * p.tiles_m * splits, full = (blocks + 255) / 256 * t.full;
             p.ns = 2000 + 2LL * p.each * (full > t.alone ? full : t.alone);
-            if (splits > 1) p.ns += 2500 + splits * out * 8 / 4000;
+            if (splits > 1) p.ns += 4500 + splits * out * 8 / 4000;
             if (best.bn == 0 || p.ns < best.ns) best = p;
         }
     return best;
