@@ -594,7 +594,7 @@ typedef struct qtts_fp8_weight {
     const float *scales;   /* [(n + 127) / 128][(k + 127) / 128] */
     int32_t n;             /* 1..131072 */
     int32_t k;             /* 16..131072, a multiple of 16 */
-    int32_t ld;
+    int32_t ld;            /* to 2^23 */
 } qtts_fp8_weight;
 
 /* y = x W^T (+ add): x rows of k floats, y and add (NULL: none; may be y itself

@@ -12,6 +12,7 @@ namespace qtts {
 
 constexpr int kFp8Block = 128;                    // side of a weight's block, length of a row's
 constexpr int kFp8MaxSide = 1 << 17;              // of n and k
+constexpr int kFp8MaxStride = 1 << 23;            // a tile's rows are reached by 32-bit offsets
 constexpr long long kFp8MaxRows = 1LL << 24;
 constexpr size_t kFp8ScratchBytes = (size_t)128 << 20;  // a context's: rows, in bfloat16
 constexpr int kFp8RowStep = 256;                  // rows that a tile takes at most
@@ -33,6 +34,7 @@ inline Refusal check_fp8_weight(const qtts_fp8_weight &w) {
     if (w.n < 1 || w.k < 16 || w.k % 16 != 0 || w.n > kFp8MaxSide || w.k > kFp8MaxSide)
         return {QTTS_ESHAPE, "fp8 weight: n and k must be 1..131072, k a multiple of 16"};
     if (w.ld < w.k) return {QTTS_ESHAPE, "fp8 weight: a row stride below the row"};
+    if (w.ld > kFp8MaxStride) return {QTTS_ERANGE, "fp8 weight: a row stride above 2^23"};
     if (w.ld % 16 != 0) return {QTTS_EINVAL, "fp8 weight: the row stride must be a multiple of 16"};
     if (!w.codes || !w.scales) return {QTTS_EINVAL, "fp8 weight: null buffer"};
     if (!aligned_to(w.codes, 16) || !aligned_to(w.scales, 4))
@@ -112,6 +114,7 @@ inline Fp8Plan fp8_plan(int rows, int n, int k) {
             const long long out = (long long)rows * ((n + 3) & ~3);
             if (splits > 1 && splits * out > kFp8PartFloats) break;
             const long long blocks = (long long)p.tiles_n * p.tiles_m * splits, full = (blocks + 255) / 256 * t.full;
+            if (blocks > (1 << 22)) continue;  // a launch counts its threads in 32 bits
             p.ns = 2000 + 2LL * p.each * (full > t.alone ? full : t.alone);
             if (splits > 1) p.ns += 4500 + splits * out * 8 / 4000;
             if (best.bn == 0 || p.ns < best.ns) best = p;

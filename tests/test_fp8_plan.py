@@ -31,7 +31,7 @@ extern "C" void plan(int rows, int n, int k, long long *o) {
 }
 """
 
-OK, EINVAL, ESHAPE = qtts.QTTS_OK, qtts.QTTS_EINVAL, qtts.QTTS_ESHAPE
+OK, EINVAL, ESHAPE, ERANGE = qtts.QTTS_OK, qtts.QTTS_EINVAL, qtts.QTTS_ESHAPE, qtts.QTTS_ERANGE
 AT = 1 << 20  # an address that is never read
 
 
@@ -57,7 +57,7 @@ def _weight(**over):
 @pytest.mark.parametrize("weight,status", [
     (dict(), OK), (dict(n=1), OK), (dict(n=1 << 17), OK), (dict(n=0), ESHAPE), (dict(n=(1 << 17) + 1), ESHAPE),
     (dict(k=16), OK), (dict(k=0), ESHAPE), (dict(k=264), ESHAPE), (dict(k=288), ESHAPE), (dict(ld=256), ESHAPE),
-    (dict(ld=280), EINVAL), (dict(ld=288), OK), (dict(codes=0), EINVAL), (dict(scales=0), EINVAL),
+    (dict(ld=280), EINVAL), (dict(ld=288), OK), (dict(ld=1 << 23), OK), (dict(ld=(1 << 23) + 16), ERANGE), (dict(codes=0), EINVAL), (dict(scales=0), EINVAL),
     (dict(codes=AT + 8), EINVAL), (dict(scales=AT + 2), EINVAL), (dict(n=-5), ESHAPE),
 ])
 def test_weights(lib, weight, status):
@@ -94,18 +94,21 @@ def test_plans(lib):
     """Tiles cover the output, splits the contraction, none of them empty; parts
     and the rows' scratch hold what a launch uses."""
     o = (C.c_longlong * 13)()
-    for rows in [*range(1, 300, 7), 512, 1064, 4096, 8192, 100000]:
+    for rows in [*range(1, 300, 7), 512, 1064, 4096, 8192, 100000, 1 << 24]:
         for n in (1, 31, 128, 1000, 2048, 12288, 131072):
             for k in (16, 128, 144, 2048, 6144, 131072):
-                lib.plan(rows, n, k, o)
+                lib.plan(1, n, k, o)
+                rows_now = min(rows, o[5])  # what a launch takes
+                lib.plan(rows_now, n, k, o)
                 bn, bm, tn, tm, splits, at_once, part, most, step, scratch, kb, waves, per = list(o)
-                assert (tn - 1) * bn < n <= tn * bn and (tm - 1) * bm < rows <= tm * bm
+                assert (tn - 1) * bn < n <= tn * bn and (tm - 1) * bm < rows_now <= tm * bm
+                assert tn * tm * splits * 512 < 1 << 32
                 assert step % bm == 0 and at_once % step == 0 and at_once >= step
                 assert at_once * kb * 256 <= scratch
                 assert 1 <= splits <= min(kb, most) and most <= 64
                 assert (splits - 1) * per < kb <= splits * per
                 if splits > 1:
-                    assert min(rows, at_once) * -(-n // 4) * 4 * splits <= part
+                    assert rows_now * -(-n // 4) * 4 * splits <= part
                 if bm == 16:  # the kernel for up to 16 rows: its LDS
                     assert splits == 1 and rows <= 16 and waves in (4, 8, 16)
                     assert waves * 1024 + (rows * kb * 256 if lib.own(rows, kb) else 0) <= 160 * 1024

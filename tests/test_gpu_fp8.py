@@ -187,6 +187,97 @@ def test_not_finite(ctx, rows, bad):
     assert np.array_equal(dc.cpu().numpy(), codes)
 
 
+@pytest.mark.parametrize("rows", [2, 10, 40, 300])
+def test_scales_of_any_size(ctx, rows):
+    """Scales of 0 (whose codes count as 0, NaN among them), negative ones, the least
+    and the largest, in any order along k and beside each other along n; x so that
+    the results stay f32's."""
+    n, k = 400, 1168
+    codes = _weight(40, n, k).host[0].copy()
+    scales = np.array([[0.01, 0.0, -0.02, 0.0, 0.03, -0.5, 1e-3, 0.0, 0.0, 0.7],
+                       [0.0] * 10,
+                       [1e-40, 3e38, 1e-30, 2.0 ** -149, 1e20, 0.0, 1.0, -3e38, 1e-38, 2e30],
+                       [2.0 ** -126, 2.0 ** -118, 2.0 ** -117, 2.0 ** 117, 2.0 ** 118, 2.0 ** 127, 1.5, 1.0, 0.75, 3.0]],
+                      np.float32)
+    x = _rows(41, rows, k)
+    for b in range(10):  # the third and fourth row's products of one size
+        x[:, b * 128:(b + 1) * 128] *= np.float32(0.2)
+    codes[5, 130], codes[150, 7], codes[395, 300] = 0x7f, 0xff, 0x11
+    x2 = x.copy()
+    w = Weight(codes, scales)
+    got = _gemm(ctx, w, x2)
+    assert np.array_equal(got[:, 128:256], np.zeros((rows, 128), np.float32))
+    clean = codes.copy()
+    clean[5, 130] = clean[150, 7] = 0
+    ref, mass = fm.product(x2, clean, scales)
+    fine = np.r_[0:256]
+    off, bound = np.abs(got - ref), (128 + 10 + 66) * 2.0 ** -24 * mass + 2.0 ** -140
+    assert np.all(off[:, fine] <= bound[:, fine])
+    # sums of up to 3e38 * 448 * 448: f32's where the definition's are, to the same bound
+    for cols in (np.r_[256:384], np.r_[384:400]):
+        for b in range(10):
+            alone = np.zeros_like(scales)
+            alone[:, b] = scales[:, b]
+            tiny = (x2 * np.float32(2.0 ** -20)).astype(np.float32)
+            got = _gemm(ctx, Weight(clean, alone), tiny)
+            ref, mass = fm.product(tiny, clean, alone)
+            inside = mass[:, cols] < 1e37
+            # a scale below 2^-117 leaves a sum in f32's subnormals
+            off = np.abs(got[:, cols] - ref[:, cols])
+            assert np.all((off <= 204 * 2.0 ** -24 * mass[:, cols] + 2.0 ** -140)[inside]), b
+
+
+@pytest.mark.parametrize("rows,n,k", [(4, 100, 8192), (1, 70, 32768), (3, 40, 11008), (4, 33, 8208), (16, 20, 20000)])
+def test_long_rows(ctx, rows, n, k):
+    """As much of x in LDS as a few rows may have there, and one block more."""
+    w, x = _weight(50, n, k), _rows(51, rows, k)
+    _check(_gemm(ctx, w, x), x, w)
+
+
+def test_more_rows_than_the_scratch_holds(ctx):
+    rows, k, n = 524288 + 300, 16, 7
+    w = _weight(52, n, k)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((rows, k), generator=g, device="cuda")
+    y = torch.full((rows + 1, 8), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), 8)
+    ctx.synchronize()
+    assert bool(torch.all(y[rows:] == 7)) and bool(torch.all(y[:, 7] == 7))
+    some = np.r_[0:20, 524270:524310, rows - 20:rows]
+    _check(y.cpu().numpy()[some, :7], x.cpu().numpy()[some], w)
+
+
+def test_two_contexts_at_once(ctx):
+    other = qtts.Context(0)
+    try:
+        jobs = []
+        for c, seed in ((ctx, 60), (other, 70)):
+            for rows, n, k in ((40, 640, 2048), (7, 500, 512), (300, 260, 1024)):
+                w, x = _weight(seed, n, k), _up(_rows(seed + 1, rows, k))
+                y = torch.zeros((rows, n), device="cuda")
+                jobs.append((c, w, x, rows, k, n, y))
+        torch.cuda.synchronize()
+
+        def go():
+            for c, w, x, rows, k, n, y in jobs:
+                c.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), n)
+        go()
+        torch.cuda.synchronize()
+        alone = []
+        for c, w, x, rows, k, n, y in jobs:
+            c.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), n)
+            c.synchronize()
+            alone.append(y.clone())
+        torch.cuda.synchronize()
+        for _ in range(20):
+            go()
+        torch.cuda.synchronize()
+        assert all(torch.equal(job[-1], a) for job, a in zip(jobs, alone))
+    finally:
+        other.close()
+
+
 def test_no_rows(ctx):
     w = _weight(1, 32, 64)
     ctx.fp8_gemm_device(w.w, 0, 64, 0, 0, 32)
