@@ -77,7 +77,7 @@ struct Fp8Plan {
 struct Fp8Tile {
     int bn, bm, alone, full;
 };
-constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1620, 1900}, {256, 128, 1000, 1080}, {128, 128, 600, 540}, {64, 64, 330, 200}};
+constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 495}, {64, 64, 330, 205}};
 
 // Whether the kernel for up to 16 rows brings them to 8 bits itself, in each block anew.
 inline bool fp8_own_rows(int rows, int kb) { return rows <= kFewRows && rows * kb <= kFewItems; }
@@ -92,12 +92,12 @@ inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
 }
 
 // The tile and number of splits that are taken to cost least.  A block's start costs
-// some 2 us, a CU works off ceil(blocks / CUs) of them, and joining costs a launch, the
-// host's share of it too, and the parts' way to memory and back.  What it chooses is within 10 % of the best of
-// all of them but for a few sizes: 1064 x 2048 -> 4096, 64 x 64 30 us (chosen), 128 x
-// 128 31, 256 x 256 52; 8192 rows of it 90 (4096 rows), 134 and 124 (chosen); 128 x 6144
-// -> 2048 in 64 x 64, 14 us in four parts, 37 in one; 512 x 1552 -> 1001 10 us in one,
-// 12 in four.
+// some 2 us; the fullest CU works off its blocks, where there are more than two a CU
+// nearly their mean; joining costs a launch, the host's share of it too, and the parts'
+// way to memory and back.  In 256 x 256, 128 x 128 and 64 x 64, us, the chosen one with a
+// star: 1064 x 2048 -> 4096 52, 31.6, 29.6*; 4096 rows of it 63.9*, 66.1, 83.6; 512 x
+// 1552 -> 1001 22, 13, 9.9*; 2048 x 6144 -> 2048 127, 52.8*, 63.6; 8192 x 2048 -> 12288
+// 362*, 410, -.  128 x 6144 -> 2048 in 64 x 64: 14 in four parts, 37 in one.
 inline Fp8Plan fp8_plan(int rows, int n, int k) {
     const int kb = fp8_blocks(k);
     if (rows <= 16) {
@@ -113,7 +113,8 @@ inline Fp8Plan fp8_plan(int rows, int n, int k) {
             if (p.splits != splits) continue;
             const long long out = (long long)rows * ((n + 3) & ~3);
             if (splits > 1 && splits * out > kFp8PartFloats) break;
-            const long long blocks = (long long)p.tiles_n * p.tiles_m * splits, full = (blocks + 255) / 256 * t.full;
+            const long long blocks = (long long)p.tiles_n * p.tiles_m * splits;
+            const long long full = blocks <= 512 ? (blocks + 255) / 256 * t.full : blocks * t.full * 27 / (256 * 25);
             if (blocks > (1 << 22)) continue;  // a launch counts its threads in 32 bits
             p.ns = 2000 + 2LL * p.each * (full > t.alone ? full : t.alone);
             if (splits > 1) p.ns += 4500 + splits * out * 8 / 4000;
