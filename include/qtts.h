@@ -504,13 +504,15 @@ typedef struct qtts_paged_pool {
  * goes on from another shares that one's full pages.  A source outside the batch
  * ends the row: it holds nothing.  With window > 0, pages whose tokens the next row
  * of attention with this window and these sinks does not see are dropped.  What a
- * row no longer holds is given back.  To go back into a full page, make tokens[b]
- * its first token: a shared page is then not written again.
+ * row no longer holds is given back.  As an append's start, tokens[b] is a token of
+ * the page that its source is filling or a page's first, as a full page's rows are not
+ * kept: to go on from its middle, make tokens[b] its first token.  The row then takes
+ * another page, and one that is shared is not written again.
  * Slots: a row that goes on from itself keeps its slot; the slot of one that only
  * others go on from goes to the first of them; the other rows take those of the rows
- * that ended, in order.  copied (NULL or [batch]) receives the slot whose open rows
- * row b has to copy before its next append (qtts_paged_copy_open_device, every
- * layer), or -1.
+ * that ended, in order.  copied (NULL or [batch], none of the other arrays) receives
+ * the slot whose open rows row b has to copy (qtts_paged_copy_open_device, every
+ * layer) before any row is appended to, or -1.
  * Enqueued on the context stream, allocates nothing and can be captured; larger
  * tables use context scratch, as attention does. */
 qtts_status qtts_paged_remap_device(qtts_ctx *ctx, const qtts_paged_pool *pool, const int32_t *d_source,

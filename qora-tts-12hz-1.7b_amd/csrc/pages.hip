@@ -94,9 +94,9 @@ __device__ void hand_on_slots(const RemapParams &A, Slots &S) {
     }
 }
 
-// What N entries from `first` on, kThreads apart, become; references change where they
-// do; the table has entries.  Loads of one kind are asked for together, one kind after another: what an entry
-// was, its row's heir, the heir's entry.
+// What N entries from `first` on, kThreads apart, become, of a table that has some;
+// references change where they do.  Loads of one kind are asked for together, one kind
+// after another: what an entry was, its row's heir, the heir's entry.
 template <int N>
 __device__ __forceinline__ void remapped(const RemapParams &A, int first, int (&now)[N]) {
     const int n = A.pool.batch * A.pool.max_pages, wide = A.pool.max_pages;

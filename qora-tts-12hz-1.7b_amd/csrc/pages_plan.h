@@ -46,6 +46,8 @@ inline Refusal check_remap(const qtts_paged_pool &p, const int32_t *source, cons
     if (!tokens) return {QTTS_EINVAL, "paged remap: null tokens"};
     if (!aligned_to(source, 4) || !aligned_to(tokens, 4) || !aligned_to(copied, 4))
         return {QTTS_EINVAL, "paged remap: misaligned array"};
+    if (copied && (copied == source || copied == tokens || copied == p.slots || copied == p.page_table))
+        return {QTTS_EINVAL, "paged remap: copied must be an array of its own"};
     return kAccepted;
 }
 

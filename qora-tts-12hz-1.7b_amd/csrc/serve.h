@@ -1,6 +1,6 @@
 // serve.h — kernel parameter blocks and launches of the serving operators: the
-// paged 8-bit cache (paged.hip) and its pages (pages.hip), row sampling (sample_rows.hip) and products on
-// 8-bit floats (fp8.hip).
+// paged 8-bit cache (paged.hip) and its pages (pages.hip), row sampling
+// (sample_rows.hip) and products on 8-bit floats (fp8.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -100,7 +100,8 @@ struct Fp8Params {
     int tiles_n, splits, each;  // Fp8Plan; blocks of a split
 };
 
-// The host's checks (paged_plan.h, pages_plan.h, fp8_plan.h) have refused what a launch cannot hold.
+// The host's checks (paged_plan.h, pages_plan.h, fp8_plan.h) have refused what a
+// launch cannot hold.
 void launch_paged_append(hipStream_t st, const PagedAppendParams &p);
 void launch_paged_attention(hipStream_t st, const PagedAttnParams &p);
 void launch_paged_read(hipStream_t st, const PagedReadParams &p);

@@ -378,7 +378,8 @@ def exported_symbols() -> List[str]:
         "qtts_paged_append_device", "qtts_paged_attention_device", "qtts_paged_attention_sinks_device",
         "qtts_paged_read_device",
         "qtts_paged_remap_device", "qtts_paged_reserve_device", "qtts_paged_compact_device",
-        "qtts_paged_copy_pages_device", "qtts_paged_copy_open_device", "qtts_sample_rows_device", "qtts_fp8_gemm_device", "qtts_fp8_quantize_device",
+        "qtts_paged_copy_pages_device", "qtts_paged_copy_open_device", "qtts_sample_rows_device",
+        "qtts_fp8_gemm_device", "qtts_fp8_quantize_device",
     ]
 
 

@@ -91,7 +91,7 @@ def test_pools(lib, pool, status):
 
 def test_arrays(lib):
     p = C.byref(_pool())
-    assert lib.remap(p, None, AT, 5, 3, AT) == OK
+    assert lib.remap(p, None, AT, 5, 3, AT + 4096) == OK
     for args in ((AT, None, 0, 0, None), (AT + 2, AT, 0, 0, None), (AT, AT + 1, 0, 0, None), (AT, AT, 0, 0, AT + 2),
                  (AT, AT, -1, 0, None), (AT, AT, 0, -1, None)):
         assert lib.remap(p, *args) == EINVAL
@@ -100,6 +100,15 @@ def test_arrays(lib):
     for args in ((None, AT, AT), (AT, None, AT), (AT + 2, AT, AT), (AT, AT + 2, AT), (AT + 4, AT, AT + 2), (AT, AT, None)):
         assert lib.compact(p, *args) == EINVAL
     assert lib.compact(C.byref(_pool(num_pages=1)), None, None, AT) == OK
+
+
+def test_what_a_remap_writes_is_an_array_of_its_own(lib):
+    names = ("source", "tokens", "slots", "page_table")
+    for same in (None,) + names:
+        at = {n: AT + 4096 * (i + 1) for i, n in enumerate(names)}
+        p = C.byref(_pool(slots=at["slots"], page_table=at["page_table"]))
+        copied = at[same] if same else AT + 4096 * 9
+        assert lib.remap(p, at["source"], at["tokens"], 0, 0, copied) == (EINVAL if same else OK)
 
 
 def _kv(**over):
