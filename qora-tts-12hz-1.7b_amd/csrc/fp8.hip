@@ -186,9 +186,11 @@ __device__ __forceinline__ void each(F &&f) {
     }
 }
 
-// Four columns of a row of a split's sums.
-__device__ __forceinline__ float *part_of(const Fp8Params &A, int split, int row, int n) {
-    return A.part + ((size_t)split * A.rows + row) * ((A.w.n + 3) & ~3) + n;
+// Where a lane's four sums of a part of a divided tile lie: by fragments, each as a wave
+// stores it.
+template <int BN, int BM>
+__device__ __forceinline__ f32x4 *part_of(const Fp8Params &A, size_t part, int fragment, int lane) {
+    return reinterpret_cast<f32x4 *>(A.part) + (part * (BN / 16 * (BM / 16)) + fragment) * 64 + lane;
 }
 
 // Four columns of a row of y.
@@ -245,11 +247,15 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
     const unsigned ring_at = lds_address(ring);
     const int lane = threadIdx.x & 63, r = lane & 15, G = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
-    int id = blockIdx.x;
-    const int split = id % A.splits;
-    id /= A.splits;
+    int id = blockIdx.x, first = 0, last = (A.w.k + 63) / 64;
+    const int part = id - A.whole;
+    const bool divided = A.splits > 1 && part >= 0;
+    if (divided) {
+        id = A.whole + part / A.splits;
+        first = 2 * A.each * (part % A.splits);
+        last = min(first + 2 * A.each, last);
+    }
     const int n0 = id % A.tiles_n * BN, m0 = id / A.tiles_n * BM;
-    const int first = 2 * split * A.each, last = min(first + 2 * A.each, (A.w.k + 63) / 64);
     // A load of codes brings 8 rows of 128 bytes; their eight pieces lie in LDS at
     // their number exclusive-or half of the row's.
     const uint8_t *codes = A.w.codes + (size_t)n0 * A.w.ld, *xs = A.xc + (size_t)(m0 / 16 + wave * LB) * A.kb * 4096;
@@ -394,23 +400,28 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
         for (int i = 0; i < NF; i++) {
             const int n = n0 + (wn * NF + i) * 16 + 4 * G;
             if (row >= A.rows || n >= A.w.n) continue;
-            if (A.splits > 1) *glb(reinterpret_cast<f32x4 *>(part_of(A, split, row, n))) = acc[i][j];
+            if (divided) *glb(part_of<BN, BM>(A, part, (wave * NF + i) * MF + j, lane)) = acc[i][j];
             else put(A, row, n, acc[i][j]);
         }
     }
 }
 
-// The splits' sums, in their order.  Four columns a thread.
+// The parts' sums of the divided tiles, in their order.  Four columns a thread.
+template <int BN, int BM, int WN, int WM>
 __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
-    const int fours = (A.w.n + 3) / 4;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= (long long)A.rows * fours) return;
-    const int row = (int)(at / fours), n = (int)(at % fours) * 4;
+    constexpr int F = BN / 16 * (BM / 16), NF = BN / WN / 16, MF = BM / WM / 16;
+    const int lane = threadIdx.x & 63, r = lane & 15, G = lane >> 4;
+    const int at = blockIdx.x * 4 + (threadIdx.x >> 6), tile = at / F, f = at % F;  // a wave a fragment
+    const int wave = f / (NF * MF), i = f / MF % NF, j = f % MF, id = A.whole + tile;
+    const int row = id / A.tiles_n * BM + (wave / WN * MF + j) * 16 + r;
+    const int n = id % A.tiles_n * BN + (wave % WN * NF + i) * 16 + 4 * G;
+    if (row >= A.rows || n >= A.w.n) return;
     f32x4 v = {0, 0, 0, 0};
     for (int k0 = 0; k0 < A.splits; k0 += 8) {
         f32x4 p[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) p[k] = load4(part_of(A, min(k0 + k, A.splits - 1), row, n));
+        for (int k = 0; k < 8; k++)
+            p[k] = *glb(part_of<BN, BM>(A, (size_t)tile * A.splits + min(k0 + k, A.splits - 1), f, lane));
 #pragma unroll
         for (int k = 0; k < 8; k++)
             if (k0 + k < A.splits) v += p[k];
@@ -512,6 +523,14 @@ void few_of(hipStream_t st, const Fp8Params &p, int waves, unsigned blocks, size
     else hipLaunchKernelGGL((k_fp8_few<16, OWN>), dim3(blocks), dim3(1024), lds, st, p);
 }
 
+template <int BN, int BM, int WN, int WM>
+void tiles_of(hipStream_t st, const Fp8Params &p, const Fp8Plan &plan) {
+    hipLaunchKernelGGL((k_fp8_tile<BN, BM, WN, WM>), dim3((unsigned)fp8_launched(plan)), dim3(64 * WN * WM), 0, st, p);
+    if (plan.splits == 1) return;
+    const unsigned waves = (unsigned)(plan.tiles_n * plan.tiles_m - plan.whole) * (BN / 16 * (BM / 16));
+    hipLaunchKernelGGL((k_fp8_join<BN, BM, WN, WM>), dim3(waves / 4), dim3(256), 0, st, p);
+}
+
 }  // namespace
 
 void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
@@ -525,9 +544,10 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
         p.kb = fp8_blocks(p.w.k);
         const Fp8Plan plan = fp8_plan(p.rows, p.w.n, p.w.k);
         p.tiles_n = plan.tiles_n;
+        p.whole = plan.whole;
         p.splits = plan.splits;
         p.each = plan.each;
-        const unsigned blocks = (unsigned)plan.tiles_n * plan.tiles_m * plan.splits;
+        const unsigned blocks = (unsigned)plan.tiles_n * plan.tiles_m;
         const bool own = plan.bm == 16 && fp8_own_rows(p.rows, p.kb);
         if (!own) {
             const long long each = 8 * kRowsAhead, rows_blocks = ((long long)p.rows * p.kb + each - 1) / each;
@@ -538,13 +558,9 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
             else few_of<false>(st, p, plan.waves, blocks, 0);
             continue;
         }
-        if (plan.bm == 256) hipLaunchKernelGGL((k_fp8_tile<256, 256, 4, 2>), dim3(blocks), dim3(512), 0, st, p);
-        else if (plan.bm == 128) hipLaunchKernelGGL((k_fp8_tile<128, 128, 4, 2>), dim3(blocks), dim3(512), 0, st, p);
-        else hipLaunchKernelGGL((k_fp8_tile<64, 64, 2, 2>), dim3(blocks), dim3(256), 0, st, p);
-        if (plan.splits > 1) {
-            const long long fours = (long long)p.rows * ((p.w.n + 3) / 4);
-            hipLaunchKernelGGL(k_fp8_join, dim3((unsigned)((fours + 255) / 256)), dim3(256), 0, st, p);
-        }
+        if (plan.bm == 256) tiles_of<256, 256, 4, 2>(st, p, plan);
+        else if (plan.bm == 128) tiles_of<128, 128, 4, 2>(st, p, plan);
+        else tiles_of<64, 64, 2, 2>(st, p, plan);
     }
 }
 

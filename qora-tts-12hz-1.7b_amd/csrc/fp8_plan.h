@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/qtts.h"
 #include "paged_plan.h"
@@ -62,42 +63,47 @@ inline Refusal check_fp8_quantize(const float *src, int32_t ld_src, const qtts_f
     return check_rows(src, ld_src, w.k);
 }
 
-// A product's tiles: bn columns of the output (rows of the weight) by bm rows; the
-// blocks of 128 of the contraction are divided over `splits` blocks of a tile, `each`
-// of them each.
+// A product's tiles: bn columns of the output (rows of the weight) by bm rows.  The
+// first `whole` have a block each; the blocks of 128 of the contraction of the others
+// are divided over `splits` blocks, `each` of them each.
 struct Fp8Plan {
     int bn, bm;  // bm == 16: the kernel for up to 16 rows
-    int tiles_n, tiles_m, splits, each;
+    int tiles_n, tiles_m, whole, splits, each;
     long long ns;  // what it is taken to cost
     int waves;     // of a block, for a few rows
 };
+inline long long fp8_launched(const Fp8Plan &p) {
+    return p.whole + ((long long)p.tiles_n * p.tiles_m - p.whole) * p.splits;
+}
 
 // A tile's step of 64, in ns: with a CU to itself and where blocks fill it, as measured
 // (4096 deep, 64 to 4096 blocks).
 struct Fp8Tile {
     int bn, bm, alone, full;
 };
-constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 495}, {64, 64, 330, 205}};
+constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 520}, {64, 64, 330, 210}};
 
 // Whether the kernel for up to 16 rows brings them to 8 bits itself, in each block anew.
 inline bool fp8_own_rows(int rows, int kb) { return rows <= kFewRows && rows * kb <= kFewItems; }
 
 inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
     const int kb = fp8_blocks(k);
-    Fp8Plan p{bn, bm, (n + bn - 1) / bn, (rows + bm - 1) / bm, 1, 0, 0, 0};
+    Fp8Plan p{bn, bm, (n + bn - 1) / bn, (rows + bm - 1) / bm, 0, 1, 0, 0, 0};
     p.each = (kb + splits - 1) / splits;
     p.splits = (kb + p.each - 1) / p.each;
     p.each = (kb + p.splits - 1) / p.splits;
     return p;
 }
 
-// The tile and number of splits that are taken to cost least.  A block's start costs
-// some 2 us; the fullest CU works off its blocks, where there are more than two a CU
-// nearly their mean; joining costs a launch, the host's share of it too, and the parts'
-// way to memory and back.  In 256 x 256, 128 x 128 and 64 x 64, us, the chosen one with a
-// star: 1064 x 2048 -> 4096 52, 31.6, 29.6*; 4096 rows of it 63.9*, 66.1, 83.6; 512 x
-// 1552 -> 1001 22, 13, 9.9*; 2048 x 6144 -> 2048 127, 52.8*, 63.6; 8192 x 2048 -> 12288
-// 362*, 410, -.  128 x 6144 -> 2048 in 64 x 64: 14 in four parts, 37 in one.
+// The tile and division that are taken to cost least: no tile divided, all of them, or
+// those past the last whole round of 256.  A block's start costs some 2 us; the fullest
+// CU works off its blocks; joining costs a launch and the parts' way to memory and back.
+// Against all that can be chosen, 1 % more over 26 shapes (17 to 8192 rows), 8 % at
+// worst.  us, the chosen one with a star, tiles of 256, 128 and 64 whole and the last
+// round divided in 128 and in 64: 512 x 1552 -> 1001 22, 13, 9.9*; 900 x 2048 -> 4096 57,
+// 24.3*, 26.1; 1064 rows of it 54, 34, 33, 29*, 30; 2112 rows 58, 57, 51, 44*, 50;
+// 4096 rows 63.9*, 66.1, 83.6; 2100 x 6144 -> 2048 132, 85, 82, 62*, 72; 8192 x 2048 ->
+// 12288 362*, 410, -.  128 x 6144 -> 2048 in 64: 14 in four parts, 37 in one.
 inline Fp8Plan fp8_plan(int rows, int n, int k) {
     const int kb = fp8_blocks(k);
     if (rows <= 16) {
@@ -111,14 +117,22 @@ inline Fp8Plan fp8_plan(int rows, int n, int k) {
         for (int splits = 1; splits <= kFp8MaxSplits && splits <= kb; splits++) {
             Fp8Plan p = fp8_divided(rows, n, k, t.bn, t.bm, splits);
             if (p.splits != splits) continue;
-            const long long out = (long long)rows * ((n + 3) & ~3);
-            if (splits > 1 && splits * out > kFp8PartFloats) break;
-            const long long blocks = (long long)p.tiles_n * p.tiles_m * splits;
-            const long long full = blocks <= 512 ? (blocks + 255) / 256 * t.full : blocks * t.full * 27 / (256 * 25);
-            if (blocks > (1 << 22)) continue;  // a launch counts its threads in 32 bits
-            p.ns = 2000 + 2LL * p.each * (full > t.alone ? full : t.alone);
-            if (splits > 1) p.ns += 4500 + splits * out * 8 / 4000;
-            if (best.bn == 0 || p.ns < best.ns) best = p;
+            const long long tiles = (long long)p.tiles_n * p.tiles_m, rounds = splits > 1 ? tiles / 256 : 0;
+            for (long long round : {0LL, rounds}) {
+                p.whole = (int)(256 * round);
+                const long long rest = tiles - p.whole, pieces = rest * splits, floats = pieces * t.bn * t.bm;
+                if (splits > 1 && (rest == 0 || floats > kFp8PartFloats)) continue;
+                if (fp8_launched(p) > (1 << 22)) continue;  // a launch counts its threads in 32 bits
+                const long long most = (pieces + 255) / 256, step = 2LL * p.each, all = 2LL * kb;
+                long long work = most * step * t.full;
+                if (round) work = round * all * t.full + (most == 1 ? step * t.alone : work);
+                const long long alone = (round ? all : step) * t.alone;
+                p.ns = 2000 + (work > alone ? work : alone);
+                // (the last tiles' rows may be few)
+                const long long low = rest < p.tiles_n ? rest : p.tiles_n, few = (long long)p.tiles_m * t.bm - rows;
+                if (splits > 1) p.ns += 3500 + (floats - low * few * splits * t.bn) * 8 / 4000;
+                if (best.bn == 0 || p.ns < best.ns) best = p;
+            }
         }
     return best;
 }

@@ -97,7 +97,7 @@ struct Fp8Params {
     float *part;          // kFp8PartFloats: split sums
     // the launch's own
     int kb;               // blocks of the contraction
-    int tiles_n, splits, each;  // Fp8Plan; blocks of a split
+    int tiles_n, whole, splits, each;  // Fp8Plan
 };
 
 // The host's checks (paged_plan.h, pages_plan.h, fp8_plan.h) have refused what a

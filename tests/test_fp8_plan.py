@@ -27,7 +27,8 @@ extern "C" void plan(int rows, int n, int k, long long *o) {
     const Fp8Plan p = fp8_plan(rows, n, k);
     o[0] = p.bn; o[1] = p.bm; o[2] = p.tiles_n; o[3] = p.tiles_m; o[4] = p.splits;
     o[5] = fp8_rows_at_once(k); o[6] = kFp8PartFloats; o[7] = kFp8MaxSplits; o[8] = kFp8RowStep;
-    o[9] = (long long)kFp8ScratchBytes; o[10] = fp8_blocks(k); o[11] = p.waves; o[12] = p.each;
+    o[9] = (long long)kFp8ScratchBytes; o[10] = fp8_blocks(k); o[11] = p.waves; o[12] = p.each; o[13] = p.whole;
+    o[14] = fp8_launched(p);
 }
 """
 
@@ -93,22 +94,23 @@ def test_sources(lib):
 def test_plans(lib):
     """Tiles cover the output, splits the contraction, none of them empty; parts
     and the rows' scratch hold what a launch uses."""
-    o = (C.c_longlong * 13)()
+    o = (C.c_longlong * 15)()
     for rows in [*range(1, 300, 7), 512, 1064, 4096, 8192, 100000, 1 << 24]:
         for n in (1, 31, 128, 1000, 2048, 12288, 131072):
             for k in (16, 128, 144, 2048, 6144, 131072):
                 lib.plan(1, n, k, o)
                 rows_now = min(rows, o[5])  # what a launch takes
                 lib.plan(rows_now, n, k, o)
-                bn, bm, tn, tm, splits, at_once, part, most, step, scratch, kb, waves, per = list(o)
+                bn, bm, tn, tm, splits, at_once, part, most, step, scratch, kb, waves, per, whole, launched = list(o)
                 assert (tn - 1) * bn < n <= tn * bn and (tm - 1) * bm < rows_now <= tm * bm
-                assert tn * tm * splits * 512 < 1 << 32
+                assert launched * 512 < 1 << 32 and launched == whole + (tn * tm - whole) * splits
                 assert step % bm == 0 and at_once % step == 0 and at_once >= step
                 assert at_once * kb * 256 <= scratch
                 assert 1 <= splits <= min(kb, most) and most <= 64
                 assert (splits - 1) * per < kb <= splits * per
+                assert 0 <= whole <= tn * tm and whole % 256 == 0
                 if splits > 1:
-                    assert rows_now * -(-n // 4) * 4 * splits <= part
+                    assert whole < tn * tm and (tn * tm - whole) * splits * bn * bm <= part
                 if bm == 16:  # the kernel for up to 16 rows: its LDS
                     assert splits == 1 and rows <= 16 and waves in (4, 8, 16)
                     assert waves * 1024 + (rows * kb * 256 if lib.own(rows, kb) else 0) <= 160 * 1024

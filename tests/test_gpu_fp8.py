@@ -97,6 +97,14 @@ def test_large(ctx, rows, n, k):
     _check(_gemm(ctx, w, x, add=add), x, w, add)
 
 
+@pytest.mark.parametrize("rows,n,k", [(646, 5378, 1040), (1051, 2047, 6144), (3337, 4740, 528)])
+def test_the_last_round_divided(ctx, rows, n, k):
+    """Tiles of 128, 64 and 256 of which 256 or 512 have a block each and the others
+    several, and the join of these."""
+    w, x, add = _weight(1, n, k), _rows(2, rows, k), _rows(3, rows, n)
+    _check(_gemm(ctx, w, x, add=add), x, w, add)
+
+
 @pytest.mark.parametrize("rows", [5, 40])
 def test_residual_in_place(ctx, rows):
     w, x, add = _weight(4, 260, 384), _rows(5, rows, 384), _rows(6, rows, 260)
