@@ -76,14 +76,12 @@ __device__ __forceinline__ unsigned dpp_bits(unsigned v) {
     return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
 }
 
-// Largest over 32 lanes, of magnitudes as bits (as integers: a NaN is the largest).
-__device__ __forceinline__ unsigned half_max(unsigned v) {
+// Largest over 16 lanes, of magnitudes as bits (as integers: a NaN is the largest).
+__device__ __forceinline__ unsigned row_max(unsigned v) {
     v = max(v, dpp_bits<kDppXor1>(v));
     v = max(v, dpp_bits<kDppXor2>(v));
     v = max(v, dpp_bits<kDppHalfMirror>(v));
-    v = max(v, dpp_bits<kDppMirror>(v));
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return max((unsigned)r[0], (unsigned)r[1]);
+    return max(v, dpp_bits<kDppMirror>(v));
 }
 
 // Where a row's 16-byte pieces lie in LDS, of four: at place_of(piece) exclusive-or a
@@ -93,39 +91,41 @@ __device__ __forceinline__ unsigned half_max(unsigned v) {
 // twice as long).
 __device__ __forceinline__ int place_of(int piece) { return (piece & 1 ? 3 : 0) ^ (piece >> 1); }
 
-// 128 values of a row as the products take them, in 8 bits and back: four a lane of 32.
-__device__ __forceinline__ u32x2 block_values(f32x4 x) {
-    const int e = scale_exponent(half_max(top4(x, 0)));
-    const int c = codes4(x, e);
+// 128 values of a row as the products take them, in 8 bits and back: eight a lane of 16.
+__device__ __forceinline__ u32x4 block_values(f32x4 x, f32x4 y) {
+    const int e = scale_exponent(row_max(top4(y, top4(x, 0))));
     const float s = e == 255 ? 1.0f : power_of(e);
-    const unsigned lo = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, false));
-    const unsigned hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, true));
-    return e == 255 ? u32x2{0x7fc07fc0u, 0x7fc07fc0u} : u32x2{lo, hi};
+    const bf16x8 v = values8(codes4(x, e), codes4(y, e), s);
+    return e == 255 ? u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u} : __builtin_bit_cast(u32x4, v);
 }
 
 // Rows lie in pieces of 1 KB, 16 of them and half of 64 of the contraction (of every 16
 // the first 8, or the others), as they are to lie in LDS.
-// All rows to scratch, [row / 16][k / 64][half], zeros behind k.  32 lanes a block of 128,
-// kRowsAhead blocks one after another whose loads are in flight together.
-constexpr int kRowsAhead = 4;
+// All rows to scratch, [row / 16][k / 64][half], zeros behind k.  A wave a block of 128
+// of four rows, kRowsAhead blocks one after another whose loads are in flight together.
+// Bound by memory: 8192 rows of 2048, 101 MB, in 18 to 26 us; 2100 of 6144 12.6 (four
+// blocks a wave 13.6); small ones by latency, 17 of 6144 3.4 us (4.2).
+constexpr int kRowsAhead = 2;
 __global__ __launch_bounds__(256) void k_fp8_rows(Fp8Params A) {
-    const int lane = threadIdx.x & 31;
-    const long long at = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kRowsAhead, blocks = (long long)A.rows * A.kb;
-    f32x4 x[kRowsAhead];
+    const int lane = threadIdx.x & 15, sub = threadIdx.x >> 4 & 3;
+    const long long at = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * kRowsAhead;
+    const long long blocks = (long long)((A.rows + 3) / 4) * A.kb;
+    f32x4 x[kRowsAhead][2];
 #pragma unroll
     for (int i = 0; i < kRowsAhead; i++) {
         const long long b = min(at + i, blocks - 1);
-        const int col = (int)(b % A.kb) * kFp8Block + 4 * lane;
-        x[i] = load4(A.x + (size_t)(b / A.kb) * A.ld_x + (col < A.w.k ? col : 0));
-        if (col >= A.w.k) x[i] = f32x4{0, 0, 0, 0};
+        const int col = (int)(b % A.kb) * kFp8Block + 8 * lane, row = min((int)(b / A.kb) * 4 + sub, A.rows - 1);
+        const float *from = A.x + (size_t)row * A.ld_x + (col < A.w.k ? col : 0);
+        x[i][0] = load4(from), x[i][1] = load4(from + 4);
+        if (col >= A.w.k) x[i][0] = x[i][1] = f32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < kRowsAhead; i++) {
-        if (at + i >= blocks) return;
-        const int row = (int)((at + i) / A.kb), b = (int)((at + i) % A.kb);
-        uint8_t *to = A.xc + ((size_t)(row >> 4) * A.kb + b) * 4096 + (lane >> 4) * 2048 + (lane & 2) * 512;
-        const int place = place_of(lane >> 2 & 3) ^ (row >> 2 & 3);
-        *glb(reinterpret_cast<u32x2 *>(to + (row & 15) * 64 + place * 16 + (lane & 1) * 8)) = block_values(x[i]);
+        const u32x4 v = block_values(x[i][0], x[i][1]);
+        const int row = (int)((at + i) / A.kb) * 4 + sub, b = (int)((at + i) % A.kb);
+        uint8_t *to = A.xc + ((size_t)(row >> 4) * A.kb + b) * 4096 + (lane >> 3) * 2048 + (lane & 1) * 1024;
+        const int place = place_of(lane >> 1 & 3) ^ (row >> 2 & 3);
+        if (at + i < blocks && row < A.rows) *glb(reinterpret_cast<u32x4 *>(to + (row & 15) * 64 + place * 16)) = v;
     }
 }
 
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
 // straight from memory to registers, four asked for at once.  OWN: of up to kFewRows
 // rows the block meanwhile brings x to 8 bits itself, into LDS; more come from scratch,
 // which k_fp8_rows has filled.  Bound by reading the weight and by one chain of
-// latencies: one row, 2048 to 12288, 25 MB in 7.7 us (3.3 TB/s); 6144 to 2048 8.5 us.
+// latencies: one row, 2048 to 12288, 25 MB in 7.2 us (3.5 TB/s); 6144 to 2048 8.5 us.
 // (With the contraction divided over blocks and joined through memory 12 us, most of it
 // the joining.)
 template <int W, bool OWN>
@@ -466,22 +466,23 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A)
         }
     };
     ask(wave);
-    const int items = OWN ? A.rows * A.kb : 0;  // 32 lanes a row's block of 128
-    for (int i0 = threadIdx.x >> 5; i0 < items; i0 += 8 * W) {
-        f32x4 x[4];
-        const int l = threadIdx.x & 31;
+    const int items = OWN ? A.rows * A.kb : 0;  // 16 lanes a row's block of 128
+    for (int i0 = threadIdx.x >> 4; i0 < items; i0 += 8 * W) {
+        f32x4 x[2][2];
+        const int l = threadIdx.x & 15;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int it = min(i0 + 2 * W * i, items - 1), col = it % A.kb * kFp8Block + 4 * l;
-            x[i] = load4(A.x + (size_t)(it / A.kb) * A.ld_x + (col < A.w.k ? col : 0));
-            if (col >= A.w.k) x[i] = f32x4{0, 0, 0, 0};
+        for (int i = 0; i < 2; i++) {
+            const int it = min(i0 + 4 * W * i, items - 1), col = it % A.kb * kFp8Block + 8 * l;
+            const float *from = A.x + (size_t)(it / A.kb) * A.ld_x + (col < A.w.k ? col : 0);
+            x[i][0] = load4(from), x[i][1] = load4(from + 4);
+            if (col >= A.w.k) x[i][0] = x[i][1] = f32x4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int it = i0 + 2 * W * i;
-            const u32x2 v = block_values(x[i]);
+        for (int i = 0; i < 2; i++) {
+            const int it = i0 + 4 * W * i;
+            const u32x4 v = block_values(x[i][0], x[i][1]);
             if (it < items)
-                *reinterpret_cast<u32x2 *>(xs + it * 256 + (l >> 4) * 128 + (l & 2) * 32 + (l >> 2 & 3) * 16 + (l & 1) * 8) = v;
+                *reinterpret_cast<u32x4 *>(xs + it * 256 + (l >> 3) * 128 + (l & 1) * 64 + (l >> 1 & 3) * 16) = v;
         }
     }
     if (OWN) __syncthreads();
@@ -550,7 +551,7 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
         const unsigned blocks = (unsigned)plan.tiles_n * plan.tiles_m;
         const bool own = plan.bm == 16 && fp8_own_rows(p.rows, p.kb);
         if (!own) {
-            const long long each = 8 * kRowsAhead, rows_blocks = ((long long)p.rows * p.kb + each - 1) / each;
+            const long long each = 4 * kRowsAhead, rows_blocks = ((long long)(p.rows + 3) / 4 * p.kb + each - 1) / each;
             hipLaunchKernelGGL(k_fp8_rows, dim3((unsigned)rows_blocks), dim3(256), 0, st, p);
         }
         if (plan.bm == 16) {
