@@ -17,6 +17,9 @@ constexpr int kPoolPages = (4 << 20) - 64;          // names of pages, and their
 // Entries that one block remaps in its registers, in 3.5 us; more go through scratch in
 // two launches, which take 6.5 (one block 9 to 13 for 8128).
 constexpr int kRemapThreads = 1024, kRemapEach = 2;
+// Entries that the block which finds the moves renames itself, 8192 in 2 us: with 8128
+// it takes 12.5 us, with a second launch 10.4 and 4.7; with 144 6.6, or 6.2 and 1.5.
+constexpr int kRenameOne = 16384;
 constexpr int kPoolChunk = 16384;                   // pages that a block looks at in one go (counted in 16 bits)
 
 inline Refusal check_pool(const qtts_paged_pool &p) {
