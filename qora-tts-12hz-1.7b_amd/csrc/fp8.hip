@@ -429,40 +429,45 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
     put(A, row, n, v);
 }
 
-// Up to 16 rows: 16 weight rows a block, whose blocks of 128 its W waves take in turn,
-// straight from memory to registers, four asked for at once.  OWN: of up to kFewRows
-// rows the block meanwhile brings x to 8 bits itself, into LDS; more come from scratch,
-// which k_fp8_rows has filled.  Bound by reading the weight and by one chain of
-// latencies: one row, 2048 to 12288, 25 MB in 7.2 us (3.5 TB/s); 6144 to 2048 8.5 us.
-// (With the contraction divided over blocks and joined through memory 12 us, most of it
-// the joining.)
-template <int W, bool OWN>
-__global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A) {
+// Up to 64 rows: 16 weight rows a block, whose blocks of 128 its W waves take in turn,
+// straight from memory to registers; RF times 16 rows of x.  OWN: of up to kFewRows rows
+// the block meanwhile brings x to 8 bits itself, into LDS; more come from scratch, which
+// k_fp8_rows has filled.  Bound by a chain of latencies, by reading the weight, and by
+// reading x from L2 in every block (60 GB/s a CU): one row, 2048 to 12288, 25 MB in 7.2
+// us (3.5 TB/s); 16 rows, 6144 to 2048 8.5 us, 2048 to 4096 4.2, 32 of these 5.3, 64 7.5
+// (in tiles of 64 and joined 8.7 to 9.5).  With 32 weight rows a block, half of x's reads
+// and half of the blocks: 5.6, 7.0 and 9.5.
+template <int W, bool OWN, int RF>
+__global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few(Fp8Params A) {
+    constexpr int kAhead = 4 / RF;  // blocks of 128 asked for at once
     extern __shared__ __align__(16) uint8_t lds[];  // sums of the waves, then x, [row][128s][half of 64][piece]
     f32x4 *so = reinterpret_cast<f32x4 *>(lds);
-    uint8_t *xs = lds + W * 1024;
+    uint8_t *xs = lds + W * RF * 1024;
     const int lane = threadIdx.x & 63, r = lane & 15, G = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
     const uint8_t *wr = A.w.codes + (size_t)min(n0 + r, A.w.n - 1) * A.w.ld;
     const KCONST float *ws = (const KCONST float *)(A.w.scales + (size_t)(n0 / kFp8Block) * A.kb);
-    i32x4 w[4][2];
-    bf16x8 xv[OWN ? 1 : 4][4];
-    float scale[4];
+    i32x4 w[kAhead][2];
+    bf16x8 xv[OWN ? 1 : kAhead][RF][4];
+    float scale[kAhead];
     const uint8_t *xr = OWN ? xs + min(r, A.rows - 1) * A.kb * 256 + 16 * G : A.xc + r * 64 + 16 * (place_of(G) ^ (r >> 2));
     auto ask = [&](int b0) {
 #pragma unroll
-        for (int a = 0; a < 4; a++) {
+        for (int a = 0; a < kAhead; a++) {
             const int b = min(b0 + W * a, A.kb - 1);
-            if (!OWN)
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    xv[OWN ? 0 : a][q] = *glb(reinterpret_cast<const bf16x8 *>(xr + (size_t)b * 4096 + q * 1024));
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int at = b * 128 + 64 * h + 16 * G;  // behind k any codes: x has zeros there
                 w[a][h] = __builtin_nontemporal_load(glb(reinterpret_cast<const i32x4 *>(wr + (at < A.w.k ? at : 0))));
             }
             scale[a] = ws[b];
+            if (!OWN)
+#pragma unroll
+                for (int f = 0; f < RF; f++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        xv[OWN ? 0 : a][f][q] =
+                            *glb(reinterpret_cast<const bf16x8 *>(xr + ((size_t)f * A.kb + b) * 4096 + q * 1024));
         }
     };
     ask(wave);
@@ -486,42 +491,45 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : 4) void k_fp8_few(Fp8Params A)
         }
     }
     if (OWN) __syncthreads();
-    f32x4 acc = {0, 0, 0, 0};
-    for (int b0 = wave; b0 < A.kb; b0 += 4 * W) {
+    f32x4 acc[RF] = {};
+    for (int b0 = wave; b0 < A.kb; b0 += kAhead * W) {
         if (b0 != wave) ask(b0);
 #pragma unroll
-        for (int a = 0; a < 4; a++) {
+        for (int a = 0; a < kAhead; a++) {
             const int b = b0 + W * a;
             if (b >= A.kb) break;
             const Scale s(scale[a]);
             const int mask = s.none ? 0 : -1;  // codes under a scale of 0 are zeros
-            f32x4 p = {0, 0, 0, 0};
+            const float by = s.bad ? __uint_as_float(0x7fc00000u) : s.rest;
+            f32x4 p[RF] = {};
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const i32x4 c = w[a][q >> 1];
-                p = mma(values8(c[2 * (q & 1)] & mask, c[2 * (q & 1) + 1] & mask, s.power),
-                        OWN ? *reinterpret_cast<const bf16x8 *>(xr + b * 256 + q * 64) : xv[OWN ? 0 : a][q], p);
-            }
-            const float by = s.bad ? __uint_as_float(0x7fc00000u) : s.rest;
+                const bf16x8 v = values8(c[2 * (q & 1)] & mask, c[2 * (q & 1) + 1] & mask, s.power);
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] = fmaf(by, p[i], acc[i]);
+                for (int f = 0; f < RF; f++)
+                    p[f] = mma(v, OWN ? *reinterpret_cast<const bf16x8 *>(xr + b * 256 + q * 64) : xv[OWN ? 0 : a][f][q], p[f]);
+            }
+#pragma unroll
+            for (int f = 0; f < RF; f++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[f][i] = fmaf(by, p[f][i], acc[f][i]);
         }
     }
-    so[threadIdx.x] = acc;
-    __syncthreads();
-    if (wave != 0) return;
 #pragma unroll
-    for (int k = 1; k < W; k++) acc += so[k * 64 + lane];
-    const int n = n0 + 4 * G;
-    if (r < A.rows && n < A.w.n) put(A, r, n, acc);
+    for (int f = 0; f < RF; f++) so[(f * W + wave) * 64 + lane] = acc[f];
+    __syncthreads();
+    if (wave >= RF) return;  // a wave for 16 rows
+    f32x4 sum = so[wave * W * 64 + lane];
+#pragma unroll
+    for (int k = 1; k < W; k++) sum += so[(wave * W + k) * 64 + lane];
+    const int n = n0 + 4 * G, row = 16 * wave + r;
+    if (row < A.rows && n < A.w.n) put(A, row, n, sum);
 }
 
-template <bool OWN>
-void few_of(hipStream_t st, const Fp8Params &p, int waves, unsigned blocks, size_t x_bytes) {
-    const size_t lds = (size_t)waves * 1024 + x_bytes;
-    if (waves == 4) hipLaunchKernelGGL((k_fp8_few<4, OWN>), dim3(blocks), dim3(256), lds, st, p);
-    else if (waves == 8) hipLaunchKernelGGL((k_fp8_few<8, OWN>), dim3(blocks), dim3(512), lds, st, p);
-    else hipLaunchKernelGGL((k_fp8_few<16, OWN>), dim3(blocks), dim3(1024), lds, st, p);
+template <int W, bool OWN, int RF>
+void few_of(hipStream_t st, const Fp8Params &p, size_t x_bytes) {
+    hipLaunchKernelGGL((k_fp8_few<W, OWN, RF>), dim3((unsigned)p.tiles_n), dim3(64 * W), W * RF * 1024 + x_bytes, st, p);
 }
 
 template <int BN, int BM, int WN, int WM>
@@ -548,15 +556,19 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
         p.whole = plan.whole;
         p.splits = plan.splits;
         p.each = plan.each;
-        const unsigned blocks = (unsigned)plan.tiles_n * plan.tiles_m;
-        const bool own = plan.bm == 16 && fp8_own_rows(p.rows, p.kb);
-        if (!own) {
-            const long long each = 4 * kRowsAhead, rows_blocks = ((long long)(p.rows + 3) / 4 * p.kb + each - 1) / each;
-            hipLaunchKernelGGL(k_fp8_rows, dim3((unsigned)rows_blocks), dim3(256), 0, st, p);
+        if (fp8_own_rows(p.rows, p.kb)) {
+            const size_t x_bytes = (size_t)p.rows * p.kb * 256;
+            if (plan.waves == 4) few_of<4, true, 1>(st, p, x_bytes);
+            else if (plan.waves == 8) few_of<8, true, 1>(st, p, x_bytes);
+            else few_of<16, true, 1>(st, p, x_bytes);
+            continue;
         }
-        if (plan.bm == 16) {
-            if (own) few_of<true>(st, p, plan.waves, blocks, (size_t)p.rows * p.kb * 256);
-            else few_of<false>(st, p, plan.waves, blocks, 0);
+        const long long each = 4 * kRowsAhead, rows_blocks = ((long long)(p.rows + 3) / 4 * p.kb + each - 1) / each;
+        hipLaunchKernelGGL(k_fp8_rows, dim3((unsigned)rows_blocks), dim3(256), 0, st, p);
+        if (plan.bn == 16) {
+            if (plan.bm == 16) few_of<8, false, 1>(st, p, 0);
+            else if (plan.bm == 32) few_of<8, false, 2>(st, p, 0);
+            else few_of<8, false, 4>(st, p, 0);
             continue;
         }
         if (plan.bm == 256) tiles_of<256, 256, 4, 2>(st, p, plan);

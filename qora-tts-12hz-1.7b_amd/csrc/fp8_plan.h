@@ -67,10 +67,10 @@ inline Refusal check_fp8_quantize(const float *src, int32_t ld_src, const qtts_f
 // first `whole` have a block each; the blocks of 128 of the contraction of the others
 // are divided over `splits` blocks, `each` of them each.
 struct Fp8Plan {
-    int bn, bm;  // bm == 16: the kernel for up to 16 rows
+    int bn, bm;  // bn == 16: the kernel for up to 64 rows, all of them in a block
     int tiles_n, tiles_m, whole, splits, each;
     long long ns;  // what it is taken to cost
-    int waves;     // of a block, for a few rows
+    int waves;     // of a block of that kernel
 };
 inline long long fp8_launched(const Fp8Plan &p) {
     return p.whole + ((long long)p.tiles_n * p.tiles_m - p.whole) * p.splits;
@@ -83,7 +83,7 @@ struct Fp8Tile {
 };
 constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 520}, {64, 64, 330, 210}};
 
-// Whether the kernel for up to 16 rows brings them to 8 bits itself, in each block anew.
+// Whether the kernel for few rows brings them to 8 bits itself, in each block anew.
 inline bool fp8_own_rows(int rows, int kb) { return rows <= kFewRows && rows * kb <= kFewItems; }
 
 inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
@@ -104,15 +104,26 @@ inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
 // 24.3*, 26.1; 1064 rows of it 54, 34, 33, 29*, 30; 2112 rows 58, 57, 51, 44*, 50;
 // 4096 rows 63.9*, 66.1, 83.6; 2100 x 6144 -> 2048 132, 85, 82, 62*, 72; 8192 x 2048 ->
 // 12288 362*, 410, -.  128 x 6144 -> 2048 in 64: 14 in four parts, 37 in one.
+//
+// To 64 rows also the kernel for few: rows of 2048 -> 4096, 32 4.9 us and 64 7.0 (tiles
+// 8.4 and 9.2); 6144 -> 2048 16 8.3* (8.7), 32 11.9 (10.2*), 64 17.9 (10.5*); 2048 ->
+// 30000 16 20 (16*).
 inline Fp8Plan fp8_plan(int rows, int n, int k) {
     const int kb = fp8_blocks(k);
-    if (rows <= 16) {
-        // waves enough to fill the card with a few tiles, but a block of 128 for each
-        Fp8Plan p = fp8_divided(rows, n, k, 16, 16, 1);
-        p.waves = p.tiles_n >= 512 || kb <= 4 ? 4 : p.tiles_n >= 256 || kb <= 8 ? 8 : 16;
-        return p;
-    }
     Fp8Plan best{};
+    if (rows <= 64) {
+        const int side = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+        best = fp8_divided(rows, n, k, 16, side, 1);
+        best.waves = 8;
+        if (fp8_own_rows(rows, kb)) {
+            // waves enough to fill the card with a few tiles, but a block of 128 for each
+            best.waves = best.tiles_n >= 512 || kb <= 4 ? 4 : best.tiles_n >= 256 || kb <= 8 ? 8 : 16;
+            return best;
+        }
+        // a CU's blocks' reads of x in bfloat16 and of codes, and the weight from memory
+        const long long reads = 16LL * k * (2 * side / 16 + 1), blocks = best.tiles_n > 256 ? best.tiles_n : 256;
+        best.ns = 2400 + (long long)n * k / 10000 + blocks * reads / 256 * 33 / 2000;
+    }
     for (const Fp8Tile &t : kFp8Tiles)
         for (int splits = 1; splits <= kFp8MaxSplits && splits <= kb; splits++) {
             Fp8Plan p = fp8_divided(rows, n, k, t.bn, t.bm, splits);

@@ -111,9 +111,10 @@ def test_plans(lib):
                 assert 0 <= whole <= tn * tm and whole % 256 == 0
                 if splits > 1:
                     assert whole < tn * tm and (tn * tm - whole) * splits * bn * bm <= part
-                if bm == 16:  # the kernel for up to 16 rows: its LDS
-                    assert splits == 1 and rows <= 16 and waves in (4, 8, 16)
-                    assert waves * 1024 + (rows * kb * 256 if lib.own(rows, kb) else 0) <= 160 * 1024
+                if bn == 16:  # the kernel for few rows: all in a block, its LDS
+                    own = lib.own(rows, kb)
+                    assert splits == 1 and tm == 1 and bm in (16, 32, 64) and waves in ((4, 8, 16) if own else (8,))
+                    assert waves * bm // 16 * 1024 + (rows * kb * 256 if own else 0) <= 160 * 1024
 
 
 def test_oracle_rounds_to_the_nearest():

@@ -97,6 +97,15 @@ def test_large(ctx, rows, n, k):
     _check(_gemm(ctx, w, x, add=add), x, w, add)
 
 
+@pytest.mark.parametrize("rows", [5, 16, 17, 31, 32, 33, 49, 64, 65])
+@pytest.mark.parametrize("n,k", [(4090, 1552), (30, 8208), (9001, 272), (300, 16)])
+def test_few_rows(ctx, rows, n, k):
+    """The kernel for them and tiles of 64, on either side of where one gives way to
+    the other."""
+    w, x, add = _weight(1, n, k), _rows(2, rows, k), _rows(3, rows, n)
+    _check(_gemm(ctx, w, x, add=add), x, w, add)
+
+
 @pytest.mark.parametrize("rows,n,k", [(646, 5378, 1040), (1051, 2047, 6144), (3337, 4740, 528)])
 def test_the_last_round_divided(ctx, rows, n, k):
     """Tiles of 128, 64 and 256 of which 256 or 512 have a block each and the others
