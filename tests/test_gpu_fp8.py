@@ -114,7 +114,7 @@ def test_the_last_round_divided(ctx, rows, n, k):
     _check(_gemm(ctx, w, x, add=add), x, w, add)
 
 
-@pytest.mark.parametrize("rows", [5, 40])
+@pytest.mark.parametrize("rows", [5, 40, 130])
 def test_residual_in_place(ctx, rows):
     w, x, add = _weight(4, 260, 384), _rows(5, rows, 384), _rows(6, rows, 260)
     dx, y = _up(x), _up(add)
@@ -139,7 +139,7 @@ def _edges():
     return np.stack(rows).astype(np.float32)
 
 
-@pytest.mark.parametrize("each", [7, 64])
+@pytest.mark.parametrize("each", [7, 64, 200])
 def test_rows_are_rounded_exactly(ctx, each):
     """Through a weight of ones on the diagonal a row comes back as its codes'
     values."""
@@ -173,7 +173,7 @@ def test_weights_are_rounded_exactly(ctx, n, k):
 
 
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
-@pytest.mark.parametrize("rows", [3, 30])
+@pytest.mark.parametrize("rows", [3, 30, 90])
 def test_not_finite(ctx, rows, bad):
     """A row with an Inf or NaN is NaN, the others are not; a weight's code or
     scale makes its outputs NaN; a block of a weight that is not finite has
@@ -300,15 +300,16 @@ def test_no_rows(ctx):
     ctx.fp8_gemm_device(w.w, 0, 64, 0, 0, 32)
 
 
-def test_graph_and_own_stream(ctx):
+@pytest.mark.parametrize("rows", [40, 290])
+def test_graph_and_own_stream(ctx, rows):
     """Captured and replayed on other values, between plain calls that use the
     scratch for other sizes."""
     w, big = _weight(11, 640, 2048), _weight(12, 200, 1024)
-    xs = [_rows(20 + i, 40, 2048) for i in range(3)]
-    x, y = _up(xs[0]), torch.zeros((40, 640), device="cuda")
+    xs = [_rows(20 + i, rows, 2048) for i in range(3)]
+    x, y = _up(xs[0]), torch.zeros((rows, 640), device="cuda")
     bx, by = _up(_rows(30, 300, 1024)), torch.zeros((300, 200), device="cuda")
     stream = torch.cuda.ExternalStream(ctx.stream)
-    call = lambda: ctx.fp8_gemm_device(w.w, x.data_ptr(), 2048, 40, y.data_ptr(), 640)
+    call = lambda: ctx.fp8_gemm_device(w.w, x.data_ptr(), 2048, rows, y.data_ptr(), 640)
     torch.cuda.synchronize()
     alone = []
     for a in xs:
