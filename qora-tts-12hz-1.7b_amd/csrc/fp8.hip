@@ -430,17 +430,17 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
 }
 
 // Up to 64 rows: 16 weight rows a block, whose blocks of 128 its W waves take in turn,
-// straight from memory to registers; RF times 16 rows of x.  OWN: of up to kFewRows rows
-// the block meanwhile brings x to 8 bits itself, into LDS; more come from scratch, which
-// k_fp8_rows has filled.  Bound by a chain of latencies, by reading the weight, and by
-// reading x from L2 in every block (60 GB/s a CU): one row, 2048 to 12288, 25 MB in 7.2
-// us (3.5 TB/s); 16 rows, 6144 to 2048 8.5 us, 2048 to 4096 4.2, 32 of these 5.3, 64 7.5
-// (in tiles of 64 and joined 8.7 to 9.5).  With 32 weight rows a block, half of x's reads
-// and half of the blocks: 5.6, 7.0 and 9.5.
+// straight from memory to registers; RF times 16 rows of x.  OWN: the block meanwhile
+// brings x to 8 bits itself, into LDS (fp8_own_rows); otherwise it comes from scratch,
+// which k_fp8_rows has filled.  Bound by a chain of latencies, by reading the weight, and
+// by reading x from L2 in every block (60 GB/s a CU): one row, 2048 to 12288, 25 MB in
+// 7.2 us (3.5 TB/s); 16 rows, 6144 to 2048 8.5 us, 2048 to 4096 4.2, 32 of these 5.3, 64
+// 7.5 (in tiles of 64 and joined 8.7 to 9.5).  With 32 weight rows a block, half of x's
+// reads and half of the blocks: 5.6, 7.0 and 9.5.
 template <int W, bool OWN, int RF>
 __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few(Fp8Params A) {
     constexpr int kAhead = 4 / RF;  // blocks of 128 asked for at once
-    extern __shared__ __align__(16) uint8_t lds[];  // sums of the waves, then x, [row][128s][half of 64][piece]
+    extern __shared__ __align__(16) uint8_t lds[];  // sums of the waves, then x as in scratch, `side` rows a piece
     f32x4 *so = reinterpret_cast<f32x4 *>(lds);
     uint8_t *xs = lds + W * RF * 1024;
     const int lane = threadIdx.x & 63, r = lane & 15, G = lane >> 4;
@@ -450,7 +450,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
     i32x4 w[kAhead][2];
     bf16x8 xv[OWN ? 1 : kAhead][RF][4];
     float scale[kAhead];
-    const uint8_t *xr = OWN ? xs + min(r, A.rows - 1) * A.kb * 256 + 16 * G : A.xc + r * 64 + 16 * (place_of(G) ^ (r >> 2));
+    const int side = OWN && A.rows <= kFewRows ? A.rows : 16, mine = min(r, side - 1);
+    const uint8_t *xr = (OWN ? xs : A.xc) + mine * 64 + 16 * (place_of(G) ^ (mine >> 2));
     auto ask = [&](int b0) {
 #pragma unroll
         for (int a = 0; a < kAhead; a++) {
@@ -472,22 +473,23 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
     };
     ask(wave);
     const int items = OWN ? A.rows * A.kb : 0;  // 16 lanes a row's block of 128
-    for (int i0 = threadIdx.x >> 4; i0 < items; i0 += 8 * W) {
-        f32x4 x[2][2];
+    for (int i0 = threadIdx.x >> 4; i0 < items; i0 += 16 * W) {
+        f32x4 x[4][2];
         const int l = threadIdx.x & 15;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) {
             const int it = min(i0 + 4 * W * i, items - 1), col = it % A.kb * kFp8Block + 8 * l;
             const float *from = A.x + (size_t)(it / A.kb) * A.ld_x + (col < A.w.k ? col : 0);
             x[i][0] = load4(from), x[i][1] = load4(from + 4);
             if (col >= A.w.k) x[i][0] = x[i][1] = f32x4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int it = i0 + 4 * W * i;
+        for (int i = 0; i < 4; i++) {
+            const int it = i0 + 4 * W * i, row = it / A.kb, b = it % A.kb, in = row & 15;
             const u32x4 v = block_values(x[i][0], x[i][1]);
+            const int piece = ((row >> 4) * A.kb + b) * 4 + 2 * (l >> 3) + (l & 1);
             if (it < items)
-                *reinterpret_cast<u32x4 *>(xs + it * 256 + (l >> 3) * 128 + (l & 1) * 64 + (l >> 1 & 3) * 16) = v;
+                *reinterpret_cast<u32x4 *>(xs + (piece * side + in) * 64 + 16 * (place_of(l >> 1 & 3) ^ (in >> 2))) = v;
         }
     }
     if (OWN) __syncthreads();
@@ -508,7 +510,10 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
                 const bf16x8 v = values8(c[2 * (q & 1)] & mask, c[2 * (q & 1) + 1] & mask, s.power);
 #pragma unroll
                 for (int f = 0; f < RF; f++)
-                    p[f] = mma(v, OWN ? *reinterpret_cast<const bf16x8 *>(xr + b * 256 + q * 64) : xv[OWN ? 0 : a][f][q], p[f]);
+                    {
+                    const uint8_t *at = xr + ((f * A.kb + b) * 4 + q) * side * 64;
+                    p[f] = mma(v, OWN ? *reinterpret_cast<const bf16x8 *>(at) : xv[OWN ? 0 : a][f][q], p[f]);
+                }
             }
 #pragma unroll
             for (int f = 0; f < RF; f++)
@@ -556,11 +561,10 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
         p.whole = plan.whole;
         p.splits = plan.splits;
         p.each = plan.each;
-        if (fp8_own_rows(p.rows, p.kb)) {
-            const size_t x_bytes = (size_t)p.rows * p.kb * 256;
+        if (fp8_own_rows(p.rows, p.w.n, p.kb)) {
+            const size_t x_bytes = (size_t)fp8_own_bytes(p.rows, p.kb);
             if (plan.waves == 4) few_of<4, true, 1>(st, p, x_bytes);
-            else if (plan.waves == 8) few_of<8, true, 1>(st, p, x_bytes);
-            else few_of<16, true, 1>(st, p, x_bytes);
+            else few_of<8, true, 1>(st, p, x_bytes);
             continue;
         }
         const long long each = 4 * kRowsAhead, rows_blocks = ((long long)(p.rows + 3) / 4 * p.kb + each - 1) / each;

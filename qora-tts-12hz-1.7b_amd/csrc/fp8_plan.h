@@ -19,8 +19,7 @@ constexpr size_t kFp8ScratchBytes = (size_t)128 << 20;  // a context's: rows, in
 constexpr int kFp8RowStep = 256;                  // rows that a tile takes at most
 constexpr int kFp8MaxSplits = 16;                 // parts of a sum
 constexpr long long kFp8PartFloats = 4LL << 20;   // all parts' sums
-constexpr int kFewRows = 4;                       // that each block brings to 8 bits itself,
-constexpr int kFewItems = 256;                    // with so many blocks of 128: 64 KB of LDS
+constexpr int kFewRows = 4;                       // that a block may hold by themselves, not 16 at once
 
 inline int fp8_blocks(int k) { return (k + kFp8Block - 1) / kFp8Block; }
 
@@ -83,8 +82,16 @@ struct Fp8Tile {
 };
 constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 520}, {64, 64, 330, 210}};
 
-// Whether the kernel for few rows brings them to 8 bits itself, in each block anew.
-inline bool fp8_own_rows(int rows, int kb) { return rows <= kFewRows && rows * kb <= kFewItems; }
+// Whether the kernel for few rows brings them to 8 bits itself, in each block anew, for a
+// launch less: up to four rows while they fit 64 KB of LDS, up to 16 while a CU's blocks
+// have no more than 128 times 128 values to bring over (us so and with a launch for it:
+// 8 rows of 2048 -> 4096 6.7 and 6.8, 8 of 1024 -> 8000 6.2 and 7.0, but 16 of these 8.3
+// and 6.7, 8 of 2048 -> 12288 12.4 and 10.1; one of 6144 -> 2048 7.9 and 10.1).
+inline bool fp8_own_rows(int rows, int n, int kb) {
+    const long long items = (long long)rows * kb;
+    return rows <= kFewRows ? items <= 256 : rows <= 16 && items * ((n + 4095) / 4096) <= 128;
+}
+inline long long fp8_own_bytes(int rows, int kb) { return (rows <= kFewRows ? rows : 16LL) * kb * 256; }
 
 inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
     const int kb = fp8_blocks(k);
@@ -115,9 +122,10 @@ inline Fp8Plan fp8_plan(int rows, int n, int k) {
         const int side = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
         best = fp8_divided(rows, n, k, 16, side, 1);
         best.waves = 8;
-        if (fp8_own_rows(rows, kb)) {
-            // waves enough to fill the card with a few tiles, but a block of 128 for each
-            best.waves = best.tiles_n >= 512 || kb <= 4 ? 4 : best.tiles_n >= 256 || kb <= 8 ? 8 : 16;
+        if (fp8_own_rows(rows, n, kb)) {
+            // more waves for a long row where they do not stand in another block's way (one
+            // row of 6144 -> 2048 7.9 us, 8.5 with four; -> 12288 20.7 and 17.5)
+            best.waves = best.tiles_n > 256 || kb <= 16 ? 4 : 8;
             return best;
         }
         // a CU's blocks' reads of x in bfloat16 and of codes, and the weight from memory

@@ -22,7 +22,7 @@ extern "C" int gemm(const qtts_fp8_weight *w, const float *x, int ld_x, int rows
     return told(check_fp8_gemm(*w, x, ld_x, rows, add, ld_add, y, ld_y));
 }
 extern "C" int quantize(const float *src, int ld, const qtts_fp8_weight *w) { return told(check_fp8_quantize(src, ld, *w)); }
-extern "C" int own(int rows, int kb) { return fp8_own_rows(rows, kb); }
+extern "C" int own(int rows, int n, int kb) { return fp8_own_rows(rows, n, kb) ? (int)fp8_own_bytes(rows, kb) : 0; }
 extern "C" void plan(int rows, int n, int k, long long *o) {
     const Fp8Plan p = fp8_plan(rows, n, k);
     o[0] = p.bn; o[1] = p.bm; o[2] = p.tiles_n; o[3] = p.tiles_m; o[4] = p.splits;
@@ -111,10 +111,11 @@ def test_plans(lib):
                 assert 0 <= whole <= tn * tm and whole % 256 == 0
                 if splits > 1:
                     assert whole < tn * tm and (tn * tm - whole) * splits * bn * bm <= part
+                own = lib.own(rows, n, kb)
+                assert not own or bn == 16
                 if bn == 16:  # the kernel for few rows: all in a block, its LDS
-                    own = lib.own(rows, kb)
-                    assert splits == 1 and tm == 1 and bm in (16, 32, 64) and waves in ((4, 8, 16) if own else (8,))
-                    assert waves * bm // 16 * 1024 + (rows * kb * 256 if own else 0) <= 160 * 1024
+                    assert splits == 1 and tm == 1 and bm in (16, 32, 64) and waves in ((4, 8) if own else (8,))
+                    assert waves * bm // 16 * 1024 + own <= 160 * 1024
 
 
 def test_oracle_rounds_to_the_nearest():

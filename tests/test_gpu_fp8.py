@@ -97,8 +97,8 @@ def test_large(ctx, rows, n, k):
     _check(_gemm(ctx, w, x, add=add), x, w, add)
 
 
-@pytest.mark.parametrize("rows", [5, 16, 17, 31, 32, 33, 49, 64, 65])
-@pytest.mark.parametrize("n,k", [(4090, 1552), (30, 8208), (9001, 272), (300, 16)])
+@pytest.mark.parametrize("rows", [2, 5, 9, 16, 17, 31, 32, 33, 49, 64, 65])
+@pytest.mark.parametrize("n,k", [(4090, 1552), (30, 8208), (9001, 272), (300, 16), (260, 3184)])
 def test_few_rows(ctx, rows, n, k):
     """The kernel for them and tiles of 64, on either side of where one gives way to
     the other."""
