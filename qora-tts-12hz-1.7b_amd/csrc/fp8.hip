@@ -429,14 +429,14 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
     put(A, row, n, v);
 }
 
-// Up to 64 rows: 16 weight rows a block, whose blocks of 128 its W waves take in turn,
-// straight from memory to registers; RF times 16 rows of x.  OWN: the block meanwhile
+// Without tiles: 16 weight rows by RF times 16 of x a block, whose blocks of 128 its W
+// waves take in turn, straight from memory to registers.  OWN: the block meanwhile
 // brings x to 8 bits itself, into LDS (fp8_own_rows); otherwise it comes from scratch,
-// which k_fp8_rows has filled.  Bound by a chain of latencies, by reading the weight, and
-// by reading x from L2 in every block (60 GB/s a CU): one row, 2048 to 12288, 25 MB in
-// 7.2 us (3.5 TB/s); 16 rows, 6144 to 2048 8.5 us, 2048 to 4096 4.2, 32 of these 5.3, 64
-// 7.5 (in tiles of 64 and joined 8.7 to 9.5).  With 32 weight rows a block, half of x's
-// reads and half of the blocks: 5.6, 7.0 and 9.5.
+// which k_fp8_rows has filled.  Bound by a chain of latencies and by what every block
+// reads of the weight and of x from L2 (75 GB/s a CU): one row, 2048 to 12288, 25 MB in
+// 7.2 us (3.5 TB/s); 16 rows, 6144 to 2048 7.4 us, 2048 to 4096 3.8, 32 of these 4.9, 64
+// 7.0.  With 32 weight rows a block, half of x's reads and half of the blocks: 5.2, 6.7
+// and 9.0.
 template <int W, bool OWN, int RF>
 __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few(Fp8Params A) {
     constexpr int kAhead = 4 / RF;  // blocks of 128 asked for at once
@@ -444,14 +444,15 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
     f32x4 *so = reinterpret_cast<f32x4 *>(lds);
     uint8_t *xs = lds + W * RF * 1024;
     const int lane = threadIdx.x & 63, r = lane & 15, G = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x % A.tiles_n * 16, group = blockIdx.x / A.tiles_n;
     const uint8_t *wr = A.w.codes + (size_t)min(n0 + r, A.w.n - 1) * A.w.ld;
     const KCONST float *ws = (const KCONST float *)(A.w.scales + (size_t)(n0 / kFp8Block) * A.kb);
     i32x4 w[kAhead][2];
     bf16x8 xv[OWN ? 1 : kAhead][RF][4];
     float scale[kAhead];
     const int side = OWN && A.rows <= kFewRows ? A.rows : 16, mine = min(r, side - 1);
-    const uint8_t *xr = (OWN ? xs : A.xc) + mine * 64 + 16 * (place_of(G) ^ (mine >> 2));
+    const uint8_t *xr = (OWN ? xs : A.xc + (size_t)group * RF * A.kb * 4096) + mine * 64 + 16 * (place_of(G) ^ (mine >> 2));
     auto ask = [&](int b0) {
 #pragma unroll
         for (int a = 0; a < kAhead; a++) {
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int at = b * 128 + 64 * h + 16 * G;  // behind k any codes: x has zeros there
-                w[a][h] = __builtin_nontemporal_load(glb(reinterpret_cast<const i32x4 *>(wr + (at < A.w.k ? at : 0))));
+                w[a][h] = *glb(reinterpret_cast<const i32x4 *>(wr + (at < A.w.k ? at : 0)));
             }
             scale[a] = ws[b];
             if (!OWN)
@@ -528,13 +529,14 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
     f32x4 sum = so[wave * W * 64 + lane];
 #pragma unroll
     for (int k = 1; k < W; k++) sum += so[(wave * W + k) * 64 + lane];
-    const int n = n0 + 4 * G, row = 16 * wave + r;
+    const int n = n0 + 4 * G, row = 16 * (group * RF + wave) + r;
     if (row < A.rows && n < A.w.n) put(A, row, n, sum);
 }
 
 template <int W, bool OWN, int RF>
 void few_of(hipStream_t st, const Fp8Params &p, size_t x_bytes) {
-    hipLaunchKernelGGL((k_fp8_few<W, OWN, RF>), dim3((unsigned)p.tiles_n), dim3(64 * W), W * RF * 1024 + x_bytes, st, p);
+    const unsigned blocks = (unsigned)p.tiles_n * (unsigned)((p.rows + 16 * RF - 1) / (16 * RF));
+    hipLaunchKernelGGL((k_fp8_few<W, OWN, RF>), dim3(blocks), dim3(64 * W), W * RF * 1024 + x_bytes, st, p);
 }
 
 template <int BN, int BM, int WN, int WM>

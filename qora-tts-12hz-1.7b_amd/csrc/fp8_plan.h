@@ -66,7 +66,7 @@ inline Refusal check_fp8_quantize(const float *src, int32_t ld_src, const qtts_f
 // first `whole` have a block each; the blocks of 128 of the contraction of the others
 // are divided over `splits` blocks, `each` of them each.
 struct Fp8Plan {
-    int bn, bm;  // bn == 16: the kernel for up to 64 rows, all of them in a block
+    int bn, bm;  // bn == 16: the kernel without tiles in LDS, 16, 32 or 64 rows a block
     int tiles_n, tiles_m, whole, splits, each;
     long long ns;  // what it is taken to cost
     int waves;     // of a block of that kernel
@@ -80,9 +80,9 @@ inline long long fp8_launched(const Fp8Plan &p) {
 struct Fp8Tile {
     int bn, bm, alone, full;
 };
-constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 520}, {64, 64, 330, 210}};
+constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 520}, {64, 64, 310, 205}};
 
-// Whether the kernel for few rows brings them to 8 bits itself, in each block anew, for a
+// Whether that kernel brings few rows to 8 bits itself, in each block anew, for a
 // launch less: up to four rows while they fit 64 KB of LDS, up to 16 while a CU's blocks
 // have no more than 128 times 128 values to bring over (us so and with a launch for it:
 // 8 rows of 2048 -> 4096 6.7 and 6.8, 8 of 1024 -> 8000 6.2 and 7.0, but 16 of these 8.3
@@ -103,8 +103,8 @@ inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
 }
 
 // The tile and division that are taken to cost least: no tile divided, all of them, or
-// those past the last whole round of 256.  A block's start costs some 2 us; the fullest
-// CU works off its blocks; joining costs a launch and the parts' way to memory and back.
+// those past the last whole round of 256.  A block's start and end cost some 3 us;
+// the fullest CU works off its blocks; joining costs a launch and the parts' way to memory and back.
 // Against all that can be chosen, 1 % more over 26 shapes (17 to 8192 rows), 8 % at
 // worst.  us, the chosen one with a star, tiles of 256, 128 and 64 whole and the last
 // round divided in 128 and in 64: 512 x 1552 -> 1001 22, 13, 9.9*; 900 x 2048 -> 4096 57,
@@ -112,25 +112,27 @@ inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
 // 4096 rows 63.9*, 66.1, 83.6; 2100 x 6144 -> 2048 132, 85, 82, 62*, 72; 8192 x 2048 ->
 // 12288 362*, 410, -.  128 x 6144 -> 2048 in 64: 14 in four parts, 37 in one.
 //
-// To 64 rows also the kernel for few: rows of 2048 -> 4096, 32 4.9 us and 64 7.0 (tiles
-// 8.4 and 9.2); 6144 -> 2048 16 8.3* (8.7), 32 11.9 (10.2*), 64 17.9 (10.5*); 2048 ->
-// 30000 16 20 (16*).
+// Where the reads that every block repeats cost less, the kernel without tiles, in as
+// many rows a block as cost least: 32 rows of 2048 -> 4096 4.9 us (in tiles 8.4), 64 7.0
+// (9.2); 128 of 2048 -> 2048 6.7 (9.2); 333 of 1552 -> 1001 7.8 (10.1); 230 of 3248 -> 150
+// 3.9 (7.7); but 200 of 6144 -> 2048 29 (17*).  Over 110 drawn shapes 4 % more than
+// the best of all that can be chosen.
 inline Fp8Plan fp8_plan(int rows, int n, int k) {
     const int kb = fp8_blocks(k);
     Fp8Plan best{};
-    if (rows <= 64) {
-        const int side = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-        best = fp8_divided(rows, n, k, 16, side, 1);
-        best.waves = 8;
+    for (int side = 16; side <= 64; side *= 2) {
+        Fp8Plan p = fp8_divided(rows, n, k, 16, side, 1);
+        p.waves = 8;
         if (fp8_own_rows(rows, n, kb)) {
             // more waves for a long row where they do not stand in another block's way (one
             // row of 6144 -> 2048 7.9 us, 8.5 with four; -> 12288 20.7 and 17.5)
-            best.waves = best.tiles_n > 256 || kb <= 16 ? 4 : 8;
-            return best;
+            p.waves = p.tiles_n > 256 || kb <= 16 ? 4 : 8;
+            return p;
         }
-        // a CU's blocks' reads of x in bfloat16 and of codes, and the weight from memory
-        const long long reads = 16LL * k * (2 * side / 16 + 1), blocks = best.tiles_n > 256 ? best.tiles_n : 256;
-        best.ns = 2400 + (long long)n * k / 10000 + blocks * reads / 256 * 33 / 2000;
+        // what a block reads of x in bfloat16 and of codes
+        const long long reads = 16LL * k * (2 * side / 16 + 1), blocks = (long long)p.tiles_n * p.tiles_m;
+        p.ns = 2200 + (blocks + 255) / 256 * (200 + reads * 13 / 1000);
+        if (blocks <= (1 << 22) && (best.bn == 0 || p.ns < best.ns)) best = p;
     }
     for (const Fp8Tile &t : kFp8Tiles)
         for (int splits = 1; splits <= kFp8MaxSplits && splits <= kb; splits++) {
@@ -146,7 +148,7 @@ inline Fp8Plan fp8_plan(int rows, int n, int k) {
                 long long work = most * step * t.full;
                 if (round) work = round * all * t.full + (most == 1 ? step * t.alone : work);
                 const long long alone = (round ? all : step) * t.alone;
-                p.ns = 2000 + (work > alone ? work : alone);
+                p.ns = 3000 + (work > alone ? work : alone);
                 // (the last tiles' rows may be few)
                 const long long low = rest < p.tiles_n ? rest : p.tiles_n, few = (long long)p.tiles_m * t.bm - rows;
                 if (splits > 1) p.ns += 3500 + (floats - low * few * splits * t.bn) * 8 / 4000;

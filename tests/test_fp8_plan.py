@@ -113,8 +113,9 @@ def test_plans(lib):
                     assert whole < tn * tm and (tn * tm - whole) * splits * bn * bm <= part
                 own = lib.own(rows, n, kb)
                 assert not own or bn == 16
-                if bn == 16:  # the kernel for few rows: all in a block, its LDS
-                    assert splits == 1 and tm == 1 and bm in (16, 32, 64) and waves in ((4, 8) if own else (8,))
+                if bn == 16:  # the kernel without tiles: its LDS
+                    assert splits == 1 and bm in (16, 32, 64) and waves in ((4, 8) if own else (8,))
+                    assert not own or (bm == 16 and tm == 1)
                     assert waves * bm // 16 * 1024 + own <= 160 * 1024
 
 

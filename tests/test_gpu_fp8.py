@@ -106,6 +106,16 @@ def test_few_rows(ctx, rows, n, k):
     _check(_gemm(ctx, w, x, add=add), x, w, add)
 
 
+@pytest.mark.parametrize("rows,n,k", [(258, 5737, 16), (321, 5471, 16), (2694, 4369, 16), (400, 6001, 144),
+                                      (300, 5737, 272), (2694, 4369, 272), (69, 5737, 1040), (321, 5452, 784),
+                                      (72, 5733, 2064), (69, 3267, 4112), (20, 4103, 6160), (132, 5452, 4112)])
+def test_tiles(ctx, rows, n, k):
+    """Tiles of 64, 128 and 256, whole and divided, cut short on every side."""
+    w = _weight(n + k, n, k, ld=-(-k // 16) * 16 + 32)
+    x, add = _rows(rows + k, rows, k), _rows(3, rows, n)
+    _check(_gemm(ctx, w, x, add=add, ld_x=k + 4, ld_y=-(-n // 4) * 4 + 4), x, w, add)
+
+
 @pytest.mark.parametrize("rows,n,k", [(646, 5378, 1040), (1051, 2047, 6144), (3337, 4740, 528)])
 def test_the_last_round_divided(ctx, rows, n, k):
     """Tiles of 128, 64 and 256 of which 256 or 512 have a block each and the others
@@ -114,12 +124,12 @@ def test_the_last_round_divided(ctx, rows, n, k):
     _check(_gemm(ctx, w, x, add=add), x, w, add)
 
 
-@pytest.mark.parametrize("rows", [5, 40, 130])
-def test_residual_in_place(ctx, rows):
-    w, x, add = _weight(4, 260, 384), _rows(5, rows, 384), _rows(6, rows, 260)
+@pytest.mark.parametrize("rows,n", [(5, 260), (40, 260), (130, 260), (300, 5500)])
+def test_residual_in_place(ctx, rows, n):
+    w, x, add = _weight(4, n, 384), _rows(5, rows, 384), _rows(6, rows, n)
     dx, y = _up(x), _up(add)
     torch.cuda.synchronize()
-    ctx.fp8_gemm_device(w.w, dx.data_ptr(), 384, rows, y.data_ptr(), 260, add=y.data_ptr(), ld_add=260)
+    ctx.fp8_gemm_device(w.w, dx.data_ptr(), 384, rows, y.data_ptr(), n, add=y.data_ptr(), ld_add=n)
     ctx.synchronize()
     _check(y.cpu().numpy(), x, w, add)
 
@@ -173,12 +183,12 @@ def test_weights_are_rounded_exactly(ctx, n, k):
 
 
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
-@pytest.mark.parametrize("rows", [3, 30, 90])
-def test_not_finite(ctx, rows, bad):
+@pytest.mark.parametrize("rows,n", [(3, 300), (30, 300), (90, 300), (300, 5737)])
+def test_not_finite(ctx, rows, n, bad):
     """A row with an Inf or NaN is NaN, the others are not; a weight's code or
     scale makes its outputs NaN; a block of a weight that is not finite has
     scale NaN."""
-    n, k = 300, 272
+    k = 272
     w, x = _weight(8, n, k), _rows(9, rows, k)
     x[1, 260] = bad
     got = _gemm(ctx, w, x)
@@ -190,12 +200,12 @@ def test_not_finite(ctx, rows, bad):
     x = np.abs(_rows(9, rows, k)) + 1
     got = _gemm(ctx, Weight(codes, scales), x)
     assert np.all(np.isnan(got[:, 17])) and not np.any(np.isfinite(got[:, 128:256]))
-    some = np.r_[0:17, 18:128, 256:300]
+    some = np.r_[0:17, 18:128, 256:n]
     ref, mass = fm.product(x, w.host[0], w.host[1])
     assert np.all(np.abs(got[:, some] - ref[:, some]) <= 200 * 2.0 ** -24 * mass[:, some])
     src = _rows(10, n, k)
     src[130, 200] = bad
-    dsrc, dc, ds = _up(src), torch.zeros((n, k), dtype=torch.uint8, device="cuda"), torch.zeros((3, 3), device="cuda")
+    dsrc, dc, ds = _up(src), torch.zeros((n, k), dtype=torch.uint8, device="cuda"), torch.zeros((-(-n // 128), 3), device="cuda")
     torch.cuda.synchronize()
     ctx.fp8_quantize_device(dsrc.data_ptr(), k, qtts.Fp8Weight(dc.data_ptr(), ds.data_ptr(), n, k, k))
     ctx.synchronize()
@@ -204,18 +214,20 @@ def test_not_finite(ctx, rows, bad):
     assert np.array_equal(dc.cpu().numpy(), codes)
 
 
-@pytest.mark.parametrize("rows", [2, 10, 40, 300])
-def test_scales_of_any_size(ctx, rows):
+@pytest.mark.parametrize("rows,times", [(2, 1), (10, 1), (40, 1), (300, 1), (128, 11), (330, 11)])
+def test_scales_of_any_size(ctx, rows, times):
     """Scales of 0 (whose codes count as 0, NaN among them), negative ones, the least
     and the largest, in any order along k and beside each other along n; x so that
     the results stay f32's."""
-    n, k = 400, 1168
+    n, k = 512 * times - 112, 1168
     codes = _weight(40, n, k).host[0].copy()
-    scales = np.array([[0.01, 0.0, -0.02, 0.0, 0.03, -0.5, 1e-3, 0.0, 0.0, 0.7],
+    scales = np.tile(np.array([[0.01, 0.0, -0.02, 0.0, 0.03, -0.5, 1e-3, 0.0, 0.0, 0.7],
                        [0.0] * 10,
                        [1e-40, 3e38, 1e-30, 2.0 ** -149, 1e20, 0.0, 1.0, -3e38, 1e-38, 2e30],
                        [2.0 ** -126, 2.0 ** -118, 2.0 ** -117, 2.0 ** 117, 2.0 ** 118, 2.0 ** 127, 1.5, 1.0, 0.75, 3.0]],
-                      np.float32)
+                      np.float32), (times, 1))
+    each = 512 * np.arange(times)[:, None]
+    columns = lambda a, b: np.sort((each + np.arange(a, b)).reshape(-1))  # of every turn of the scales
     x = _rows(41, rows, k)
     for b in range(10):  # the third and fourth row's products of one size
         x[:, b * 128:(b + 1) * 128] *= np.float32(0.2)
@@ -223,15 +235,15 @@ def test_scales_of_any_size(ctx, rows):
     x2 = x.copy()
     w = Weight(codes, scales)
     got = _gemm(ctx, w, x2)
-    assert np.array_equal(got[:, 128:256], np.zeros((rows, 128), np.float32))
+    assert not np.any(got[:, columns(128, 256)])
     clean = codes.copy()
     clean[5, 130] = clean[150, 7] = 0
     ref, mass = fm.product(x2, clean, scales)
-    fine = np.r_[0:256]
+    fine = columns(0, 256)
     off, bound = np.abs(got - ref), (128 + 10 + 66) * 2.0 ** -24 * mass + 2.0 ** -140
     assert np.all(off[:, fine] <= bound[:, fine])
     # sums of up to 3e38 * 448 * 448: f32's where the definition's are, to the same bound
-    for cols in (np.r_[256:384], np.r_[384:400]):
+    for cols in (columns(256, 384), columns(384, 400)):
         for b in range(10):
             alone = np.zeros_like(scales)
             alone[:, b] = scales[:, b]
@@ -270,20 +282,20 @@ def test_two_contexts_at_once(ctx):
     try:
         jobs = []
         for c, seed in ((ctx, 60), (other, 70)):
-            for rows, n, k in ((40, 640, 2048), (7, 500, 512), (300, 260, 1024)):
+            for rows, n, k in ((40, 640, 2048), (7, 500, 512), (300, 260, 1024), (20, 4103, 6160), (70, 5737, 1040)):
                 w, x = _weight(seed, n, k), _up(_rows(seed + 1, rows, k))
-                y = torch.zeros((rows, n), device="cuda")
+                y = torch.zeros((rows, -(-n // 4) * 4), device="cuda")
                 jobs.append((c, w, x, rows, k, n, y))
         torch.cuda.synchronize()
 
         def go():
             for c, w, x, rows, k, n, y in jobs:
-                c.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), n)
+                c.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), y.stride(0))
         go()
         torch.cuda.synchronize()
         alone = []
         for c, w, x, rows, k, n, y in jobs:
-            c.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), n)
+            c.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), y.stride(0))
             c.synchronize()
             alone.append(y.clone())
         torch.cuda.synchronize()
@@ -300,16 +312,16 @@ def test_no_rows(ctx):
     ctx.fp8_gemm_device(w.w, 0, 64, 0, 0, 32)
 
 
-@pytest.mark.parametrize("rows", [40, 290])
-def test_graph_and_own_stream(ctx, rows):
+@pytest.mark.parametrize("rows,n,k", [(40, 640, 2048), (290, 640, 2048), (20, 4104, 6160)])
+def test_graph_and_own_stream(ctx, rows, n, k):
     """Captured and replayed on other values, between plain calls that use the
     scratch for other sizes."""
-    w, big = _weight(11, 640, 2048), _weight(12, 200, 1024)
-    xs = [_rows(20 + i, rows, 2048) for i in range(3)]
-    x, y = _up(xs[0]), torch.zeros((rows, 640), device="cuda")
+    w, big = _weight(11, n, k), _weight(12, 200, 1024)
+    xs = [_rows(20 + i, rows, k) for i in range(3)]
+    x, y = _up(xs[0]), torch.zeros((rows, n), device="cuda")
     bx, by = _up(_rows(30, 300, 1024)), torch.zeros((300, 200), device="cuda")
     stream = torch.cuda.ExternalStream(ctx.stream)
-    call = lambda: ctx.fp8_gemm_device(w.w, x.data_ptr(), 2048, rows, y.data_ptr(), 640)
+    call = lambda: ctx.fp8_gemm_device(w.w, x.data_ptr(), k, rows, y.data_ptr(), n)
     torch.cuda.synchronize()
     alone = []
     for a in xs:
