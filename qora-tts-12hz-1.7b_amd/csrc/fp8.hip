@@ -434,7 +434,7 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
 // brings x to 8 bits itself, into LDS (fp8_own_rows); otherwise it comes from scratch,
 // which k_fp8_rows has filled.  Bound by a chain of latencies and by what every block
 // reads of the weight and of x from L2 (75 GB/s a CU): one row, 2048 to 12288, 25 MB in
-// 7.2 us (3.5 TB/s); 16 rows, 6144 to 2048 7.4 us, 2048 to 4096 3.8, 32 of these 4.9, 64
+// 7 to 9 us (2.8 to 3.5 TB/s); 16 rows, 6144 to 2048 7.4 us, 2048 to 4096 3.8, 32 of these 4.9, 64
 // 7.0.  With 32 weight rows a block, half of x's reads and half of the blocks: 5.2, 6.7
 // and 9.0.
 template <int W, bool OWN, int RF>
