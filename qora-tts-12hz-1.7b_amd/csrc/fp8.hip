@@ -272,7 +272,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
                ring_at + 2 * kCodes + (2 * slot + u) * kHalf + (wave * LB + i) * 1024);
     };
     auto load_codes = [&](int s, int i) {  // of the block that begins with step s
-        // behind k a row's first codes: x has zeros there
+        // behind k the block's first codes: x has zeros there
         const unsigned at = piece[i] < A.w.k - s * 64 ? piece[i] : 0;
         to_lds(codes + (size_t)s * 64, row_at[i] + at, ring_at + (s >> 1 & 1) * kCodes + (wave * LA + i) * 1024);
     };
@@ -434,9 +434,9 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
 // brings x to 8 bits itself, into LDS (fp8_own_rows); otherwise it comes from scratch,
 // which k_fp8_rows has filled.  Bound by a chain of latencies and by what every block
 // reads of the weight and of x from L2 (75 GB/s a CU): one row, 2048 to 12288, 25 MB in
-// 7 to 9 us (2.8 to 3.5 TB/s); 16 rows, 6144 to 2048 7.4 us, 2048 to 4096 3.8, 32 of these 4.9, 64
-// 7.0.  With 32 weight rows a block, half of x's reads and half of the blocks: 5.2, 6.7
-// and 9.0.
+// 7 to 9 us (2.8 to 3.5 TB/s); 16 rows, 6144 to 2048 7.4 us, 2048 to 4096 3.8, 32 of
+// these 4.9, 64 7.0.  With 32 weight rows a block, half of x's reads and half of the
+// blocks: 5.2, 6.7 and 9.0.
 template <int W, bool OWN, int RF>
 __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few(Fp8Params A) {
     constexpr int kAhead = 4 / RF;  // blocks of 128 asked for at once
@@ -459,8 +459,8 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
             const int b = min(b0 + W * a, A.kb - 1);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int at = b * 128 + 64 * h + 16 * G;  // behind k any codes: x has zeros there
-                w[a][h] = *glb(reinterpret_cast<const i32x4 *>(wr + (at < A.w.k ? at : 0)));
+                const int at = b * 128 + 64 * h + 16 * G;  // behind k the block's first codes: x has zeros there
+                w[a][h] = *glb(reinterpret_cast<const i32x4 *>(wr + (at < A.w.k ? at : b * 128)));
             }
             scale[a] = ws[b];
             if (!OWN)
@@ -510,8 +510,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
                 const i32x4 c = w[a][q >> 1];
                 const bf16x8 v = values8(c[2 * (q & 1)] & mask, c[2 * (q & 1) + 1] & mask, s.power);
 #pragma unroll
-                for (int f = 0; f < RF; f++)
-                    {
+                for (int f = 0; f < RF; f++) {
                     const uint8_t *at = xr + ((f * A.kb + b) * 4 + q) * side * 64;
                     p[f] = mma(v, OWN ? *reinterpret_cast<const bf16x8 *>(at) : xv[OWN ? 0 : a][f][q], p[f]);
                 }

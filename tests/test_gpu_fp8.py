@@ -256,6 +256,21 @@ def test_scales_of_any_size(ctx, rows, times):
             assert np.all((off <= 204 * 2.0 ** -24 * mass[:, cols] + 2.0 ** -140)[inside]), b
 
 
+@pytest.mark.parametrize("rows,n", [(1, 20), (9, 20), (60, 300), (258, 5737), (400, 6001)])
+@pytest.mark.parametrize("k", [144, 208])
+def test_nan_codes_under_a_scale_of_zero(ctx, rows, n, k):
+    """They count as 0 wherever they lie, also where a later block is cut short."""
+    codes = _weight(80, n, k).host[0].copy()
+    scales = np.full((-(-n // 128), 2), 0.5, np.float32)
+    scales[0, 0] = 0
+    codes[:16, :128:3] = 0x7f
+    x = _rows(81, rows, k)
+    clean = codes.copy()
+    clean[:16, :128] = 0
+    got, (ref, mass) = _gemm(ctx, Weight(codes, scales), x), fm.product(x, clean, scales)
+    assert np.all(np.abs(got - ref) <= (128 + 2 + 66) * 2.0 ** -24 * mass + 2.0 ** -149)
+
+
 @pytest.mark.parametrize("rows,n,k", [(4, 100, 8192), (1, 70, 32768), (3, 40, 11008), (4, 33, 8208), (16, 20, 20000)])
 def test_long_rows(ctx, rows, n, k):
     """As much of x in LDS as a few rows may have there, and one block more."""
