@@ -473,24 +473,23 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few
         }
     };
     ask(wave);
-    const int items = OWN ? A.rows * A.kb : 0;  // 16 lanes a row's block of 128
+    const int items = OWN ? min(A.rows - 16 * group, 16) * A.kb : 0;  // 16 lanes a row's block of 128
     for (int i0 = threadIdx.x >> 4; i0 < items; i0 += 16 * W) {
         f32x4 x[4][2];
         const int l = threadIdx.x & 15;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int it = min(i0 + 4 * W * i, items - 1), col = it % A.kb * kFp8Block + 8 * l;
-            const float *from = A.x + (size_t)(it / A.kb) * A.ld_x + (col < A.w.k ? col : 0);
+            const float *from = A.x + (size_t)(16 * group + it / A.kb) * A.ld_x + (col < A.w.k ? col : 0);
             x[i][0] = load4(from), x[i][1] = load4(from + 4);
             if (col >= A.w.k) x[i][0] = x[i][1] = f32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int it = i0 + 4 * W * i, row = it / A.kb, b = it % A.kb, in = row & 15;
+            const int it = i0 + 4 * W * i, row = it / A.kb, piece = it % A.kb * 4 + 2 * (l >> 3) + (l & 1);
             const u32x4 v = block_values(x[i][0], x[i][1]);
-            const int piece = ((row >> 4) * A.kb + b) * 4 + 2 * (l >> 3) + (l & 1);
             if (it < items)
-                *reinterpret_cast<u32x4 *>(xs + (piece * side + in) * 64 + 16 * (place_of(l >> 1 & 3) ^ (in >> 2))) = v;
+                *reinterpret_cast<u32x4 *>(xs + (piece * side + row) * 64 + 16 * (place_of(l >> 1 & 3) ^ (row >> 2))) = v;
         }
     }
     if (OWN) __syncthreads();

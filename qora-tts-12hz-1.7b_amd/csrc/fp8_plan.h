@@ -82,14 +82,15 @@ struct Fp8Tile {
 };
 constexpr Fp8Tile kFp8Tiles[] = {{256, 256, 1600, 1850}, {128, 128, 570, 520}, {64, 64, 310, 205}};
 
-// Whether that kernel brings few rows to 8 bits itself, in each block anew, for a
-// launch less: up to four rows while they fit 64 KB of LDS, up to 16 while a CU's blocks
-// have no more than 128 times 128 values to bring over (us so and with a launch for it:
-// 8 rows of 2048 -> 4096 6.7 and 6.8, 8 of 1024 -> 8000 6.2 and 7.0, but 16 of these 8.3
-// and 6.7, 8 of 2048 -> 12288 12.4 and 10.1; one of 6144 -> 2048 7.9 and 10.1).
+// Whether that kernel brings x to 8 bits itself, in each block anew, for a launch less: up
+// to four rows while they fit 64 KB of LDS, more while a CU's blocks of 16 rows have no
+// more than 128 times 128 values to bring over (us so and with a launch for it: 8 rows of
+// 2048 -> 4096 6.7 and 6.8, 8 of 1024 -> 8000 6.2 and 7.0, but 16 of these 8.3 and 6.7, 8
+// of 2048 -> 12288 12.4 and 10.1; one of 6144 -> 2048 7.9 and 10.1).
 inline bool fp8_own_rows(int rows, int n, int kb) {
-    const long long items = (long long)rows * kb;
-    return rows <= kFewRows ? items <= 256 : rows <= 16 && items * ((n + 4095) / 4096) <= 128;
+    if (rows <= kFewRows) return rows * kb <= 256;
+    const long long blocks = (n + 15) / 16 * ((rows + 15) / 16LL);
+    return (rows < 16 ? rows : 16) * kb * ((blocks + 255) / 256) <= 128;
 }
 inline long long fp8_own_bytes(int rows, int kb) { return (rows <= kFewRows ? rows : 16LL) * kb * 256; }
 

@@ -115,7 +115,7 @@ def test_plans(lib):
                 assert not own or bn == 16
                 if bn == 16:  # the kernel without tiles: its LDS
                     assert splits == 1 and bm in (16, 32, 64) and waves in ((4, 8) if own else (8,))
-                    assert not own or (bm == 16 and tm == 1)
+                    assert not own or bm == 16
                     assert waves * bm // 16 * 1024 + own <= 160 * 1024
 
 
