@@ -3012,7 +3012,8 @@ qtts_status qtts_paged_remap_device(qtts_ctx *c, const qtts_paged_pool *pool, co
     QTTS_CHECK(c, check_remap(*pool, d_source, d_tokens, window, sinks, d_copied));
     if (pool->batch == 0) return QTTS_OK;
     DeviceGuard guard(c->device);
-    launch_paged_remap(c->stream, {*pool, d_source, d_tokens, window, sinks, d_copied, (int32_t *)c->attn_part});
+    launch_paged_remap(c->stream, {*pool, d_source, d_tokens, window, sinks, d_copied, (int32_t *)c->attn_part,
+                                   c->paged_counters});
     return check_launch(c, "k_paged_remap");
 }
 

@@ -127,8 +127,8 @@ __device__ __forceinline__ void remapped(const RemapParams &A, int first, int (&
 }
 
 // Tables of up to kRemapThreads * kRemapEach entries: block 0 reads them all, then
-// writes; block 1 hands on the slots.  8 rows of 18: 4 us.  64 of 127 13 us, most of it
-// one CU's atomics: 4.1 + 2.3 us in many blocks and two launches.
+// writes; block 1 hands on the slots.  8 rows of 18: 3.5 us.  64 of 127 13 us, most of it
+// one CU's atomics.
 __global__ __launch_bounds__(kThreads) void k_paged_remap_one(RemapParams A) {
     __shared__ Slots S;
     if (blockIdx.x == 1) return hand_on_slots(A, S);
@@ -144,14 +144,38 @@ __global__ __launch_bounds__(kThreads) void k_paged_remap_one(RemapParams A) {
     }
 }
 
-// Larger ones: new rows to scratch, block 0 the slots; then scratch to the table.
+// Larger ones: new rows to scratch, block 0 the slots; then scratch to the table: up to
+// kRemapStored entries by the block that ends last (64 of 127 4.8 to 5.9 us), more in a launch
+// of their own (4.1 + 2.3 us).
+template <bool LAST>
 __global__ __launch_bounds__(kThreads) void k_paged_remap(RemapParams A) {
     __shared__ Slots S;
+    __shared__ bool last;
     if (blockIdx.x == 0) return hand_on_slots(A, S);
-    const int i = (blockIdx.x - 1) * kThreads + threadIdx.x;
+    const int n = A.pool.batch * A.pool.max_pages, i = (blockIdx.x - 1) * kThreads + threadIdx.x;
     int now[1];
     remapped(A, i, now);
-    if (i < A.pool.batch * A.pool.max_pages) A.scratch[i] = now[0];
+    if (!LAST) {
+        if (i < n) A.scratch[i] = now[0];
+        return;
+    }
+    if (i < n) st_dev_i32(A.scratch + i, now[0]);
+    wait_stores();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = arrive_dev(A.counter) == gridDim.x - 2;
+        if (last) reset_dev(A.counter);
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int j = threadIdx.x; j < n; j += 8 * kThreads) {
+        int x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = ld_dev_i32(A.scratch + min(j + k * kThreads, n - 1));
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (j + k * kThreads < n) A.pool.page_table[j + k * kThreads] = x[k];
+    }
 }
 
 __global__ __launch_bounds__(256) void k_paged_remap_store(RemapParams A) {
@@ -392,7 +416,12 @@ void launch_paged_remap(hipStream_t st, const RemapParams &p) {
         hipLaunchKernelGGL(k_paged_remap_one, dim3(2), dim3(kThreads), 0, st, p);
         return;
     }
-    hipLaunchKernelGGL(k_paged_remap, dim3(1 + (unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, p);
+    const unsigned blocks = 1 + (unsigned)((n + kThreads - 1) / kThreads);
+    if (n <= kRemapStored) {
+        hipLaunchKernelGGL(k_paged_remap<true>, dim3(blocks), dim3(kThreads), 0, st, p);
+        return;
+    }
+    hipLaunchKernelGGL(k_paged_remap<false>, dim3(blocks), dim3(kThreads), 0, st, p);
     hipLaunchKernelGGL(k_paged_remap_store, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);
 }
 

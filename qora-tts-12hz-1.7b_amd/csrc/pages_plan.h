@@ -14,9 +14,11 @@ namespace qtts {
 constexpr int kPoolBatch = 8192;                    // rows whose slots one block hands on through LDS
 constexpr long long kPoolEntries = 4LL << 20;       // of a page table: its copy lies in scratch
 constexpr int kPoolPages = (4 << 20) - 64;          // names of pages, and their number, in scratch
-// Entries that one block remaps in its registers, in 3.5 us; more go through scratch in
-// two launches, which take 6.5 (one block 9 to 13 for 8128).
+// Entries that one block remaps in its registers, in 3.5 us; more go through scratch
+// (8128 in 4.8 to 5.9 us, one block 9 to 13), from there to the table by one block or, above
+// kRemapStored, in a second launch.
 constexpr int kRemapThreads = 1024, kRemapEach = 2;
+constexpr int kRemapStored = 16384;
 // Entries that the block which finds the moves renames itself, 8192 in 2 us: with 8128
 // it takes 12.5 us, with a second launch 10.4 and 4.7; with 144 6.6, or 6.2 and 1.5.
 constexpr int kRenameOne = 16384;

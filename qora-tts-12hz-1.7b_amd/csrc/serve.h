@@ -50,7 +50,8 @@ struct RemapParams {
     const int32_t *source, *tokens;
     int window, sinks;
     int32_t *copied;
-    int32_t *scratch;  // kPoolEntries
+    int32_t *scratch;   // kPoolEntries
+    unsigned *counter;  // 0 between launches
 };
 
 struct ReserveParams {
