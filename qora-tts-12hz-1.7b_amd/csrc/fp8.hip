@@ -22,6 +22,7 @@ namespace qtts {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ f32x4 load4(const float *p) { return *glb(reinterpret_cast<const f32x4 *>(p)); }
@@ -156,15 +157,15 @@ __global__ __launch_bounds__(256) void k_fp8_weight(const float *src, int ld_src
 }
 
 // A weight's scale in two factors: a power of two that its codes take as they
-// become bfloat16, within 2^-117 and 2^117, and the rest (1 to 2, but at the ends of
-// f32).  A sum then is of the result's size: a large x beside a small scale does not
-// leave f32.
+// become bfloat16, within 2^-117 and 2^117, and the rest: 1 to 2, but 2^-32 and on,
+// or to 2^11, for a scale that is `far` out, at the ends of f32.  A sum then is of the
+// result's size: a large x beside a small scale does not leave f32.
 struct Scale {
     float power, rest;
-    bool none, bad;  // 0; Inf or NaN
+    bool none, bad, far;  // 0; Inf or NaN
     __device__ __forceinline__ explicit Scale(float s) {
         const int e = (int)(__float_as_uint(s) >> 23 & 255), c = min(max(e, 10), 244);
-        none = s == 0.0f, bad = e == 255;
+        none = s == 0.0f, bad = e == 255, far = !none && !bad && e != c;
         power = none || bad ? 1.0f : power_of(c);
         rest = none || bad ? 1.0f : s * power_of(254 - c);
     }
@@ -225,7 +226,9 @@ __device__ __forceinline__ unsigned lds_address(void *p) {
 // conversion wait for a barrier of their own.
 //
 // Sums are held in units of the current block's `rest`, one multiplication for each
-// 128: a second set of sums for the block would take the registers of the tile.
+// 128: a second set of sums for the block would take the registers of the tile.  The
+// unit stays within 1 and 2, or a sum would leave f32 in it: blocks whose scale is far
+// out are zeros in the steps and are added after them, each under its own scale.
 //
 // 256 x 256, 8192 rows, 2048 to 12288: 350 us, 1.18 PFLOP/s, where 8192 cubed in
 // bfloat16 is 1.24 in the library.  Of a step's 2950 cycles the products take 2048 (two
@@ -290,7 +293,7 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
         (const KCONST float *)(A.w.scales + (size_t)(min(n0 + wn * NF * 16, A.w.n - 1) / kFp8Block) * A.kb);
     f32x4 acc[NF][MF] = {};
     float next = ws[first >> 1], power = 1.0f, rest = 1.0f;
-    bool none = false, bad = false;
+    bool none = false, bad = false, far = false;
     i32x4 c[NF];    // this step's codes
     bf16x8 w[NF];   // the half at hand
     auto half = [&](int slot, int u, float by, bool scaled, auto &&between) {
@@ -306,13 +309,19 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
     };
     auto nothing = [](int) {};
     float by = 1.0f;
-    auto new_block = [&](int s) {  // its scale
-        const Scale z(next);
+    // a block's scale, as Scale has it; in integers, which a wave has once
+    auto new_block = [&](int s) {
+        const unsigned bits = __float_as_uint(next), e = bits >> 23 & 255;
         next = ws[min((s >> 1) + 1, A.kb - 1)];
-        power = z.power, none = z.none, bad |= z.bad;
-        by = rest * __builtin_amdgcn_rcpf(z.rest), rest = z.rest;
+        const bool held = e - 10 <= 234;
+        none = !held && e != 255;
+        bad |= e == 255, far |= none && bits << 1;
+        power = __uint_as_float(e << 23);  // (of zeros, or of what becomes NaN: any)
+        const float unit = held ? __uint_as_float((bits & 0x807fffffu) | 0x3f800000u) : rest;
+        by = rest * __builtin_amdgcn_rcpf(unit), rest = unit;
     };
-    // codes under a scale of 0 are zeros; every wave that reads these writes them
+    // codes under a scale of 0 are zeros, and for now under one far out; every wave that
+    // reads these writes them
     auto clear_codes = [&](int s) {
         for (int i = 0; i < NF; i++)
             *reinterpret_cast<i32x4 *>(ring + (s >> 1 & 1) * kCodes + (wn * NF + i) * 2048 + (my_code ^ (s & 1) * 64)) =
@@ -393,6 +402,33 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
     for (int i = 0; i < NF; i++)
 #pragma unroll
         for (int j = 0; j < MF; j++) acc[i][j] *= rest;
+    // straight from memory to registers, as without tiles
+    for (int b = first >> 1; far && 2 * b < last; b++) {
+        const Scale z(ws[b]);
+        if (!z.far) continue;
+#pragma unroll 1
+        for (int q = 0; q < 4; q++) {
+            const int at = b * 128 + 64 * (q >> 1) + 16 * G + 8 * (q & 1);
+            const uint8_t *wr = A.w.codes + (at < A.w.k ? at : b * 128);
+            const uint8_t *xr = A.xc + ((size_t)(m0 / 16 + wm * MF) * A.kb + b) * 4096 + q * 1024 + my_x;
+#pragma unroll
+            for (int i = 0; i < NF; i++) {
+                const int n = min(n0 + (wn * NF + i) * 16 + r, A.w.n - 1);
+                const i32x2 v = *glb(reinterpret_cast<const i32x2 *>(wr + (size_t)n * A.w.ld));
+                w[i] = values8(v[0], v[1], z.power);
+            }
+#pragma unroll
+            for (int j = 0; j < MF; j++) {
+                const bf16x8 x = *glb(reinterpret_cast<const bf16x8 *>(xr + (size_t)j * A.kb * 4096));
+#pragma unroll
+                for (int i = 0; i < NF; i++) {
+                    const f32x4 p = mma(w[i], x, f32x4{0, 0, 0, 0});
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(z.rest, p[e], acc[i][j][e]);
+                }
+            }
+        }
+    }
 #pragma unroll
     for (int j = 0; j < MF; j++) {
         const int row = m0 + (wm * MF + j) * 16 + r;
