@@ -49,7 +49,7 @@ struct qtts_ctx {
     float *attn_part = nullptr;
     unsigned *attn_counters = nullptr;
     unsigned *paged_counters = nullptr;
-    uint8_t *fp8_x = nullptr;  // rows of the products on 8-bit floats
+    uint8_t *fp8_x = nullptr;  // rows of the products on 8-bit floats, and their weight's scales
     // staging for the stand-alone operators
     float *d_in = nullptr;
     size_t d_in_cap = 0;
@@ -1598,7 +1598,7 @@ qtts_status qtts_ctx_create(int32_t device, qtts_ctx **out) {
     if (bad(hipMalloc(&c->attn_part, kAttnPartFloats * sizeof(float)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->attn_counters, kAttnCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->paged_counters, kPagedCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
-    if (bad(hipMalloc(&c->fp8_x, kFp8ScratchBytes))) return QTTS_ENOMEM;
+    if (bad(hipMalloc(&c->fp8_x, kFp8ScratchBytes + kFp8ChangesBytes))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->d_small, 256))) return QTTS_ENOMEM;
     if (bad(hipMemset(c->counters, 0, kCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
     if (bad(hipMemset(c->attn_counters, 0, kAttnCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
@@ -3093,6 +3093,7 @@ qtts_status qtts_fp8_gemm_device(qtts_ctx *c, const qtts_fp8_weight *w, const fl
     p.ld_y = ld_y;
     p.rows = rows;
     p.xc = c->fp8_x;
+    p.changes = (int2 *)(c->fp8_x + kFp8ScratchBytes);
     p.part = c->attn_part;
     DeviceGuard guard(c->device);
     launch_fp8_gemm(c->stream, p);

@@ -106,8 +106,58 @@ __device__ __forceinline__ u32x4 block_values(f32x4 x, f32x4 y) {
 // of four rows, kRowsAhead blocks one after another whose loads are in flight together.
 // Bound by memory: 8192 rows of 2048, 101 MB, in 18 to 26 us; 2100 of 6144 12.6 (four
 // blocks a wave 13.6); small ones by latency, 17 of 6144 3.4 us (4.2).
+//
+// The blocks behind those of the rows find how the tiles' unit changes along k
+// (Fp8Params::changes), a wave a row of the weight's scales, 64 at a time: 40 rows of 33
+// blocks 3.8 us, 3.6 without them, and no more where there are more rows.  (A factor found
+// in the tiles themselves, its rounding carried on, took their step 2 to 5 % longer.)
 constexpr int kRowsAhead = 2;
+__device__ void unit_changes(const Fp8Params &A, int nb) {
+    const int lane = threadIdx.x & 63;
+    if (nb * kFp8Block >= A.w.n) return;
+    const float *ws = A.w.scales + (size_t)nb * A.kb;
+    int carried = 0;
+    for (int b0 = 0; b0 < A.kb; b0 += 64) {
+        const int b = min(b0 + lane, A.kb - 1);
+        const unsigned scale = __float_as_uint(*glb(ws + b)), last = __float_as_uint(*glb(ws + max(b - 1, 0)));
+        const float from = __uint_as_float(fp8_unit(last)), to = __uint_as_float(fp8_unit(scale));
+        const Fp8Change c = fp8_change(from, to, __builtin_amdgcn_rcpf(from), __builtin_amdgcn_rcpf(to));
+        // Carried from lane to lane of 16, a block in each turn, and from 16 to 16 what the
+        // last of them has left (a product of factors is so within 2^-23).
+        int factor = c.quotient, before = 0;
+        if (carried != 0 || __any(c.left != 0)) {
+#pragma unroll
+            for (int turn = 0; turn < 15; turn++)  // row_shr:1, the first gets 0
+                before = __builtin_amdgcn_update_dpp(0, fp8_carry(c, before), 0x111, 0xF, 0xF, true);
+            factor += fp8_step(c, before);
+            const unsigned long long apart = __ballot(fp8_apart(c.quotient));
+            const int after = fp8_carry(c, before);
+#pragma unroll
+            for (int row = 0; row < 4; row++) {
+                const unsigned at = (unsigned)(apart >> 16 * row) & 0xffffu;
+                carried += __builtin_amdgcn_readlane(after, 16 * row + 15);
+                if (at == 0) continue;
+                const int l = 16 * row + 31 - __builtin_clz(at);
+                const Fp8Change all{0, 0, __builtin_amdgcn_readlane(c.half, l)};
+                const int step = fp8_step(all, carried);
+                factor += lane == l ? step : 0;
+                carried = fp8_carry(all, carried);
+            }
+        }
+        if (b0 + lane < A.kb) A.changes[(size_t)nb * A.kb + b0 + lane] = {(int)fp8_power(scale), factor};
+    }
+}
+
+__host__ __device__ __forceinline__ int rows_blocks(int rows, int kb) {
+    return (int)(((rows + 3) / 4 * (long long)kb + 4 * kRowsAhead - 1) / (4 * kRowsAhead));
+}
+
+template <bool TILES>
 __global__ __launch_bounds__(256) void k_fp8_rows(Fp8Params A) {
+    if (TILES) {
+        const int beyond = (int)blockIdx.x - rows_blocks(A.rows, A.kb);
+        if (beyond >= 0) return unit_changes(A, 4 * beyond + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    }
     const int lane = threadIdx.x & 15, sub = threadIdx.x >> 4 & 3;
     const long long at = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * kRowsAhead;
     const long long blocks = (long long)((A.rows + 3) / 4) * A.kb;
@@ -225,10 +275,13 @@ __device__ __forceinline__ unsigned lds_address(void *p) {
 // read and multiplied in one stretch, so that neither the reads nor the codes'
 // conversion wait for a barrier of their own.
 //
-// Sums are held in units of the current block's `rest`, one multiplication for each
-// 128: a second set of sums for the block would take the registers of the tile.  The
-// unit stays within 1 and 2, or a sum would leave f32 in it: blocks whose scale is far
-// out are zeros in the steps and are added after them, each under its own scale.
+// Sums are held in units of the current block's `rest` (fp8_unit), one multiplication
+// for each 128: a second set of sums for the block would take the registers of the tile.
+// The unit stays within 1 and 2, or a sum would leave f32 in it: blocks whose scale is far
+// out are zeros in the steps and are added after them, each under its own scale.  The
+// factors between units are k_fp8_rows', which has their roundings not add up: found here
+// as rest * (1 / rest), a product of them was up to 2.4e-6 off after 48 blocks, always to
+// one side, and 1 only by chance between equal scales.
 //
 // 256 x 256, 8192 rows, 2048 to 12288: 350 us, 1.18 PFLOP/s, where 8192 cubed in
 // bfloat16 is 1.24 in the library.  Of a step's 2950 cycles the products take 2048 (two
@@ -288,12 +341,20 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
     auto half_at = [&](int slot, int u, int j) {
         return *reinterpret_cast<const bf16x8 *>(ring + 2 * kCodes + (2 * slot + u) * kHalf + (wm * MF + j) * 1024 + my_x);
     };
-    // (scalar loads: they do not wait behind the others)
-    const KCONST float *ws =
-        (const KCONST float *)(A.w.scales + (size_t)(min(n0 + wn * NF * 16, A.w.n - 1) / kFp8Block) * A.kb);
+    const size_t scales_at = (size_t)(min(n0 + wn * NF * 16, A.w.n - 1) / kFp8Block) * A.kb;
+    const KCONST float *ws = (const KCONST float *)A.w.scales + scales_at;
     f32x4 acc[NF][MF] = {};
-    float next = ws[first >> 1], power = 1.0f, rest = 1.0f;
-    bool none = false, bad = false, far = false;
+    // 64 blocks' power and factor, a lane each, from block `ahead` on: a scalar load in each
+    // block would be waited for there
+    i32x2 changes;
+    int ahead;
+    auto look_ahead = [&](int b) {
+        ahead = b;
+        changes = *glb(reinterpret_cast<const i32x2 *>(A.changes) + scales_at + min(b + lane, A.kb - 1));
+    };
+    float rest = ws[(last - 1) >> 1], power = 1.0f, by = 1.0f;
+    int met = 0;
+    bool none = false;
     i32x4 c[NF];    // this step's codes
     bf16x8 w[NF];   // the half at hand
     auto half = [&](int slot, int u, float by, bool scaled, auto &&between) {
@@ -308,17 +369,10 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
         });
     };
     auto nothing = [](int) {};
-    float by = 1.0f;
-    // a block's scale, as Scale has it; in integers, which a wave has once
-    auto new_block = [&](int s) {
-        const unsigned bits = __float_as_uint(next), e = bits >> 23 & 255;
-        next = ws[min((s >> 1) + 1, A.kb - 1)];
-        const bool held = e - 10 <= 234;
-        none = !held && e != 255;
-        bad |= e == 255, far |= none && bits << 1;
-        power = __uint_as_float(e << 23);  // (of zeros, or of what becomes NaN: any)
-        const float unit = held ? __uint_as_float((bits & 0x807fffffu) | 0x3f800000u) : rest;
-        by = rest * __builtin_amdgcn_rcpf(unit), rest = unit;
+    auto new_block = [&](int s) {  // its scale
+        const int l = (s >> 1) - ahead, bits = __builtin_amdgcn_readlane(changes[0], l);
+        power = __int_as_float(bits), by = __int_as_float(__builtin_amdgcn_readlane(changes[1], l));
+        none = bits & kFp8None, met |= bits;
     };
     // codes under a scale of 0 are zeros, and for now under one far out; every wave that
     // reads these writes them
@@ -371,8 +425,14 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
         begin(next_slot, s + 1, odd);
         return next_slot;
     };
+    auto more_ahead = [&](int s) {
+        if ((s >> 1) + 1 - ahead < 64) return;
+        look_ahead((s >> 1) + 1);
+        asm volatile("" : "+v"(changes));  // waited for here, not in every block
+    };
     const auto yes = std::true_type{};
     const auto no = std::false_type{};
+    look_ahead(first >> 1);
     each<LA>([&](auto i) { load_codes(first, i); });
     each<LB>([&](auto i) { load_half(0, first, 0, i), load_half(0, first, 1, i); });
     if (first + 1 < last) each<LB>([&](auto i) { load_half(1, first + 1, 0, i), load_half(1, first + 1, 1, i); });
@@ -388,22 +448,24 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void k_fp8_tile(Fp8Params A) {
     int slot = 0, s = first;
     begin(slot, first, yes);
     for (; s + 4 < last; s += 2) {
+        more_ahead(s);
         slot = through(slot, s, no, yes);
         slot = through(slot, s + 1, yes, yes);
     }
     for (; s + 2 < last; s += 2) {
+        more_ahead(s);
         slot = through(slot, s, no, no);
         slot = through(slot, s + 1, yes, no);
     }
     if (s + 1 < last) slot = through(slot, s, no, no);
     half(slot, 1, 1.0f, false, nothing);
-    if (bad) rest = __uint_as_float(0x7fc00000u);
+    rest = __uint_as_float(met & kFp8Bad ? 0x7fc00000u : fp8_unit(__float_as_uint(rest)));
 #pragma unroll
     for (int i = 0; i < NF; i++)
 #pragma unroll
         for (int j = 0; j < MF; j++) acc[i][j] *= rest;
     // straight from memory to registers, as without tiles
-    for (int b = first >> 1; far && 2 * b < last; b++) {
+    for (int b = first >> 1; met & kFp8Far && 2 * b < last; b++) {
         const Scale z(ws[b]);
         if (!z.far) continue;
 #pragma unroll 1
@@ -603,14 +665,16 @@ void launch_fp8_gemm(hipStream_t st, const Fp8Params &in) {
             else few_of<8, true, 1>(st, p, x_bytes);
             continue;
         }
-        const long long each = 4 * kRowsAhead, rows_blocks = ((long long)(p.rows + 3) / 4 * p.kb + each - 1) / each;
-        hipLaunchKernelGGL(k_fp8_rows, dim3((unsigned)rows_blocks), dim3(256), 0, st, p);
+        const unsigned blocks = rows_blocks(p.rows, p.kb);
         if (plan.bn == 16) {
+            hipLaunchKernelGGL(k_fp8_rows<false>, dim3(blocks), dim3(256), 0, st, p);
             if (plan.bm == 16) few_of<8, false, 1>(st, p, 0);
             else if (plan.bm == 32) few_of<8, false, 2>(st, p, 0);
             else few_of<8, false, 4>(st, p, 0);
             continue;
         }
+        const unsigned scale_rows = fp8_blocks(p.w.n);
+        hipLaunchKernelGGL(k_fp8_rows<true>, dim3(blocks + (scale_rows + 3) / 4), dim3(256), 0, st, p);
         if (plan.bm == 256) tiles_of<256, 256, 4, 2>(st, p, plan);
         else if (plan.bm == 128) tiles_of<128, 128, 4, 2>(st, p, plan);
         else tiles_of<64, 64, 2, 2>(st, p, plan);

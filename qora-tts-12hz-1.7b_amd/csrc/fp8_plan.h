@@ -3,6 +3,7 @@
 // device code, so that the CPU tests run the same lines.
 #pragma once
 
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 
@@ -16,10 +17,13 @@ constexpr int kFp8MaxSide = 1 << 17;              // of n and k
 constexpr int kFp8MaxStride = 1 << 23;            // a tile's rows are reached by 32-bit offsets
 constexpr long long kFp8MaxRows = 1LL << 24;
 constexpr size_t kFp8ScratchBytes = (size_t)128 << 20;  // a context's: rows, in bfloat16
+constexpr size_t kFp8ChangesBytes = (size_t)8 << 20;    // and a weight's scales, as tiles take them
 constexpr int kFp8RowStep = 256;                  // rows that a tile takes at most
 constexpr int kFp8MaxSplits = 16;                 // parts of a sum
 constexpr long long kFp8PartFloats = 4LL << 20;   // all parts' sums
 constexpr int kFewRows = 4;                       // that a block may hold by themselves, not 16 at once
+
+static_assert(kFp8ChangesBytes >= (size_t)(kFp8MaxSide / kFp8Block) * (kFp8MaxSide / kFp8Block) * 8, "all blocks");
 
 inline int fp8_blocks(int k) { return (k + kFp8Block - 1) / kFp8Block; }
 
@@ -93,6 +97,52 @@ inline bool fp8_own_rows(int rows, int n, int kb) {
     return (rows < 16 ? rows : 16) * kb * ((blocks + 255) / 256) <= 128;
 }
 inline long long fp8_own_bytes(int rows, int kb) { return (rows <= kFewRows ? rows : 16LL) * kb * 256; }
+
+// The unit that a tile's sums are held in under a block's scale: the scale without its
+// power of two, 1 to 2 with its sign; 1 where the codes do not hold that power (under
+// 2^-117 or over 2^117, 0, Inf, NaN).
+QTTS_HD bool fp8_held(unsigned scale) { return (scale >> 23 & 255) - 10 <= 234; }
+QTTS_HD unsigned fp8_unit(unsigned scale) { return fp8_held(scale) ? (scale & 0x807fffffu) | 0x3f800000u : 0x3f800000u; }
+
+// A block's power of two, which its codes take, for an instruction that uses only the
+// exponent; below it what a tile has to know of the block.
+constexpr int kFp8None = 1, kFp8Bad = 2, kFp8Far = 4;  // zeros in the steps; Inf or NaN; added behind them
+QTTS_HD unsigned fp8_power(unsigned scale) {
+    const unsigned e = scale & 0x7f800000u;
+    if (fp8_held(scale)) return e;
+    return e == 0x7f800000u ? e | kFp8Bad : e | kFp8None | (scale << 1 ? kFp8Far : 0);
+}
+
+// From one unit to another: the quotient, rounded, as bits; what the rounding leaves of
+// it, and half of the quotient's last place, both in 2^-48 of it.  Of the reciprocals a
+// step or two may be wrong.
+struct Fp8Change {
+    int quotient, left, half;
+};
+QTTS_HD Fp8Change fp8_change(float from, float to, float from_inverse, float to_inverse) {
+    const float near = from * to_inverse, q = fmaf(fmaf(-near, to, from), to_inverse, near), size = fabsf(q);
+    union {
+        float f;
+        int i;
+    } bits{q};
+    const float half = (size < 1.0f ? 0x1p23f : 0x1p24f) * fabsf(to * from_inverse);
+    return {bits.i, (int)(fmaf(-q, to, from) * from_inverse * 0x1p48f), size == 1.0f ? 1 << 29 : (int)half};
+}
+// What the roundings of the quotients before have left is carried on; once it is half a
+// place, the quotient's neighbour is taken in its place.  The factors' product then is
+// never further than 2^-24 from the units' quotient, however often these change, and
+// equal units change nothing.
+QTTS_HD int fp8_step(const Fp8Change &c, int carried) {  // from the quotient to the factor
+    const int all = carried + c.left;
+    return all > c.half ? 1 : all < -c.half ? -1 : 0;
+}
+QTTS_HD int fp8_carry(const Fp8Change &c, int carried) {  // on to the next change
+    const int all = carried + c.left, place = 2 * c.half;
+    return all - (all > c.half ? place : all < -c.half ? -place : 0);
+}
+// Whether a quotient can go on by one more place of the same size: away from 1, where
+// places change theirs.
+QTTS_HD bool fp8_apart(int quotient) { return (unsigned)(quotient & 0x7fffffff) - 0x3f7fffffu > 2; }
 
 inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
     const int kb = fp8_blocks(k);

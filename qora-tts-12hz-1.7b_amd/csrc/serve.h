@@ -95,6 +95,7 @@ struct Fp8Params {
     float *y;
     int ld_x, ld_add, ld_y, rows;
     uint8_t *xc;          // kFp8ScratchBytes: rows as the products take them
+    int2 *changes;        // kFp8ChangesBytes: fp8_power and the factor into its unit, for each block of the weight
     float *part;          // kFp8PartFloats: split sums
     // the launch's own
     int kb;               // blocks of the contraction
