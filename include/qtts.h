@@ -607,9 +607,11 @@ typedef struct qtts_fp8_weight {
  * at least).  Products of codes are exact, their sums f32.  A row with an Inf or
  * NaN is NaN, as is a column whose weight or scale has one (codes under a scale of 0
  * count as 0).  rows 0..2^24.
- * Enqueued on the context stream, allocates nothing and can be captured (context
- * scratch, as above).  How the sum over k is divided goes by the sizes of a call,
- * so a row's last bits may depend on how many others there are. */
+ * Enqueued on the context stream, can be captured (context scratch, as above).  A
+ * context's first product of more than a few rows allocates 136 MiB for that, captured
+ * or not (QTTS_ENOMEM without them); later ones allocate nothing.  How the sum over k
+ * is divided goes by the sizes of a call, so a row's last bits may depend on how many
+ * others there are. */
 qtts_status qtts_fp8_gemm_device(qtts_ctx *ctx, const qtts_fp8_weight *w, const float *d_x, int32_t ld_x, int32_t rows,
                                  const float *d_add, int32_t ld_add, float *d_y, int32_t ld_y);
 

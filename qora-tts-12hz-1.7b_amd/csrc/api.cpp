@@ -512,6 +512,19 @@ qtts_status mfma_reserve(qtts_ctx *c, const Q4Mfma &w) {
     return grow_kept(c, &c->mfma_part, &c->mfma_part_cap, w.scratch_part);
 }
 
+// The products on 8-bit floats: their scratch with the first call that uses it.  A
+// capture on the stream may be that call: relaxed, a thread may allocate in one.
+qtts_status fp8_reserve(qtts_ctx *c) {
+    if (c->fp8_x) return QTTS_OK;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    HIP_TRY(c, hipThreadExchangeStreamCaptureMode(&mode));
+    const hipError_t e = hipMalloc(&c->fp8_x, kFp8ScratchBytes + kFp8ChangesBytes);
+    HIP_TRY(c, hipThreadExchangeStreamCaptureMode(&mode));
+    if (e == hipSuccess) return QTTS_OK;
+    c->fp8_x = nullptr;
+    return fail(c, QTTS_ENOMEM, "hipMalloc scratch of products on 8-bit floats");
+}
+
 // y[m] (+)= f(x[m]) . W (+ bias) for M rows on the matrix cores
 // (csrc/mfma.hip), f the row prologue (MfmaRowsMode): the prologue and
 // binary16 split, then the product.  Up to kMfmaPassRows rows: one block per
@@ -1598,7 +1611,6 @@ qtts_status qtts_ctx_create(int32_t device, qtts_ctx **out) {
     if (bad(hipMalloc(&c->attn_part, kAttnPartFloats * sizeof(float)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->attn_counters, kAttnCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->paged_counters, kPagedCounters * sizeof(unsigned)))) return QTTS_ENOMEM;
-    if (bad(hipMalloc(&c->fp8_x, kFp8ScratchBytes + kFp8ChangesBytes))) return QTTS_ENOMEM;
     if (bad(hipMalloc(&c->d_small, 256))) return QTTS_ENOMEM;
     if (bad(hipMemset(c->counters, 0, kCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
     if (bad(hipMemset(c->attn_counters, 0, kAttnCounters * sizeof(unsigned)))) return QTTS_EDEVICE;
@@ -3083,6 +3095,8 @@ qtts_status qtts_fp8_gemm_device(qtts_ctx *c, const qtts_fp8_weight *w, const fl
     if (!c || !w) return QTTS_EINVAL;
     QTTS_CHECK(c, check_fp8_gemm(*w, d_x, ld_x, rows, d_add, ld_add, d_y, ld_y));
     if (rows == 0) return QTTS_OK;
+    DeviceGuard guard(c->device);
+    if (fp8_scratch(rows, w->n, w->k)) QTTS_TRY(fp8_reserve(c));
     Fp8Params p{};
     p.w = *w;
     p.x = d_x;
@@ -3093,9 +3107,8 @@ qtts_status qtts_fp8_gemm_device(qtts_ctx *c, const qtts_fp8_weight *w, const fl
     p.ld_y = ld_y;
     p.rows = rows;
     p.xc = c->fp8_x;
-    p.changes = (int2 *)(c->fp8_x + kFp8ScratchBytes);
+    p.changes = c->fp8_x ? (int2 *)(c->fp8_x + kFp8ScratchBytes) : nullptr;
     p.part = c->attn_part;
-    DeviceGuard guard(c->device);
     launch_fp8_gemm(c->stream, p);
     return check_launch(c, "k_fp8_tile");
 }

@@ -144,6 +144,11 @@ QTTS_HD int fp8_carry(const Fp8Change &c, int carried) {  // on to the next chan
 // places change theirs.
 QTTS_HD bool fp8_apart(int quotient) { return (unsigned)(quotient & 0x7fffffff) - 0x3f7fffffu > 2; }
 
+// Whether a call uses the scratch.  (One of more rows than that holds does.)
+inline bool fp8_scratch(int rows, int n, int k) {
+    return rows > fp8_rows_at_once(k) || !fp8_own_rows(rows, n, fp8_blocks(k));
+}
+
 inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
     const int kb = fp8_blocks(k);
     Fp8Plan p{bn, bm, (n + bn - 1) / bn, (rows + bm - 1) / bm, 0, 1, 0, 0, 0};
