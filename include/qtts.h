@@ -520,8 +520,9 @@ qtts_status qtts_paged_remap_device(qtts_ctx *ctx, const qtts_paged_pool *pool, 
 
 /* Gives row b pages for its tokens starts[b] .. ends[b] - 1 (device, [batch]) where
  * the table has none: the lowest free ones, in order of rows and entries.  lacking
- * (NULL or [batch]) receives 0 for a row that has them all now, -1 for one whose
- * start is negative or whose end is below 0 or past the table, which is left out.
+ * (NULL or [batch], none of the pool's arrays; it may be starts or ends) receives 0
+ * for a row that has them all now, -1 for one whose start is negative or whose end is
+ * below 0 or past the table, which is left out.
  * From the first row that the free pages do not serve whole, rows receive none, and
  * lacking says how many each wants.  Enqueued on the context stream, allocates
  * nothing and can be captured (context scratch, as above). */
@@ -531,10 +532,10 @@ qtts_status qtts_paged_reserve_device(qtts_ctx *ctx, const qtts_paged_pool *pool
 /* Packs the pool: the pages in use become its first ones.  The i-th page in use
  * behind that border takes the id of the i-th free one before it; refs and table
  * follow.  from and to (device, [num_pages / 2]) receive the moves, -1 behind them,
- * live (NULL or one int) how many pages are in use.  Then every layer copies its
- * pages (qtts_paged_copy_pages_device with num_pages / 2) before they are read or
- * written.  Enqueued on the context stream, allocates nothing and can be captured
- * (context scratch, as above). */
+ * live (NULL or one int) how many pages are in use: three arrays of their own.  Then
+ * every layer copies its pages (qtts_paged_copy_pages_device with num_pages / 2) before
+ * they are read or written.  Enqueued on the context stream, allocates nothing and can
+ * be captured (context scratch, as above). */
 qtts_status qtts_paged_compact_device(qtts_ctx *ctx, const qtts_paged_pool *pool, int32_t *d_from, int32_t *d_to,
                                       int32_t *d_live);
 

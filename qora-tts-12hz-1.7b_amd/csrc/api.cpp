@@ -3043,6 +3043,7 @@ qtts_status qtts_paged_compact_device(qtts_ctx *c, const qtts_paged_pool *pool, 
                                       int32_t *d_live) {
     if (!c || !pool) return QTTS_EINVAL;
     QTTS_CHECK(c, check_compact(*pool, d_from, d_to, d_live));
+    QTTS_CHECK(c, check_compact_own(*pool, d_from, d_to, d_live));
     DeviceGuard guard(c->device);
     launch_paged_compact(c->stream, {*pool, d_from, d_to, d_live, (int32_t *)c->attn_part});
     return check_launch(c, "k_paged_compact");

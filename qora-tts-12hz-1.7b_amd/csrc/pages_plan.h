@@ -43,6 +43,13 @@ inline Refusal check_pool(const qtts_paged_pool &p) {
     return kAccepted;
 }
 
+// Whether an array that a call writes is one of others.
+inline bool one_of(const void *p, std::initializer_list<const void *> others) {
+    for (const void *o : others)
+        if (p && p == o) return true;
+    return false;
+}
+
 inline Refusal check_remap(const qtts_paged_pool &p, const int32_t *source, const int32_t *tokens, int32_t window,
                            int32_t sinks, const int32_t *copied) {
     QTTS_REFUSE(check_pool(p));
@@ -51,7 +58,7 @@ inline Refusal check_remap(const qtts_paged_pool &p, const int32_t *source, cons
     if (!tokens) return {QTTS_EINVAL, "paged remap: null tokens"};
     if (!aligned_to(source, 4) || !aligned_to(tokens, 4) || !aligned_to(copied, 4))
         return {QTTS_EINVAL, "paged remap: misaligned array"};
-    if (copied && (copied == source || copied == tokens || copied == p.slots || copied == p.page_table))
+    if (one_of(copied, {source, tokens, p.slots, p.page_table, p.refs}))
         return {QTTS_EINVAL, "paged remap: copied must be an array of its own"};
     return kAccepted;
 }
@@ -63,6 +70,8 @@ inline Refusal check_reserve(const qtts_paged_pool &p, const int32_t *starts, co
     if (!starts || !ends) return {QTTS_EINVAL, "paged reserve: null array"};
     if (!aligned_to(starts, 4) || !aligned_to(ends, 4) || !aligned_to(lacking, 4))
         return {QTTS_EINVAL, "paged reserve: misaligned array"};
+    if (one_of(lacking, {p.slots, p.page_table, p.refs}))
+        return {QTTS_EINVAL, "paged reserve: lacking must be none of the pool's arrays"};
     return kAccepted;
 }
 
@@ -72,6 +81,15 @@ inline Refusal check_compact(const qtts_paged_pool &p, const int32_t *from, cons
     if (!aligned_to(from, 4) || !aligned_to(to, 4) || !aligned_to(live, 4))
         return {QTTS_EINVAL, "paged compact: misaligned array"};
     if (from && from == to) return {QTTS_EINVAL, "paged compact: two lists"};
+    return kAccepted;
+}
+
+// What it writes beside the pool is arrays of their own.
+inline Refusal check_compact_own(const qtts_paged_pool &p, const int32_t *from, const int32_t *to,
+                                 const int32_t *live) {
+    if (one_of(from, {to, live, p.slots, p.page_table, p.refs}) || one_of(to, {live, p.slots, p.page_table, p.refs}) ||
+        one_of(live, {p.slots, p.page_table, p.refs}))
+        return {QTTS_EINVAL, "paged compact: from, to and live must be arrays of their own"};
     return kAccepted;
 }
 
