@@ -503,7 +503,9 @@ typedef struct qtts_paged_pool {
  * A row that goes on from itself keeps its pages up to the last one begun; one that
  * goes on from another shares that one's full pages.  A source outside the batch
  * ends the row: it holds nothing.  With window > 0, pages whose tokens the next row
- * of attention with this window and these sinks does not see are dropped.  What a
+ * of attention with this window and these sinks does not see are dropped, and do not
+ * return: a row that goes back later sees nothing in their place.  To be able to go
+ * back by n tokens, let every remap have a window n wider than attention's.  What a
  * row no longer holds is given back.  As an append's start, tokens[b] is a token of
  * the page that its source is filling or a page's first, as a full page's rows are not
  * kept: to go on from its middle, make tokens[b] its first token.  The row then takes
