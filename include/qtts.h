@@ -607,7 +607,8 @@ typedef struct qtts_fp8_weight {
  * strides multiples of 4; y is neither x nor overlaps it.  Each 128 values of a
  * row of x (the last ones fewer) go to e4m3 on the way, the nearest to x / s, ties
  * to even, with s the least power of two with which they stay within 448 (2^-110
- * at least).  Products of codes are exact, their sums f32.  A row with an Inf or
+ * at least; under 2^120, where 256 s would leave f32, codes end at 240).  Products of
+ * codes are exact, their sums f32.  A row with an Inf or
  * NaN is NaN, as is a column whose weight or scale has one (codes under a scale of 0
  * count as 0).  rows 0..2^24.
  * Enqueued on the context stream, can be captured (context scratch, as above).  A

@@ -8,8 +8,9 @@
 // code.  The products are taken on bfloat16 matrix instructions, whose sums keep
 // 2^-23 of the largest term.  The instructions on 8-bit floats would be twice as
 // fast, but within each eight products they drop what is 2^-13 below the largest
-// (measured term by term, with and without their scaling): 2.3e-5 of a result on
-// ordinary values, where f32 sums are at 1e-7.
+// (measured term by term, with and without their scaling): over 128 products of normal
+// values 1.5e-5 of the result, of values of many sizes 5e-5, where the bfloat16 ones have
+// 9e-9 and 2.6e-8.
 #include <algorithm>
 #include <type_traits>
 
@@ -104,8 +105,8 @@ __device__ __forceinline__ u32x4 block_values(f32x4 x, f32x4 y) {
 // the first 8, or the others), as they are to lie in LDS.
 // All rows to scratch, [row / 16][k / 64][half], zeros behind k.  A wave a block of 128
 // of four rows, kRowsAhead blocks one after another whose loads are in flight together.
-// Bound by memory: 8192 rows of 2048, 101 MB, in 18 to 26 us; 2100 of 6144 12.6 (four
-// blocks a wave 13.6); small ones by latency, 17 of 6144 3.4 us (4.2).
+// Bound by memory: 8192 rows of 2048, 101 MB, in 27 us; 2100 of 6144 12.6 (four blocks a
+// wave 13.6); small ones by latency, 17 of 6144 3.4 us (4.2).
 //
 // The blocks behind those of the rows find how the tiles' unit changes along k
 // (Fp8Params::changes), a wave a row of the weight's scales, 64 at a time: 40 rows of 33
@@ -180,7 +181,8 @@ __global__ __launch_bounds__(256) void k_fp8_rows(Fp8Params A) {
     }
 }
 
-// A weight in 8 bits, a block of 128 x 128 each: the same scales.
+// A weight in 8 bits, a block of 128 x 128 each: the same scales.  Bound by memory: 12288
+// rows of 2048, 126 MB, in 21.7 us (5.8 TB/s); 256 of 256 4.1, latency.
 __global__ __launch_bounds__(256) void k_fp8_weight(const float *src, int ld_src, qtts_fp8_weight w, int kb) {
     __shared__ unsigned tops[4];
     const int b = blockIdx.x % kb, nb = blockIdx.x / kb, c = b * kFp8Block + 4 * (threadIdx.x & 31);
@@ -283,13 +285,14 @@ __device__ __forceinline__ unsigned lds_address(void *p) {
 // as rest * (1 / rest), a product of them was up to 2.4e-6 off after 48 blocks, always to
 // one side, and 1 only by chance between equal scales.
 //
-// 256 x 256, 8192 rows, 2048 to 12288: 350 us, 1.18 PFLOP/s, where 8192 cubed in
-// bfloat16 is 1.24 in the library.  Of a step's 2950 cycles the products take 2048 (two
-// waves a SIMD); the multiplications, the conversions and the loads' addresses, some
-// 300 each, overlap with them in part, and at 1.9 to 2.1 GHz the card's power bounds
-// both.  Measured on the way: all loads right behind the barrier 3400 cycles, a
-// barrier behind each half 4000; a pattern of products and other instructions imposed
-// on the compiler's order 3150 to 4200.
+// 256 x 256, 8192 rows, 2048 to 12288: a call takes 382 us of which the rows are 27,
+// so some 355, 1.16 PFLOP/s, where 8192 cubed in bfloat16 is 1.24 in the library (375
+// to 420 in a kernel trace, under which the clock is lower).  Of a step's 2950 cycles
+// the products take 2048 (two waves a SIMD); the multiplications, the conversions and
+// the loads' addresses, some 300 each, overlap with them in part, and at 1.9 to 2.1
+// GHz the card's power bounds both.  Measured on the way: all loads right behind the
+// barrier 3400 cycles, a barrier behind each half 4000; a pattern of products and
+// other instructions imposed on the compiler's order 3150 to 4200.
 //
 // Eight waves on 128 x 128 rather than four: 512 rows, 2048 to 4096, 20.6 us against
 // 23.5; 2048 rows, 6144 to 2048, 52.8 against 59.9.
@@ -531,10 +534,10 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8Params A) {
 // waves take in turn, straight from memory to registers.  OWN: the block meanwhile
 // brings x to 8 bits itself, into LDS (fp8_own_rows); otherwise it comes from scratch,
 // which k_fp8_rows has filled.  Bound by a chain of latencies and by what every block
-// reads of the weight and of x from L2 (75 GB/s a CU): one row, 2048 to 12288, 25 MB in
-// 7 to 9 us (2.8 to 3.5 TB/s); 16 rows, 6144 to 2048 7.4 us, 2048 to 4096 3.8, 32 of
-// these 4.9, 64 7.0.  With 32 weight rows a block, half of x's reads and half of the
-// blocks: 5.2, 6.7 and 9.0.
+// reads of the weight and of x from L2 (75 GB/s a CU).  In a kernel trace one row, 2048 to
+// 12288, 25 MB, takes 9 to 9.9 us (2.5 to 2.8 TB/s; 8.8 among calls in a graph); 16 rows,
+// 6144 to 2048 8.1 us, 2048 to 4096 4.4, 32 of these 5.6, 64 8.1.  With 32 weight rows a
+// block, half of x's reads and half of the blocks, these three took 1.3 to 1.4 times as long.
 template <int W, bool OWN, int RF>
 __global__ __launch_bounds__(64 * W, W == 4 ? 3 : RF > 1 ? 2 : 4) void k_fp8_few(Fp8Params A) {
     constexpr int kAhead = 4 / RF;  // blocks of 128 asked for at once

@@ -169,10 +169,11 @@ inline Fp8Plan fp8_divided(int rows, int n, int k, int bn, int bm, int splits) {
 // 12288 362*, 410, -.  128 x 6144 -> 2048 in 64: 14 in four parts, 37 in one.
 //
 // Where the reads that every block repeats cost less, the kernel without tiles, in as
-// many rows a block as cost least: 32 rows of 2048 -> 4096 4.9 us (in tiles 8.4), 64 7.0
-// (9.2); 128 of 2048 -> 2048 6.7 (9.2); 333 of 1552 -> 1001 7.8 (10.1); 230 of 3248 -> 150
-// 3.9 (7.7); but 200 of 6144 -> 2048 29 (17*).  Over 110 drawn shapes 4 % more than
-// the best of all that can be chosen.
+// many rows a block as cost least (kernels' times, both sides of one session): 32 rows
+// of 2048 -> 4096 4.9 us (in tiles 8.4), 64 7.0 (9.2); 128 of 2048 -> 2048 6.7 (9.2);
+// 333 of 1552 -> 1001 7.8 (10.1); 230 of 3248 -> 150 3.9 (7.7); but 200 of 6144 ->
+// 2048 29 (17*).  Over 110 drawn shapes 4 % more than the best of all that can be
+// chosen.
 inline Fp8Plan fp8_plan(int rows, int n, int k) {
     const int kb = fp8_blocks(k);
     Fp8Plan best{};

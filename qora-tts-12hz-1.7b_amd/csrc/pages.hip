@@ -127,8 +127,8 @@ __device__ __forceinline__ void remapped(const RemapParams &A, int first, int (&
 }
 
 // Tables of up to kRemapThreads * kRemapEach entries: block 0 reads them all, then
-// writes; block 1 hands on the slots.  8 rows of 18: 3.5 us.  64 of 127 13 us, most of it
-// one CU's atomics.
+// writes; block 1 hands on the slots.  8 rows of 18: 3.5 us.  (64 of 127 took 13 us this
+// way, most of it one CU's atomics.)
 __global__ __launch_bounds__(kThreads) void k_paged_remap_one(RemapParams A) {
     __shared__ Slots S;
     if (blockIdx.x == 1) return hand_on_slots(A, S);
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kThreads) void k_paged_remap_one(RemapParams A) {
 
 // Larger ones: new rows to scratch, block 0 the slots; then scratch to the table: up to
 // kRemapStored entries by the block that ends last (64 of 127 4.8 to 5.9 us), more in a launch
-// of their own (4.1 + 2.3 us).
+// of their own (4.1 + 2.3 us; 64 of 500 5.6 together, 2^20 entries 12.7, 2^22 31).
 template <bool LAST>
 __global__ __launch_bounds__(kThreads) void k_paged_remap(RemapParams A) {
     __shared__ Slots S;
@@ -283,7 +283,8 @@ __global__ __launch_bounds__(kThreads) void k_paged_reserve(ReserveParams A) {
 // behind that border to the i-th free one before it.  Their new names go to scratch,
 // the border to its end.  One block, which renames a smaller table too; the moves of a
 // pool of one chunk stay in LDS (12532 pages, 2300 moves, without the renaming: 10.5 us,
-// 12.5 by way of the lists).
+// 12.5 by way of the lists).  Larger pools are the one block's to read twice: 65536 pages,
+// half of them in use anywhere, 52 us with the renaming, 2^20 0.75 ms, 2^22 3.0 ms.
 template <bool ONE>
 __global__ __launch_bounds__(kThreads) void k_paged_compact(CompactParams A) {
     __shared__ int sums[kWaves];
