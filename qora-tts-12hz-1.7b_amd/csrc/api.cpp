@@ -521,6 +521,7 @@ qtts_status fp8_reserve(qtts_ctx *c) {
     const hipError_t e = hipMalloc(&c->fp8_x, kFp8ScratchBytes + kFp8ChangesBytes);
     HIP_TRY(c, hipThreadExchangeStreamCaptureMode(&mode));
     if (e == hipSuccess) return QTTS_OK;
+    (void)hipGetLastError();  // or the next launch's check finds it
     c->fp8_x = nullptr;
     return fail(c, QTTS_ENOMEM, "hipMalloc scratch of products on 8-bit floats");
 }

@@ -1,6 +1,5 @@
 """The scratch of products on 8-bit floats: a context takes it with the first product
 that uses it, in a capture too, and no other."""
-import numpy as np
 import pytest
 import torch
 
@@ -76,4 +75,36 @@ def test_first_product_in_a_capture():
             assert torch.equal(y, got)
         del g
     finally:
+        ctx.close()
+
+
+def test_a_full_card():
+    """Refused where the scratch cannot be had, and nothing is left of it: products that
+    do without go on, and the others when there is room."""
+    w, few, rows = _weight(8, 260, 2048), _rows(9, 1, 2048), _rows(10, 90, 2048)
+    x, y, hold = _up(rows), torch.zeros((90, 260), device="cuda"), []
+    one = _up(few)
+    ctx = qtts.Context(0)
+    try:
+        _call(ctx, w, one, y)
+        ctx.synchronize()
+        for _ in range(4):
+            room = _free() - 100 * MIB
+            if room > 30 * MIB:
+                hold.append(torch.empty(room, dtype=torch.uint8, device="cuda"))
+        assert _free() < 136 * MIB
+        with pytest.raises(qtts.QttsError) as e:
+            _call(ctx, w, x, y)
+        assert e.value.status == qtts.QTTS_ENOMEM
+        _call(ctx, w, one, y)
+        ctx.synchronize()
+        hold.clear()
+        torch.cuda.empty_cache()
+        _check(y.cpu().numpy()[:1], few, w)
+        _call(ctx, w, x, y)
+        ctx.synchronize()
+        _check(y.cpu().numpy(), rows, w)
+    finally:
+        hold.clear()
+        torch.cuda.empty_cache()
         ctx.close()
